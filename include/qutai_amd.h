@@ -405,6 +405,37 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
                             int64_t heads, int64_t kv_heads, int64_t time, int64_t dim, int dtype, int layout,
                             double scale, int causal, void* stream);
 
+/* RMSNorm of every query and key head and the rotation of its position, in one
+ * launch: for each row x of `dim` values (even, at most 256) of [batch][time]
+ * positions and heads (kv_heads) heads,
+ *   n = x / sqrt(mean(x^2) + eps) * weight,
+ *   (out[2i], out[2i+1]) = (n[2i], n[2i+1]) turned by p * theta^(-2i/dim),
+ * p = offset + t + starts[b] (starts: int64 per sequence, or NULL).  Weights are
+ * fp32 [dim]; NULL for both leaves the norm out.  A position's rows start q_row
+ * (k_row) elements after the previous position's, so q and k may be columns of
+ * one wider matrix; q_out and k_out are contiguous.  Either side may be absent
+ * (0 heads, NULL pointers).  dtype QA_F32 or QA_BF16 for rows and outputs; the
+ * norm, the angles' sine and cosine and the products are fp32, the angles'
+ * reduction fp64.  Outputs share no memory with inputs.  The unfused form is
+ * qutai_amd_rms_norm per head and qutai_amd_rope_rows. */
+int qutai_amd_qk_norm_rope(const void* q, const void* k, const float* q_weight, const float* k_weight, void* q_out,
+                           void* k_out, const int64_t* starts, int64_t offset, int64_t batch, int64_t time,
+                           int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, double theta,
+                           double eps, int dtype, void* stream);
+
+/* The gradients of qutai_amd_qk_norm_rope: gq and gk contiguous gradients of its
+ * outputs, q and k its inputs; dq and dk of `dtype`, dq_row (dk_row) elements
+ * from position to position; dq_weight and dk_weight fp32 [dim] (NULL where not
+ * wanted), summed over all rows in a fixed order, which needs a workspace of
+ * qutai_amd_qk_norm_rope_workspace(dim) floats. */
+int qutai_amd_qk_norm_rope_backward(const void* gq, const void* gk, const void* q, const void* k,
+                                    const float* q_weight, const float* k_weight, void* dq, void* dk,
+                                    float* dq_weight, float* dk_weight, const int64_t* starts, int64_t offset,
+                                    int64_t batch, int64_t time, int64_t heads, int64_t kv_heads, int64_t dim,
+                                    int64_t q_row, int64_t k_row, int64_t dq_row, int64_t dk_row, double theta,
+                                    double eps, int dtype, float* workspace, int64_t workspace_floats, void* stream);
+int64_t qutai_amd_qk_norm_rope_workspace(int64_t dim);
+
 /* Attention of `length` new positions over a key/value cache of `total`
  * positions whose last `length` are the new ones: query i sees the first
  * total - length + i + 1 keys.  q and out are [batch][length][heads][dim], k

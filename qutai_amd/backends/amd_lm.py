@@ -733,6 +733,96 @@ def rope(values, batch, time, heads, dim, theta, offset=0, inverse=False, *, col
     return out
 
 
+def _qk_rows(values, positions, heads, dim, column, row, dtype):
+    """(pointer, elements per position) of one side's head rows: columns
+    column .. column + heads*dim of ``values``; (None, 0) without heads."""
+    if not heads:
+        return None, 0
+    width = heads * dim
+    row = width if row is None else row
+    if values.dtype != dtype or column < 0 or column + width > row or values.size < positions * row:
+        raise ValueError("query and key rows need one dtype and columns inside their storages")
+    return values.ptr + column * _TYPES[dtype][1], row
+
+
+def _qk_arguments(q, k, q_weight, k_weight, batch, time, heads, kv_heads, dim, starts):
+    sides = [(x, w) for x, w, n in ((q, q_weight, heads), (k, k_weight, kv_heads)) if n]
+    if min(batch, time, heads, kv_heads) < 0 or not sides or dim <= 0 or dim % 2 or dim > 256:
+        raise ValueError("qk_norm_rope needs query or key heads of an even width up to 256")
+    dtype = sides[0][0].dtype
+    if dtype not in ("bfloat16", "float32"):
+        raise ValueError("qk_norm_rope takes bfloat16 or float32 rows")
+    weights = [w for _, w in sides if w is not None]
+    if len(weights) not in (0, len(sides)) or any(w.dtype != "float32" or w.size != dim for w in weights):
+        raise ValueError("qk_norm_rope takes fp32 weights of dim values for every side, or none")
+    if starts is not None and (starts.dtype != "int64" or starts.size != batch):
+        raise ValueError("starts holds one int64 position per sequence")
+    return dtype
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, batch, time, heads, kv_heads, dim, theta, eps=1e-6, *, offset=0, starts=None,
+                 q_column=0, q_row=None, k_column=0, k_row=None):
+    """RMSNorm of every query and key head (rows of ``dim``, an fp32 weight of
+    ``dim`` values for each side) and its rotary embedding, one launch and one
+    rounding: (q, k), contiguous [batch][time][heads][dim].  Position t of
+    sequence b is offset + t, plus ``starts[b]`` (int64 storage) where given.  q
+    and k may be columns q_column .. (k_column ..) of a wider matrix of q_row
+    (k_row) elements per position, as in ``rope``.  Weights of None leave the
+    norm out; 0 heads leave a side out (its result is None)."""
+    dtype = _qk_arguments(q, k, q_weight, k_weight, batch, time, heads, kv_heads, dim, starts)
+    positions = batch * time
+    (q_at, q_row), (k_at, k_row) = (_qk_rows(q, positions, heads, dim, q_column, q_row, dtype),
+                                    _qk_rows(k, positions, kv_heads, dim, k_column, k_row, dtype))
+    out_q, out_k = (AMDStorage(positions * n * dim, dtype) if n else None for n in (heads, kv_heads))
+    if positions:
+        get_runtime().call("qutai_amd_qk_norm_rope", q_at, k_at, amd._p(q_weight), amd._p(k_weight), amd._p(out_q),
+                           amd._p(out_k), amd._p(starts), offset, batch, time, heads, kv_heads, dim, q_row, k_row,
+                           float(theta), float(eps), code(dtype))
+    return out_q, out_k
+
+
+def qk_norm_rope_backward(gq, gk, q, k, q_weight, k_weight, batch, time, heads, kv_heads, dim, theta, eps=1e-6, *,
+                          offset=0, starts=None, q_column=0, q_row=None, k_column=0, k_row=None, out=None):
+    """(dq, dk, dq_weight, dk_weight) of ``qk_norm_rope``: gq and gk the
+    contiguous gradients of its results in the rows' dtype, the other arguments
+    its own.  The input gradients are new contiguous storages, or with ``out`` (a
+    storage laid out like the wider matrix that holds both q and k: q_row and
+    k_row elements per position) its columns q_column .. and k_column ..; the
+    weights' gradients (None without weights) are fp32 sums over all rows in a
+    fixed order."""
+    dtype = _qk_arguments(q, k, q_weight, k_weight, batch, time, heads, kv_heads, dim, starts)
+    positions = batch * time
+    for g, n in ((gq, heads), (gk, kv_heads)):
+        if n and (g.dtype != dtype or g.size != positions * n * dim):
+            raise ValueError("gq and gk need the rows' dtype and one value for each of theirs")
+    (q_at, q_step), (k_at, k_step) = (_qk_rows(q, positions, heads, dim, q_column, q_row, dtype),
+                                      _qk_rows(k, positions, kv_heads, dim, k_column, k_row, dtype))
+    if out is None:
+        dq, dk = (AMDStorage(positions * n * dim, dtype) if n else None for n in (heads, kv_heads))
+        (dq_at, dq_step), (dk_at, dk_step) = (amd._p(dq), heads * dim), (amd._p(dk), kv_heads * dim)
+    else:
+        if heads and kv_heads and (q_step != k_step or not (q_column + heads * dim <= k_column
+                                                            or k_column + kv_heads * dim <= q_column)):
+            raise ValueError("out holds q's and k's gradients in separate columns of one row")
+        for x in (gq, gk, q, k):
+            if x is not None and out.nbytes and out.ptr < x.ptr + x.nbytes and x.ptr < out.ptr + out.nbytes:
+                raise ValueError("out must not share memory with an input")
+        dq = out if heads else None
+        dk = out if kv_heads else None
+        (dq_at, dq_step), (dk_at, dk_step) = (_qk_rows(out, positions, heads, dim, q_column, q_row, dtype),
+                                              _qk_rows(out, positions, kv_heads, dim, k_column, k_row, dtype))
+    dwq, dwk = (AMDStorage(dim, "float32") if n and w is not None else None
+                for n, w in ((heads, q_weight), (kv_heads, k_weight)))
+    runtime = get_runtime()
+    need = runtime.lib.qutai_amd_qk_norm_rope_workspace(dim) if dwq is not None or dwk is not None else 0
+    workspace = AMDStorage(need, "float32") if need else None
+    runtime.call("qutai_amd_qk_norm_rope_backward", amd._p(gq), amd._p(gk), q_at, k_at, amd._p(q_weight),
+                 amd._p(k_weight), dq_at, dk_at, amd._p(dwq), amd._p(dwk), amd._p(starts), offset, batch, time, heads,
+                 kv_heads, dim, q_step, k_step, dq_step, dk_step, float(theta), float(eps), code(dtype),
+                 amd._p(workspace), need)
+    return dq, dk, dwq, dwk
+
+
 def copy_rows(source, rows, width, *, column=0, row=None, out=None, out_column=0, out_row=None):
     """Columns column .. column + width of the ``rows`` rows of ``source``
     (``row`` elements each) into a new contiguous [rows][width] block, or into

@@ -76,6 +76,11 @@ SIGNATURES = {
     "qutai_amd_silu": [_p, _p, _p, _i64, _i32, _i32, _p],
     "qutai_amd_rope": [_p, _p, _i64, _i64, _i64, _i64, _f64, _i64, _i32, _i32, _p],
     "qutai_amd_rope_rows": [_p, _p, _i64, _i64, _i64, _i64, _f64, _i64, _i32, _i64, _i64, _i32, _p],
+    "qutai_amd_qk_norm_rope": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f64, _f64,
+                               _i32, _p],
+    "qutai_amd_qk_norm_rope_backward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+                                        _i64, _i64, _i64, _i64, _f64, _f64, _i32, _p, _i64, _p],
+    "qutai_amd_qk_norm_rope_workspace": [_i64],
     "qutai_amd_head_rows": [_p, _p, _i64, _i64, _i64, _i64, _i32, _i32, _p],
     "qutai_amd_head_loss": [_p, _p, _p, _i64, _i64, _i32, _p],
     "qutai_amd_head_gradient": [_p, _p, _p, _i64, _i64, _f64, _i32, _p],
@@ -98,7 +103,7 @@ SIGNATURES = {
                               _i32, _p],
     "qutai_amd_gemm_static_capacity": [],
 }
-RESTYPES = {"qutai_amd_gemm_workspace_size": _sz, "qutai_amd_rms_norm_workspace": _i64,
+RESTYPES = {"qutai_amd_gemm_workspace_size": _sz, "qutai_amd_qk_norm_rope_workspace": _i64, "qutai_amd_rms_norm_workspace": _i64,
             "qutai_amd_attention_bwd_workspace_size": _sz, "qutai_amd_reduce_sum_workspace_size": _sz,
             "qutai_amd_gemm_static_capacity": _sz, "qutai_amd_route_workspace_size": _sz}
 

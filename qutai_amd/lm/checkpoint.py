@@ -52,6 +52,8 @@ def _file_hash(path):
 
 def _config(model):
     config = getattr(model, "config", None)
+    if hasattr(config, "to_dict"):
+        return config.to_dict()
     return asdict(config) if is_dataclass(config) else config
 
 

@@ -1,5 +1,6 @@
 """Decoder configuration (src/qutai/lm/config.py:5-71): the same fields,
-defaults, validation and parameter-count formula."""
+defaults, validation and parameter-count formula, and ``qk_norm``: an RMSNorm of
+every query and key head before its rotation, off by default."""
 from __future__ import annotations
 
 from dataclasses import asdict, dataclass
@@ -23,6 +24,7 @@ class Config:
     norm_eps: float = 1e-06
     aux_loss_coef: float = 0.01
     activation_checkpointing: bool = True
+    qk_norm: bool = False
 
     def __post_init__(self):
         sizes = (self.vocab_size, self.n_layers, self.d_model, self.n_heads, self.n_kv_heads, self.d_ff,
@@ -39,17 +41,26 @@ class Config:
         real = (self.norm_eps, self.rope_theta, self.aux_loss_coef)
         if any(not isinstance(v, (int, float)) or not isfinite(v) for v in real):
             raise ValueError("norm_eps, rope_theta and aux_loss_coef must be finite numbers")
+        if type(self.qk_norm) is not bool:
+            raise ValueError("qk_norm must be True or False")
         if self.norm_eps <= 0 or self.rope_theta <= 0 or self.aux_loss_coef < 0:
             raise ValueError("norm_eps and rope_theta must be positive, aux_loss_coef non-negative")
 
     def to_dict(self):
-        return asdict(self)
+        """The fields as a dict; qk_norm only where it is set, so that a
+        configuration without it is the reference's."""
+        fields = asdict(self)
+        if not self.qk_norm:
+            del fields["qk_norm"]
+        return fields
 
     def parameter_counts(self):
         d = self.d_model
         kv_width = self.n_kv_heads * (d // self.n_heads)
         shared = self.vocab_size * d + d  # tied embedding / head and the final norm
         per_attention = 2 * d * d + 2 * d * kv_width + 2 * d  # q, out, k, v and the two norms
+        if self.qk_norm:
+            per_attention += 2 * (d // self.n_heads)
         if self.ffn_type == "dense":
             total = shared + self.n_layers * (per_attention + 3 * d * self.d_ff)
             return {"total_parameters": total, "active_parameters": total}

@@ -58,6 +58,8 @@ class Decoder:
             p = f"blocks.{i}."
             result += [(p + "attn_norm.weight", block.attn_norm.weight), (p + "ffn_norm.weight", block.ffn_norm.weight)]
             result += [(p + f"attn.{n}.weight", getattr(block.attn, n).weight) for n in ("q", "k", "v", "out")]
+            if block.attn.q_norm is not None:
+                result += [(p + f"attn.{n}.weight", getattr(block.attn, n).weight) for n in ("q_norm", "k_norm")]
             if block.is_moe:
                 result.append((p + "ffn.router.weight", block.ffn.router.weight))
                 result += [(p + "ffn.experts.gate.weight", block.ffn.w_gate), (p + "ffn.experts.up.weight", block.ffn.w_up),

@@ -234,6 +234,29 @@ def rope(x, heads, theta, offset=0):
                   lambda g: (b.rope(g, *dims, inverse=True),))
 
 
+def qk_norm_rope(q, k, q_weight, k_weight, heads, kv_heads, theta, eps, offset=0):
+    """RMSNorm of every head of q (batch, time, heads*dim) and k (batch, time,
+    kv_heads*dim), weights of dim values each, and their rotary embedding in
+    one launch; (q, k), recorded."""
+    b = backend(q)
+    batch, time, features = q.shape
+    dims = (batch, time, heads, kv_heads, features // heads, theta, eps)
+    values = b.qk_norm_rope(q.storage, k.storage, q_weight.storage, k_weight.storage, *dims, offset=offset)
+
+    def query_gradients(g):
+        dq, _, dweight, _ = b.qk_norm_rope_backward(g, None, q.storage, None, q_weight.storage, None, batch, time, heads,
+                                                    0, *dims[4:], offset=offset)
+        return owned(dq), owned(dweight)
+
+    def key_gradients(g):
+        _, dk, _, dweight = b.qk_norm_rope_backward(None, g, None, k.storage, None, k_weight.storage, batch, time, 0,
+                                                    kv_heads, *dims[4:], offset=offset)
+        return owned(dk), owned(dweight)
+
+    return (record(Tensor(values[0], shape=q.shape), (q, q_weight), query_gradients),
+            record(Tensor(values[1], shape=k.shape), (k, k_weight), key_gradients))
+
+
 def silu_mul(gate, up):
     """silu(gate) * up as one recorded op (SwiGLU's activation, lm/layers.py:310-311)."""
     b = backend(gate)
@@ -399,7 +422,8 @@ class RMSNorm:
 
 class GQA:
     """Grouped-query attention block: q/k/v projections (seeds seed..seed+2),
-    RoPE on q and k, fused causal attention, out projection (seed+3, std
+    RoPE on q and k (with ``config.qk_norm`` after an RMSNorm of every head,
+    in the same pass), fused causal attention, out projection (seed+3, std
     0.02/sqrt(2 n_layers)) (src/qutai/lm/layers.py:317-350)."""
 
     def __init__(self, config, *, device="amd", dtype="float32", seed=None):
@@ -415,17 +439,25 @@ class GQA:
         self.out = Projection(width, width, device=device, dtype=dtype, seed=offset(3),
                               std=0.02 / sqrt(2 * config.n_layers))
         self.heads, self.kv_heads, self.theta = config.n_heads, config.n_kv_heads, config.rope_theta
+        self.q_norm, self.k_norm = (RMSNorm(width // config.n_heads, config.norm_eps, device=device, dtype=dtype)
+                                    if getattr(config, "qk_norm", False) else None for _ in range(2))
 
     def __call__(self, x):
         weights = (self.q.weight, self.k.weight, self.v.weight)
+        norms = () if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
         if _stacked_qkv(x, *weights):
-            return self.out(gqa_attention(x, *weights, self.heads, self.kv_heads, self.theta))
-        q = rope(self.q(x), self.heads, self.theta)
-        k = rope(self.k(x), self.kv_heads, self.theta)
+            return self.out(gqa_attention(x, *weights, self.heads, self.kv_heads, self.theta, *norms,
+                                          **({"eps": self.q_norm.eps} if norms else {})))
+        if norms:
+            q, k = qk_norm_rope(self.q(x), self.k(x), *norms, self.heads, self.kv_heads, self.theta, self.q_norm.eps)
+        else:
+            q = rope(self.q(x), self.heads, self.theta)
+            k = rope(self.k(x), self.kv_heads, self.theta)
         return self.out(attention(q, k, self.v(x), self.heads, self.kv_heads))
 
     def parameters(self):
-        return (*self.q.parameters(), *self.k.parameters(), *self.v.parameters(), *self.out.parameters())
+        layers = (self.q, self.k, self.v, self.out) + (() if self.q_norm is None else (self.q_norm, self.k_norm))
+        return tuple(p for layer in layers for p in layer.parameters())
 
 
 class Block:
@@ -630,7 +662,7 @@ def _stacked_qkv(x, wq, wk, wv):
     return _bf16_path(x, wq) and activation_dtype(x, wq) == "bfloat16"
 
 
-def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta):
+def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=None, *, eps=1e-6):
     """RoPE(x Wq^T), RoPE(x Wk^T), x Wv^T and causal grouped-query attention
     as one recorded op: GQA up to its out projection (src/qutai/lm/layers.py:
     317-350 with rope 108-116 and attention 119-130) on the bf16 path.  The
@@ -642,7 +674,9 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta):
     GEMM.  The forward values are those of the separate projections (every
     output element sums K in the same order whatever the tile); the input
     gradient sums its three terms in one accumulator where the separate
-    projections add three rounded products."""
+    projections add three rounded products.  With norm weights q_norm and k_norm
+    (of a head's width) every head is normed before its rotation, in the pass
+    that reads the product's columns; the product is then kept for the backward."""
     b = backend(x)
     batch, time, width = x.shape
     rows = batch * time
@@ -655,10 +689,17 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta):
     for w, start in ((wq, 0), (wk, dq), (wv, dq + dkv)):
         amd.cast_into(amd.view(ws, start * width, w.size), w.storage)
     qkv = b.gemm(xs, ws, rows, width, total, transpose_right=True, out_dtype="bfloat16")
-    q = b.rope(qkv, batch, time, heads, head, theta, row=total)
-    k = b.rope(qkv, batch, time, kv_heads, head, theta, column=dq, row=total)
     v = b.copy_rows(qkv, rows, dkv, column=dq + dkv, row=total)
-    del qkv
+    if q_norm is None:
+        q = b.rope(qkv, batch, time, heads, head, theta, row=total)
+        k = b.rope(qkv, batch, time, kv_heads, head, theta, column=dq, row=total)
+        del qkv
+        parents = (x, wq, wk, wv)
+    else:
+        norm_dims = (q_norm.storage, k_norm.storage, batch, time, heads, kv_heads, head, theta, eps)
+        columns = dict(q_row=total, k_column=dq, k_row=total)
+        q, k = b.qk_norm_rope(qkv, qkv, *norm_dims, **columns)
+        parents = (x, wq, wk, wv, q_norm, k_norm)
     dims = (batch, time, heads, kv_heads, head)
     out, lse = b.attention(q, k, v, *dims)
 
@@ -666,8 +707,12 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta):
         with set_matmul_precision(precision):
             gq, gk, gv = b.attention_backward(g, q, k, v, out, lse, *dims)
             d = amd.AMDStorage(rows * total, gq.dtype)
-            b.rope(gq, batch, time, heads, head, theta, inverse=True, out=d, out_row=total)
-            b.rope(gk, batch, time, kv_heads, head, theta, inverse=True, out=d, out_column=dq, out_row=total)
+            dnorms = ()
+            if q_norm is None:
+                b.rope(gq, batch, time, heads, head, theta, inverse=True, out=d, out_row=total)
+                b.rope(gk, batch, time, kv_heads, head, theta, inverse=True, out=d, out_column=dq, out_row=total)
+            else:
+                dnorms = tuple(map(owned, b.qk_norm_rope_backward(gq, gk, qkv, qkv, *norm_dims, **columns, out=d)[2:]))
             b.copy_rows(gv, rows, dkv, out=d, out_column=dq + dkv, out_row=total)
             dx = None
             if x.requires_grad:
@@ -678,9 +723,9 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta):
                 dw = b.gemm(d, xs, total, rows, width, transpose_left=True, out_dtype=wq.dtype)
                 dws = tuple(owned(amd.view(dw, start * width, w.size)) if w.requires_grad else None
                             for w, start in ((wq, 0), (wk, dq), (wv, dq + dkv)))
-        return (dx, *dws)
+        return (dx, *dws, *dnorms)
 
-    return record(Tensor(out, shape=(batch, time, dq)), (x, wq, wk, wv), backward)
+    return record(Tensor(out, shape=(batch, time, dq)), parents, backward)
 
 
 def attention_fused(q, k, v, *, scale=None, causal=False):
