@@ -436,6 +436,26 @@ int qutai_amd_qk_norm_rope_backward(const void* gq, const void* gk, const void* 
                                     double eps, int dtype, float* workspace, int64_t workspace_floats, void* stream);
 int64_t qutai_amd_qk_norm_rope_workspace(int64_t dim);
 
+/* One token for each of `rows` rows of `vocab` logits (dtype QA_F32 or QA_BF16;
+ * at most 2^20 of them, rows below 2^22).  With the weights w_i = exp((l_i - max)
+ * / temperature) and the tokens ordered by falling logits, equal ones by index:
+ *   top_k (> 0) keeps the first top_k tokens,
+ *   top_p (< 1) of those the shortest prefix that holds top_p of their weight
+ *   (one token at least),
+ *   min_p of those the ones with w_i >= min_p,
+ * and the token is the first, by index, at which the running sum of the kept
+ * weights exceeds u times their sum; u = uniforms[row] (QA_F32 or QA_F64, taken
+ * as 0 below 0 and as 1, the last kept token, above 1).  Its probability
+ * among the kept tokens goes to probabilities (fp32).  Temperature 0 takes the
+ * largest logit, the lowest index of equal ones, with probability 1.  A NaN
+ * counts as -inf; a row of nothing else gives token -1 with probability 0; beside
+ * +inf every finite logit weighs nothing.  Weights and their sums are 64-bit.
+ * Each parameter is one number, or where its pointer is not NULL one per row. */
+int qutai_amd_sample(const void* logits, const void* uniforms, int64_t* tokens, float* probabilities, int64_t rows,
+                     int64_t vocab, const float* temperatures, double temperature, const int64_t* top_ks,
+                     int64_t top_k, const float* top_ps, double top_p, const float* min_ps, double min_p, int dtype,
+                     int uniform_dtype, void* stream);
+
 /* Attention of `length` new positions over a key/value cache of `total`
  * positions whose last `length` are the new ones: query i sees the first
  * total - length + i + 1 keys.  q and out are [batch][length][heads][dim], k
@@ -446,6 +466,53 @@ int64_t qutai_amd_qk_norm_rope_workspace(int64_t dim);
  * sequence of the cache path (src/qutai/nn/layers.py:345-355). */
 int qutai_amd_attention_cached(const void* q, const void* k, const void* v, void* out, int64_t batch, int64_t heads,
                                int64_t length, int64_t total, int64_t dim, int dtype, double scale, void* stream);
+
+/* New keys and values quantised into a cache of `capacity` positions for each of
+ * [batch][kv_heads] rows.  keys and values hold [batch][fresh] positions of
+ * kv_heads x dim values (dim <= 256) of `dtype` (QA_BF16 or QA_F32), key_row
+ * (value_row) elements from one position to the next; position t of sequence b
+ * is written as cache position start + starts[b] + t (starts, counts: int64 per
+ * sequence, or NULL), unless t >= counts[b] or it lies outside the capacity.
+ *
+ * bits 8: a scale per row, codes -127 .. 127; bits 4: a scale per 32 channels,
+ * codes -7 .. 7.  A scale is the smallest bfloat16 from 2^-100 up whose product
+ * with 127 (7) reaches the group's largest magnitude; a code is x / scale rounded
+ * to nearest, ties to even, and stands for code x scale (exact in fp32).  A group
+ * with an infinity or NaN stands for NaN.  key_codes and value_codes (16-byte
+ * aligned) hold qutai_amd_cache_pitch(dim) x bits / 8 bytes for each cached
+ * position, in an order of the library's own; key_scales and value_scales one
+ * bfloat16 (bits 8) or pitch / 32 of them (bits 4).  batch x fresh x kv_heads
+ * below 2^25. */
+int qutai_amd_cache_quantize(const void* keys, const void* values, void* key_codes, void* key_scales,
+                             void* value_codes, void* value_scales, const int64_t* starts, const int64_t* counts,
+                             int64_t start, int64_t batch, int64_t fresh, int64_t kv_heads, int64_t dim,
+                             int64_t capacity, int64_t key_row, int64_t value_row, int bits, int dtype, void* stream);
+int64_t qutai_amd_cache_pitch(int64_t dim);
+
+/* The values that one side's codes stand for (keys != 0: the keys'), rounded once
+ * to dtype: out is [batch][kv_heads][length][dim], zeros from position shift +
+ * lengths[b] on (lengths: int64 per sequence, or NULL for shift alone);
+ * length <= capacity. */
+int qutai_amd_cache_dequantize(const void* codes, const void* scales, void* out, const int64_t* lengths,
+                               int64_t shift, int64_t batch, int64_t kv_heads, int64_t dim, int64_t capacity,
+                               int64_t length, int bits, int keys, int dtype, void* stream);
+
+/* Attention of `fresh` new positions over such a cache: q and out are
+ * [batch][fresh][heads][dim] of dtype, heads a multiple of kv_heads (head h reads
+ * kv head h / (heads / kv_heads)); query t of sequence b sees the cache positions
+ * up to start + starts[b] + t, and is zero where t >= counts[b] or it sees none.
+ * longest bounds the positions that any sequence sees (it decides how the work is
+ * split, not what is computed).  Scores, probabilities and sums are fp32, the
+ * cache's values those its codes stand for.  workspace:
+ * qutai_amd_attention_quantized_workspace_size bytes; too small a one is
+ * QA_EWORKSPACE.  batch x fresh x heads at most 2^25. */
+int qutai_amd_attention_quantized(const void* q, const void* key_codes, const void* key_scales,
+                                  const void* value_codes, const void* value_scales, void* out, const int64_t* starts,
+                                  const int64_t* counts, int64_t start, int64_t batch, int64_t fresh, int64_t heads,
+                                  int64_t kv_heads, int64_t dim, int64_t capacity, int64_t longest, int bits, int dtype,
+                                  double scale, void* workspace, size_t workspace_bytes, void* stream);
+size_t qutai_amd_attention_quantized_workspace_size(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads,
+                                                    int64_t dim, int64_t longest);
 
 /* A key and a value cache extended in one launch: out[r] = past[r] followed by
  * new[r] for each of `rows` (batch, head) rows of past_bytes and new_bytes, both

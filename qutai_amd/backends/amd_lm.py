@@ -538,6 +538,103 @@ def cache_join(past, new, rows):
     return out
 
 
+class QuantizedCache:
+    """Device memory of a quantised key and value cache: codes of 8 bits (a
+    scale per row) or 4 bits (a scale per 32 channels) for ``capacity``
+    positions of each (sequence, kv head), laid out by the library
+    (qutai_amd_cache_quantize)."""
+
+    def __init__(self, batch, kv_heads, dim, capacity, bits):
+        if bits not in (8, 4):
+            raise ValueError("a quantised cache has codes of 8 or 4 bits")
+        if batch <= 0 or not 0 < kv_heads <= 65536 or not 0 < dim <= 256 or not 0 < capacity <= 1 << 31:
+            raise ValueError("a quantised cache needs sequences, kv heads, a head width up to 256 and a capacity")
+        self.batch, self.kv_heads, self.dim, self.capacity, self.bits = batch, kv_heads, dim, capacity, bits
+        pitch = get_runtime().lib.qutai_amd_cache_pitch(dim)
+        rows, scales = batch * kv_heads * capacity, 1 if bits == 8 else pitch // 32
+        # codes are raw bytes: eight to a word (a row has 16 at least)
+        self.key_codes, self.value_codes = (AMDStorage(rows * pitch * bits // 64, "int64") for _ in range(2))
+        self.key_scales, self.value_scales = (AMDStorage(rows * scales, "bfloat16") for _ in range(2))
+
+
+def _cache_positions(cache, *arrays):
+    for values in arrays:
+        if values is not None and (values.dtype != "int64" or values.size != cache.batch):
+            raise ValueError("a cache's positions and counts are one int64 per sequence")
+
+
+def cache_quantize(cache, keys, values, new, *, start=0, starts=None, counts=None, key_column=0, key_row=None,
+                   value_column=0, value_row=None):
+    """Quantise ``new`` positions of every sequence into ``cache`` from position
+    start + starts[b] on (``starts``, ``counts``: int64 storages of one value per
+    sequence; only the first counts[b] positions are written, and none outside
+    the capacity).  keys and values are [batch][new][kv_heads][dim], or columns
+    key_column .. (value_column ..) of wider matrices of key_row (value_row)
+    elements per position."""
+    width, positions = cache.kv_heads * cache.dim, cache.batch * new
+    key_row, value_row = (width if row is None else row for row in (key_row, value_row))
+    if new < 0 or keys.dtype != values.dtype or keys.dtype not in ("bfloat16", "float32"):
+        raise ValueError("cached keys and values are bfloat16 or float32, of one dtype")
+    for x, column, row in ((keys, key_column, key_row), (values, value_column, value_row)):
+        if column < 0 or column + width > row or x.size < positions * row:
+            raise ValueError("keys and values need new positions of kv_heads * dim values for every sequence")
+    _cache_positions(cache, starts, counts)
+    if positions:
+        item = _TYPES[keys.dtype][1]
+        cache.key_codes.runtime.call(
+            "qutai_amd_cache_quantize", keys.ptr + key_column * item, values.ptr + value_column * item,
+            cache.key_codes.ptr, cache.key_scales.ptr, cache.value_codes.ptr, cache.value_scales.ptr, amd._p(starts),
+            amd._p(counts), start, cache.batch, new, cache.kv_heads, cache.dim, cache.capacity, key_row, value_row,
+            cache.bits, code(keys.dtype))
+
+
+def cache_dequantize(cache, length, *, lengths=None, shift=0, dtype="float32"):
+    """(keys, values) that the cache holds at its first ``length`` positions,
+    [batch][kv_heads][length][dim] in ``dtype``; zeros from position shift +
+    lengths[b] on (without ``lengths``: from ``length`` on)."""
+    if not 0 <= length <= cache.capacity or dtype not in ("bfloat16", "float32"):
+        raise ValueError("a cache is read up to its capacity, as bfloat16 or float32")
+    _cache_positions(cache, lengths)
+    shift = shift if lengths is not None else length
+    out = []
+    for codes, scales, keys in ((cache.key_codes, cache.key_scales, 1), (cache.value_codes, cache.value_scales, 0)):
+        values = AMDStorage(cache.batch * cache.kv_heads * length * cache.dim, dtype)
+        if values.size:
+            values.runtime.call("qutai_amd_cache_dequantize", codes.ptr, scales.ptr, values.ptr, amd._p(lengths), shift,
+                                cache.batch, cache.kv_heads, cache.dim, cache.capacity, length, cache.bits, keys,
+                                code(dtype))
+        out.append(values)
+    return tuple(out)
+
+
+def attention_quantized(cache, q, new, heads, *, start=0, starts=None, counts=None, longest=None, scale=None):
+    """Attention of ``new`` positions over a quantised cache that holds them:
+    q and the result are [batch][new][heads][dim]; query t of sequence b sees
+    the cache up to position start + starts[b] + t.  Rows t >= counts[b] are
+    zero.  ``longest`` (the capacity if not given) bounds the positions that any
+    sequence sees and sizes the split of the work."""
+    if q.dtype not in ("bfloat16", "float32"):
+        raise ValueError("attention_quantized takes bfloat16 or float32 queries")
+    if new < 0 or heads <= 0 or heads % cache.kv_heads or q.size != cache.batch * new * heads * cache.dim:
+        raise ValueError("queries need new positions of heads * dim values, heads a multiple of the cache's")
+    _cache_positions(cache, starts, counts)
+    longest = cache.capacity if longest is None else longest
+    if not 0 <= longest <= cache.capacity:
+        raise ValueError("longest lies between 0 and the capacity")
+    scale = cache.dim ** -0.5 if scale is None else scale
+    out = AMDStorage(q.size, q.dtype)
+    if q.size:
+        runtime = out.runtime
+        need = runtime.lib.qutai_amd_attention_quantized_workspace_size(cache.batch, new, heads, cache.kv_heads,
+                                                                        cache.dim, longest)
+        workspace = AMDStorage((need + 3) // 4, "float32") if need else None
+        runtime.call("qutai_amd_attention_quantized", q.ptr, cache.key_codes.ptr, cache.key_scales.ptr,
+                     cache.value_codes.ptr, cache.value_scales.ptr, out.ptr, amd._p(starts), amd._p(counts), start,
+                     cache.batch, new, heads, cache.kv_heads, cache.dim, cache.capacity, longest, cache.bits,
+                     code(q.dtype), float(scale), amd._p(workspace), need)
+    return out
+
+
 def attention_backward(gradient, q, k, v, out, lse, batch, time, heads, kv_heads, dim, *, causal=True, layout=1,
                        scale=None):
     """(dq, dk, dv) of ``attention`` (cuda_lm.attention_backward,
@@ -908,6 +1005,47 @@ def head_block_gradient(logits, labels, stats, gradient, rows, cols, col0, count
         logits.runtime.call("qutai_amd_head_block_gradient", logits.ptr, ids.ptr, stats.ptr, g.ptr, rows, cols, col0,
                             1.0 / count, code(logits.dtype))
     return logits
+
+
+def _sampling_parameter(value, name, rows, dtype, valid):
+    """(device pointer or None, number) of a parameter that is one number or a
+    storage of one per row."""
+    if isinstance(value, AMDStorage):
+        if value.dtype != dtype or value.size != rows:
+            raise ValueError(f"{name} for every row is a {dtype} storage of that many values")
+        return value.ptr, 0
+    if not isinstance(value, (int, float)) or isinstance(value, bool) or not valid(value):
+        raise ValueError(f"{name} is out of range")
+    return None, value
+
+
+def sample(logits, uniforms, rows, vocab, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(tokens int64, probabilities float32): one token for each row of
+    [rows][vocab] logits, picked by ``uniforms`` (float32 or float64 numbers in
+    [0, 1), one per row) among the tokens that are kept.  In the order of falling
+    logits (equal ones: lowest index first) ``top_k`` keeps that many (0: all),
+    ``top_p`` the shortest prefix of them that holds this share of their weight
+    exp((logit - max) / temperature), ``min_p`` those of them that weigh at least
+    that much of the largest.  The token is the first, by index, at which the
+    running sum of the kept weights exceeds the row's number times their sum; the
+    probability is its share.  Temperature 0 takes the largest logit.  Each
+    parameter is a number, or a storage of one per row (float32; top_k int64).  A
+    NaN logit counts as -inf; a row of -inf gives token -1."""
+    if logits.dtype not in ("bfloat16", "float32") or uniforms.dtype not in ("float32", "float64"):
+        raise ValueError("sample takes bfloat16 or float32 logits and float32 or float64 uniforms")
+    if rows < 0 or not 0 < vocab <= 1 << 20 or rows >= 1 << 22 or logits.size != rows * vocab or uniforms.size != rows:
+        raise ValueError("sample needs rows * vocab logits (vocab at most 2^20) and a number for every row")
+    temperatures, temperature = _sampling_parameter(temperature, "temperature", rows, "float32",
+                                                    lambda x: 0 <= x < float("inf"))
+    top_ks, top_k = _sampling_parameter(top_k, "top_k", rows, "int64", lambda x: type(x) is int and 0 <= x < 1 << 62)
+    top_ps, top_p = _sampling_parameter(top_p, "top_p", rows, "float32", lambda x: 0 <= x <= 1)
+    min_ps, min_p = _sampling_parameter(min_p, "min_p", rows, "float32", lambda x: 0 <= x <= 1)
+    tokens, probabilities = AMDStorage(rows, "int64"), AMDStorage(rows, "float32")
+    if rows:
+        tokens.runtime.call("qutai_amd_sample", logits.ptr, uniforms.ptr, tokens.ptr, probabilities.ptr, rows, vocab,
+                            temperatures, float(temperature), top_ks, top_k, top_ps, float(top_p), min_ps, float(min_p),
+                            code(logits.dtype), code(uniforms.dtype))
+    return tokens, probabilities
 
 
 def head_gradient(logits, labels, rows, vocab, gradient, count, *, start=0):

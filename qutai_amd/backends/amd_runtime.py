@@ -86,6 +86,14 @@ SIGNATURES = {
     "qutai_amd_head_gradient": [_p, _p, _p, _i64, _i64, _f64, _i32, _p],
     "qutai_amd_attention_fwd": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _f64, _i32, _p],
     "qutai_amd_attention_cached": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _f64, _p],
+    "qutai_amd_sample": [_p, _p, _p, _p, _i64, _i64, _p, _f64, _p, _i64, _p, _f64, _p, _f64, _i32, _i32, _p],
+    "qutai_amd_cache_quantize": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
+                                 _i32, _p],
+    "qutai_amd_cache_pitch": [_i64],
+    "qutai_amd_cache_dequantize": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p],
+    "qutai_amd_attention_quantized": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                      _i32, _i32, _f64, _p, _sz, _p],
+    "qutai_amd_attention_quantized_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64],
     "qutai_amd_cache_join": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p],
     "qutai_amd_attention_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _i64, _i64, _i64, _i64, _i64, _i32,
                                 _i32, _f64, _i32, _p],
@@ -103,7 +111,8 @@ SIGNATURES = {
                               _i32, _p],
     "qutai_amd_gemm_static_capacity": [],
 }
-RESTYPES = {"qutai_amd_gemm_workspace_size": _sz, "qutai_amd_qk_norm_rope_workspace": _i64, "qutai_amd_rms_norm_workspace": _i64,
+RESTYPES = {"qutai_amd_cache_pitch": _i64, "qutai_amd_attention_quantized_workspace_size": _sz,
+            "qutai_amd_gemm_workspace_size": _sz, "qutai_amd_qk_norm_rope_workspace": _i64, "qutai_amd_rms_norm_workspace": _i64,
             "qutai_amd_attention_bwd_workspace_size": _sz, "qutai_amd_reduce_sum_workspace_size": _sz,
             "qutai_amd_gemm_static_capacity": _sz, "qutai_amd_route_workspace_size": _sz}
 

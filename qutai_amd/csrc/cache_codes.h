@@ -1,0 +1,60 @@
+// How a quantised key or value cache holds a row of `dim` channels.
+//
+// A group of channels -- the row where codes have 8 bits, 32 channels where they
+// have 4 -- shares a scale: the smallest bfloat16 s >= 2^-100 with M s >= the
+// group's largest magnitude, M = 127 or 7; a code is x / s rounded to nearest,
+// ties to even, and stands for code * s, a product that fp32 holds exactly.  A
+// group with an infinity or NaN has the scale NaN (and codes 0).
+//
+// Rows are padded to a pitch P of channels (zeros).  Eight bits: a byte per
+// channel, in order.  Four bits: two's complement nibbles in the order in which
+// the attention kernel's lanes take them, 16 lanes or 4 x 16 lanes to a row:
+//   keys: lane group g of 4 holds P/8 bytes, a dword for each 32 channels c, of
+//     channels 32c + 8g + j; nibble n of the dword is j = 2 (n % 4) + n / 4;
+//   values: lane r of 16 holds P/32 bytes, one for each 32 channels c, of
+//     channels 32c + 2r (low nibble) and 32c + 2r + 1.
+#pragma once
+#include "common.h"
+
+namespace qa {
+
+inline int64_t cache_pitch(int64_t dim) {
+  for (const int64_t p : {32, 64, 96, 128, 192, 256})
+    if (dim <= p) return p;
+  return 0;
+}
+
+inline int64_t cache_groups(int64_t pitch, int bits) { return bits == 8 ? 1 : pitch / 32; }
+inline int64_t cache_row_bytes(int64_t pitch, int bits) { return pitch * bits / 8; }
+
+// The scale's bfloat16 bits for a largest magnitude; `most` is 127 or 7.
+__device__ __forceinline__ uint32_t scale_bits(float amax, float most) {
+  if (!(amax <= 3.4028234663852886e38f)) return 0x7fc0u;  // infinity or NaN
+  // the rounded quotient upwards; one step more where it was rounded down onto a bfloat16 (M s is exact)
+  uint32_t s = (__float_as_uint(amax / most) + 0xffffu) >> 16;
+  if (s < 0x0d80u) s = 0x0d80u;  // 2^-100
+  if (most * __uint_as_float(s << 16) < amax) s++;
+  return s;
+}
+
+// x / s rounded to nearest, ties to even: an estimate, and its exact remainder.
+__device__ __forceinline__ int code_of(float x, float s, float inverse) {
+  float q = rintf(x * inverse);
+  const float rest = fmaf(-q, s, x), twice = 2.f * fabsf(rest);
+  if (twice > s || (twice == s && ((int)q & 1))) q += rest > 0.f ? 1.f : -1.f;
+  return (int)q;
+}
+
+// byte and shift of a channel's nibble within a 4-bit row
+__device__ __forceinline__ int key_nibble(int d, int pitch, int& shift) {
+  const int c = d >> 5, g = (d >> 3) & 3, j = d & 7, n = (j >> 1) + 4 * (j & 1);
+  shift = 4 * (n & 1);
+  return g * (pitch >> 3) + 4 * c + (n >> 1);
+}
+__device__ __forceinline__ int value_nibble(int d, int pitch, int& shift) {
+  shift = 4 * (d & 1);
+  return ((d & 31) >> 1) * (pitch >> 5) + (d >> 5);
+}
+__device__ __forceinline__ int nibble_value(uint32_t byte, int shift) { return (int)(byte << (28 - shift)) >> 28; }
+
+}  // namespace qa

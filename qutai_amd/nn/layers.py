@@ -16,7 +16,8 @@ inference over new positions only: their projections, the cached keys and
 values appended, the score product against every cached key with the
 causal mask shifted by the cached length, softmax and the value product (a
 few positions in one launch), all with graph recording off
-(src/qutai/nn/layers.py:334-355).
+(src/qutai/nn/layers.py:334-355).  ``cache=QuantizedKVCache(capacity)`` does
+the same over codes of 8 or 4 bits, quantised as they are written.
 """
 from __future__ import annotations
 
@@ -29,7 +30,7 @@ from ..core import operations
 from ..core.context import set_recording
 from ..core.grad import owned, record
 from ..core.tensor import Tensor, _result, matmul
-from .cache import KVCache  # noqa: F401 - the reference exposes it beside the layers
+from .cache import KVCache, QuantizedKVCache  # noqa: F401 - the reference exposes KVCache beside the layers
 
 
 def _tensor(data, like):
@@ -170,6 +171,10 @@ class MultiHeadAttention(Attention):
         with set_recording(False):
             tensor = self._input(data)
             queries, keys, values = (layer(tensor) for layer in (self.query, self.key, self.value))
+            if isinstance(cache, QuantizedKVCache):
+                shape = (*queries.shape[:2], self.heads, queries.shape[2] // self.heads)
+                cache.append(keys.reshape(shape), values.reshape(shape))
+                return self.output(cache.attend(queries.reshape(shape)).reshape(queries.shape))
             keys, values = cache.update(self._split(keys), self._split(values))
             batch, length, features = tensor.shape
             total, dim = keys.shape[2:]

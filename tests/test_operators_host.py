@@ -8,6 +8,7 @@ import pytest
 
 from qutai_amd.backends import amd, amd_lm, amd_runtime
 from qutai_amd.lm import Config
+from qutai_amd.nn import QuantizedKVCache
 
 LIBRARY = Path(__file__).resolve().parent.parent / "qutai_amd" / "libqutai_amd.so"
 built = pytest.mark.skipif(not LIBRARY.exists(), reason="libqutai_amd.so not built")
@@ -97,3 +98,123 @@ def test_config_with_normed_heads():
     assert extra == plain.n_layers * 2 * 16
     with pytest.raises(ValueError):
         Config(qk_norm=1)
+
+
+# ---- the quantised cache -----------------------------------------------------------
+
+def fake_cache(batch=2, kv_heads=2, dim=8, capacity=10, bits=8):
+    cache = object.__new__(amd_lm.QuantizedCache)
+    cache.batch, cache.kv_heads, cache.dim, cache.capacity, cache.bits = batch, kv_heads, dim, capacity, bits
+    return cache
+
+
+def test_a_cache_of_impossible_sizes_is_refused():
+    for sizes in ((2, 2, 8, 10, 2), (0, 2, 8, 10, 8), (2, 0, 8, 10, 8), (2, 2, 0, 10, 8), (2, 2, 257, 10, 8), (2, 2, 8, 0, 4)):
+        with pytest.raises(ValueError):
+            amd_lm.QuantizedCache(*sizes)
+    for arguments in ((0, 8), (-3, 8), (8, 16), (2.0, 8)):
+        with pytest.raises(ValueError):
+            QuantizedKVCache(arguments[0], bits=arguments[1])
+    cache = QuantizedKVCache(8)
+    cache.truncate(0)
+    assert cache.length == 0
+    for lengths in (1, (1, 0)):
+        with pytest.raises(ValueError):
+            cache.truncate(lengths)
+
+
+@pytest.mark.parametrize("change", [
+    dict(new=-1), dict(keys=fake(96, "float32")), dict(keys=fake(96, "int64"), values=fake(96, "int64")),
+    dict(values=fake(95, "bfloat16")), dict(key_column=1), dict(value_row=15), dict(starts=fake(3, "int64")),
+    dict(counts=fake(2, "float32")),
+])
+def test_cache_quantize_refuses(change):
+    a = dict(cache=fake_cache(), keys=fake(96, "bfloat16"), values=fake(96, "bfloat16"), new=3)
+    with pytest.raises(ValueError):
+        amd_lm.cache_quantize(**{**a, **change})
+
+
+@pytest.mark.parametrize("change", [
+    dict(q=fake(192, "int64")), dict(q=fake(191, "float32")), dict(heads=3), dict(heads=0), dict(new=-1), dict(longest=11),
+    dict(starts=fake(1, "int64")), dict(counts=fake(2, "bfloat16")),
+])
+def test_attention_quantized_refuses(change):
+    a = dict(cache=fake_cache(), q=fake(2 * 3 * 4 * 8, "float32"), new=3, heads=4)
+    with pytest.raises(ValueError):
+        amd_lm.attention_quantized(**{**a, **change})
+
+
+def test_cache_dequantize_refuses():
+    for change in (dict(length=11), dict(length=-1), dict(length=4, dtype="float64"), dict(length=4, lengths=fake(3, "int64"))):
+        with pytest.raises(ValueError):
+            amd_lm.cache_dequantize(fake_cache(), **change)
+
+
+@built
+def test_cache_entry_points_refuse():
+    library, p = amd_runtime.load_library(), FAKE
+
+    def write(key_codes=p, start=0, batch=2, new=3, heads=2, dim=8, capacity=10, key_row=16, value_row=16, bits=8, dtype=5,
+              keys=p):
+        return library.qutai_amd_cache_quantize(keys, p, key_codes, p, p, p, None, None, start, batch, new, heads, dim,
+                                                capacity, key_row, value_row, bits, dtype, None)
+
+    for change in (dict(key_codes=p + 8), dict(start=1 << 60), dict(batch=-1), dict(new=-1), dict(heads=0), dict(dim=257),
+                   dict(dim=0), dict(capacity=0), dict(key_row=15), dict(value_row=15), dict(bits=5), dict(dtype=0 + 4),
+                   dict(keys=None), dict(batch=1 << 13, new=1 << 13), dict(key_codes=None), dict(capacity=1 << 40)):
+        assert write(**change) == amd_runtime.QA_EINVAL, change
+    assert write(batch=0) == 0 and write(new=0) == 0
+
+    def read(shift=0, batch=2, heads=2, dim=8, capacity=10, length=4, bits=8, dtype=5, codes=p):
+        return library.qutai_amd_cache_dequantize(codes, p, p, None, shift, batch, heads, dim, capacity, length, bits, 1,
+                                                  dtype, None)
+
+    for change in (dict(length=11), dict(length=-1), dict(bits=16), dict(dtype=1), dict(codes=None), dict(codes=p + 4),
+                   dict(dim=300), dict(shift=1 << 50)):
+        assert read(**change) == amd_runtime.QA_EINVAL, change
+
+    def attend(q=p, start=0, batch=2, new=3, heads=4, kv_heads=2, dim=8, capacity=10, longest=10, bits=8, dtype=5, scale=1.0,
+               codes=p):
+        size = library.qutai_amd_attention_quantized_workspace_size(batch, new, heads, kv_heads, dim, longest)
+        return library.qutai_amd_attention_quantized(q, codes, p, p, p, p, None, None, start, batch, new, heads, kv_heads,
+                                                     dim, capacity, longest, bits, dtype, scale, p, size, None)
+
+    for change in (dict(q=None), dict(start=-(1 << 50)), dict(batch=-1), dict(new=-1), dict(heads=3), dict(kv_heads=0),
+                   dict(dim=0), dict(dim=257), dict(capacity=0), dict(longest=11), dict(bits=3), dict(dtype=4),
+                   dict(scale=0.0), dict(scale=float("nan")), dict(codes=p + 8), dict(batch=1 << 12, new=1 << 12)):
+        assert attend(**change) == amd_runtime.QA_EINVAL, change
+    assert attend(batch=0) == 0 and attend(new=0) == 0
+    pitch = library.qutai_amd_cache_pitch
+    assert [pitch(d) for d in (0, 1, 32, 33, 80, 100, 129, 193, 256, 257)] == [0, 32, 32, 64, 96, 128, 192, 256, 256, 0]
+
+
+# ---- sampling ------------------------------------------------------------------------
+
+@pytest.mark.parametrize("change", [
+    dict(logits=fake(40, "float64")), dict(logits=fake(39, "float32")), dict(uniforms=fake(4, "bfloat16")),
+    dict(uniforms=fake(5, "float32")), dict(rows=-1), dict(vocab=0), dict(vocab=1 << 21), dict(temperature=-1.0),
+    dict(temperature=float("inf")), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=1.5), dict(top_k=True),
+    dict(top_p=1.1), dict(top_p=-0.1), dict(min_p=2), dict(min_p=float("nan")), dict(top_k=fake(4, "float32")),
+    dict(temperature=fake(3, "float32")), dict(top_p=fake(4, "float64")), dict(min_p="0"),
+])
+def test_sample_refuses(change):
+    a = dict(logits=fake(40, "float32"), uniforms=fake(4, "float32"), rows=4, vocab=10)
+    with pytest.raises(ValueError):
+        amd_lm.sample(**{**a, **change})
+
+
+@built
+def test_sample_entry_point_refuses():
+    library, p = amd_runtime.load_library(), FAKE
+
+    def call(logits=p, uniforms=p, tokens=p, probabilities=p, rows=4, vocab=10, temperature=1.0, top_k=0, top_p=1.0,
+             min_p=0.0, dtype=0, uniform_dtype=0):
+        return library.qutai_amd_sample(logits, uniforms, tokens, probabilities, rows, vocab, None, temperature, None, top_k,
+                                        None, top_p, None, min_p, dtype, uniform_dtype, None)
+
+    for change in (dict(logits=None), dict(uniforms=None), dict(tokens=None), dict(probabilities=None), dict(rows=-1),
+                   dict(rows=1 << 22), dict(vocab=0), dict(vocab=(1 << 20) + 1), dict(temperature=-1.0),
+                   dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_k=-1), dict(top_p=-1.0),
+                   dict(top_p=float("nan")), dict(min_p=1.5), dict(min_p=float("nan")), dict(dtype=1), dict(uniform_dtype=5)):
+        assert call(**change) == amd_runtime.QA_EINVAL, change
+    assert call(rows=0, logits=None) == 0
