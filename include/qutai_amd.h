@@ -505,14 +505,16 @@ int qutai_amd_cache_dequantize(const void* codes, const void* scales, void* out,
  * split, not what is computed).  Scores, probabilities and sums are fp32, the
  * cache's values those its codes stand for.  workspace:
  * qutai_amd_attention_quantized_workspace_size bytes; too small a one is
- * QA_EWORKSPACE.  batch x fresh x heads at most 2^25. */
+ * QA_EWORKSPACE.  capacity is a multiple of 32 (at most 2^30; what lies behind a
+ * sequence's last position may be anything), the scales are 4-byte aligned;
+ * batch x fresh x heads at most 2^25. */
 int qutai_amd_attention_quantized(const void* q, const void* key_codes, const void* key_scales,
                                   const void* value_codes, const void* value_scales, void* out, const int64_t* starts,
                                   const int64_t* counts, int64_t start, int64_t batch, int64_t fresh, int64_t heads,
                                   int64_t kv_heads, int64_t dim, int64_t capacity, int64_t longest, int bits, int dtype,
                                   double scale, void* workspace, size_t workspace_bytes, void* stream);
 size_t qutai_amd_attention_quantized_workspace_size(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads,
-                                                    int64_t dim, int64_t longest);
+                                                    int64_t dim, int64_t longest, int dtype);
 
 /* A key and a value cache extended in one launch: out[r] = past[r] followed by
  * new[r] for each of `rows` (batch, head) rows of past_bytes and new_bytes, both

@@ -541,14 +541,15 @@ def cache_join(past, new, rows):
 class QuantizedCache:
     """Device memory of a quantised key and value cache: codes of 8 bits (a
     scale per row) or 4 bits (a scale per 32 channels) for ``capacity``
-    positions of each (sequence, kv head), laid out by the library
-    (qutai_amd_cache_quantize)."""
+    positions (rounded up to whole blocks of 32) of each (sequence, kv head),
+    laid out by the library (qutai_amd_cache_quantize)."""
 
     def __init__(self, batch, kv_heads, dim, capacity, bits):
         if bits not in (8, 4):
             raise ValueError("a quantised cache has codes of 8 or 4 bits")
-        if batch <= 0 or not 0 < kv_heads <= 65536 or not 0 < dim <= 256 or not 0 < capacity <= 1 << 31:
+        if batch <= 0 or not 0 < kv_heads <= 65536 or not 0 < dim <= 256 or not 0 < capacity <= 1 << 30:
             raise ValueError("a quantised cache needs sequences, kv heads, a head width up to 256 and a capacity")
+        capacity = (capacity + 31) // 32 * 32
         self.batch, self.kv_heads, self.dim, self.capacity, self.bits = batch, kv_heads, dim, capacity, bits
         pitch = get_runtime().lib.qutai_amd_cache_pitch(dim)
         rows, scales = batch * kv_heads * capacity, 1 if bits == 8 else pitch // 32
@@ -626,7 +627,7 @@ def attention_quantized(cache, q, new, heads, *, start=0, starts=None, counts=No
     if q.size:
         runtime = out.runtime
         need = runtime.lib.qutai_amd_attention_quantized_workspace_size(cache.batch, new, heads, cache.kv_heads,
-                                                                        cache.dim, longest)
+                                                                        cache.dim, longest, code(q.dtype))
         workspace = AMDStorage((need + 3) // 4, "float32") if need else None
         runtime.call("qutai_amd_attention_quantized", q.ptr, cache.key_codes.ptr, cache.key_scales.ptr,
                      cache.value_codes.ptr, cache.value_scales.ptr, out.ptr, amd._p(starts), amd._p(counts), start,

@@ -135,7 +135,7 @@ void launch_write(const WriteArgs& a, hipStream_t stream) {
 }
 
 bool sizes_ok(int64_t batch, int64_t heads, int64_t dim, int64_t capacity, int bits, int dtype) {
-  return batch >= 0 && heads > 0 && heads <= 65536 && dim > 0 && dim <= 256 && capacity > 0 && capacity <= (1ll << 31) &&
+  return batch >= 0 && heads > 0 && heads <= 65536 && dim > 0 && dim <= 256 && capacity > 0 && capacity <= (1ll << 30) &&
          batch <= (1ll << 24) && (bits == 8 || bits == 4) && (dtype == BF16 || dtype == F32);
 }
 

@@ -173,17 +173,18 @@ def test_cache_entry_points_refuse():
                    dict(dim=300), dict(shift=1 << 50)):
         assert read(**change) == amd_runtime.QA_EINVAL, change
 
-    def attend(q=p, start=0, batch=2, new=3, heads=4, kv_heads=2, dim=8, capacity=10, longest=10, bits=8, dtype=5, scale=1.0,
-               codes=p):
-        size = library.qutai_amd_attention_quantized_workspace_size(batch, new, heads, kv_heads, dim, longest)
+    def attend(q=p, start=0, batch=2, new=3, heads=4, kv_heads=2, dim=8, capacity=1024, longest=1000, bits=8, dtype=5,
+               scale=1.0, codes=p, less=0):
+        size = library.qutai_amd_attention_quantized_workspace_size(batch, new, heads, kv_heads, dim, longest, dtype) - less
         return library.qutai_amd_attention_quantized(q, codes, p, p, p, p, None, None, start, batch, new, heads, kv_heads,
-                                                     dim, capacity, longest, bits, dtype, scale, p, size, None)
+                                                     dim, capacity, longest, bits, dtype, scale, p, max(size, 0), None)
 
     for change in (dict(q=None), dict(start=-(1 << 50)), dict(batch=-1), dict(new=-1), dict(heads=3), dict(kv_heads=0),
-                   dict(dim=0), dict(dim=257), dict(capacity=0), dict(longest=11), dict(bits=3), dict(dtype=4),
+                   dict(dim=0), dict(dim=257), dict(capacity=0), dict(capacity=1000), dict(longest=1025), dict(bits=3), dict(dtype=4),
                    dict(scale=0.0), dict(scale=float("nan")), dict(codes=p + 8), dict(batch=1 << 12, new=1 << 12)):
         assert attend(**change) == amd_runtime.QA_EINVAL, change
     assert attend(batch=0) == 0 and attend(new=0) == 0
+    assert attend(less=4) == amd_runtime.QA_EWORKSPACE
     pitch = library.qutai_amd_cache_pitch
     assert [pitch(d) for d in (0, 1, 32, 33, 80, 100, 129, 193, 256, 257)] == [0, 32, 32, 64, 96, 128, 192, 256, 256, 0]
 
