@@ -17,6 +17,7 @@ import atexit
 import ctypes
 import os
 import threading
+from collections import deque
 from pathlib import Path
 
 _runtime = None
@@ -160,7 +161,7 @@ class Runtime:
         self.debug_sync = os.environ.get("QUTAI_AMD_SYNC") == "1"
         self._closed = False
         # pinned staging ring for asynchronous host-to-device uploads
-        self._staging, self._staging_at, self._staging_pending = None, 0, []
+        self._staging, self._staging_at, self._staging_pending = None, 0, deque()
         self.hip = _hip_library()
         self._bind_hip()
         self.lib = load_library()
@@ -334,22 +335,21 @@ class Runtime:
                 self._staging = value.value
             start = self._staging_at if self._staging_at + nbytes <= self.STAGING_BYTES else 0
             end = start + nbytes
-            # wait for the copies that still read the region about to be overwritten
-            keep = []
-            for lo, hi, event in self._staging_pending:
-                if lo < end and start < hi:
-                    self._check(self._event_sync(event), "hipEventSynchronize")
-                    self._event_destroy(event)
-                else:
-                    keep.append((lo, hi, event))
+            # wait for the copies that still read the region about to be overwritten: regions follow each
+            # other around the ring, so these are the oldest (and where this one starts over, what an earlier
+            # turn left behind the last one)
+            pending = self._staging_pending
+            while pending and (start < pending[0][1] and pending[0][0] < end
+                               or start < self._staging_at <= pending[0][0]):
+                self._check(self._event_sync(pending[0][2]), "hipEventSynchronize")
+                self._event_destroy(pending.popleft()[2])
             ctypes.memmove(self._staging + start, host, nbytes)
             self._check(self._memcpy_async(ptr, self._staging + start, nbytes, _MEMCPY_H2D, None),
                         "hipMemcpyAsync HtoD")
             event = ctypes.c_void_p()
             self._check(self._event_create_flags(ctypes.byref(event), 2), "hipEventCreateWithFlags")  # no timing
             self._check(self._event_record(event, None), "hipEventRecord")
-            keep.append((start, end, event.value))
-            self._staging_pending = keep
+            pending.append((start, end, event.value))
             self._staging_at = (end + 255) // 256 * 256
 
     def download(self, ptr: int, buffer):
@@ -436,7 +436,7 @@ class Runtime:
             self._sync()
             for _, _, event in self._staging_pending:
                 self._event_destroy(event)
-            self._staging_pending = []
+            self._staging_pending.clear()
             if self._staging is not None:
                 self._host_free(self._staging)
                 self._staging = None
