@@ -416,7 +416,7 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * one wider matrix; q_out and k_out are contiguous.  Either side may be absent
  * (0 heads, NULL pointers).  dtype QA_F32 or QA_BF16 for rows and outputs; the
  * norm, the angles' sine and cosine and the products are fp32, the angles'
- * reduction fp64.  Outputs share no memory with inputs.  The unfused form is
+ * reduction fp64.  batch x time is below 2^31.  Outputs share no memory with inputs.  The unfused form is
  * qutai_amd_rms_norm per head and qutai_amd_rope_rows. */
 int qutai_amd_qk_norm_rope(const void* q, const void* k, const float* q_weight, const float* k_weight, void* q_out,
                            void* k_out, const int64_t* starts, int64_t offset, int64_t batch, int64_t time,
