@@ -8,11 +8,20 @@
 // The given number u picks the first token, in the order of indices, at which the
 // running sum of the kept weights exceeds u times their sum.
 //
-// What is kept is a threshold on a logit's key (its bits, in an order of unsigned
-// integers) and, among the tokens that lie on it, a number of them from the
-// lowest index on: nothing is sorted.  The threshold is found digit by digit, from
-// histograms of counts (top_k) or of weights (top_p).  Weights in a histogram are
-// 64-bit integers, w_i 2^(62 - log2 vocab): their sums are exact, in any order.
+// What is kept is a threshold on the logit and, among the tokens that lie on it, a
+// number of them from the lowest index on: nothing is sorted.  A workgroup of 1024
+// threads owns a row and keeps its first 16 steps (of 16 bytes per thread: 131072
+// bf16 or 65536 fp32 logits) in registers; what lies behind is read again by every
+// pass.  A NaN, which no comparison lets through, stands behind the last token.
+//  top_k: the k-th largest of the threads' maxima bounds the k-th largest logit
+//  from below; the few logits from there on go into a list in LDS, where the
+//  threshold is found.
+//  top_p: weights in bins of 1/32 of a power of two, whose sums are 64-bit integers
+//  (weight times 2^45, or less for very large vocabularies): exact in any order.
+//  The logits of the bin that the prefix ends in go into the list.
+// A list is searched digit by digit of its keys (bits in an order of unsigned
+// integers), from histograms.  Where it overflows (thousands of equal or nearly
+// equal logits, or a large k) the whole row is.
 #include "common.h"
 #include "qutai_amd.h"
 
@@ -24,7 +33,7 @@ namespace {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int64_t VOCAB_LIMIT = 1 << 20;
-constexpr int BINS = 2048;
+constexpr int BINS = 2048, LIST = 4096, HELD = 8;  // HELD: steps of a register vector
 
 struct SampleArgs {
   const void* logits;
@@ -37,81 +46,66 @@ struct SampleArgs {
   const float* min_ps;
   double temperature, top_p, min_p;
   int64_t top_k;
-  int vocab, wide_uniforms, vector, fraction;  // fraction: bits of a weight in a histogram
+  int vocab, wide_uniforms, vector, fraction;  // fraction: bits of a weight in a bin
 };
 
-// Keys: larger for larger logits, equal for equal ones (both zeros, every NaN
-// with -inf); 0 is below all of them.
-template <class T> struct Key;
-template <> struct Key<float> {
-  static constexpr int E = 4, BITS = 32;
-  static __device__ __forceinline__ uint32_t of(uint32_t bits) {
-    float v = __uint_as_float(bits);
-    v = v == v ? v + 0.f : -INFINITY;
-    const uint32_t u = __float_as_uint(v);
-    return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
-  }
-  static __device__ __forceinline__ float value(uint32_t key) {
-    return __uint_as_float(key ^ ((int32_t)key < 0 ? 0x80000000u : 0xffffffffu));
-  }
-};
-template <> struct Key<bf16_t> {
-  static constexpr int E = 8, BITS = 16;
-  static __device__ __forceinline__ uint32_t of(uint32_t bits) { return Key<float>::of(bits << 16) >> 16; }
-  static __device__ __forceinline__ float value(uint32_t key) {
-    return __uint_as_float(((key ^ (key & 0x8000u ? 0x8000u : 0xffffu)) & 0xffffu) << 16);
-  }
-};
+typedef uint32_t u32x32 __attribute__((ext_vector_type(4 * HELD)));
 
-template <class T>
-struct Row {
-  static constexpr int E = Key<T>::E;
-  const T* p;
-  int vocab, vector;
-  __device__ __forceinline__ int steps() const { return (vocab + THREADS * E - 1) / (THREADS * E); }
-  // the keys of tokens (step THREADS + thread) E .. + E; 0 behind the last
-  __device__ __forceinline__ void keys(int step, uint32_t (&k)[E]) const {
-    const int first = (step * THREADS + (int)threadIdx.x) * E;
-    if (vector && first + E <= vocab) {
-      const u32x4 w = global_load<u32x4>(p + first);
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        if constexpr (E == 4) k[e] = Key<T>::of(w[e]);
-        else k[e] = Key<T>::of((w[e >> 1] >> (16 * (e & 1))) & 0xffffu);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        k[e] = 0;
-        if (first + e < vocab) {
-          if constexpr (E == 4) k[e] = Key<T>::of(__float_as_uint(p[first + e]));
-          else k[e] = Key<T>::of(p[first + e]);
-        }
-      }
-    }
-  }
-};
+// Larger for larger logits, equal for equal ones (both zeros); above 0 for all but NaN.
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t u = __float_as_uint(v + 0.f);
+  return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t key) {
+  return __uint_as_float(key ^ ((int32_t)key < 0 ? 0x80000000u : 0xffffffffu));
+}
 
 struct Shared {
   union {
-    uint32_t counts[BINS];
-    unsigned long long masses[BINS];
+    struct {
+      union {
+        uint32_t counts[BINS];
+        unsigned long long masses[BINS];
+      };
+      float list[LIST];
+    };
     double sums[VOCAB_LIMIT / (THREADS * 4) * WAVES];  // kept weights of each step and wave
   };
   uint32_t ties[VOCAB_LIMIT / (THREADS * 4) * WAVES];
+  double powers[32];  // 2^(-j / 32)
   unsigned long long part[WAVES];
-  double wide[WAVES];
+  double wide[2];
   unsigned long long found[3];
+  uint32_t bound[2], listed;
   int chosen;
 };
 
-template <class T>
-__device__ __forceinline__ double weight(uint32_t key, float top, double scale) {
-  const float l = Key<T>::value(key);
-  if (l == top) return 1.0;
-  const double behind = (double)top - (double)l;
-  return behind < INFINITY ? exp(-behind * scale) : 0.0;
-}
+// w = 2^(-t / 32), t = (top - l) 32 log2(e) / T: a table of 32 powers and a polynomial of degree five for
+// the rest, |x| <= ln 2 / 64 (the next term is 2e-15), with t's nearest integer n.
+struct Weigh {
+  const double* powers;
+  float top;
+  double wide_top, scale;
+  __device__ __forceinline__ double behind(float l) const {  // 65536, which weighs nothing, for NaN and infinities
+    return fmin(l == top ? 0.0 : (wide_top - (double)l) * scale, 65536.0);
+  }
+  __device__ __forceinline__ int bin(float l) const { return __double2loint(behind(l) + 6755399441055744.0); }
+  __device__ __forceinline__ double operator()(float l, int& n) const {
+    const double t = behind(l), whole = t + 6755399441055744.0;  // 1.5 2^52
+    n = __double2loint(whole);
+    const double x = (t - (whole - 6755399441055744.0)) * -0.021660849392498290;  // ln 2 / 32
+    double y = fma(x, 1.0 / 120, 1.0 / 24);
+    y = fma(x, y, 1.0 / 6);
+    y = fma(x, y, 0.5);
+    y = fma(x, y, 1.0);
+    y = fma(x, y, 1.0);
+    return ldexp(powers[n & 31] * y, -(n >> 5));
+  }
+  __device__ __forceinline__ double operator()(float l) const {
+    int n;
+    return (*this)(l, n);
+  }
+};
 
 // The bin, from the top, at which a running sum of bins reaches `target` (> 0, at
 // most their sum); found: bin, sum of the bins above it, its own value.  Threads
@@ -135,144 +129,311 @@ __device__ __forceinline__ void find_bin(Shared& s, const V* bins, unsigned long
   __syncthreads();
 }
 
+template <class V>
+__device__ __forceinline__ unsigned long long sum_bins(Shared& s, const V* bins) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned long long total = (unsigned long long)bins[2 * threadIdx.x] + bins[2 * threadIdx.x + 1];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
+  if (lane == 0) s.part[wave] = total;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) total += s.part[w];
+  __syncthreads();
+  return total;
+}
+
+// The key at which a running sum over the visited keys, from the largest on, reaches
+// `target` (0: goal(their sum)), digit by digit: visit(f) calls f(key, amount) for
+// every key of this thread.  Returns the key; above: the sum of the larger keys;
+// own: that of its equals.
+template <class V, class Visit, class Goal>
+__device__ __forceinline__ uint32_t find_key(Shared& s, V* bins, unsigned long long& target, Visit visit, Goal goal,
+                                             unsigned long long& above, unsigned long long& own) {
+  uint32_t prefix = 0;
+  above = 0;
+#pragma nounroll
+  for (int low = 21, width = 11, done = 0;;) {  // digits of 11, 11 and 10 bits
+    for (int i = threadIdx.x; i < BINS; i += THREADS) bins[i] = 0;
+    __syncthreads();
+    visit([&](uint32_t key, V amount) {
+      if (done == 0 || key >> (32 - done) == prefix) atomicAdd(&bins[(key >> low) & ((1u << width) - 1)], amount);
+    });
+    __syncthreads();
+    if (target == 0) target = goal(sum_bins(s, bins));
+    find_bin(s, bins, target - above);
+    prefix = prefix << width | (uint32_t)s.found[0];
+    above += s.found[1];
+    own = s.found[2];
+    done += width;
+    __syncthreads();
+    if (low == 0) return prefix;
+    width = low > 10 ? 11 : low;
+    low -= width;
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
-  constexpr int E = Key<T>::E, KEY = Key<T>::BITS;
+  constexpr int E = 16 / (int)sizeof(T);
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x;
-  const Row<T> row = {(const T*)a.logits + r * a.vocab, a.vocab, a.vector};
-  const int steps = row.steps();
+  const T* row = (const T*)a.logits + r * a.vocab;
+  const int steps = (a.vocab + THREADS * E - 1) / (THREADS * E);
   const double temperature = a.temperatures ? (double)a.temperatures[r] : a.temperature;
   const int64_t top_k = a.top_ks ? a.top_ks[r] : a.top_k;
   const double top_p = a.top_ps ? (double)a.top_ps[r] : a.top_p;
   const double asked = a.min_ps ? (double)a.min_ps[r] : a.min_p, min_p = asked <= 1.0 ? asked : 1.0;
+  if (tid < 32) s.powers[tid] = exp2(tid * -0.03125);
+  if (tid == 0) s.listed = 0;
 
-  // ---- the largest key and its lowest index
-  uint32_t k[E], best = 0;
-  int at = 0;
-  for (int step = 0; step < steps; step++) {
-    row.keys(step, k);
+  // the logits of tokens (step THREADS + thread) E .. + E as they lie in memory, NaN behind the last
+  auto load = [&](int step, uint32_t (&w)[4]) {
+    const int first = (step * THREADS + tid) * E;
+    if (a.vector && first + E <= a.vocab) {
+      const u32x4 v = global_load<u32x4>(row + first);
 #pragma unroll
-    for (int e = 0; e < E; e++)
-      if (k[e] > best) best = k[e], at = (step * THREADS + tid) * E + e;
-  }
-  unsigned long long both = (unsigned long long)best << 32 | (0xffffffffu - (uint32_t)at);
+      for (int i = 0; i < 4; i++) w[i] = v[i];
+    } else {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    const unsigned long long other = __shfl_xor(both, o);
-    both = other > both ? other : both;
-  }
-  if (lane == 0) s.part[wave] = both;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WAVES; w++) both = s.part[w] > both ? s.part[w] : both;
-  __syncthreads();
-  const uint32_t top_key = (uint32_t)(both >> 32);
-  const int top_at = (int)(0xffffffffu - (uint32_t)both);
-  const float top = Key<T>::value(top_key);
-  const bool none = top == -INFINITY;
-  if (none || !(temperature > 0.0)) {
-    if (tid == 0) {
-      a.tokens[r] = none ? -1 : top_at;
-      a.probabilities[r] = none ? 0.f : 1.f;
-    }
-    return;
-  }
-  const double scale = 1.0 / temperature;
-
-  // ---- the threshold: keys above it are kept, and `keep` of the `tied` on it
-  uint32_t threshold = 0;
-  unsigned long long keep = 0, tied = 0;
-  const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0;
-  constexpr int FIRST = KEY == 32 ? 21 : 5;  // digits of 11, 11 and 10 bits, or 11 and 5
-  if (by_count) {
-    unsigned long long wanted = (unsigned long long)top_k;
-    uint32_t prefix = 0;
-    for (int low = FIRST, width = 11, done = 0;;) {
-      for (int i = tid; i < BINS; i += THREADS) s.counts[i] = 0;
-      __syncthreads();
-      for (int step = 0; step < steps; step++) {
-        row.keys(step, k);
-#pragma unroll
-        for (int e = 0; e < E; e++)
-          if (done == 0 || k[e] >> (KEY - done) == prefix) atomicAdd(&s.counts[(k[e] >> low) & ((1u << width) - 1)], 1u);
-      }
-      __syncthreads();
-      find_bin(s, s.counts, wanted);
-      prefix = prefix << width | (uint32_t)s.found[0];
-      wanted -= s.found[1];
-      tied = s.found[2];
-      done += width;
-      __syncthreads();
-      if (low == 0) break;
-      width = low < 11 ? low : low - 10 < 11 ? low - 10 : 11;
-      low -= width;
-    }
-    threshold = prefix, keep = wanted;
-  }
-  const double unit = (double)(1ull << a.fraction);
-  if (by_mass) {
-    unsigned long long target = 0, above = 0, mass = 0;
-    uint32_t prefix = 0;
-    for (int low = FIRST, width = 11, done = 0;;) {
-      for (int i = tid; i < BINS; i += THREADS) s.masses[i] = 0;
-      __syncthreads();
-      for (int step = 0; step < steps; step++) {
-        row.keys(step, k);
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          if (k[e] == 0 || k[e] < threshold || (by_count && k[e] == threshold)) continue;
-          if (done == 0 || k[e] >> (KEY - done) == prefix)
-            atomicAdd(&s.masses[(k[e] >> low) & ((1u << width) - 1)],
-                      (unsigned long long)(weight<T>(k[e], top, scale) * unit + 0.5));
+      for (int i = 0; i < 4; i++) {
+        if constexpr (E == 4) {
+          w[i] = first + i < a.vocab ? __float_as_uint(row[first + i]) : 0x7fc00000u;
+        } else {
+          w[i] = first + 2 * i < a.vocab ? row[first + 2 * i] : 0x7fc0u;
+          w[i] |= (first + 2 * i + 1 < a.vocab ? row[first + 2 * i + 1] : 0x7fc0u) << 16;
         }
       }
-      if (by_count && tid == 0 && (done == 0 || threshold >> (KEY - done) == prefix))
-        atomicAdd(&s.masses[(threshold >> low) & ((1u << width) - 1)],
-                  keep * (unsigned long long)(weight<T>(threshold, top, scale) * unit + 0.5));
-      __syncthreads();
-      if (done == 0) {
-        unsigned long long total = s.masses[2 * tid] + s.masses[2 * tid + 1];
-#pragma unroll
-        for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-        if (lane == 0) s.part[wave] = total;
-        __syncthreads();
-        total = 0;
-        for (int w = 0; w < WAVES; w++) total += s.part[w];
-        __syncthreads();
-        const double wanted = ceil(top_p * (double)total);
-        target = wanted < 1.0 ? 1ull : (unsigned long long)wanted;
-        target = target > total ? total : target;
-      }
-      find_bin(s, s.masses, target - above);
-      prefix = prefix << width | (uint32_t)s.found[0];
-      above += s.found[1];
-      mass = s.found[2];
-      done += width;
-      __syncthreads();
-      if (low == 0) break;
-      width = low < 11 ? low : low - 10 < 11 ? low - 10 : 11;
-      low -= width;
     }
-    // the tokens on the threshold weigh the same
-    const unsigned long long each = (unsigned long long)(weight<T>(prefix, top, scale) * unit + 0.5);
-    tied = by_count && prefix == threshold ? tied : mass / each;
-    keep = (target - above + each - 1) / each;
-    threshold = prefix;
+  };
+  // all loads of the steps held are in flight together
+  u32x32 held0, held1;
+  float largest = -INFINITY;
+  auto unpack = [](const uint32_t (&w)[4], float (&v)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      if constexpr (E == 4) v[e] = __uint_as_float(w[e]);
+      else v[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    }
+  };
+#pragma unroll
+  for (int step = 0; step < 2 * HELD; step++) {
+    uint32_t w[4] = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+    if (step < steps) load(step, w);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (step < HELD) held0[4 * step + i] = w[i];
+      else held1[4 * (step - HELD) + i] = w[i];
+    }
+  }
+  // f(step, logits) for every step; those not held are loaded one step ahead
+  auto each = [&](auto f) {
+    uint32_t next[4] = {0u, 0u, 0u, 0u};
+#pragma nounroll
+    for (int step = 0; step < steps; step++) {
+      uint32_t w[4];
+      if (step < HELD) {
+        const int i = 4 * step;
+        w[0] = held0[i], w[1] = held0[i + 1], w[2] = held0[i + 2], w[3] = held0[i + 3];
+      } else if (step < 2 * HELD) {
+        const int i = 4 * (step - HELD);
+        w[0] = held1[i], w[1] = held1[i + 1], w[2] = held1[i + 2], w[3] = held1[i + 3];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = next[i];
+      }
+      if (step + 1 >= 2 * HELD && step + 1 < steps) load(step + 1, next);
+      float v[E];
+      unpack(w, v);
+      f(step, v);
+    }
+  };
+
+  // ---- the largest logit
+  each([&](int, const float (&v)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e++) largest = fmaxf(largest, v[e]);
+  });
+  float top = largest;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if (lane == 0) s.part[wave] = __float_as_uint(top);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) top = fmaxf(top, __uint_as_float((uint32_t)s.part[w]));
+  __syncthreads();
+  if (top == -INFINITY) {
+    if (tid == 0) a.tokens[r] = -1, a.probabilities[r] = 0.f;
+    return;
+  }
+  if (!(temperature > 0.0)) {  // its lowest index
+    uint32_t at = 0xffffffffu;
+    each([&](int step, const float (&v)[E]) {
+#pragma unroll
+      for (int e = E - 1; e >= 0; e--) {
+        const uint32_t i = (uint32_t)(step * THREADS + tid) * E + e;
+        if (v[e] == top && i < at) at = i;
+      }
+    });
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+      const uint32_t other = __shfl_xor(at, o);
+      at = other < at ? other : at;
+    }
+    if (lane == 0) s.part[wave] = at;
+    __syncthreads();
+    for (int w = 0; w < WAVES; w++) at = (uint32_t)s.part[w] < at ? (uint32_t)s.part[w] : at;
+    if (tid == 0) a.tokens[r] = at, a.probabilities[r] = 1.f;
+    return;
+  }
+  const Weigh weigh = {s.powers, top, (double)top, 46.166241308446829 / temperature};  // 32 log2(e)
+  const double unit = (double)(1ull << a.fraction);
+  auto units = [&](double w) -> unsigned long long {  // w unit, rounded: at most 2^45
+    return (unsigned long long)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffull;
+  };
+
+  // ---- the threshold: logits above it are kept, and `keep` of the `tied` on it
+  float threshold = -INFINITY;
+  unsigned long long keep = 0, tied = 0;
+  const bool by_count = top_k > 0 && top_k < a.vocab, by_mass = top_p < 1.0;
+  // the logits that the search is left with: from `low` on, below `high` (or all)
+  float low = -INFINITY, high = 0.f;
+  bool open = true, listed = false;
+  unsigned long long target = 0, over = 0;  // of weights: what the prefix has to hold, and what lies above `high`
+  auto target_of = [&](unsigned long long total) -> unsigned long long {
+    const double wanted = ceil(top_p * (double)total);
+    const unsigned long long least = wanted < 1.0 ? 1ull : (unsigned long long)wanted;
+    return least < total ? least : total;
+  };
+  if (by_count) {
+    // a bound that top_k logits reach: one that as many threads' maxima do
+    if (a.vocab > LIST && top_k <= THREADS / 2) {
+      s.list[tid] = largest;
+      __syncthreads();
+      if (wave == 0) {
+        uint32_t k[WAVES], least = 0, most = key_of(top) + 1;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) k[i] = key_of(s.list[64 * i + lane]);
+        while (most - least > 1) {  // least: reached by top_k maxima or more; most: by fewer
+          const uint32_t mid = least + (most - least) / 2;
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < WAVES; i++) n += __popcll(__ballot(k[i] >= mid));
+          if (n >= top_k) least = mid;
+          else most = mid;
+          if (n >= top_k && n <= top_k + top_k / 4 + 8) break;
+        }
+        if (lane == 0) s.bound[0] = least;
+      }
+      __syncthreads();
+      low = s.bound[0] <= key_of(-INFINITY) ? -INFINITY : value_of(s.bound[0]);
+    }
+  } else if (by_mass) {
+    for (int i = tid; i < BINS; i += THREADS) s.masses[i] = 0;
+    __syncthreads();
+    each([&](int, const float (&v)[E]) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        int n;
+        const unsigned long long amount = units(weigh(v[e], n));
+        if (amount) atomicAdd(&s.masses[BINS - 1 - n], amount);  // an amount of 1 lies 46 powers of two below
+      }
+    });
+    __syncthreads();
+    target = target_of(sum_bins(s, s.masses));
+    find_bin(s, s.masses, target);
+    const int bin = BINS - 1 - (int)s.found[0];
+    over = s.found[1];
+    // the smallest keys of this bin and of the one above it: 64 candidates at a time, of which the largest
+    // that lies in a lower bin is searched on
+    if (wave < 2) {
+      uint32_t base = 0;
+      const int wanted = bin - wave;
+#pragma nounroll
+      for (int shift = 26; shift >= 0; shift = shift == 2 ? 0 : shift - 6) {
+        const uint32_t candidate = base + ((uint32_t)lane << shift);
+        bool below = candidate == 0;
+        if (candidate && candidate < key_of(top)) {
+          const float l = value_of(candidate);
+          below = !(l >= -INFINITY) || weigh.bin(l) > wanted;
+        }
+        const unsigned long long lanes = __ballot(below && (shift || lane < 4));
+        base += (uint32_t)(63 - __clzll(lanes)) << shift;
+      }
+      if (lane == 0) s.bound[wave] = base + 1;
+    }
+    __syncthreads();
+    low = value_of(s.bound[0]), high = value_of(s.bound[1]), open = bin == 0;
+  }
+  // these logits into the list, if they fit
+  if (by_count ? a.vocab <= LIST || top_k <= THREADS / 2 : by_mass) {
+    each([&](int, const float (&v)[E]) {
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        const bool in = v[e] >= low && (open || v[e] < high);
+        const unsigned long long lanes = __ballot(in);
+        if (!lanes) continue;
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&s.listed, (uint32_t)__popcll(lanes));
+        at = __shfl(at, 0) + (uint32_t)__popcll(lanes & ((1ull << lane) - 1));
+        if (in && at < LIST) s.list[at] = v[e];
+      }
+    });
+    __syncthreads();
+    listed = s.listed <= LIST;
+  }
+  // f(logit) for this thread's logits of the search
+  auto visit = [&](auto f) {
+    if (listed) {
+      const int n = (int)s.listed;
+      for (int i = tid; i < n; i += THREADS) f(s.list[i]);
+    } else {
+      each([&](int, const float (&v)[E]) {
+#pragma unroll
+        for (int e = 0; e < E; e++)
+          if (v[e] >= low && (open || v[e] < high)) f(v[e]);
+      });
+    }
+  };
+  if (by_count) {
+    unsigned long long above, wanted = 0;
+    auto goal = [&](unsigned long long n) { return (unsigned long long)top_k < n ? (unsigned long long)top_k : n; };
+    const uint32_t key = find_key(s, s.counts, wanted, [&](auto f) { visit([&](float l) { f(key_of(l), 1u); }); }, goal,
+                                  above, tied);
+    threshold = value_of(key);
+    keep = (unsigned long long)top_k - above;
+    if (keep > tied) keep = tied;  // fewer numbers than top_k
+    low = value_of(key + 1);       // for what lies above
+  }
+  if (by_mass) {
+    unsigned long long above, own;
+    target -= over;
+    const uint32_t key = find_key(s, s.masses, target, [&](auto f) {
+      visit([&](float l) {
+        if (l >= low) f(key_of(l), units(weigh(l)));
+      });
+      // and what top_k keeps of its own threshold
+      if (by_count && tid == 0) f(key_of(threshold), keep * units(weigh(threshold)));
+    }, target_of, above, own);
+    const float l = value_of(key);
+    const unsigned long long each_one = units(weigh(l));  // the tokens on a threshold weigh the same
+    if (!by_count || l > threshold) tied = own / each_one;
+    keep = (target - above + each_one - 1) / each_one;
+    threshold = l;
   }
 
   // ---- where tokens on the threshold are left out: how many lie before each step's wave
-  const bool cut = (by_count || by_mass) && keep < tied;
+  const bool filtered = by_count || by_mass, cut = filtered && keep < tied;
   const int slots = steps * WAVES;
   if (cut) {
-    for (int step = 0; step < steps; step++) {
-      row.keys(step, k);
+    each([&](int step, const float (&v)[E]) {
       int n = 0;
 #pragma unroll
-      for (int e = 0; e < E; e++) n += __popcll(__ballot(k[e] == threshold));
+      for (int e = 0; e < E; e++) n += __popcll(__ballot(v[e] == threshold));
       if (lane == 0) s.ties[step * WAVES + wave] = n;
-    }
+    });
     __syncthreads();
     if (wave == 0) {
       uint32_t before = 0;
@@ -288,43 +449,38 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
         before += __shfl(run, 63);
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
 
-  // the kept weights of this thread's tokens of a step
-  auto kept = [&](int step, double (&w)[E]) {
-    row.keys(step, k);
+  // add(e, weight) for this thread's tokens of a step, 0 where they are not kept
+  auto kept = [&](int step, const float (&v)[E], auto add) {
     unsigned long long rank = 0;
     if (cut) {
       rank = s.ties[step * WAVES + wave];
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        const unsigned long long on = __ballot(k[e] == threshold);
-        rank += __popcll(on & ((1ull << lane) - 1));
-      }
+      for (int e = 0; e < E; e++) rank += __popcll(__ballot(v[e] == threshold) & ((1ull << lane) - 1));
     }
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      bool in = k[e] != 0 && k[e] >= threshold;
-      if (cut && k[e] == threshold) in = rank++ < keep;
-      w[e] = 0.0;
-      if (in) {
-        w[e] = weight<T>(k[e], top, scale);
-        if (w[e] < min_p) w[e] = 0.0;
+      bool in = v[e] >= threshold;
+      if (cut && v[e] == threshold) in = rank++ < keep;
+      double x = 0.0;
+      if (!filtered || __any(in)) {
+        x = weigh(v[e]);
+        x = in && !(x < min_p) ? x : 0.0;
       }
+      add(e, x);
     }
   };
 
   // ---- their sums, step by step and wave by wave (the order of indices)
-  for (int step = 0; step < steps; step++) {
-    double w[E], sum = 0.0;
-    kept(step, w);
-#pragma unroll
-    for (int e = 0; e < E; e++) sum += w[e];
+  each([&](int step, const float (&v)[E]) {
+    double sum = 0.0;
+    kept(step, v, [&](int, double x) { sum += x; });
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     if (lane == 0) s.sums[step * WAVES + wave] = sum;
-  }
+  });
   __syncthreads();
   if (wave == 0) {
     double before = 0.0;
@@ -368,7 +524,13 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   if (wave != chosen % WAVES) return;
   const double goal = s.wide[0], all = s.wide[1];
   double w[E], sum = 0.0;
-  kept(chosen / WAVES, w);
+  {
+    uint32_t words[4];
+    load(chosen / WAVES, words);
+    float v[E];
+    unpack(words, v);
+    kept(chosen / WAVES, v, [&](int e, double x) { w[e] = x; });
+  }
 #pragma unroll
   for (int e = 0; e < E; e++) sum += w[e];
   double run = sum;
@@ -378,18 +540,18 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
     if (lane >= o) run += other;
   }
   const double base = chosen ? s.sums[chosen - 1] : 0.0;
-  const unsigned long long over = __ballot(sum > 0.0 && base + run > goal), any = __ballot(sum > 0.0);
-  const int owner = over ? __ffsll(over) - 1 : 63 - __clzll(any);
+  const unsigned long long past = __ballot(sum > 0.0 && base + run > goal), any = __ballot(sum > 0.0);
+  const int owner = past ? __ffsll(past) - 1 : 63 - __clzll(any);
   if (lane != owner) return;
-  double walk = base + run - sum, weigh = 0.0;
+  double walk = base + run - sum, share = 0.0;
   int token = -1;
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    if (w[e] > 0.0 && !(token >= 0 && walk > goal)) token = (chosen / WAVES * THREADS + tid) * E + e, weigh = w[e];
+    if (w[e] > 0.0 && !(token >= 0 && walk > goal)) token = (chosen / WAVES * THREADS + tid) * E + e, share = w[e];
     walk += w[e];
   }
   a.tokens[r] = token;
-  a.probabilities[r] = (float)(weigh / all);
+  a.probabilities[r] = (float)(share / all);
 }
 
 }  // namespace
@@ -409,7 +571,7 @@ extern "C" int qutai_amd_sample(const void* logits, const void* uniforms, int64_
   const int es = dtype == BF16 ? 2 : 4;
   const SampleArgs a = {logits, uniforms, tokens, probabilities, temperatures, top_ks, top_ps, min_ps, temperature,
                         top_p, min_p, top_k, (int)vocab, uniform_dtype == F64, (uintptr_t)logits % 16 == 0 && vocab * es % 16 == 0,
-                        62 - log2};
+                        62 - log2 < 45 ? 62 - log2 : 45};
   hipStream_t stream = (hipStream_t)stream_;
   if (dtype == BF16) hipLaunchKernelGGL(sample_rows<bf16_t>, dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
   else hipLaunchKernelGGL(sample_rows<float>, dim3((unsigned)rows), dim3(THREADS), 0, stream, a);
