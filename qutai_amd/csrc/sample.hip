@@ -9,11 +9,11 @@
 // running sum of the kept weights exceeds u times their sum.
 //
 // What is kept is a threshold on the logit and, among the tokens that lie on it, a
-// number of them from the lowest index on: nothing is sorted.  A workgroup of 1024
-// threads owns a row and keeps its first 16 steps (of 16 bytes per thread: 131072
+// number of them from the lowest index on: nothing is sorted.  A workgroup of 512
+// threads owns a row and keeps its first 32 steps (of 16 bytes per thread: 131072
 // bf16 or 65536 fp32 logits) in registers; what lies behind is read again by every
 // pass.  A NaN, which no comparison lets through, stands behind the last token.
-//  top_k: the k-th largest of the threads' maxima bounds the k-th largest logit
+//  top_k: the k-th largest of the threads' maxima (two each) bounds the k-th largest logit
 //  from below; the few logits from there on go into a list in LDS, where the
 //  threshold is found.
 //  top_p: weights in bins of 1/32 of a power of two, whose sums are 64-bit integers
@@ -31,9 +31,10 @@ using namespace qa;
 
 namespace {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr int THREADS = 512, WAVES = THREADS / 64;
 constexpr int64_t VOCAB_LIMIT = 1 << 20;
-constexpr int BINS = 2048, LIST = 4096, HELD = 8;  // HELD: steps of a register vector
+constexpr int BINS = 2048, LIST = 4096, FEW = 192;
+constexpr int SPAN = 8, HELD = 4 * SPAN;  // steps of a register vector, and of all of them
 
 struct SampleArgs {
   const void* logits;
@@ -49,7 +50,7 @@ struct SampleArgs {
   int vocab, wide_uniforms, vector, fraction;  // fraction: bits of a weight in a bin
 };
 
-typedef uint32_t u32x32 __attribute__((ext_vector_type(4 * HELD)));
+typedef uint32_t u32x32 __attribute__((ext_vector_type(4 * SPAN)));
 
 // Larger for larger logits, equal for equal ones (both zeros); above 0 for all but NaN.
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -75,31 +76,31 @@ struct Shared {
   double powers[32];  // 2^(-j / 32)
   unsigned long long part[WAVES];
   double wide[2];
-  unsigned long long found[3];
-  uint32_t bound[2], listed;
+  unsigned long long found[4];
+  float bound[4];
+  uint32_t listed;
   int chosen;
 };
 
-// w = 2^(-t / 32), t = (top - l) 32 log2(e) / T: a table of 32 powers and a polynomial of degree five for
-// the rest, |x| <= ln 2 / 64 (the next term is 2e-15), with t's nearest integer n.
+// w = 2^(-t / 32), t = (top - l) 32 log2(e) / T: a table of 32 powers for the nearest
+// integer n of t, and for the rest, at most half, a polynomial of degree four (the
+// exponential's series up to the fifth power, that power economised: within 9e-14).
+// Means nothing where t lies above 32000, or l is not finite: see `least_of`.
+constexpr double ROUND = 6755399441055744.0;  // 1.5 2^52: adding it leaves an integer in the low bits
+
 struct Weigh {
   const double* powers;
-  float top;
-  double wide_top, scale;
-  __device__ __forceinline__ double behind(float l) const {  // 65536, which weighs nothing, for NaN and infinities
-    return fmin(l == top ? 0.0 : (wide_top - (double)l) * scale, 65536.0);
-  }
-  __device__ __forceinline__ int bin(float l) const { return __double2loint(behind(l) + 6755399441055744.0); }
+  double top, scale;
+  __device__ __forceinline__ double behind(float l) const { return (top - (double)l) * scale; }
   __device__ __forceinline__ double operator()(float l, int& n) const {
-    const double t = behind(l), whole = t + 6755399441055744.0;  // 1.5 2^52
+    const double t = behind(l), whole = t + ROUND, x = t - (whole - ROUND);
     n = __double2loint(whole);
-    const double x = (t - (whole - 6755399441055744.0)) * -0.021660849392498290;  // ln 2 / 32
-    double y = fma(x, 1.0 / 120, 1.0 / 24);
-    y = fma(x, y, 1.0 / 6);
-    y = fma(x, y, 0.5);
+    double y = fma(x, 9.172562701824643e-09, -1.6938633902808837e-06);
+    y = fma(x, y, 0.0002345961982022468);
+    y = fma(x, y, -0.021660849391722175);
     y = fma(x, y, 1.0);
-    y = fma(x, y, 1.0);
-    return ldexp(powers[n & 31] * y, -(n >> 5));
+    y *= powers[n & 31];
+    return __hiloint2double(__double2hiint(y) - ((n & ~31) << 15), __double2loint(y));  // times 2^-(n / 32)
   }
   __device__ __forceinline__ double operator()(float l) const {
     int n;
@@ -107,14 +108,38 @@ struct Weigh {
   }
 };
 
+// The smallest logit (by a wave, all lanes) that `enough` accepts, which accepts
+// every larger one up to top; 64 candidates at a time, of which the largest that
+// is not enough is searched on.
+template <class F>
+__device__ __forceinline__ float least_of(float top, F enough) {
+  const int lane = threadIdx.x & 63;
+  uint32_t base = 0;
+#pragma nounroll
+  for (int shift = 26; shift >= 0; shift = shift == 2 ? 0 : shift - 6) {
+    const uint32_t candidate = base + ((uint32_t)lane << shift);
+    bool below = candidate == 0;
+    if (candidate && candidate < key_of(top)) {
+      const float l = value_of(candidate);
+      below = !(l > -INFINITY) || !enough(l);
+    }
+    const unsigned long long lanes = __ballot(below && (shift || lane < 4));
+    base += (uint32_t)(63 - __clzll(lanes)) << shift;
+  }
+  return value_of(base + 1);
+}
+
 // The bin, from the top, at which a running sum of bins reaches `target` (> 0, at
 // most their sum); found: bin, sum of the bins above it, its own value.  Threads
 // take neighbouring bins, the highest first.
 template <class V>
 __device__ __forceinline__ void find_bin(Shared& s, const V* bins, unsigned long long target) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, high = BINS - 1 - 2 * (int)threadIdx.x;
-  const unsigned long long a = bins[high], b = bins[high - 1];
-  unsigned long long run = a + b;
+  constexpr int PER = BINS / THREADS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, high = BINS - 1 - PER * (int)threadIdx.x;
+  unsigned long long own[PER], run = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) run += own[i] = bins[high - i];
+  const unsigned long long mine = run;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const unsigned long long other = __shfl_up(run, o);
@@ -122,17 +147,32 @@ __device__ __forceinline__ void find_bin(Shared& s, const V* bins, unsigned long
   }
   if (lane == 63) s.part[wave] = run;
   __syncthreads();
-  for (int w = 0; w < wave; w++) run += s.part[w];
-  const unsigned long long above = run - a - b;
-  if (above < target && above + a >= target) s.found[0] = high, s.found[1] = above, s.found[2] = a;
-  else if (above + a < target && run >= target) s.found[0] = high - 1, s.found[1] = above + a, s.found[2] = b;
+  unsigned long long before[WAVES];  // read together
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) before[w] = s.part[w];
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) run += w < wave ? before[w] : 0;
+  if (run - mine < target && run >= target) {
+    unsigned long long above = run - mine;
+    int i = 0;
+#pragma unroll
+    for (int n = 0; n < PER - 1; n++)
+      if (i == n && above + own[n] < target) above += own[n], i = n + 1;
+    s.found[0] = high - i, s.found[1] = above;
+    unsigned long long value = own[0];
+#pragma unroll
+    for (int n = 1; n < PER; n++) value = i == n ? own[n] : value;
+    s.found[2] = value;
+  }
   __syncthreads();
 }
 
 template <class V>
 __device__ __forceinline__ unsigned long long sum_bins(Shared& s, const V* bins) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned long long total = (unsigned long long)bins[2 * threadIdx.x] + bins[2 * threadIdx.x + 1];
+  unsigned long long total = 0;
+#pragma unroll
+  for (int i = 0; i < BINS / THREADS; i++) total += bins[threadIdx.x + i * THREADS];
 #pragma unroll
   for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
   if (lane == 0) s.part[wave] = total;
@@ -209,23 +249,35 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
     }
   };
   // all loads of the steps held are in flight together
-  u32x32 held0, held1;
-  float largest = -INFINITY;
-  auto unpack = [](const uint32_t (&w)[4], float (&v)[E]) {
+  bool infinite = false;  // the row has +inf: those stand at 0, the others at -inf
+  auto unpack = [&](const uint32_t (&w)[4], float (&v)[E]) {
 #pragma unroll
     for (int e = 0; e < E; e++) {
       if constexpr (E == 4) v[e] = __uint_as_float(w[e]);
       else v[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     }
-  };
+    if (infinite) {
 #pragma unroll
-  for (int step = 0; step < 2 * HELD; step++) {
-    uint32_t w[4] = {0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+      for (int e = 0; e < E; e++) v[e] = v[e] == INFINITY ? 0.f : -INFINITY;
+    }
+  };
+  float largest[2] = {-INFINITY, -INFINITY};  // two maxima of each thread
+  u32x32 held0, held1, held2, held3;
+#pragma unroll
+  for (int step = 0; step < HELD; step++) {
+    uint32_t w[4] = {0xffc0ffc0u, 0xffc0ffc0u, 0xffc0ffc0u, 0xffc0ffc0u};  // NaN
     if (step < steps) load(step, w);
+    float v[E];
+    unpack(w, v);
+#pragma unroll
+    for (int e = 0; e < E; e++) largest[e & 1] = fmaxf(largest[e & 1], v[e]);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      if (step < HELD) held0[4 * step + i] = w[i];
-      else held1[4 * (step - HELD) + i] = w[i];
+      const int at = 4 * (step % SPAN) + i;
+      if (step < SPAN) held0[at] = w[i];
+      else if (step < 2 * SPAN) held1[at] = w[i];
+      else if (step < 3 * SPAN) held2[at] = w[i];
+      else held3[at] = w[i];
     }
   }
   // f(step, logits) for every step; those not held are loaded one step ahead
@@ -234,17 +286,13 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
 #pragma nounroll
     for (int step = 0; step < steps; step++) {
       uint32_t w[4];
-      if (step < HELD) {
-        const int i = 4 * step;
-        w[0] = held0[i], w[1] = held0[i + 1], w[2] = held0[i + 2], w[3] = held0[i + 3];
-      } else if (step < 2 * HELD) {
-        const int i = 4 * (step - HELD);
-        w[0] = held1[i], w[1] = held1[i + 1], w[2] = held1[i + 2], w[3] = held1[i + 3];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = next[i];
-      }
-      if (step + 1 >= 2 * HELD && step + 1 < steps) load(step + 1, next);
+      const int i = 4 * (step % SPAN);
+      if (step < SPAN) w[0] = held0[i], w[1] = held0[i + 1], w[2] = held0[i + 2], w[3] = held0[i + 3];
+      else if (step < 2 * SPAN) w[0] = held1[i], w[1] = held1[i + 1], w[2] = held1[i + 2], w[3] = held1[i + 3];
+      else if (step < 3 * SPAN) w[0] = held2[i], w[1] = held2[i + 1], w[2] = held2[i + 2], w[3] = held2[i + 3];
+      else if (step < HELD) w[0] = held3[i], w[1] = held3[i + 1], w[2] = held3[i + 2], w[3] = held3[i + 3];
+      else w[0] = next[0], w[1] = next[1], w[2] = next[2], w[3] = next[3];
+      if (step + 1 >= HELD && step + 1 < steps) load(step + 1, next);
       float v[E];
       unpack(w, v);
       f(step, v);
@@ -252,11 +300,15 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   };
 
   // ---- the largest logit
-  each([&](int, const float (&v)[E]) {
+  for (int step = HELD; step < steps; step++) {
+    uint32_t w[4];
+    float v[E];
+    load(step, w);
+    unpack(w, v);
 #pragma unroll
-    for (int e = 0; e < E; e++) largest = fmaxf(largest, v[e]);
-  });
-  float top = largest;
+    for (int e = 0; e < E; e++) largest[e & 1] = fmaxf(largest[e & 1], v[e]);
+  }
+  float top = fmaxf(largest[0], largest[1]);
 #pragma unroll
   for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   if (lane == 0) s.part[wave] = __float_as_uint(top);
@@ -288,11 +340,27 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
     if (tid == 0) a.tokens[r] = at, a.probabilities[r] = 1.f;
     return;
   }
-  const Weigh weigh = {s.powers, top, (double)top, 46.166241308446829 / temperature};  // 32 log2(e)
+  if (top == INFINITY) {
+    infinite = true;
+    top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) largest[i] = largest[i] == INFINITY ? 0.f : -INFINITY;
+  }
+  const Weigh weigh = {s.powers, (double)top, fmin(46.166241308446829 / temperature, 1e300)};  // 32 log2(e)
   const double unit = (double)(1ull << a.fraction);
   auto units = [&](double w) -> unsigned long long {  // w unit, rounded: at most 2^45
     return (unsigned long long)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffull;
   };
+  // the smallest logits that weigh something (2^-1000 and min_p), and anything in a bin
+  if (wave == 0) {
+    const float least = least_of(top, [&](float l) { return weigh.behind(l) < 32000.0 && !(weigh(l) < min_p); });
+    if (lane == 0) s.bound[0] = least;
+  } else if (wave == 1) {
+    const float least = least_of(top, [&](float l) { return weigh.behind(l) < 32.0 * (a.fraction + 1); });
+    if (lane == 0) s.bound[1] = least;
+  }
+  __syncthreads();
+  const float lightest = s.bound[0], binned = s.bound[1];
 
   // ---- the threshold: logits above it are kept, and `keep` of the `tied` on it
   float threshold = -INFINITY;
@@ -309,70 +377,65 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   };
   if (by_count) {
     // a bound that top_k logits reach: one that as many threads' maxima do
-    if (a.vocab > LIST && top_k <= THREADS / 2) {
-      s.list[tid] = largest;
+    if (a.vocab > LIST && top_k <= THREADS) {
+      s.list[tid] = largest[0];
+      s.list[THREADS + tid] = largest[1];
       __syncthreads();
       if (wave == 0) {
-        uint32_t k[WAVES], least = 0, most = key_of(top) + 1;
+        uint32_t k[2 * WAVES], least = 0, most = key_of(top) + 1;
 #pragma unroll
-        for (int i = 0; i < WAVES; i++) k[i] = key_of(s.list[64 * i + lane]);
+        for (int i = 0; i < 2 * WAVES; i++) k[i] = key_of(s.list[64 * i + lane]);
         while (most - least > 1) {  // least: reached by top_k maxima or more; most: by fewer
           const uint32_t mid = least + (most - least) / 2;
           int n = 0;
 #pragma unroll
-          for (int i = 0; i < WAVES; i++) n += __popcll(__ballot(k[i] >= mid));
+          for (int i = 0; i < 2 * WAVES; i++) n += __popcll(__ballot(k[i] >= mid));
           if (n >= top_k) least = mid;
           else most = mid;
           if (n >= top_k && n <= top_k + top_k / 4 + 8) break;
         }
-        if (lane == 0) s.bound[0] = least;
+        if (lane == 0) s.bound[2] = least <= key_of(-INFINITY) ? -INFINITY : value_of(least);
       }
       __syncthreads();
-      low = s.bound[0] <= key_of(-INFINITY) ? -INFINITY : value_of(s.bound[0]);
+      low = s.bound[2];
     }
   } else if (by_mass) {
     for (int i = tid; i < BINS; i += THREADS) s.masses[i] = 0;
     __syncthreads();
     each([&](int, const float (&v)[E]) {
+      int n[E];
+      unsigned long long amount[E];
 #pragma unroll
-      for (int e = 0; e < E; e++) {
-        int n;
-        const unsigned long long amount = units(weigh(v[e], n));
-        if (amount) atomicAdd(&s.masses[BINS - 1 - n], amount);  // an amount of 1 lies 46 powers of two below
-      }
+      for (int e = 0; e < E; e++) amount[e] = units(weigh(v[e], n[e]));
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (v[e] >= binned) atomicAdd(&s.masses[BINS - 1 - n[e]], amount[e]);
     });
     __syncthreads();
     target = target_of(sum_bins(s, s.masses));
     find_bin(s, s.masses, target);
     const int bin = BINS - 1 - (int)s.found[0];
     over = s.found[1];
-    // the smallest keys of this bin and of the one above it: 64 candidates at a time, of which the largest
-    // that lies in a lower bin is searched on
+    // the smallest logits of this bin and of the one above it
     if (wave < 2) {
-      uint32_t base = 0;
-      const int wanted = bin - wave;
-#pragma nounroll
-      for (int shift = 26; shift >= 0; shift = shift == 2 ? 0 : shift - 6) {
-        const uint32_t candidate = base + ((uint32_t)lane << shift);
-        bool below = candidate == 0;
-        if (candidate && candidate < key_of(top)) {
-          const float l = value_of(candidate);
-          below = !(l >= -INFINITY) || weigh.bin(l) > wanted;
-        }
-        const unsigned long long lanes = __ballot(below && (shift || lane < 4));
-        base += (uint32_t)(63 - __clzll(lanes)) << shift;
-      }
-      if (lane == 0) s.bound[wave] = base + 1;
+      const double edge = bin - wave;
+      const float least = least_of(top, [&](float l) { return weigh.behind(l) + ROUND - ROUND <= edge; });
+      if (lane == 0) s.bound[2 + wave] = least;
     }
     __syncthreads();
-    low = value_of(s.bound[0]), high = value_of(s.bound[1]), open = bin == 0;
+    low = fmaxf(s.bound[2], binned), high = s.bound[3], open = bin == 0;
   }
   // these logits into the list, if they fit
-  if (by_count ? a.vocab <= LIST || top_k <= THREADS / 2 : by_mass) {
+  if (by_count ? a.vocab <= LIST || top_k <= THREADS : by_mass) {
+    const float end = open ? INFINITY : high;  // (no logit here is +inf)
     each([&](int, const float (&v)[E]) {
+      bool some = false;
+#pragma unroll
+      for (int e = 0; e < E; e++) some |= v[e] >= low && v[e] < end;
+      if (!__any(some)) return;
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const bool in = v[e] >= low && (open || v[e] < high);
+        const bool in = v[e] >= low && v[e] < end;
         const unsigned long long lanes = __ballot(in);
         if (!lanes) continue;
         uint32_t at = 0;
@@ -397,35 +460,76 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       });
     }
   };
-  if (by_count) {
-    unsigned long long above, wanted = 0;
-    auto goal = [&](unsigned long long n) { return (unsigned long long)top_k < n ? (unsigned long long)top_k : n; };
-    const uint32_t key = find_key(s, s.counts, wanted, [&](auto f) { visit([&](float l) { f(key_of(l), 1u); }); }, goal,
-                                  above, tied);
-    threshold = value_of(key);
-    keep = (unsigned long long)top_k - above;
-    if (keep > tied) keep = tied;  // fewer numbers than top_k
-    low = value_of(key + 1);       // for what lies above
+  const int few = listed ? (int)s.listed : 0;
+  if (few > 0 && few <= FEW) {
+    // each logit of a short list against all of them
+    const float l = tid < few ? s.list[tid] : -INFINITY;
+    const unsigned long long amount = by_mass && tid < few && l >= binned ? units(weigh(l)) : 0;
+    if (tid < FEW) s.masses[tid] = amount;
+    if (tid < 4 && few + tid < LIST) s.list[few + tid] = NAN;
+    __syncthreads();
+    unsigned long long heavier = 0;
+    int larger = 0, equal = 0;
+    if (wave * 64 < few) {
+      for (int j = 0; j < few; j += 2) {
+        const float m0 = s.list[j], m1 = s.list[j + 1];
+        const unsigned long long w0 = s.masses[j], w1 = s.masses[j + 1];
+        larger += (m0 > l) + (m1 > l);
+        equal += (m0 == l) + (m1 == l);
+        heavier += (m0 > l ? w0 : 0) + (m1 > l ? w1 : 0);
+      }
+    }
+    unsigned long long each_one = amount, goal = target - over;
+    if (by_count) {
+      const int wanted = (int)(top_k < few ? top_k : few);
+      if (tid < few && larger < wanted && larger + equal >= wanted)  // those on the threshold, which agree
+        s.found[0] = __float_as_uint(l), s.found[1] = wanted - larger, s.found[2] = equal, s.found[3] = heavier + amount * (unsigned long long)(wanted - larger);
+      __syncthreads();
+      threshold = __uint_as_float((uint32_t)s.found[0]);
+      keep = s.found[1], tied = s.found[2];
+      if (by_mass) goal = target_of(s.found[3]);
+      __syncthreads();
+    }
+    if (by_mass) {
+      const unsigned long long held = by_count && l == threshold ? keep : (unsigned long long)equal;
+      if (tid < few && l >= threshold && heavier < goal && heavier + held * each_one >= goal)
+        s.found[0] = __float_as_uint(l), s.found[1] = (goal - heavier + each_one - 1) / each_one, s.found[2] = equal;
+      __syncthreads();
+      threshold = __uint_as_float((uint32_t)s.found[0]);
+      keep = s.found[1], tied = s.found[2];
+    }
+  } else if (by_count || by_mass) {
+    if (by_count) {
+      unsigned long long above, wanted = 0;
+      auto goal = [&](unsigned long long n) { return (unsigned long long)top_k < n ? (unsigned long long)top_k : n; };
+      const uint32_t key = find_key(s, s.counts, wanted, [&](auto f) { visit([&](float l) { f(key_of(l), 1u); }); }, goal,
+                                    above, tied);
+      threshold = value_of(key);
+      keep = (unsigned long long)top_k - above;
+      if (keep > tied) keep = tied;  // fewer numbers than top_k
+      low = value_of(key + 1);       // for what lies above
+    }
+    if (by_mass) {
+      unsigned long long above, own;
+      target -= over;
+      const uint32_t key = find_key(s, s.masses, target, [&](auto f) {
+        visit([&](float l) {
+          if (l >= low && l >= binned) f(key_of(l), units(weigh(l)));
+        });
+        // and what top_k keeps of its own threshold
+        if (by_count && tid == 0 && threshold >= binned) f(key_of(threshold), keep * units(weigh(threshold)));
+      }, target_of, above, own);
+      const float l = value_of(key);
+      const unsigned long long each_one = units(weigh(l));  // the tokens on a threshold weigh the same
+      if (!by_count || l > threshold) tied = own / each_one;
+      keep = (target - above + each_one - 1) / each_one;
+      threshold = l;
+    }
   }
-  if (by_mass) {
-    unsigned long long above, own;
-    target -= over;
-    const uint32_t key = find_key(s, s.masses, target, [&](auto f) {
-      visit([&](float l) {
-        if (l >= low) f(key_of(l), units(weigh(l)));
-      });
-      // and what top_k keeps of its own threshold
-      if (by_count && tid == 0) f(key_of(threshold), keep * units(weigh(threshold)));
-    }, target_of, above, own);
-    const float l = value_of(key);
-    const unsigned long long each_one = units(weigh(l));  // the tokens on a threshold weigh the same
-    if (!by_count || l > threshold) tied = own / each_one;
-    keep = (target - above + each_one - 1) / each_one;
-    threshold = l;
-  }
+  if (threshold < lightest) threshold = lightest, keep = tied = 0;
 
   // ---- where tokens on the threshold are left out: how many lie before each step's wave
-  const bool filtered = by_count || by_mass, cut = filtered && keep < tied;
+  const bool cut = keep < tied;
   const int slots = steps * WAVES;
   if (cut) {
     each([&](int step, const float (&v)[E]) {
@@ -452,33 +556,39 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   }
   __syncthreads();
 
-  // add(e, weight) for this thread's tokens of a step, 0 where they are not kept
-  auto kept = [&](int step, const float (&v)[E], auto add) {
-    unsigned long long rank = 0;
+  // the weights of this thread's tokens of a step, 0 where they are not kept; false where the wave keeps none
+  auto kept = [&](int step, const float (&v)[E], double (&w)[E]) -> bool {
+    float most = v[0];
+#pragma unroll
+    for (int e = 1; e < E; e++) most = fmaxf(most, v[e]);
+    if (!__any(most >= threshold)) return false;
+    uint32_t in = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) in |= v[e] >= threshold ? 1u << e : 0u;
     if (cut) {
-      rank = s.ties[step * WAVES + wave];
+      unsigned long long rank = s.ties[step * WAVES + wave];
 #pragma unroll
       for (int e = 0; e < E; e++) rank += __popcll(__ballot(v[e] == threshold) & ((1ull << lane) - 1));
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (v[e] == threshold && rank++ >= keep) in &= ~(1u << e);
     }
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      bool in = v[e] >= threshold;
-      if (cut && v[e] == threshold) in = rank++ < keep;
-      double x = 0.0;
-      if (!filtered || __any(in)) {
-        x = weigh(v[e]);
-        x = in && !(x < min_p) ? x : 0.0;
-      }
-      add(e, x);
-    }
+    for (int e = 0; e < E; e++) w[e] = weigh(v[e]);
+#pragma unroll
+    for (int e = 0; e < E; e++) w[e] = in >> e & 1 ? w[e] : 0.0;
+    return true;
   };
 
   // ---- their sums, step by step and wave by wave (the order of indices)
   each([&](int step, const float (&v)[E]) {
-    double sum = 0.0;
-    kept(step, v, [&](int, double x) { sum += x; });
+    double w[E], sum = 0.0;
+    if (kept(step, v, w)) {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      for (int e = 0; e < E; e++) sum += w[e];
+#pragma unroll
+      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    }
     if (lane == 0) s.sums[step * WAVES + wave] = sum;
   });
   __syncthreads();
@@ -523,13 +633,13 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   const int chosen = s.chosen;
   if (wave != chosen % WAVES) return;
   const double goal = s.wide[0], all = s.wide[1];
-  double w[E], sum = 0.0;
+  double w[E] = {}, sum = 0.0;
   {
     uint32_t words[4];
     load(chosen / WAVES, words);
     float v[E];
     unpack(words, v);
-    kept(chosen / WAVES, v, [&](int e, double x) { w[e] = x; });
+    kept(chosen / WAVES, v, w);
   }
 #pragma unroll
   for (int e = 0; e < E; e++) sum += w[e];
