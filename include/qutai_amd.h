@@ -489,13 +489,14 @@ int qutai_amd_cache_quantize(const void* keys, const void* values, void* key_cod
                              int64_t capacity, int64_t key_row, int64_t value_row, int bits, int dtype, void* stream);
 int64_t qutai_amd_cache_pitch(int64_t dim);
 
-/* The values that one side's codes stand for (keys != 0: the keys'), rounded once
- * to dtype: out is [batch][kv_heads][length][dim], zeros from position shift +
- * lengths[b] on (lengths: int64 per sequence, or NULL for shift alone);
- * length <= capacity. */
-int qutai_amd_cache_dequantize(const void* codes, const void* scales, void* out, const int64_t* lengths,
+/* The values that the codes stand for, rounded once to dtype: keys and values are
+ * [batch][kv_heads][length][dim], zeros from position shift + lengths[b] on
+ * (lengths: int64 per sequence, or NULL for shift alone); length <= capacity,
+ * batch x kv_heads x length at most 2^28. */
+int qutai_amd_cache_dequantize(const void* key_codes, const void* key_scales, const void* value_codes,
+                               const void* value_scales, void* keys, void* values, const int64_t* lengths,
                                int64_t shift, int64_t batch, int64_t kv_heads, int64_t dim, int64_t capacity,
-                               int64_t length, int bits, int keys, int dtype, void* stream);
+                               int64_t length, int bits, int dtype, void* stream);
 
 /* Attention of `fresh` new positions over such a cache: q and out are
  * [batch][fresh][heads][dim] of dtype, heads a multiple of kv_heads (head h reads

@@ -597,15 +597,12 @@ def cache_dequantize(cache, length, *, lengths=None, shift=0, dtype="float32"):
         raise ValueError("a cache is read up to its capacity, as bfloat16 or float32")
     _cache_positions(cache, lengths)
     shift = shift if lengths is not None else length
-    out = []
-    for codes, scales, keys in ((cache.key_codes, cache.key_scales, 1), (cache.value_codes, cache.value_scales, 0)):
-        values = AMDStorage(cache.batch * cache.kv_heads * length * cache.dim, dtype)
-        if values.size:
-            values.runtime.call("qutai_amd_cache_dequantize", codes.ptr, scales.ptr, values.ptr, amd._p(lengths), shift,
-                                cache.batch, cache.kv_heads, cache.dim, cache.capacity, length, cache.bits, keys,
-                                code(dtype))
-        out.append(values)
-    return tuple(out)
+    out = tuple(AMDStorage(cache.batch * cache.kv_heads * length * cache.dim, dtype) for _ in range(2))
+    if length:
+        out[0].runtime.call("qutai_amd_cache_dequantize", cache.key_codes.ptr, cache.key_scales.ptr, cache.value_codes.ptr,
+                            cache.value_scales.ptr, *(x.ptr for x in out), amd._p(lengths), shift, cache.batch,
+                            cache.kv_heads, cache.dim, cache.capacity, length, cache.bits, code(dtype))
+    return out
 
 
 def attention_quantized(cache, q, new, heads, *, start=0, starts=None, counts=None, longest=None, scale=None):

@@ -91,7 +91,7 @@ SIGNATURES = {
     "qutai_amd_cache_quantize": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
                                  _i32, _p],
     "qutai_amd_cache_pitch": [_i64],
-    "qutai_amd_cache_dequantize": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _p],
+    "qutai_amd_cache_dequantize": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _p],
     "qutai_amd_attention_quantized": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                                       _i32, _i32, _f64, _p, _sz, _p],
     "qutai_amd_attention_quantized_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64, _i32],

@@ -37,24 +37,18 @@ __device__ __forceinline__ uint32_t scale_bits(float amax, float most) {
   return s;
 }
 
-// x / s rounded to nearest, ties to even: an estimate, and its exact remainder.
-__device__ __forceinline__ int code_of(float x, float s, float inverse) {
-  float q = rintf(x * inverse);
-  const float rest = fmaf(-q, s, x), twice = 2.f * fabsf(rest);
-  if (twice > s || (twice == s && ((int)q & 1))) q += rest > 0.f ? 1.f : -1.f;
-  return (int)q;
+// x / s rounded to nearest, ties to even, as a float: an estimate, and its exact remainder.
+__device__ __forceinline__ float code_of(float x, float s, float inverse) {
+  const float q = rintf(x * inverse), rest = fmaf(-q, s, x), twice = 2.f * fabsf(rest);
+  const bool off = twice > s || (twice == s && ((int)q & 1));
+  return off ? q + copysignf(1.f, rest) : q;
 }
-
-// byte and shift of a channel's nibble within a 4-bit row
-__device__ __forceinline__ int key_nibble(int d, int pitch, int& shift) {
-  const int c = d >> 5, g = (d >> 3) & 3, j = d & 7, n = (j >> 1) + 4 * (j & 1);
-  shift = 4 * (n & 1);
-  return g * (pitch >> 3) + 4 * c + (n >> 1);
+// The same where x is a bfloat16: x and s have 8 bits each, so a quotient that is
+// no tie lies 2^-9 off it at least, and one step of 2^-11 takes away the estimate's error.
+__device__ __forceinline__ float code_of_bf16(float x, float inverse) {
+  return rintf(fmaf(x, inverse, 6144.f) - 6144.f);
 }
-__device__ __forceinline__ int value_nibble(int d, int pitch, int& shift) {
-  shift = 4 * (d & 1);
-  return ((d & 31) >> 1) * (pitch >> 5) + (d >> 5);
-}
-__device__ __forceinline__ int nibble_value(uint32_t byte, int shift) { return (int)(byte << (28 - shift)) >> 28; }
+// The low byte of an integer's two's complement, |q| below 2^22, in the low byte of a float's bits.
+__device__ __forceinline__ uint32_t low_byte(float q) { return __float_as_uint(q + 12582912.f); }
 
 }  // namespace qa

@@ -165,12 +165,13 @@ def test_cache_entry_points_refuse():
         assert write(**change) == amd_runtime.QA_EINVAL, change
     assert write(batch=0) == 0 and write(new=0) == 0
 
-    def read(shift=0, batch=2, heads=2, dim=8, capacity=10, length=4, bits=8, dtype=5, codes=p):
-        return library.qutai_amd_cache_dequantize(codes, p, p, None, shift, batch, heads, dim, capacity, length, bits, 1,
-                                                  dtype, None)
+    def read(shift=0, batch=2, heads=2, dim=8, capacity=10, length=4, bits=8, dtype=5, codes=p, out=p):
+        return library.qutai_amd_cache_dequantize(codes, p, p, p, out, p, None, shift, batch, heads, dim, capacity, length,
+                                                  bits, dtype, None)
 
     for change in (dict(length=11), dict(length=-1), dict(bits=16), dict(dtype=1), dict(codes=None), dict(codes=p + 4),
-                   dict(dim=300), dict(shift=1 << 50)):
+                   dict(dim=300), dict(shift=1 << 50), dict(out=None),
+                   dict(batch=1 << 12, capacity=1 << 20, length=1 << 18)):
         assert read(**change) == amd_runtime.QA_EINVAL, change
 
     def attend(q=p, start=0, batch=2, new=3, heads=4, kv_heads=2, dim=8, capacity=1024, longest=1000, bits=8, dtype=5,
