@@ -147,28 +147,45 @@ __device__ __forceinline__ int key_channel(int k, int g) {
   else return k < DP / 64 * 2 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : DP / 64 * 64 + 8 * g;
 }
 
-template <int BITS>
+// Nibbles hold code + 8.  RAISED: as they are, in the high fraction bits of bf16
+// numbers of 16 .. 31, code + 24: three operations for two codes, against five;
+// what the 24 adds is taken away by the products (see `attend`).  Otherwise the
+// code itself.
+__device__ __forceinline__ uint32_t raised(uint32_t w, int nibble) {  // nibbles `nibble` and `nibble` + 4
+  return ((nibble ? w >> (4 * nibble - 3) : w << 3) & 0x00780078u) | 0x41804180u;
+}
+constexpr uint32_t RAISE = 0xc1c0c1c0u;  // -24 twice
+
+template <int BITS, bool RAISED>
 __device__ __forceinline__ bf16x8 key_operand(const uint32_t* w, int k) {
   if constexpr (BITS == 8) {
     return bytes_bf16(w[2 * k], w[2 * k + 1]);
   } else {
     u32x4 out;
+    const uint32_t x = w[k] ^ 0x88888888u;
 #pragma unroll
-    for (int e = 0; e < 4; e++)  // nibbles e and e + 4
-      out[e] = pack_bf16x2((float)((int32_t)(w[k] << (28 - 4 * e)) >> 28), (float)((int32_t)(w[k] << (12 - 4 * e)) >> 28));
+    for (int e = 0; e < 4; e++) {  // nibbles e and e + 4
+      if constexpr (RAISED) out[e] = raised(w[k], e);
+      else out[e] = pack_bf16x2((float)((int32_t)(x << (28 - 4 * e)) >> 28), (float)((int32_t)(x << (12 - 4 * e)) >> 28));
+    }
     return __builtin_bit_cast(bf16x8, out);
   }
 }
 
-// operand i of the value product from the eight keys' dwords
-template <int BITS, int DP, int W>
+// operand i of the value product from the eight keys' dwords (RAISED: of 16-bit halves of two keys each)
+template <int BITS, bool RAISED, int W>
 __device__ __forceinline__ bf16x8 value_operand(const uint32_t (&w)[8][W], int i) {
   u32x4 out;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const uint32_t a = w[2 * e][i * BITS / 32], b = w[2 * e + 1][i * BITS / 32];
-    const int s = 32 - BITS - i * BITS % 32;
-    out[e] = pack_bf16x2((float)((int32_t)(a << s) >> (32 - BITS)), (float)((int32_t)(b << s) >> (32 - BITS)));
+    if constexpr (BITS == 4 && RAISED) {
+      out[e] = raised(w[2 * e + (i >> 2 & 1)][i >> 3], i & 3);
+    } else {
+      uint32_t a = w[2 * e][i * BITS / 32], b = w[2 * e + 1][i * BITS / 32];
+      if constexpr (BITS == 4) a ^= 0x88888888u, b ^= 0x88888888u;
+      const int s = 32 - BITS - i * BITS % 32;
+      out[e] = pack_bf16x2((float)((int32_t)(a << s) >> (32 - BITS)), (float)((int32_t)(b << s) >> (32 - BITS)));
+    }
   }
   return __builtin_bit_cast(bf16x8, out);
 }
@@ -184,6 +201,7 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   constexpr int G = BITS == 8 ? 1 : DP / 32;                      // scales of a row
   constexpr int KS = DP / 32, NV = DP / 16, QP = Parts<T>::Q, PP = Parts<T>::P;
   constexpr int ROWS = 16 / SPREAD;                               // rows of a tile of 16 columns
+  constexpr bool RAISED = BITS == 4 && sizeof(T) == 2;
   static_assert(SPREAD == 1 || (TILE == 1 && SPREAD >= PP), "a row's parts need a column each");
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
   const int total = (int)gridDim.x, id = a.tiles > 1 ? xcd_remap(blockIdx.x, total) : (int)blockIdx.x;
@@ -233,6 +251,19 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
     }
   }
 
+  // what the raised keys add to a group's products, taken off in fp32: some six times a code's size, whose
+  // rounding stays far below a bf16 output's
+  f32x4 drop[TILE][RAISED ? G : 1];
+  if constexpr (RAISED) {
+    const u32x4 raise = {RAISE, RAISE, RAISE, RAISE};
+#pragma unroll
+    for (int i = 0; i < TILE; i++)
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+        drop[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, raise), q[i][k][0],
+                                                             f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+  }
+
   f32x4 acc[TILE][NV];
   float top[TILE], sum[TILE];
 #pragma unroll
@@ -264,8 +295,18 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; j++)
       load_value<BITS, DP>(V + (int64_t)(s0 + 16 * (j >> 2) + 4 * g + (j & 3)) * (DP * BITS / 8), r, vw[j]);
+    if constexpr (RAISED) {  // the halves of two keys' dwords beside each other
+#pragma unroll
+      for (int j = 0; j < 8; j += 2)
+#pragma unroll
+        for (int n = 0; n < VW; n++) {
+          const uint32_t lo = __builtin_amdgcn_perm(vw[j + 1][n], vw[j][n], 0x05040100u);
+          vw[j + 1][n] = __builtin_amdgcn_perm(vw[j + 1][n], vw[j][n], 0x07060302u);
+          vw[j][n] = lo;
+        }
+    }
 
-    // scores, in powers of two
+    // scores, before the factor that makes them powers of two
     f32x4 score[TILE][2];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -273,10 +314,13 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
 #pragma unroll
       for (int i = 0; i < TILE; i++)
 #pragma unroll
-        for (int n = 0; n < G; n++) dot[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < G; n++) {
+          if constexpr (RAISED) dot[i][n] = drop[i][n];
+          else dot[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        const bf16x8 key = key_operand<BITS>(kw[u], k);
+        const bf16x8 key = key_operand<BITS, RAISED>(kw[u], k);
 #pragma unroll
         for (int i = 0; i < TILE; i++)
 #pragma unroll
@@ -293,7 +337,7 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
             const float s = scale_at(ks[u], e * G + n);
             x = G == 1 ? dot[i][0][e] * s : __builtin_fmaf(dot[i][n][e], s, x);
           }
-          score[i][u][e] = x * a.scale;
+          score[i][u][e] = x;
         }
       }
     }
@@ -312,6 +356,7 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
     for (int i = 0; i < TILE; i++) {
       float m = fmaxf(fmaxf(fmaxf(score[i][0][0], score[i][0][1]), fmaxf(score[i][0][2], score[i][0][3])),
                       fmaxf(fmaxf(score[i][1][0], score[i][1][1]), fmaxf(score[i][1][2], score[i][1][3])));
+      m *= a.scale;
       if (__any(m > top[i] + RISE)) {
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(fmaxf(m, __shfl_xor(m, 32)), top[i]);
@@ -323,7 +368,7 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        p[i][j] = __builtin_amdgcn_exp2f(score[i][j >> 2][j & 3] - top[i]);
+        p[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(score[i][j >> 2][j & 3], a.scale, -top[i]));
         sum[i] += p[i][j];
       }
     }
@@ -341,31 +386,42 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
           for (int j = 0; j < 8; j++)
             if (s0 + 16 * (j >> 2) + 4 * g + (j & 3) >= limit[i]) x[j] = 0.f;
         }
-        bf16x8 parts[PP];
-        split_bf16<PP>(x, parts);
-        if constexpr (SPREAD > 1) {
-          const int mine = r / ROWS;
-          u32x4 w = {0u, 0u, 0u, 0u};
+        if constexpr (SPREAD > 1) {  // part number r / ROWS alone
+          u32x4 w;
 #pragma unroll
           for (int n2 = 0; n2 < PP; n2++) {
-            const u32x4 c = __builtin_bit_cast(u32x4, parts[n2]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = mine == n2 ? c[e] : w[e];
+            for (int e = 0; e < 4; e++) {
+              w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
+              if (n2 + 1 < PP) {
+                const float more = r / ROWS > n2 ? 1.f : 0.f;
+                x[2 * e] = __builtin_fmaf(-more, __uint_as_float(w[e] << 16), x[2 * e]);
+                x[2 * e + 1] = __builtin_fmaf(-more, __uint_as_float(w[e] & 0xffff0000u), x[2 * e + 1]);
+              }
+            }
           }
+          if (r / ROWS >= PP) w = u32x4{0u, 0u, 0u, 0u};  // more columns than parts
           weights[i][0] = __builtin_bit_cast(bf16x8, w);
         } else {
-#pragma unroll
-          for (int n2 = 0; n2 < PP; n2++) weights[i][n2] = parts[n2];
+          split_bf16<PP>(x, weights[i]);
         }
       }
 #pragma unroll
       for (int v = n * (NV / G); v < (n + 1) * (NV / G); v++) {
-        const bf16x8 value = value_operand<BITS, DP, VW>(vw, v);
+        const bf16x8 value = value_operand<BITS, RAISED, VW>(vw, v);
 #pragma unroll
         for (int i = 0; i < TILE; i++)
 #pragma unroll
           for (int n2 = 0; n2 < (SPREAD > 1 ? 1 : PP); n2++)
             acc[i][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, weights[i][n2], acc[i][v], 0, 0, 0);
+        if constexpr (RAISED) {  // block by block: the sums never hold more than a block's excess
+          const u32x4 raise = {RAISE, RAISE, RAISE, RAISE};
+#pragma unroll
+          for (int i = 0; i < TILE; i++)
+#pragma unroll
+            for (int n2 = 0; n2 < (SPREAD > 1 ? 1 : PP); n2++)
+              acc[i][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, raise), weights[i][n2], acc[i][v], 0, 0, 0);
+        }
       }
     }
   }
@@ -430,27 +486,49 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   }
 }
 
-// The ranges of split rows joined: a wave per row.
+// The ranges of split rows joined: a wave per row.  Bound by latency (a chain of
+// two loads): the lanes hold a range's maximum and weight each.
 template <class T, int DP>
 __global__ void __launch_bounds__(64) attend_join(AttendArgs a, int tile_rows) {
+  constexpr int N = (DP + 63) / 64, RANGES = 256 / 64;
+  __shared__ float fades[256];
   const int lane = threadIdx.x;
-  const int64_t at = blockIdx.x, h = at % a.heads, bt = at / a.heads, t = bt % a.fresh, b = bt / a.fresh;
-  const int64_t row = t * a.group + h % a.group, unit = b * a.kv_heads + h / a.group;
+  const uint32_t at = blockIdx.x, h = at % (uint32_t)a.heads, bt = at / (uint32_t)a.heads, t = bt % (uint32_t)a.fresh;
+  const uint32_t b = bt / (uint32_t)a.fresh, row = t * a.group + h % a.group;
+  const int64_t unit = (int64_t)b * a.kv_heads + h / a.group;
   const int64_t slot = (unit * a.tiles + row / tile_rows) * a.splits * tile_rows + row % tile_rows;
-  float most = LOWEST;
-  for (int s = 0; s < a.splits; s++) most = fmaxf(most, a.stats[2 * (slot + (int64_t)s * tile_rows)]);
-  float whole = 0.f, v[(DP + 63) / 64] = {};
-  for (int s = 0; s < a.splits; s++) {
-    const int64_t i = slot + (int64_t)s * tile_rows;
-    const float fade = __builtin_amdgcn_exp2f(a.stats[2 * i] - most);
-    whole += a.stats[2 * i + 1] * fade;
+  float top[RANGES], weight[RANGES], most = LOWEST, whole = 0.f;
 #pragma unroll
-    for (int n = 0; n < (DP + 63) / 64; n++)
-      if (lane + 64 * n < DP) v[n] += a.part[i * DP + lane + 64 * n] * fade;
+  for (int i = 0; i < RANGES; i++) {
+    const int s = lane + 64 * i;
+    u32x2 w = {__float_as_uint(LOWEST), 0u};
+    if (s < a.splits) w = global_load<u32x2>(a.stats + 2 * (slot + (int64_t)s * tile_rows));
+    top[i] = __uint_as_float(w[0]), weight[i] = __uint_as_float(w[1]);
+    most = fmaxf(most, top[i]);
   }
-  T* out = (T*)a.out + at * a.dim;
 #pragma unroll
-  for (int n = 0; n < (DP + 63) / 64; n++) {
+  for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+#pragma unroll
+  for (int i = 0; i < RANGES; i++) {
+    const float fade = __builtin_amdgcn_exp2f(top[i] - most);
+    fades[lane + 64 * i] = fade;
+    whole += weight[i] * fade;
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) whole += __shfl_xor(whole, o);
+  __syncthreads();
+  float v[N] = {};
+#pragma unroll 8
+  for (int s = 0; s < a.splits; s++) {
+    const float* part = a.part + (slot + (int64_t)s * tile_rows) * DP;
+    const float fade = fades[s];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+      if (DP % 64 == 0 || lane + 64 * n < DP) v[n] = __builtin_fmaf(global_load<float>(part + lane + 64 * n), fade, v[n]);
+  }
+  T* out = (T*)a.out + (int64_t)at * a.dim;
+#pragma unroll
+  for (int n = 0; n < N; n++) {
     const int d = lane + 64 * n;
     if (d >= a.dim) continue;
     const float x = whole == 0.f ? 0.f : v[n] / whole;

@@ -5,7 +5,10 @@
 
 namespace {
 
-constexpr int64_t WORKGROUPS = 2048;  // wanted in a launch: eight for each of 256 CUs
+// Workgroups wanted in a launch of 256 CUs: eight for each where a tile has few
+// rows and the keys are what is read; two where it has many, whose sums a split
+// row writes and reads again.
+constexpr int64_t FEW_ROWS = 2048, MANY_ROWS = 512;
 
 AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype) {
   AttendPlan p;
@@ -16,7 +19,7 @@ AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads
   p.rows = 16 / p.spread * p.tile;
   p.tiles = (rows + p.rows - 1) / p.rows;
   const int64_t units = batch * kv_heads * p.tiles, most = (longest + WAVES * BLOCK - 1) / (WAVES * BLOCK);
-  p.splits = (WORKGROUPS + units - 1) / units;
+  p.splits = ((p.spread > 1 ? FEW_ROWS : MANY_ROWS) + units - 1) / units;
   if (p.splits > most) p.splits = most;
   if (p.splits > 256) p.splits = 256;
   if (p.splits < 1) p.splits = 1;

@@ -7,8 +7,8 @@
 // group with an infinity or NaN has the scale NaN (and codes 0).
 //
 // Rows are padded to a pitch P of channels (zeros).  Eight bits: a byte per
-// channel, in order.  Four bits: two's complement nibbles in the order in which
-// the attention kernel's lanes take them, 16 lanes or 4 x 16 lanes to a row:
+// channel, in order.  Four bits: nibbles of code + 8 in the order in which the
+// attention kernel's lanes take them, 16 lanes or 4 x 16 lanes to a row:
 //   keys: lane group g of 4 holds P/8 bytes, a dword for each 32 channels c, of
 //     channels 32c + 8g + j; nibble n of the dword is j = 2 (n % 4) + n / 4;
 //   values: lane r of 16 holds P/32 bytes, one for each 32 channels c, of

@@ -104,11 +104,11 @@ __global__ void __launch_bounds__(THREADS) cache_write(WriteArgs a) {
         uint32_t w = 0;
 #pragma unroll
         for (int n = 0; n < 8; n++) w |= (q[2 * (n & 3) + (n >> 2)] & 15) << (4 * n);
-        *(uint32_t*)(out + (part & 3) * (a.pitch >> 3) + 4 * (part >> 2)) = w;
+        *(uint32_t*)(out + (part & 3) * (a.pitch >> 3) + 4 * (part >> 2)) = w ^ 0x88888888u;
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e += 2)
-          out[(4 * (part & 3) + e / 2) * (a.pitch >> 5) + (part >> 2)] = (uint8_t)((q[e] & 15) | (q[e + 1] & 15) << 4);
+          out[(4 * (part & 3) + e / 2) * (a.pitch >> 5) + (part >> 2)] = (uint8_t)(((q[e] & 15) | (q[e + 1] & 15) << 4) ^ 0x88);
       }
       if ((part & 3) == 0) a.scales[side][slot[u] * (a.pitch / 32) + (part >> 2)] = (bf16_t)bits;
     }
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(THREADS) cache_read(ReadArgs a) {
     for (int e = 0; e < 8; e++) {
       int c;
       if constexpr (BITS == 8) c = (int8_t)(code[u][e >> 2] >> (8 * (e & 3)));
-      else c = (int32_t)(code[u][0] << (28 - 4 * (side == 0 ? (e >> 1) + 4 * (e & 1) : e))) >> 28;
+      else c = (int)(code[u][0] >> (4 * (side == 0 ? (e >> 1) + 4 * (e & 1) : e)) & 15) - 8;
       v[e] = (float)c * scale[u];
     }
     T* out = (T*)a.out[side] + (int64_t)row * a.dim;

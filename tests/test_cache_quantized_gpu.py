@@ -163,9 +163,22 @@ ATTEND = [
 ]
 
 
-def check_attention(out, q, k, v, starts, counts, scale, dtype):
+def raised_scales(x):
+    """24 times an upper bound of each value's scale where codes have 4 bits: the
+    largest code of a group is 6.5 at least (its scale is the smallest that
+    holds it, 2^-7 too large at most), so a sixth of the largest value."""
+    out = np.empty_like(x)
+    for start in range(0, x.shape[-1], 32):
+        out[..., start:start + 32] = 4 * np.abs(x[..., start:start + 32]).max(-1, keepdims=True)
+    return out
+
+
+def check_attention(out, q, k, v, starts, counts, scale, dtype, bits=8):
     """out (batch, new, heads, dim) against float64 attention over the held k, v
-    (batch, kv_heads, length, dim)."""
+    (batch, kv_heads, length, dim).  The bf16 kernels hold codes of 4 bits as
+    code + 24 and take the 24 off a product of 32 channels, or of a block of 32
+    keys, again: 16 additions (of 8 products each, and of two parts) are then
+    rounded at up to 24 scales, not at the codes' own size."""
     batch, new, heads, dim = q.shape
     group = heads // k.shape[1]
     # a weight reaches the value product as two bf16 parts (half a step of 16 bits together) or three
@@ -188,8 +201,13 @@ def check_attention(out, q, k, v, starts, counts, scale, dtype):
             size = np.abs(q[b, :n, h]) @ np.abs(keys).T * scale
             arg = np.where(hidden, 0.0, np.abs(x))
             moved = UNIT * ((dim + 40) * (size + size.max(axis=1, keepdims=True)) + 4 * arg + 8) + parts
+            raised = dtype == "bfloat16" and bits == 4
+            if raised:
+                moved += 16 * UNIT * scale * np.abs(q[b, :n, h]) @ raised_scales(keys).T
             bound = (p * (moved + (p * moved).sum(axis=1, keepdims=True) + 2 * (total + 40) * UNIT)) @ np.abs(values)
             bound += 4 * UNIT * np.abs(expected)
+            if raised:
+                bound += 16 * UNIT * p @ raised_scales(values)
             if dtype == "bfloat16":
                 bound += 2.0 ** -8 * (np.abs(expected) + bound)
             assert (np.abs(out[b, :n, h] - expected) <= bound).all(), (b, h)
@@ -214,7 +232,7 @@ def test_attention_matches_float64(dtype, bits, batch, heads, kv_heads, dim, pas
         out = cache.attend(as_tensor(q, dtype))
         assert out.dtype == dtype and out.shape == q.shape
         k, v = read(cache) if cache.length else [np.zeros((batch, kv_heads, 0, dim))] * 2
-        check_attention(download(out.storage).reshape(q.shape), q, k, v, starts, counts, dim ** -0.5, dtype)
+        check_attention(download(out.storage).reshape(q.shape), q, k, v, starts, counts, dim ** -0.5, dtype, bits)
 
 
 @pytest.mark.parametrize("bits", [8, 4])
