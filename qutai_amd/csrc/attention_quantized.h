@@ -86,9 +86,13 @@ __device__ __forceinline__ int value_channel(int i, int r) {
   else return DP / 16 * r + i;
 }
 
-// the bytes of a key's value row that lane r of 16 takes, as dwords
+// Loads take a base that is the same for the wave and a lane's 32-bit offset: no
+// 64-bit addresses in vector registers.
+
+// the bytes of a key's value row, at `offset` from `row`, that lane r of 16 takes, as dwords
 template <int BITS, int DP>
-__device__ __forceinline__ void load_value(const uint8_t* row, int r, uint32_t* w) {
+__device__ __forceinline__ void load_value(const uint8_t* base, uint32_t offset, int r, uint32_t* w) {
+  const uint8_t* row = base + offset;
   if constexpr (BITS == 4) {
     const uint8_t* p = row + r * (DP / 32);
     if constexpr (DP == 32) w[0] = global_load<uint8_t>(p);
@@ -107,7 +111,7 @@ __device__ __forceinline__ void load_value(const uint8_t* row, int r, uint32_t* 
     else if constexpr (DP == 64) w[0] = global_load<uint32_t>(row + 4 * r);
     else if constexpr (DP == 96) w[0] = global_load<uint32_t>(row + 4 * r), w[1] = global_load<uint16_t>(row + 64 + 2 * r);
     else if constexpr (DP == 128) {
-      const u32x2 v = global_load<u32x2>(row + 8 * r);
+      const u32x2 v = global_load_nt<u32x2>(row + 8 * r);  // whole 128-byte lines
       w[0] = v[0], w[1] = v[1];
     } else if constexpr (DP == 192) {
       const u32x2 v = global_load<u32x2>(row + 8 * r);
@@ -121,7 +125,8 @@ __device__ __forceinline__ void load_value(const uint8_t* row, int r, uint32_t* 
 
 // the bytes of a key's row that its lane of group g takes
 template <int BITS, int DP>
-__device__ __forceinline__ void load_key(const uint8_t* row, int g, uint32_t* w) {
+__device__ __forceinline__ void load_key(const uint8_t* base, uint32_t offset, int g, uint32_t* w) {
+  const uint8_t* row = base + offset;
   if constexpr (BITS == 4) {
     const uint8_t* p = row + g * (DP / 8);
 #pragma unroll
@@ -202,8 +207,9 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   constexpr int KS = DP / 32, NV = DP / 16, QP = Parts<T>::Q, PP = Parts<T>::P;
   constexpr int ROWS = 16 / SPREAD;                               // rows of a tile of 16 columns
   constexpr bool RAISED = BITS == 4 && sizeof(T) == 2;
+  constexpr int ROW = DP * BITS / 8;                              // bytes of a row
   static_assert(SPREAD == 1 || (TILE == 1 && SPREAD >= PP), "a row's parts need a column each");
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = uniform32(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int total = (int)gridDim.x, id = a.tiles > 1 ? xcd_remap(blockIdx.x, total) : (int)blockIdx.x;
   const int split = id % a.splits, tile = id / a.splits % a.tiles;
   const int64_t unit = id / a.splits / a.tiles, b = unit / a.kv_heads, head = unit % a.kv_heads;
@@ -277,24 +283,29 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   const int share = ((end + a.splits - 1) / a.splits + BLOCK * WAVES - 1) / (BLOCK * WAVES) * (BLOCK * WAVES);
   const int from = split * share, to = from + share < end ? from + share : end;
   const int64_t base = unit * a.capacity;
-  const uint8_t* K = a.codes[0] + base * (DP * BITS / 8);
-  const uint8_t* V = a.codes[1] + base * (DP * BITS / 8);
+  const uint8_t* K = a.codes[0] + base * ROW;
+  const uint8_t* V = a.codes[1] + base * ROW;
   const bf16_t* KSC = a.scales[0] + base * G;
   const bf16_t* VSC = a.scales[1] + base * G;
   for (int s0 = from + wave * BLOCK; s0 < to; s0 += WAVES * BLOCK) {
     uint32_t kw[2][KW], vw[8][VW], ks[2][2 * G], vs[2][2 * G];
+    const uint8_t* key_rows = K + (int64_t)s0 * ROW;
+    const uint8_t* value_rows = V + (int64_t)s0 * ROW;
+    const bf16_t* key_scales = KSC + (int64_t)s0 * G;
+    const bf16_t* value_scales = VSC + (int64_t)s0 * G;
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      load_key<BITS, DP>(K + (int64_t)(s0 + 16 * u + r) * (DP * BITS / 8), g, kw[u]);
+      load_key<BITS, DP>(key_rows, (uint32_t)((16 * u + r) * ROW), g, kw[u]);
 #pragma unroll
       for (int n = 0; n < 2 * G; n++) {
-        ks[u][n] = global_load<uint32_t>(KSC + (int64_t)(s0 + 16 * u + 4 * g) * G + 2 * n);
-        vs[u][n] = global_load<uint32_t>(VSC + (int64_t)(s0 + 16 * u + 4 * g) * G + 2 * n);
+        ks[u][n] = global_load<uint32_t>(key_scales + (uint32_t)((16 * u + 4 * g) * G + 2 * n));
+        vs[u][n] = global_load<uint32_t>(value_scales + (uint32_t)((16 * u + 4 * g) * G + 2 * n));
       }
     }
 #pragma unroll
     for (int j = 0; j < 8; j++)
-      load_value<BITS, DP>(V + (int64_t)(s0 + 16 * (j >> 2) + 4 * g + (j & 3)) * (DP * BITS / 8), r, vw[j]);
+      load_value<BITS, DP>(value_rows, (uint32_t)((16 * (j >> 2) + 4 * g + (j & 3)) * ROW), r, vw[j]);
+    __builtin_amdgcn_sched_barrier(0);  // all of a block's loads are in flight before the first is waited for
     if constexpr (RAISED) {  // the halves of two keys' dwords beside each other
 #pragma unroll
       for (int j = 0; j < 8; j += 2)

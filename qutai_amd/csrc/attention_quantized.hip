@@ -5,10 +5,12 @@
 
 namespace {
 
-// Workgroups wanted in a launch of 256 CUs: eight for each where a tile has few
-// rows and the keys are what is read; two where it has many, whose sums a split
-// row writes and reads again.
-constexpr int64_t FEW_ROWS = 2048, MANY_ROWS = 512;
+// Workgroups wanted in a launch of 256 CUs: four for each where a tile has few
+// rows and the keys are what is read (32 sequences of up to 16000 keys, 8 bits:
+// 149 us, 156 with two, 152 with twelve; 16 of up to 8000, 4 bits: 42, 40 and 57),
+// one where it has many, whose sums a split row writes and reads again (512 new
+// positions over 3500: 63 us, 79 with two, 96 with four).
+constexpr int64_t FEW_ROWS = 1024, MANY_ROWS = 256;
 
 AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype) {
   AttendPlan p;
