@@ -18,12 +18,14 @@ from __future__ import annotations
 from array import array
 from bisect import bisect_left
 from itertools import chain
+from random import Random
 
 from ..backends import amd
 from ..core.context import set_recording
 from ..core.tensor import Tensor
 from .config import Config
-from .layers import Block, Projection, RMSNorm, backend, embed, linear, projection_loss, scaled, unpack
+from ..nn.cache import QuantizedKVCache
+from .layers import Block, Projection, RMSNorm, backend, embed, linear, projection_loss, sample, scaled, unpack
 from .recompute import checkpoint
 
 
@@ -114,6 +116,64 @@ class Decoder:
         """Logits (batch, time, vocab) of the tied head (decoder.py:134-139)."""
         with set_recording(train):
             return linear(self.hidden(tokens, train=train), self.embedding.weight)
+
+    # ---- answering: new positions over quantised caches ----------------------------
+    def caches(self, capacity=None, *, bits=8):
+        """An empty QuantizedKVCache for each block (capacity: max_seq_len)."""
+        capacity = self.config.max_seq_len if capacity is None else capacity
+        return tuple(QuantizedKVCache(capacity, bits=bits) for _ in self.blocks)
+
+    def decode(self, tokens, caches, counts=None):
+        """Logits (batch, vocab) that follow the last of ``tokens`` (batch, new),
+        the positions behind those that ``caches`` hold; of sequence b only the
+        first counts[b] are there, at least one.  Nothing is recorded."""
+        ids, (batch, new) = self._tokens(tokens)
+        caches = tuple(caches)
+        counts = (new,) * batch if counts is None else tuple(counts)
+        if len(caches) != len(self.blocks) or len(counts) != batch or any(type(n) is not int or not 1 <= n <= new for n in counts):
+            raise ValueError("decode takes a cache for each block and a count of 1 to new positions for each sequence")
+        held = caches[0].lengths or (0,) * batch
+        if any((c.lengths or (0,) * batch) != held for c in caches) or len(held) != batch:
+            raise ValueError("the caches hold other sequences than the tokens'")
+        limit = min(self.config.max_seq_len, *(c.capacity for c in caches))
+        if any(n + m > limit for n, m in zip(held, counts)):
+            raise ValueError("the positions exceed max_seq_len or the caches' capacity")
+        with set_recording(False):
+            hidden = embed(ids, self.embedding.weight, (batch, new))
+            for block, cache in zip(self.blocks, caches):
+                hidden = block.decode(hidden, cache, None if min(counts) == new else counts)
+            if new > 1:  # the rows that a token follows
+                last = array("q", (b * new + n - 1 for b, n in enumerate(counts)))
+                width = self.config.d_model
+                rows = backend(hidden).embedding(hidden.storage, last, width)
+                hidden = Tensor(rows, shape=(batch, 1, width))
+            hidden = self.norm(hidden)
+            return linear(Tensor(hidden.storage, shape=(batch, self.config.d_model)), self.embedding.weight)
+
+    def generate(self, prompts, count, *, seed=None, bits=8, **filters):
+        """``count`` tokens behind each prompt (lists of ids of any lengths), one
+        list for each: every step's logits are sampled (``filters``:
+        temperature, top_k, top_p, min_p) with numbers of Random(seed), one per
+        sequence and step, keys and values cached in codes of ``bits``."""
+        prompts = [list(p) for p in prompts]
+        if type(count) is not int or count < 0 or not prompts or not all(prompts):
+            raise ValueError("generate takes prompts of one token at least and a number of tokens")
+        counts = [len(p) for p in prompts]
+        total = max(counts) + max(0, count - 1)
+        if total > self.config.max_seq_len:
+            raise ValueError("prompt and generated tokens exceed max_seq_len")
+        random, made = Random(seed), [[] for _ in prompts]
+        caches = self.caches(total, bits=bits)
+        tokens = [p + [0] * (max(counts) - len(p)) for p in prompts]
+        for _ in range(count):
+            logits = self.decode(tokens, caches, counts)
+            chosen, _ = sample(logits, [random.random() for _ in prompts], **filters)
+            if min(chosen) < 0:
+                raise RuntimeError("a row of logits holds no number that a token can be sampled from")
+            for row, token in zip(made, chosen):
+                row.append(token)
+            tokens, counts = [[token] for token in chosen], [1] * len(prompts)
+        return made
 
     # ---- loss (decoder.py:141-175) -------------------------------------------------
     def loss(self, tokens, labels=None, *, train=True, chunk_size=128):

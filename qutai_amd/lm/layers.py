@@ -455,6 +455,33 @@ class GQA:
             k = rope(self.k(x), self.kv_heads, self.theta)
         return self.out(attention(q, k, self.v(x), self.heads, self.kv_heads))
 
+    def decode(self, x, cache, counts=None):
+        """The block over new positions of (batch, new, width) alone: their keys
+        and values are appended to ``cache`` (a QuantizedKVCache; of sequence b
+        the first counts[b] where given) and they attend over all that it holds.
+        Nothing is recorded."""
+        b = backend(x)
+        batch, new, width = x.shape
+        weights = (self.q.weight, self.k.weight, self.v.weight)
+        q_width, kv_width = weights[0].shape[0], weights[1].shape[0]
+        head, rows = q_width // self.heads, batch * new
+        cache.reserve(batch, self.kv_heads, head)
+        offset, starts = cache.positions()
+        norms = (None, None) if self.q_norm is None else (self.q_norm.weight.storage, self.k_norm.weight.storage)
+        dims = (*norms, batch, new, self.heads, self.kv_heads, head, self.theta)
+        options = dict(offset=offset, starts=starts, **({} if self.q_norm is None else {"eps": self.q_norm.eps}))
+        if _stacked_qkv(x, *weights):
+            qkv, row = _stacked_product(x, *weights)
+            q, k = b.qk_norm_rope(qkv, qkv, *dims, **options, q_row=row, k_column=q_width, k_row=row)
+            v, place = qkv, dict(value_column=q_width + kv_width, value_row=row)
+        else:
+            projected = [linear(x, w).storage for w in weights]
+            q, k = b.qk_norm_rope(*projected[:2], *dims, **options)
+            v, place = projected[2], {}
+        cache.append_rows(k, v, batch, new, self.kv_heads, head, counts, **place)
+        mixed = cache.attend(Tensor(q, shape=(batch, new, self.heads, head)))
+        return self.out(Tensor(mixed.storage, shape=(batch, new, q_width)))
+
     def parameters(self):
         layers = (self.q, self.k, self.v, self.out) + (() if self.q_norm is None else (self.q_norm, self.k_norm))
         return tuple(p for layer in layers for p in layer.parameters())
@@ -489,6 +516,12 @@ class Block:
 
     def hidden(self, x):
         return self(x)[0]
+
+    def decode(self, x, cache, counts=None):
+        """The block over new positions, attending over ``cache`` (GQA.decode)."""
+        x = residual_add(x, self.attn.decode(self.attn_norm(x), cache, counts))
+        y = self.ffn(self.ffn_norm(x))
+        return residual_add(x, y[0] if self.is_moe else y)
 
     def packed(self, x):
         return pack(*self(x))
@@ -662,6 +695,18 @@ def _stacked_qkv(x, wq, wk, wv):
     return _bf16_path(x, wq) and activation_dtype(x, wq) == "bfloat16"
 
 
+def _stacked_product(x, wq, wk, wv):
+    """(x [Wq; Wk; Wv]^T in bf16, columns of a row) of the bf16 path."""
+    width, rows = x.shape[-1], x.size // x.shape[-1]
+    total = wq.shape[0] + 2 * wk.shape[0]
+    ws = amd.AMDStorage(total * width, "bfloat16")
+    start = 0
+    for w in (wq, wk, wv):
+        amd.cast_into(amd.view(ws, start * width, w.size), w.storage)
+        start += w.shape[0]
+    return backend(x).gemm(_bf16_input(x), ws, rows, width, total, transpose_right=True, out_dtype="bfloat16"), total
+
+
 def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=None, *, eps=1e-6):
     """RoPE(x Wq^T), RoPE(x Wk^T), x Wv^T and causal grouped-query attention
     as one recorded op: GQA up to its out projection (src/qutai/lm/layers.py:
@@ -737,6 +782,19 @@ def attention_fused(q, k, v, *, scale=None, causal=False):
     out, _ = backend(q).attention(q.storage, k.storage, v.storage, groups, time, 1, 1, dim, causal=causal,
                                   layout=0, scale=scale)
     return Tensor(out, shape=q.shape)
+
+
+def sample(logits, uniforms, **filters):
+    """One token for each row of (..., vocab) logits, picked by that many numbers
+    in [0, 1): (tokens, their probabilities among the tokens kept), as lists.
+    ``filters``: temperature, top_k, top_p and min_p of amd_lm.sample."""
+    vocab = logits.shape[-1]
+    rows = logits.size // vocab
+    if len(uniforms) != rows:
+        raise ValueError("sample takes one number for every row of logits")
+    numbers = amd.storage(array("d", uniforms), dtype="float64")
+    tokens, probabilities = backend(logits).sample(logits.storage, numbers, rows, vocab, **filters)
+    return tokens.tolist(), probabilities.tolist()
 
 
 def parameter_count(layer):

@@ -87,7 +87,7 @@ class QuantizedKVCache:
             self._base, self._stored, self._shift = lengths, None, 0
         self.lengths = lengths
 
-    def _positions(self):
+    def positions(self):
         """(shift, device positions or None) of the next position of every sequence."""
         if self._base is not None and self._stored is None:
             self._stored = amd.storage(self._base, dtype="int64")
@@ -125,7 +125,7 @@ class QuantizedKVCache:
         lengths = tuple(n + m for n, m in zip(self.lengths, counts))
         if max(lengths) > self.capacity:
             raise ValueError("the cache's capacity is exceeded")
-        start, starts = self._positions()
+        start, starts = self.positions()
         held = None if min(counts) == new else amd.storage(counts, dtype="int64")
         amd_lm.cache_quantize(self.codes, keys, values, new, start=start, starts=starts, counts=held, **columns)
         self._set_lengths(lengths)
@@ -151,7 +151,7 @@ class QuantizedKVCache:
         shorter sequence's end."""
         if self.codes is None:
             raise ValueError("nothing was cached yet")
-        shift, stored = self._positions()
+        shift, stored = self.positions()
         c, length = self.codes, self.length
         pair = amd_lm.cache_dequantize(c, length, lengths=stored, shift=shift, dtype=dtype)
         return tuple(Tensor(x, shape=(c.batch, c.kv_heads, length, c.dim)) for x in pair)

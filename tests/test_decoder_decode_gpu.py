@@ -1,0 +1,185 @@
+"""Answering with a Decoder: cached decoding over quantised caches (normed and
+rotated heads, codes written and read by attention, sampled tokens together)
+against a float64 forward pass that reads the values the caches hold."""
+import numpy as np
+import pytest
+
+from qutai_amd.backends import amd
+from qutai_amd.lm import Config, Decoder, autocast, sample
+from tests.helpers import download, stored, upload
+from tests.test_cache_quantized_gpu import held
+
+pytestmark = pytest.mark.gpu
+
+
+def build(qk_norm, ffn="dense", width=32, heads=4, kv_heads=2, layers=2):
+    config = Config(vocab_size=61, n_layers=layers, d_model=width, n_heads=heads, n_kv_heads=kv_heads, d_ff=40, max_seq_len=48,
+                    ffn_type=ffn, n_experts=4, top_k=2, d_expert=24, qk_norm=qk_norm)
+    model = Decoder(config, seed=1)
+    rng = np.random.default_rng(0)
+    for name, p in model.named_parameters():
+        x = rng.standard_normal(p.shape) * 0.3
+        amd.copy_into(p.storage, upload(1 + x / 3 if "norm" in name else x, "float32"))
+    return model
+
+
+def norm(x, w, eps):
+    return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w
+
+
+def turned(x, at, theta):
+    angle = at[:, None, None] * theta ** (-np.arange(0, x.shape[-1], 2) / x.shape[-1])
+    out = np.empty_like(x)
+    out[..., 0::2] = x[..., 0::2] * np.cos(angle) - x[..., 1::2] * np.sin(angle)
+    out[..., 1::2] = x[..., 0::2] * np.sin(angle) + x[..., 1::2] * np.cos(angle)
+    return out
+
+
+class Reference:
+    """One sequence's new positions in float64, over the values that the caches hold."""
+
+    def __init__(self, model):
+        self.c = model.config
+        self.p = {n: download(p.storage).astype(np.float64).reshape(p.shape) for n, p in model.named_parameters()}
+
+    def logits(self, tokens, start, caches, sequence, bits, rounded=None):
+        """``rounded``: applied where autocast stores bf16 (inputs and weights of
+        every product, and its result; the caches' values are as they are)."""
+        c, p = self.c, self.p
+        r = rounded or (lambda x: x)
+        x = p["embedding.weight"][tokens]
+        at = start + np.arange(len(tokens))
+        head, group = c.d_model // c.n_heads, c.n_heads // c.n_kv_heads
+        for i, cache in enumerate(caches):
+            a = f"blocks.{i}.attn."
+            y = r(norm(x, p[f"blocks.{i}.attn_norm.weight"], c.norm_eps))
+            q, k, v = (r(y @ r(p[a + n + ".weight"]).T) for n in "qkv")
+            q, k, v = (z.reshape(len(tokens), -1, head) for z in (q, k, v))
+            if c.qk_norm:
+                q, k = norm(q, p[a + "q_norm.weight"], c.norm_eps), norm(k, p[a + "k_norm.weight"], c.norm_eps)
+            q, k = r(turned(q, at, c.rope_theta)), r(turned(k, at, c.rope_theta))
+            keys, values = (download(z.storage).reshape(z.shape)[sequence].astype(np.float64) for z in cache.read())
+            for got, fresh in ((keys, k), (values, v)) if rounded is None else ():
+                # a code's half step, and a flip where the fp32 value lies on the other side of a border
+                exact = fresh.transpose(1, 0, 2)
+                step = np.abs(exact).max() * 1.01 / (127 if bits == 8 else 7)
+                assert np.abs(got[:, at] - exact).max() <= 0.51 * step
+            mixed = np.empty_like(q)
+            for h in range(c.n_heads):
+                s = q[:, h] @ keys[h // group, :at[-1] + 1].T / head ** 0.5
+                s[np.arange(at[-1] + 1)[None] > at[:, None]] = -np.inf
+                w = np.exp(s - s.max(1, keepdims=True))
+                mixed[:, h] = w / w.sum(1, keepdims=True) @ values[h // group, :at[-1] + 1]
+            x = x + r(r(mixed).reshape(len(tokens), -1) @ r(p[a + "out.weight"]).T)
+            y = r(norm(x, p[f"blocks.{i}.ffn_norm.weight"], c.norm_eps))
+            f = f"blocks.{i}.ffn."
+            gate, up = r(y @ r(p[f + "gate.weight"]).T), r(y @ r(p[f + "up.weight"]).T)
+            x = x + r(r(r(gate / (1 + np.exp(-gate))) * up) @ r(p[f + "down.weight"]).T)
+        return r(r(norm(x, p["norm.weight"], c.norm_eps)[-1]) @ r(p["embedding.weight"]).T)
+
+
+@pytest.mark.parametrize("qk_norm,bits,ragged", [(True, 8, True), (True, 4, False), (False, 8, True), (False, 8, False)])
+def test_cached_logits_match_float64(qk_norm, bits, ragged):
+    model = build(qk_norm)
+    reference, caches = Reference(model), model.caches(bits=bits)
+    rng = np.random.default_rng(3)
+    lengths = [0, 0, 0]
+    for new in (7, 1, 3, 1):
+        tokens = rng.integers(0, 61, (3, new)).tolist()
+        counts = [max(1, new - 2 * b) for b in range(3)] if ragged else None
+        logits = model.decode(tokens, caches, counts)
+        assert logits.shape == (3, 61) and not logits.requires_grad
+        got = download(logits.storage).reshape(3, 61)
+        for b in range(3):
+            n = counts[b] if ragged else new
+            expected = reference.logits(tokens[b][:n], lengths[b], caches, b, bits)
+            # sums of 32 to 40 fp32 products through two blocks: some thousand roundings of values of this size
+            assert np.abs(got[b] - expected).max() <= 2000 * 2.0 ** -24 * np.abs(expected).max()
+            lengths[b] += n
+        assert all(c.lengths == tuple(lengths) for c in caches)
+
+
+def test_autocast_decoding_rounds_as_bf16_does():
+    """bf16 activations (one projection product, its columns read in place)
+    against float64 over the values the caches hold.  How far the storage's
+    roundings may carry is seen from the same pass with them: another order of
+    sums gives roundings of the same sizes, so three times its own distance."""
+    model = build(True, width=64, heads=4, kv_heads=2)
+    reference, caches, rng = Reference(model), model.caches(), np.random.default_rng(5)
+    start = 0
+    for new in (6, 1, 1):
+        tokens = rng.integers(0, 61, (2, new)).tolist()
+        with autocast():
+            got = download(model.decode(tokens, caches).storage).reshape(2, 61)
+        for b in range(2):
+            exact, low = (reference.logits(tokens[b], start, caches, b, 8, r)
+                          for r in (lambda x: x, lambda x: stored(x, "bfloat16")))
+            assert np.linalg.norm(got[b] - exact) <= 3 * np.linalg.norm(low - exact)
+        start += new
+
+
+@pytest.mark.parametrize("qk_norm,ffn", [(True, "dense"), (False, "moe")])
+def test_decoding_agrees_with_the_whole_forward_pass(qk_norm, ffn):
+    """Logits of cached decoding against the uncached model on the same tokens:
+    apart by what 8-bit keys and values are off."""
+    model = build(qk_norm, ffn)
+    tokens = np.random.default_rng(8).integers(0, 61, (2, 12)).tolist()
+    whole = download(model(tokens, train=False).storage).reshape(2, 12, 61)
+    caches = model.caches()
+    model.decode([row[:9] for row in tokens], caches)
+    for t in (9, 10, 11):
+        got = download(model.decode([[row[t]] for row in tokens], caches).storage).reshape(2, 61)
+        # half a step of 1/127 of a row's largest value in each key and value, and through two blocks
+        assert np.linalg.norm(got - whole[:, t]) <= 0.05 * np.linalg.norm(whole[:, t])
+
+
+def test_generate_samples_what_decode_gives():
+    from random import Random
+
+    model = build(True)
+    prompts, filters = [[3, 4, 5, 6], [7], [8, 9]], dict(temperature=0.8, top_k=20, top_p=0.9)
+    made = model.generate(prompts, 6, seed=11, **filters)
+    assert [len(row) for row in made] == [6, 6, 6] and all(0 <= t < 61 for row in made for t in row)
+    assert made == model.generate(prompts, 6, seed=11, **filters)
+    random, caches = Random(11), model.caches(9)
+    tokens, counts = [p + [0] * (4 - len(p)) for p in prompts], [4, 1, 2]
+    for step in range(6):
+        logits = model.decode(tokens, caches, counts)
+        chosen, probabilities = sample(logits, [random.random() for _ in prompts], **filters)
+        assert chosen == [row[step] for row in made] and all(0 < x <= 1 for x in probabilities)
+        tokens, counts = [[t] for t in chosen], [1, 1, 1]
+    greedy = model.generate(prompts, 3, temperature=0.0)
+    logits = model.decode([p + [0] * (4 - len(p)) for p in prompts], model.caches(), [4, 1, 2])
+    assert [row[0] for row in greedy] == download(logits.storage).reshape(3, 61).argmax(1).tolist()
+    assert model.generate([[1]], 0) == [[]]
+
+
+def test_refusals():
+    model = build(True)
+    caches = model.caches()
+    for tokens, given, counts in (([[1, 2]], caches[:1], None), ([[1, 2]], caches, [3]), ([[1, 2]], caches, [0]),
+                                  ([[1, 2]], caches, [1, 1]), ([[61]], caches, None), ([[1] * 49], caches, None)):
+        with pytest.raises(ValueError):
+            model.decode(tokens, given, counts)
+    model.decode([[1, 2]], caches)
+    for tokens in ([[1], [2]], [[1] * 47]):
+        with pytest.raises(ValueError):
+            model.decode(tokens, caches)
+    for prompts, count in (([], 1), ([[]], 1), ([[1]], -1), ([[1] * 40], 10)):
+        with pytest.raises(ValueError):
+            model.generate(prompts, count)
+    logits = model.decode([[1]], model.caches())
+    with pytest.raises(ValueError):
+        sample(logits, [0.5, 0.5])
+
+
+def test_quantised_values_are_those_of_the_keys():
+    """What a block caches is its normed and rotated keys' and its values' codes."""
+    model = build(True, layers=1)
+    caches = model.caches()
+    model.decode([[5, 6, 7]], caches)
+    keys, values = (download(x.storage).reshape(x.shape) for x in caches[0].read())
+    again = [held(x.transpose(0, 2, 1, 3), 8).transpose(0, 2, 1, 3) for x in (keys, values)]
+    # what the codes stand for lies on the codes' own grid: quantised again it moves by half a step at most
+    for x, y in zip((keys, values), again):
+        assert np.abs(x - y).max() <= 0.51 * np.abs(x).max() / 126
