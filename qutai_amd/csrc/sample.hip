@@ -34,6 +34,8 @@ namespace {
 constexpr int THREADS = 512, WAVES = THREADS / 64;
 constexpr int64_t VOCAB_LIMIT = 1 << 20;
 constexpr int BINS = 2048, LIST = 4096, FEW = 192;
+// bf16: exponents, and entries of a table with one for each number of these exponents (see Window)
+constexpr int MAGNITUDES = 20 * 128, ENTRIES = 2 * MAGNITUDES + 4;
 constexpr int SPAN = 8, HELD = 4 * SPAN;  // steps of a register vector, and of all of them
 
 struct SampleArgs {
@@ -69,10 +71,12 @@ struct Shared {
         unsigned long long masses[BINS];
       };
       float list[LIST];
+      uint32_t numbers[ENTRIES];
     };
     double sums[VOCAB_LIMIT / (THREADS * 4) * WAVES];  // kept weights of each step and wave
   };
   uint32_t ties[VOCAB_LIMIT / (THREADS * 4) * WAVES];
+  double table[ENTRIES];  // bf16: the weight of each number
   double powers[32];  // 2^(-j / 32)
   unsigned long long part[WAVES];
   double wide[2];
@@ -105,6 +109,31 @@ struct Weigh {
   __device__ __forceinline__ double operator()(float l) const {
     int n;
     return (*this)(l, n);
+  }
+};
+
+// bf16 logits by number: entry MAGNITUDES + 3 + m for the m-th number of the window
+// of exponents, from `lo` on, MAGNITUDES - m for its negative; between them two
+// entries for what is smaller, zeros among it, at the ends two for what is larger.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+struct Window {
+  int lo;  // bits of the smallest magnitude, 1 at least
+  // the entries of a word's two logits; `small` gets a sign bit where one is below the window
+  __device__ __forceinline__ s16x2 entries(uint32_t w, uint32_t& small) const {
+    const s16x2 low = {(short)lo, (short)lo}, least = {-1, -1}, most = {MAGNITUDES, MAGNITUDES};
+    const s16x2 bits = __builtin_bit_cast(s16x2, w), sign = bits >> 15;
+    s16x2 m = __builtin_bit_cast(s16x2, w & 0x7fff7fffu) - low;
+    m = __builtin_elementwise_min(__builtin_elementwise_max(m, least), most);
+    small |= __builtin_bit_cast(uint32_t, m);
+    const s16x2 middle = {MAGNITUDES + 3, MAGNITUDES + 3};
+    return (m ^ sign) + sign + sign + middle;
+  }
+  __device__ __forceinline__ float value(int entry) const {
+    const int m = entry >= MAGNITUDES + 3 ? entry - MAGNITUDES - 3 : MAGNITUDES - entry;
+    return __uint_as_float((uint32_t)(lo + m) << 16 | (entry >= MAGNITUDES + 3 ? 0u : 0x80000000u));
+  }
+  __device__ __forceinline__ bool holds(int entry) const {
+    return entry > 0 && entry < ENTRIES - 1 && entry != MAGNITUDES + 1 && entry != MAGNITUDES + 2;
   }
 };
 
@@ -163,6 +192,43 @@ __device__ __forceinline__ void find_bin(Shared& s, const V* bins, unsigned long
 #pragma unroll
     for (int n = 1; n < PER; n++) value = i == n ? own[n] : value;
     s.found[2] = value;
+  }
+  __syncthreads();
+}
+
+// The same over amount(entry) of the bf16 entries; target 0 is goal(their sum).
+template <class F, class Goal>
+__device__ __forceinline__ void find_entry(Shared& s, F amount, unsigned long long target, Goal goal) {
+  constexpr int PER = (ENTRIES + THREADS - 1) / THREADS;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, high = ENTRIES - 1 - PER * (int)threadIdx.x;
+  unsigned long long own[PER], run = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) run += own[i] = high - i >= 0 ? amount(high - i) : 0;
+  const unsigned long long mine = run;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned long long other = __shfl_up(run, o);
+    if (lane >= o) run += other;
+  }
+  if (lane == 63) s.part[wave] = run;
+  __syncthreads();
+  unsigned long long before[WAVES], total = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) before[w] = s.part[w];
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) {
+    run += w < wave ? before[w] : 0;
+    total += before[w];
+  }
+  if (target == 0) target = goal(total);
+  if (target > total) target = total;  // fewer numbers than top_k
+  if (run - mine < target && run >= target) {
+    unsigned long long above = run - mine;
+    int i = 0;
+#pragma unroll
+    for (int n = 0; n < PER - 1; n++)
+      if (i == n && above + own[n] < target) above += own[n], i = n + 1;
+    s.found[0] = high - i, s.found[1] = above, s.found[3] = target;
   }
   __syncthreads();
 }
@@ -280,8 +346,8 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       else held3[at] = w[i];
     }
   }
-  // f(step, logits) for every step; those not held are loaded one step ahead
-  auto each = [&](auto f) {
+  // f(step, words) for every step; those not held are loaded one step ahead
+  auto each_word = [&](auto f) {
     uint32_t next[4] = {0u, 0u, 0u, 0u};
 #pragma nounroll
     for (int step = 0; step < steps; step++) {
@@ -293,10 +359,15 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       else if (step < HELD) w[0] = held3[i], w[1] = held3[i + 1], w[2] = held3[i + 2], w[3] = held3[i + 3];
       else w[0] = next[0], w[1] = next[1], w[2] = next[2], w[3] = next[3];
       if (step + 1 >= HELD && step + 1 < steps) load(step + 1, next);
+      f(step, w);
+    }
+  };
+  auto each = [&](auto f) {  // f(step, logits)
+    each_word([&](int step, const uint32_t (&w)[4]) {
       float v[E];
       unpack(w, v);
       f(step, v);
-    }
+    });
   };
 
   // ---- the largest logit
@@ -351,9 +422,9 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   auto units = [&](double w) -> unsigned long long {  // w unit, rounded: at most 2^45
     return (unsigned long long)__double_as_longlong(fma(w, unit, 4503599627370496.0)) & 0xfffffffffffffull;
   };
-  // the smallest logits that weigh something (2^-1000 and min_p), and anything in a bin
+  // the smallest logits that weigh something (2^-100 and min_p), and anything in a bin
   if (wave == 0) {
-    const float least = least_of(top, [&](float l) { return weigh.behind(l) < 32000.0 && !(weigh(l) < min_p); });
+    const float least = least_of(top, [&](float l) { return weigh.behind(l) < 3200.0 && !(weigh(l) < min_p); });
     if (lane == 0) s.bound[0] = least;
   } else if (wave == 1) {
     const float least = least_of(top, [&](float l) { return weigh.behind(l) < 32.0 * (a.fraction + 1); });
@@ -375,7 +446,91 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
     const unsigned long long least = wanted < 1.0 ? 1ull : (unsigned long long)wanted;
     return least < total ? least : total;
   };
-  if (by_count) {
+  // bf16: the logits of each number are counted, and the threshold is a number
+  bool counted = false;
+  Window window = {1};
+  if constexpr (E == 8) {
+    const uint32_t widest = __float_as_uint(fmaxf(fabsf(top), fabsf(lightest))) >> 23 & 0xff;
+    window.lo = (int)(widest < 20 ? 1 : (widest - 19) << 7);
+    if (!infinite && (by_count || by_mass)) {
+      for (int i = tid; i < ENTRIES; i += THREADS) s.numbers[i] = 0;
+      __syncthreads();
+      each_word([&](int, const uint32_t (&w)[4]) {
+        uint32_t small = 0;
+        s16x2 at[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[i] = window.entries(w[i], small);
+#pragma unroll
+        for (int i = 0; i < 4; i++) atomicAdd(&s.numbers[at[i][0]], 1u), atomicAdd(&s.numbers[at[i][1]], 1u);
+        if (!__any(small & 0x80008000u)) return;
+        float v[E];  // those below the window one by one into the list
+        unpack(w, v);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const bool in = (at[e >> 1][e & 1] == MAGNITUDES + 1 || at[e >> 1][e & 1] == MAGNITUDES + 2) && v[e] == v[e];
+          const unsigned long long lanes = __ballot(in);
+          if (!lanes) continue;
+          uint32_t place = 0;
+          if (lane == 0) place = atomicAdd(&s.listed, (uint32_t)__popcll(lanes));
+          place = __shfl(place, 0) + (uint32_t)__popcll(lanes & ((1ull << lane) - 1));
+          if (in && place < LIST) s.list[place] = v[e];
+        }
+      });
+      __syncthreads();
+      const int smaller = (int)s.listed;
+      counted = smaller <= LIST;
+      int entry = 0;
+      if (counted && by_count) {
+        // (a NaN's sign may put it above the window: it is no number)
+        find_entry(s, [&](int i) -> unsigned long long { return i < ENTRIES - 1 ? s.numbers[i] : 0; },
+                   (unsigned long long)top_k, [](unsigned long long n) { return n; });
+        entry = (int)s.found[0];
+        counted = window.holds(entry);
+        tied = s.numbers[entry];
+        keep = (unsigned long long)top_k - s.found[1];
+        if (keep > tied) keep = tied;
+        threshold = window.value(entry);
+      }
+      if (counted && by_mass) {
+        // the weights of the numbers below the window, as one sum
+        unsigned long long sum = 0;
+        for (int i = tid; i < smaller; i += THREADS) sum += s.list[i] >= binned ? units(weigh(s.list[i])) : 0;
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        __syncthreads();
+        if (lane == 0) s.part[wave] = sum;
+        __syncthreads();
+        sum = 0;
+        for (int w = 0; w < WAVES; w++) sum += s.part[w];
+        __syncthreads();
+        const int first = entry;
+        const unsigned long long kept_there = keep;
+        find_entry(s, [&](int i) -> unsigned long long {
+          if (i < first) return 0;
+          if (i == MAGNITUDES + 2) return sum;
+          if (!window.holds(i)) return 0;
+          const float l = window.value(i);
+          const unsigned long long n = by_count && i == first ? kept_there : s.numbers[i];
+          return n && l >= binned ? n * units(weigh(l)) : 0;
+        }, 0, target_of);
+        entry = (int)s.found[0];
+        counted = window.holds(entry);
+        if (counted) {
+          threshold = window.value(entry);
+          const unsigned long long one = units(weigh(threshold));
+          keep = (s.found[3] - s.found[1] + one - 1) / one;
+          tied = s.numbers[entry];
+        }
+      }
+      __syncthreads();
+      if (!counted) {  // it lies below the window (or too many do): found as fp32's is
+        if (tid == 0) s.listed = 0;
+        threshold = -INFINITY, keep = tied = 0;
+        __syncthreads();
+      }
+    }
+  }
+  if (by_count && !counted) {
     // a bound that top_k logits reach: one that as many threads' maxima do
     if (a.vocab > LIST && top_k <= THREADS) {
       s.list[tid] = largest[0];
@@ -399,7 +554,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       __syncthreads();
       low = s.bound[2];
     }
-  } else if (by_mass) {
+  } else if (by_mass && !counted) {
     for (int i = tid; i < BINS; i += THREADS) s.masses[i] = 0;
     __syncthreads();
     each([&](int, const float (&v)[E]) {
@@ -426,7 +581,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
     low = fmaxf(s.bound[2], binned), high = s.bound[3], open = bin == 0;
   }
   // these logits into the list, if they fit
-  if (by_count ? a.vocab <= LIST || top_k <= THREADS : by_mass) {
+  if (!counted && (by_count ? a.vocab <= LIST || top_k <= THREADS : by_mass)) {
     const float end = open ? INFINITY : high;  // (no logit here is +inf)
     each([&](int, const float (&v)[E]) {
       bool some = false;
@@ -498,7 +653,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       threshold = __uint_as_float((uint32_t)s.found[0]);
       keep = s.found[1], tied = s.found[2];
     }
-  } else if (by_count || by_mass) {
+  } else if (!counted && (by_count || by_mass)) {
     if (by_count) {
       unsigned long long above, wanted = 0;
       auto goal = [&](unsigned long long n) { return (unsigned long long)top_k < n ? (unsigned long long)top_k : n; };
@@ -581,16 +736,64 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   };
 
   // ---- their sums, step by step and wave by wave (the order of indices)
-  each([&](int step, const float (&v)[E]) {
-    double w[E], sum = 0.0;
-    if (kept(step, v, w)) {
+  if (E == 8 && !infinite) {
+    if constexpr (E == 8) {
+      // weights from the table, 0 for what is not kept; tokens on a cut threshold, and those below the window,
+      // one by one
+      for (int i = tid; i < ENTRIES; i += THREADS) {
+        double x = 0.0;
+        if (window.holds(i)) {
+          const float l = window.value(i);
+          if (l >= threshold && l <= top && !(cut && l == threshold)) x = weigh(l);
+        }
+        s.table[i] = x;
+      }
+      __syncthreads();
+      each_word([&](int step, const uint32_t (&w)[4]) {
+        uint32_t small = 0;
+        s16x2 at[4];
 #pragma unroll
-      for (int e = 0; e < E; e++) sum += w[e];
+        for (int i = 0; i < 4; i++) at[i] = window.entries(w[i], small);
+        double x[E], sum = 0.0;
 #pragma unroll
-      for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        for (int e = 0; e < E; e++) x[e] = s.table[at[e >> 1][e & 1]];
+#pragma unroll
+        for (int e = 0; e < E; e++) sum += x[e];
+        float v[E];
+        if (cut || __any(small & 0x80008000u)) {
+          unpack(w, v);
+          bool some = false;
+#pragma unroll
+          for (int e = 0; e < E; e++) some |= v[e] >= threshold && !window.holds(at[e >> 1][e & 1]);
+          if (cut) {
+#pragma unroll
+            for (int e = 0; e < E; e++) some |= v[e] == threshold;
+          }
+          if (__any(some)) {
+            double y[E];
+            kept(step, v, y);
+            sum = 0.0;
+#pragma unroll
+            for (int e = 0; e < E; e++) sum += y[e];
+          }
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        if (lane == 0) s.sums[step * WAVES + wave] = sum;
+      });
     }
-    if (lane == 0) s.sums[step * WAVES + wave] = sum;
-  });
+  } else {
+    each([&](int step, const float (&v)[E]) {
+      double w[E], sum = 0.0;
+      if (kept(step, v, w)) {
+#pragma unroll
+        for (int e = 0; e < E; e++) sum += w[e];
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+      }
+      if (lane == 0) s.sums[step * WAVES + wave] = sum;
+    });
+  }
   __syncthreads();
   if (wave == 0) {
     double before = 0.0;

@@ -130,6 +130,27 @@ def test_rows_without_a_finite_logit(dtype, setting):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [300, 9000])
+def test_magnitudes_of_every_size(dtype, vocab):
+    """Logits around zero of magnitudes far apart, where a cut may lie among the
+    smallest; a wide and a narrow temperature; NaN of both signs."""
+    rng = np.random.default_rng(vocab)
+    tiny = rng.choice([-1.0, 1.0], (4, vocab)) * 2.0 ** rng.integers(-40, 4, (4, vocab))
+    tiny[:, rng.random(vocab) < 0.1] = 0.0
+    tiny[1] = np.where(rng.random(vocab) < 0.5, -np.abs(tiny[1]), -0.0)  # the largest is zero
+    tiny[2] *= 2.0 ** -60  # all of them next to nothing
+    tiny[3, rng.random(vocab) < 0.2] = -np.inf
+    for setting in (dict(), dict(top_k=vocab // 2), dict(top_p=0.5), dict(top_k=vocab // 2, top_p=0.7), dict(min_p=0.9),
+                    dict(temperature=0.01, top_p=0.6), dict(temperature=300.0, top_k=vocab // 3), dict(top_k=vocab - 1)):
+        check(tiny, rng.random(4), dtype, **setting)
+    broken = rng.standard_normal((2, vocab))
+    broken[:, ::3] = np.nan
+    broken[:, 1::6] = np.copysign(np.nan, -1.0)
+    for setting in (dict(), dict(top_k=5), dict(top_k=vocab - 3, top_p=0.9), dict(top_p=0.4)):
+        check(broken, rng.random(2), dtype, **setting)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("vocab", [50, 32768, 100001])
 def test_parameters_of_every_row(dtype, vocab):
     rng = np.random.default_rng(vocab)
