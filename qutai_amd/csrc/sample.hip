@@ -683,123 +683,126 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   }
   if (threshold < lightest) threshold = lightest, keep = tied = 0;
 
-  // ---- where tokens on the threshold are left out: how many lie before each step's wave
+  // Where tokens on the threshold are left out (`cut`), a step's wave sums the weights above it and counts those
+  // on it; what it keeps of them follows from the counts before it.
   const bool cut = keep < tied;
   const int slots = steps * WAVES;
-  if (cut) {
-    each([&](int step, const float (&v)[E]) {
-      int n = 0;
-#pragma unroll
-      for (int e = 0; e < E; e++) n += __popcll(__ballot(v[e] == threshold));
-      if (lane == 0) s.ties[step * WAVES + wave] = n;
-    });
-    __syncthreads();
-    if (wave == 0) {
-      uint32_t before = 0;
-      for (int i0 = 0; i0 < slots; i0 += 64) {
-        const uint32_t n = i0 + lane < slots ? s.ties[i0 + lane] : 0;
-        uint32_t run = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const uint32_t other = __shfl_up(run, o);
-          if (lane >= o) run += other;
-        }
-        if (i0 + lane < slots) s.ties[i0 + lane] = before + run - n;
-        before += __shfl(run, 63);
-      }
-    }
-  }
+  const double edge = cut ? weigh(threshold) : 0.0;
   __syncthreads();
 
-  // the weights of this thread's tokens of a step, 0 where they are not kept; false where the wave keeps none
-  auto kept = [&](int step, const float (&v)[E], double (&w)[E]) -> bool {
+  // the weights of this thread's tokens of a step above the threshold (and on it, where none is cut), 0 for others,
+  // and how many of the wave's lie on a cut one; false where there are neither
+  auto kept = [&](const float (&v)[E], double (&w)[E], uint32_t& on) -> bool {
     float most = v[0];
 #pragma unroll
     for (int e = 1; e < E; e++) most = fmaxf(most, v[e]);
     if (!__any(most >= threshold)) return false;
-    uint32_t in = 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) in |= v[e] >= threshold ? 1u << e : 0u;
     if (cut) {
-      unsigned long long rank = s.ties[step * WAVES + wave];
 #pragma unroll
-      for (int e = 0; e < E; e++) rank += __popcll(__ballot(v[e] == threshold) & ((1ull << lane) - 1));
-#pragma unroll
-      for (int e = 0; e < E; e++)
-        if (v[e] == threshold && rank++ >= keep) in &= ~(1u << e);
+      for (int e = 0; e < E; e++) on += (uint32_t)__popcll(__ballot(v[e] == threshold));
     }
 #pragma unroll
     for (int e = 0; e < E; e++) w[e] = weigh(v[e]);
 #pragma unroll
-    for (int e = 0; e < E; e++) w[e] = in >> e & 1 ? w[e] : 0.0;
+    for (int e = 0; e < E; e++) w[e] = (cut ? v[e] > threshold : v[e] >= threshold) ? w[e] : 0.0;
     return true;
   };
 
   // ---- their sums, step by step and wave by wave (the order of indices)
   if (E == 8 && !infinite) {
     if constexpr (E == 8) {
-      // weights from the table, 0 for what is not kept; tokens on a cut threshold, and those below the window,
-      // one by one
+      // weights from the table, 0 for what is not kept; tokens below the window one by one
       for (int i = tid; i < ENTRIES; i += THREADS) {
         double x = 0.0;
         if (window.holds(i)) {
           const float l = window.value(i);
-          if (l >= threshold && l <= top && !(cut && l == threshold)) x = weigh(l);
+          if ((cut ? l > threshold : l >= threshold) && l <= top) x = weigh(l);
         }
         s.table[i] = x;
       }
+      // the entry below which nothing is kept (a threshold that is no bf16 is cut towards 0; the zeros are equal)
+      uint32_t unused = 0;
+      const int entry = window.entries(__float_as_uint(threshold) >> 16, unused)[0];
+      const int least = entry == MAGNITUDES + 2 ? MAGNITUDES + 1 : entry;
+      const s16x2 edges = {(short)entry, (short)entry};
       __syncthreads();
       each_word([&](int step, const uint32_t (&w)[4]) {
-        uint32_t small = 0;
+        uint32_t small = 0, on = 0;
         s16x2 at[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) at[i] = window.entries(w[i], small);
-        double x[E], sum = 0.0;
+        s16x2 most = __builtin_elementwise_max(__builtin_elementwise_max(at[0], at[1]), __builtin_elementwise_max(at[2], at[3]));
+        double sum = 0.0;
+        if (__any(most[0] >= least || most[1] >= least)) {
+          if (__any(small & 0x80008000u)) {
+            float v[E];
+            double x[E];
+            unpack(w, v);
+            if (kept(v, x, on)) {
 #pragma unroll
-        for (int e = 0; e < E; e++) x[e] = s.table[at[e >> 1][e & 1]];
+              for (int e = 0; e < E; e++) sum += x[e];
+            }
+          } else {
+            double x[E];
 #pragma unroll
-        for (int e = 0; e < E; e++) sum += x[e];
-        float v[E];
-        if (cut || __any(small & 0x80008000u)) {
-          unpack(w, v);
-          bool some = false;
+            for (int e = 0; e < E; e++) x[e] = at[e >> 1][e & 1] >= least ? s.table[at[e >> 1][e & 1]] : 0.0;
 #pragma unroll
-          for (int e = 0; e < E; e++) some |= v[e] >= threshold && !window.holds(at[e >> 1][e & 1]);
-          if (cut) {
+            for (int e = 0; e < E; e++) sum += x[e];
+            if (cut) {  // (the threshold is a number of the window, or the list gave it)
+              uint32_t none = 0xffffffffu;
 #pragma unroll
-            for (int e = 0; e < E; e++) some |= v[e] == threshold;
+              for (int i = 0; i < 4; i++) {
+                const uint32_t apart = __builtin_bit_cast(uint32_t, at[i] ^ edges);
+                none &= ((apart & 0x7fff7fffu) + 0x7fff7fffu) | apart;
+              }
+              if (__any((none & 0x80008000u) != 0x80008000u)) {
+                float v[E];
+                unpack(w, v);
+#pragma unroll
+                for (int e = 0; e < E; e++) on += (uint32_t)__popcll(__ballot(v[e] == threshold));
+              }
+            }
           }
-          if (__any(some)) {
-            double y[E];
-            kept(step, v, y);
-            sum = 0.0;
 #pragma unroll
-            for (int e = 0; e < E; e++) sum += y[e];
-          }
+          for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
         }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-        if (lane == 0) s.sums[step * WAVES + wave] = sum;
+        if (lane == 0) s.sums[step * WAVES + wave] = sum, s.ties[step * WAVES + wave] = on;
       });
     }
   } else {
     each([&](int step, const float (&v)[E]) {
       double w[E], sum = 0.0;
-      if (kept(step, v, w)) {
+      uint32_t on = 0;
+      if (kept(v, w, on)) {
 #pragma unroll
         for (int e = 0; e < E; e++) sum += w[e];
 #pragma unroll
         for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
       }
-      if (lane == 0) s.sums[step * WAVES + wave] = sum;
+      if (lane == 0) s.sums[step * WAVES + wave] = sum, s.ties[step * WAVES + wave] = on;
     });
   }
   __syncthreads();
   if (wave == 0) {
     double before = 0.0;
+    uint32_t ahead = 0;
     unsigned long long adds = 0;  // bit i0 / 64: this lane's sum there is not zero
     for (int i0 = 0; i0 < slots; i0 += 64) {
-      double run = i0 + lane < slots ? s.sums[i0 + lane] : 0.0;
+      const bool in = i0 + lane < slots;
+      double run = in ? s.sums[i0 + lane] : 0.0;
+      if (cut) {  // and the first `keep` of the tokens on the threshold
+        const uint32_t n = in ? s.ties[i0 + lane] : 0;
+        uint32_t count = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const uint32_t other = __shfl_up(count, o);
+          if (lane >= o) count += other;
+        }
+        const uint32_t first = ahead + count - n;
+        ahead += __shfl(count, 63);
+        if (in) s.ties[i0 + lane] = first;
+        if (first < keep) run += (double)(keep - first < n ? (uint32_t)keep - first : n) * edge;
+      }
       if (run > 0.0) adds |= 1ull << (i0 / 64);
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -807,7 +810,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
         if (lane >= o) run += other;
       }
       run += before;
-      if (i0 + lane < slots) s.sums[i0 + lane] = run;
+      if (in) s.sums[i0 + lane] = run;
       before = __shfl(run, 63);
     }
     // the first step and wave whose running sum exceeds u times the whole sum; else the last with a kept token
@@ -842,7 +845,16 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
     load(chosen / WAVES, words);
     float v[E];
     unpack(words, v);
-    kept(chosen / WAVES, v, w);
+    uint32_t on = 0;
+    if (!kept(v, w, on)) return;
+    if (cut) {
+      unsigned long long rank = s.ties[chosen];
+#pragma unroll
+      for (int e = 0; e < E; e++) rank += __popcll(__ballot(v[e] == threshold) & ((1ull << lane) - 1));
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (v[e] == threshold && rank++ < keep) w[e] = edge;
+    }
   }
 #pragma unroll
   for (int e = 0; e < E; e++) sum += w[e];
