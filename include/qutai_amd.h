@@ -450,7 +450,10 @@ int64_t qutai_amd_qk_norm_rope_workspace(int64_t dim);
  * largest logit, the lowest index of equal ones, with probability 1.  A NaN
  * counts as -inf; a row of nothing else gives token -1 with probability 0; beside
  * +inf every finite logit weighs nothing.  Weights and their sums are 64-bit.
- * Each parameter is one number, or where its pointer is not NULL one per row. */
+ * Each parameter is one number, or where its pointer is not NULL one per row
+ * (there a temperature that is not above 0 counts as 0, a top_k below 1, a top_p
+ * of 1 and more and a min_p below 0 as no filter, a min_p above 1 as 1).  A token
+ * that weighs less than 2^-100 of the largest is never taken. */
 int qutai_amd_sample(const void* logits, const void* uniforms, int64_t* tokens, float* probabilities, int64_t rows,
                      int64_t vocab, const float* temperatures, double temperature, const int64_t* top_ks,
                      int64_t top_k, const float* top_ps, double top_p, const float* min_ps, double min_p, int dtype,

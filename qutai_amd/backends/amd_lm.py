@@ -542,7 +542,8 @@ class QuantizedCache:
     """Device memory of a quantised key and value cache: codes of 8 bits (a
     scale per row) or 4 bits (a scale per 32 channels) for ``capacity``
     positions (rounded up to whole blocks of 32) of each (sequence, kv head),
-    laid out by the library (qutai_amd_cache_quantize)."""
+    laid out by the library (qutai_amd_cache_quantize), and the workspace of the
+    attention over it."""
 
     def __init__(self, batch, kv_heads, dim, capacity, bits):
         if bits not in (8, 4):
@@ -556,6 +557,7 @@ class QuantizedCache:
         # codes are raw bytes: eight to a word (a row has 16 at least)
         self.key_codes, self.value_codes = (AMDStorage(rows * pitch * bits // 64, "int64") for _ in range(2))
         self.key_scales, self.value_scales = (AMDStorage(rows * scales, "bfloat16") for _ in range(2))
+        self.workspace = AMDStorage(0, "float32")
 
 
 def _cache_positions(cache, *arrays):
@@ -622,14 +624,14 @@ def attention_quantized(cache, q, new, heads, *, start=0, starts=None, counts=No
     scale = cache.dim ** -0.5 if scale is None else scale
     out = AMDStorage(q.size, q.dtype)
     if q.size:
-        runtime = out.runtime
-        need = runtime.lib.qutai_amd_attention_quantized_workspace_size(cache.batch, new, heads, cache.kv_heads,
-                                                                        cache.dim, longest, code(q.dtype))
-        workspace = AMDStorage((need + 3) // 4, "float32") if need else None
+        runtime, dtype = out.runtime, code(q.dtype)
+        need = runtime.attention_workspace(cache.batch, new, heads, cache.kv_heads, cache.dim, longest, dtype)
+        if need > cache.workspace.nbytes:
+            cache.workspace = AMDStorage((need + 3) // 4, "float32")
         runtime.call("qutai_amd_attention_quantized", q.ptr, cache.key_codes.ptr, cache.key_scales.ptr,
                      cache.value_codes.ptr, cache.value_scales.ptr, out.ptr, amd._p(starts), amd._p(counts), start,
                      cache.batch, new, heads, cache.kv_heads, cache.dim, cache.capacity, longest, cache.bits,
-                     code(q.dtype), float(scale), amd._p(workspace), need)
+                     dtype, float(scale), cache.workspace.ptr, need)
     return out
 
 

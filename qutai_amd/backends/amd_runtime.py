@@ -167,6 +167,7 @@ class Runtime:
         self.lib = load_library()
         self._functions = {name: getattr(self.lib, name) for name in SIGNATURES}
         self._gemm_workspaces = {}  # shape and types of a product -> workspace bytes
+        self._attention_workspaces = {}  # the same of attention over a quantised cache
         self._check(self._init(0), "hipInit")
         count = ctypes.c_int()
         self._check(self._device_count(ctypes.byref(count)), "hipGetDeviceCount")
@@ -408,6 +409,18 @@ class Runtime:
             if len(self._gemm_workspaces) >= 4096:
                 self._gemm_workspaces.clear()
             need = self._gemm_workspaces[key] = self.lib.qutai_amd_gemm_workspace_size(*shape)
+        return need
+
+    def attention_workspace(self, batch, fresh, heads, kv_heads, dim, longest, dtype):
+        """qutai_amd_attention_quantized_workspace_size, asked once for each plan:
+        the longest sequence counts in blocks of 128 positions."""
+        key = (batch, fresh, heads, kv_heads, dim, (longest + 127) // 128, dtype)
+        need = self._attention_workspaces.get(key)
+        if need is None:
+            if len(self._attention_workspaces) >= 4096:
+                self._attention_workspaces.clear()
+            need = self._attention_workspaces[key] = self.lib.qutai_amd_attention_quantized_workspace_size(
+                batch, fresh, heads, kv_heads, dim, longest, dtype)
         return need
 
     # ---- events (timing on the default stream) ---------------------------------

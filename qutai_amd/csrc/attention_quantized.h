@@ -213,7 +213,8 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   const int total = (int)gridDim.x, id = a.tiles > 1 ? xcd_remap(blockIdx.x, total) : (int)blockIdx.x;
   const int split = id % a.splits, tile = id / a.splits % a.tiles;
   const int64_t unit = id / a.splits / a.tiles, b = unit / a.kv_heads, head = unit % a.kv_heads;
-  const int64_t count = a.counts ? a.counts[b] : a.fresh, first = a.start + (a.starts ? a.starts[b] : 0);
+  const int64_t given = a.counts ? a.counts[b] : a.fresh, count = given < a.fresh ? given : a.fresh;
+  const int64_t first = a.start + (a.starts ? a.starts[b] : 0);
   const int64_t rows = a.fresh * a.group, row0 = (int64_t)tile * (ROWS * TILE);
   // the keys that a row sees; none where it is not a query
   auto sees = [&](int64_t row) -> int {

@@ -269,6 +269,39 @@ def test_large_scores_and_scales():
     check_attention(out, q, *read(cache), (89,), (1,), 32 ** -0.5, "float32")
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+def test_rows_beyond_four_gigabytes(bits):
+    """The last heads' codes lie behind the 32-bit offsets."""
+    rng = np.random.default_rng(10)
+    heads, capacity = (66, 1 << 18) if bits == 8 else (132, 1 << 18)
+    cache = QuantizedKVCache(capacity, bits=bits)
+    k, v = (stored(rng.standard_normal((1, 3, heads, 256)), "bfloat16") for _ in range(2))
+    cache.append(as_tensor(k[:, :2], "bfloat16"), as_tensor(v[:, :2], "bfloat16"))
+    cache.append(as_tensor(k[:, 2:], "bfloat16"), as_tensor(v[:, 2:], "bfloat16"))
+    assert cache.codes.key_codes.nbytes > 1 << 32
+    for got, x in zip(read(cache), (k, v)):
+        assert np.array_equal(got, held(x, bits).transpose(0, 2, 1, 3))
+    q = stored(rng.standard_normal((1, 1, heads, 256)), "bfloat16")
+    out = download(cache.attend(as_tensor(q, "bfloat16")).storage).reshape(q.shape)
+    check_attention(out, q, *read(cache), (2,), (1,), 1 / 16, "bfloat16", bits)
+
+
+def test_no_new_positions_and_counts_of_the_library():
+    """An append of nothing; counts above the new positions and below none, as the
+    library's callers may pass them."""
+    rng = np.random.default_rng(14)
+    cache = QuantizedKVCache(40)
+    k, v = (stored(rng.standard_normal((3, 6, 2, 32)), "float32") for _ in range(2))
+    cache.append(as_tensor(k, "float32"), as_tensor(v, "float32"))
+    empty = Tensor(amd.AMDStorage(0, "float32"), shape=(3, 0, 2, 32))
+    cache.append(empty, empty)
+    assert cache.lengths == (6, 6, 6) and cache.attend(empty).shape == (3, 0, 2, 32)
+    q = stored(rng.standard_normal((3, 6, 4, 32)), "float32")
+    counts = amd.storage([1 << 62, -(1 << 62), 4], dtype="int64")
+    out = amd_lm.attention_quantized(cache.codes, upload(q, "float32"), 6, 4, counts=counts, longest=6)
+    check_attention(download(out).reshape(q.shape), q, *read(cache), (0, 0, 0), (6, 0, 4), 32 ** -0.5, "float32")
+
+
 def test_the_same_call_gives_the_same_bits():
     rng = np.random.default_rng(3)
     cache = QuantizedKVCache(4000)

@@ -236,3 +236,19 @@ def test_decoder_trains_with_normed_heads(cast):
         # each loss (about 5) is rounded to some 20 units of fp32: 6e-6 of slope here is 2 * 20 * 5 * 2^-24 / 0.04 = 3e-4;
         # the cubic term of a step of 2 % is of the order of 1e-3 of the slope
         assert abs(slope - expected) <= 3e-4 + 0.01 * expected
+
+
+def test_checkpoint_keeps_the_norms(tmp_path):
+    """A decoder with normed heads saved and loaded; one without refuses its files."""
+    from qutai_amd.lm import load_checkpoint, save_checkpoint
+
+    sizes = dict(vocab_size=40, n_layers=1, d_model=16, n_heads=2, n_kv_heads=1, d_ff=24, max_seq_len=8)
+    model, other = (Decoder(Config(**sizes, qk_norm=True), seed=s) for s in (1, 2))
+    weights = dict(model.named_parameters())
+    amd.copy_into(weights["blocks.0.attn.q_norm.weight"].storage, upload(np.arange(8) + 0.5, "float32"))
+    save_checkpoint(tmp_path / "saved", model)
+    load_checkpoint(tmp_path / "saved", other)
+    for name, p in other.named_parameters():
+        assert p.storage.to_array() == weights[name].storage.to_array(), name
+    with pytest.raises(ValueError):
+        load_checkpoint(tmp_path / "saved", Decoder(Config(**sizes), seed=3))
