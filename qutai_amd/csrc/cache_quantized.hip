@@ -1,6 +1,9 @@
 // A key and value cache quantised as it is written, and read back: C ABI
 // `qutai_amd_cache_quantize`, `qutai_amd_cache_dequantize` (the codes and their
-// layout: cache_codes.h).
+// layout: cache_codes.h).  Bound by HBM: 4 x 4000 positions of 8 heads of 128, keys
+// and values, bf16 to 8 bits: 24 us to write (98 MB, 4.1 TB/s; four channels per
+// lane and 64-bit row arithmetic 57), 16 us to read back (6.2 TB/s; 44 in two
+// launches of four channels per lane).
 #include "cache_codes.h"
 #include "qutai_amd.h"
 

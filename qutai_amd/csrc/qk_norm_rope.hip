@@ -11,6 +11,10 @@
 // An angle is p times its frequency in turns, in 64 bits, less its nearest
 // whole number; only the rest, at most half a turn, becomes fp32.  Squares,
 // products and sums are fp32; a result is rounded once.
+//
+// Bound by HBM.  32 x 1024 positions of 16 + 4 heads of 64, bf16: forward 34 us
+// for 168 MB (4.9 TB/s, a large copy's rate), backward 55 us for 252 MB, weight
+// sums 5 us; a wave per row (qk_rows) took 249, 425 and 17.
 #include "common.h"
 #include "qutai_amd.h"
 

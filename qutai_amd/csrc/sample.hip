@@ -20,8 +20,16 @@
 //  (weight times 2^45, or less for very large vocabularies): exact in any order.
 //  The logits of the bin that the prefix ends in go into the list.
 // A list is searched digit by digit of its keys (bits in an order of unsigned
-// integers), from histograms.  Where it overflows (thousands of equal or nearly
-// equal logits, or a large k) the whole row is.
+// integers), from histograms, a short one by comparing all with all.  Where it
+// overflows (thousands of equal or nearly equal logits, or a large k) the whole row
+// is searched.
+// bf16 logits are counted by number instead: see Window.  Their weights are then a
+// table, too.
+//
+// Bound by vector operations: one on each of a CU's 131072 logits takes 1.2 us, a
+// weight some 20 of them.  200 rows of 131072 bf16 logits: 25 us for the largest
+// alone, 52 without a filter, 52 with top_k 50, 71 with top_p .9 (passes over memory
+// with a sorted digit search: 248); a row of 32768 fp32 logits with both: 29 us.
 #include "common.h"
 #include "qutai_amd.h"
 
