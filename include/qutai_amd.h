@@ -511,7 +511,7 @@ int qutai_amd_cache_dequantize(const void* key_codes, const void* key_scales, co
  * qutai_amd_attention_quantized_workspace_size bytes; too small a one is
  * QA_EWORKSPACE.  capacity is a multiple of 32 (at most 2^30; what lies behind a
  * sequence's last position may be anything), the scales are 4-byte aligned;
- * batch x fresh x heads at most 2^25. */
+ * batch x fresh x heads at most 2^25; scale lies between 1e-30 and 1e30. */
 int qutai_amd_attention_quantized(const void* q, const void* key_codes, const void* key_scales,
                                   const void* value_codes, const void* value_scales, void* out, const int64_t* starts,
                                   const int64_t* counts, int64_t start, int64_t batch, int64_t fresh, int64_t heads,

@@ -53,7 +53,7 @@ extern "C" int qutai_amd_attention_quantized(const void* q, const void* key_code
                                              void* workspace, size_t workspace_bytes, void* stream_) {
   if (!sizes_ok(batch, fresh, heads, kv_heads, dim, longest, dtype)) return QA_EINVAL;
   if (capacity <= 0 || capacity % 32 || capacity > (1ll << 30) || longest > capacity) return QA_EINVAL;
-  if ((bits != 8 && bits != 4) || !(scale > 0.0) || scale > 1e30) return QA_EINVAL;
+  if ((bits != 8 && bits != 4) || !(scale >= 1e-30) || scale > 1e30) return QA_EINVAL;
   if (start < -(1ll << 40) || start > (1ll << 40)) return QA_EINVAL;
   if (batch == 0 || fresh == 0) return QA_OK;
   if (capacity * kv_heads > (1ll << 44) / batch) return QA_EINVAL;

@@ -94,8 +94,8 @@ class QuantizedKVCache:
         return self._shift, self._stored
 
     def _per_sequence(self, values, most, what):
-        values = (values,) * len(self.lengths) if type(values) is int else tuple(values)
-        if len(values) != len(self.lengths) or any(type(n) is not int or not 0 <= n <= m for n, m in zip(values, most)):
+        values = (values,) * len(most) if type(values) is int else tuple(values)
+        if len(values) != len(most) or any(type(n) is not int or not 0 <= n <= m for n, m in zip(values, most)):
             raise ValueError(f"{what} is one integer per sequence (or one for all), within what there is")
         return values
 
@@ -120,11 +120,11 @@ class QuantizedKVCache:
         matrix (amd_lm.cache_quantize's key_column, key_row, value_column, value_row)."""
         if min(batch, kv_heads, dim) <= 0 or new < 0:
             raise ValueError("cached keys and values need one sequence, head and channel at least")
-        self.reserve(batch, kv_heads, dim)
         counts = (new,) * batch if counts is None else self._per_sequence(counts, (new,) * batch, "counts")
-        lengths = tuple(n + m for n, m in zip(self.lengths, counts))
+        lengths = tuple(n + m for n, m in zip(self.lengths or (0,) * batch, counts))
         if max(lengths) > self.capacity:
             raise ValueError("the cache's capacity is exceeded")
+        self.reserve(batch, kv_heads, dim)  # last: a refused call settles nothing
         start, starts = self.positions()
         held = None if min(counts) == new else amd.storage(counts, dtype="int64")
         amd_lm.cache_quantize(self.codes, keys, values, new, start=start, starts=starts, counts=held, **columns)

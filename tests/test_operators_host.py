@@ -190,6 +190,23 @@ def test_cache_entry_points_refuse():
     assert [pitch(d) for d in (0, 1, 32, 33, 80, 100, 129, 193, 256, 257)] == [0, 32, 32, 64, 96, 128, 192, 256, 256, 0]
 
 
+@built
+@pytest.mark.parametrize("scale", [1e-300, 9e-31, -1.0, 2e30])
+def test_attention_scales_that_fp32_does_not_hold_are_refused(scale):
+    # (below 1e-38 a masked score's -inf would be multiplied by zero)
+    library, p = amd_runtime.load_library(), FAKE
+    assert library.qutai_amd_attention_quantized(p, p, p, p, p, p, None, None, 3, 2, 3, 4, 2, 8, 32, 32, 8, 5, scale, p,
+                                                 1 << 30, None) == amd_runtime.QA_EINVAL
+
+
+@pytest.mark.parametrize("new, counts", [(5, None), (5, (5, 1)), (3, (1,)), (3, (4, 1)), (3, 4)])
+def test_a_refused_first_append_settles_nothing(new, counts):
+    cache = QuantizedKVCache(4)
+    with pytest.raises(ValueError):
+        cache.append_rows(None, None, 2, new, 4, 64, counts)
+    assert cache.codes is None and cache.lengths == () and cache.length == 0
+
+
 # ---- sampling ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("change", [
