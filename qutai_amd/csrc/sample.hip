@@ -28,8 +28,8 @@
 //
 // Bound by vector operations: one on each of a CU's 131072 logits takes 1.2 us, a
 // weight some 20 of them.  200 rows of 131072 bf16 logits: 25 us for the largest
-// alone, 52 without a filter, 52 with top_k 50, 71 with top_p .9 (passes over memory
-// with a sorted digit search: 248); a row of 32768 fp32 logits with both: 29 us.
+// alone, 45 without a filter, 48 with top_k 50, 64 with top_p .9 (passes over memory
+// with a sorted digit search: 248); a row of 32768 fp32 logits with both: 27 us.
 #include "common.h"
 #include "qutai_amd.h"
 
@@ -93,6 +93,40 @@ struct Shared {
   uint32_t listed;
   int chosen;
 };
+
+// Another lane's value by a data-parallel move (no trip through LDS): rows are of 16
+// lanes; 0 where the source is none, or where row_mask leaves the row out.
+template <int CTRL, int ROW_MASK = 0xf, class V>
+__device__ __forceinline__ V moved(V x) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, ROW_MASK, 0xf, true));
+  } else {
+    u32x2 w = __builtin_bit_cast(u32x2, x);
+#pragma unroll
+    for (int i = 0; i < 2; i++) w[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[i], CTRL, ROW_MASK, 0xf, true);
+    return __builtin_bit_cast(V, w);
+  }
+}
+// A running sum over a wave's lanes; the last lane has the whole (which is all that
+// `wave_sum` is for: its other lanes mean nothing).
+template <class V>
+__device__ __forceinline__ V wave_scan(V x) {
+  x += moved<0x111>(x);  // the lane 1, 2, 4 and 8 below, in its row
+  x += moved<0x112>(x);
+  x += moved<0x114>(x);
+  x += moved<0x118>(x);
+  x += moved<0x142, 0xa>(x);         // the last of the row below, for rows 1 and 3
+  return x + moved<0x143, 0xc>(x);  // lane 31, for rows 2 and 3
+}
+template <class V>
+__device__ __forceinline__ V wave_sum(V x) {
+  x += moved<0xB1>(x);   // lane ^ 1
+  x += moved<0x4E>(x);   // lane ^ 2
+  x += moved<0x141>(x);  // mirrored in 8 lanes, then in 16
+  x += moved<0x140>(x);
+  x += moved<0x142, 0xa>(x);
+  return x + moved<0x143, 0xc>(x);
+}
 
 // w = 2^(-t / 32), t = (top - l) 32 log2(e) / T: a table of 32 powers for the nearest
 // integer n of t, and for the rest, at most half, a polynomial of degree four (the
@@ -177,11 +211,7 @@ __device__ __forceinline__ void find_bin(Shared& s, const V* bins, unsigned long
 #pragma unroll
   for (int i = 0; i < PER; i++) run += own[i] = bins[high - i];
   const unsigned long long mine = run;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long other = __shfl_up(run, o);
-    if (lane >= o) run += other;
-  }
+  run = wave_scan(run);
   if (lane == 63) s.part[wave] = run;
   __syncthreads();
   unsigned long long before[WAVES];  // read together
@@ -213,11 +243,7 @@ __device__ __forceinline__ void find_entry(Shared& s, F amount, unsigned long lo
 #pragma unroll
   for (int i = 0; i < PER; i++) run += own[i] = high - i >= 0 ? amount(high - i) : 0;
   const unsigned long long mine = run;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned long long other = __shfl_up(run, o);
-    if (lane >= o) run += other;
-  }
+  run = wave_scan(run);
   if (lane == 63) s.part[wave] = run;
   __syncthreads();
   unsigned long long before[WAVES], total = 0;
@@ -247,9 +273,8 @@ __device__ __forceinline__ unsigned long long sum_bins(Shared& s, const V* bins)
   unsigned long long total = 0;
 #pragma unroll
   for (int i = 0; i < BINS / THREADS; i++) total += bins[threadIdx.x + i * THREADS];
-#pragma unroll
-  for (int o = 32; o; o >>= 1) total += __shfl_xor(total, o);
-  if (lane == 0) s.part[wave] = total;
+  total = wave_sum(total);
+  if (lane == 63) s.part[wave] = total;
   __syncthreads();
   total = 0;
 #pragma unroll
@@ -503,10 +528,9 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
         // the weights of the numbers below the window, as one sum
         unsigned long long sum = 0;
         for (int i = tid; i < smaller; i += THREADS) sum += s.list[i] >= binned ? units(weigh(s.list[i])) : 0;
-#pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        sum = wave_sum(sum);
         __syncthreads();
-        if (lane == 0) s.part[wave] = sum;
+        if (lane == 63) s.part[wave] = sum;
         __syncthreads();
         sum = 0;
         for (int w = 0; w < WAVES; w++) sum += s.part[w];
@@ -771,10 +795,9 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
               }
             }
           }
-#pragma unroll
-          for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+          sum = wave_sum(sum);
         }
-        if (lane == 0) s.sums[step * WAVES + wave] = sum, s.ties[step * WAVES + wave] = on;
+        if (lane == 63) s.sums[step * WAVES + wave] = sum, s.ties[step * WAVES + wave] = on;
       });
     }
   } else {
@@ -784,10 +807,9 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       if (kept(v, w, on)) {
 #pragma unroll
         for (int e = 0; e < E; e++) sum += w[e];
-#pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        sum = wave_sum(sum);
       }
-      if (lane == 0) s.sums[step * WAVES + wave] = sum, s.ties[step * WAVES + wave] = on;
+      if (lane == 63) s.sums[step * WAVES + wave] = sum, s.ties[step * WAVES + wave] = on;
     });
   }
   __syncthreads();
@@ -800,24 +822,14 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
       double run = in ? s.sums[i0 + lane] : 0.0;
       if (cut) {  // and the first `keep` of the tokens on the threshold
         const uint32_t n = in ? s.ties[i0 + lane] : 0;
-        uint32_t count = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const uint32_t other = __shfl_up(count, o);
-          if (lane >= o) count += other;
-        }
+        const uint32_t count = wave_scan(n);
         const uint32_t first = ahead + count - n;
         ahead += __shfl(count, 63);
         if (in) s.ties[i0 + lane] = first;
         if (first < keep) run += (double)(keep - first < n ? (uint32_t)keep - first : n) * edge;
       }
       if (run > 0.0) adds |= 1ull << (i0 / 64);
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double other = __shfl_up(run, o);
-        if (lane >= o) run += other;
-      }
-      run += before;
+      run = wave_scan(run) + before;
       if (in) s.sums[i0 + lane] = run;
       before = __shfl(run, 63);
     }
@@ -866,12 +878,7 @@ __global__ void __launch_bounds__(THREADS) sample_rows(SampleArgs a) {
   }
 #pragma unroll
   for (int e = 0; e < E; e++) sum += w[e];
-  double run = sum;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double other = __shfl_up(run, o);
-    if (lane >= o) run += other;
-  }
+  const double run = wave_scan(sum);
   const double base = chosen ? s.sums[chosen - 1] : 0.0;
   const unsigned long long past = __ballot(sum > 0.0 && base + run > goal), any = __ballot(sum > 0.0);
   const int owner = past ? __ffsll(past) - 1 : 63 - __clzll(any);
