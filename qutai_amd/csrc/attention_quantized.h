@@ -20,7 +20,11 @@
 // probabilities that bf16 does not hold are sums of parts: PARTS of them, two for
 // bf16 outputs (16 bits), three for fp32.  Where a tile has few rows (SPREAD > 1)
 // the columns hold each row SPREAD times, and the parts of its probabilities go
-// into these columns: one product instead of PARTS.
+// into these columns: one product instead of PARTS.  With four rows or fewer of two
+// parts (BLOCKS = 2) half of the columns belong to a second block of keys: zeros in
+// the operands keep the other block's products out, and what is done with the scores
+// and the probabilities is done for both blocks at once (16 sequences of up to 8000
+// keys, 4 bits: 43 us with one, 37 with two).
 //
 // The running maximum of a row is only raised when a score exceeds it by 2^8
 // (in powers of two): fp32 holds the sums all the same, and nearly every block
@@ -62,6 +66,10 @@ struct AttendPlan {
   int tile, spread, rows, pitch;  // row tiles of 16 columns, copies of a row, rows of a workgroup
   int64_t tiles, splits;
 };
+
+// Two tiles of such rows do not fit in registers (4 bits, bf16, 256 channels, 512 new positions over 3000: 324 us
+// with one, 490 with two; 8 bits 198 and 158).
+constexpr bool one_tile(int item, int bits, int pitch) { return item == 4 ? pitch > 128 : bits == 4 && pitch == 256; }
 
 template <class T> struct Parts;
 template <> struct Parts<bf16_t> { static constexpr int Q = 1, P = 2; };
@@ -205,7 +213,7 @@ template <class T> __device__ __forceinline__ float element(const T* p, int64_t 
 template <> __device__ __forceinline__ float element<float>(const float* p, int64_t i) { return p[i]; }
 template <> __device__ __forceinline__ float element<bf16_t>(const bf16_t* p, int64_t i) { return bf16_to_f32(p[i]); }
 
-template <class T, int BITS, int DP, int TILE, int SPREAD>
+template <class T, int BITS, int DP, int TILE, int SPREAD, int BLOCKS = 1>
 __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   constexpr int KW = DP * BITS / 128;                             // dwords of a lane's share of a key row
   constexpr int VW = (DP * BITS / 128 + 3) / 4 < 1 ? 1 : (DP * BITS / 128 + 3) / 4;  // of a value row
@@ -214,8 +222,12 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   constexpr int ROWS = 16 / SPREAD;                               // rows of a tile of 16 columns
   constexpr bool RAISED = BITS == 4 && sizeof(T) == 2;
   constexpr int ROW = DP * BITS / 8;                              // bytes of a row
-  static_assert(SPREAD == 1 || (TILE == 1 && SPREAD >= PP), "a row's parts need a column each");
+  constexpr int COPIES = SPREAD / BLOCKS, SIDE = 16 / BLOCKS;     // columns of a row and block, columns of a block
+  constexpr int QN = BLOCKS > 1 ? BLOCKS : QP;
+  static_assert(SPREAD == 1 || (TILE == 1 && COPIES >= PP), "a row's parts need a column each");
+  static_assert(BLOCKS == 1 || QP == 1, "the queries of the other block's columns are zero");
   const int lane = threadIdx.x & 63, wave = uniform32(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int side = r / SIDE, part = r / ROWS % COPIES;  // the column's block, and which part of a probability it holds
   const int total = (int)gridDim.x, id = a.tiles > 1 ? xcd_remap(blockIdx.x, total) : (int)blockIdx.x;
   const int split = id % a.splits, tile = id / a.splits % a.tiles;
   const int64_t unit = id / a.splits / a.tiles, b = unit / a.kv_heads, head = unit % a.kv_heads;
@@ -235,7 +247,7 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
   for (int i = 0; i < TILE; i++) limit[i] = sees(row0 + i * ROWS + r % ROWS);
 
   // ---- queries: the columns' rows, PARTS of each depth
-  bf16x8 q[TILE][KS][QP];
+  bf16x8 q[TILE][KS][QN];
 #pragma unroll
   for (int i = 0; i < TILE; i++) {
     const int64_t row = row0 + i * ROWS + r % ROWS, t = row / a.group;
@@ -254,7 +266,11 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
               if (d + e < a.dim) w[e >> 1] |= (uint32_t)p[d + e] << (16 * (e & 1));
           }
         }
-        q[i][k][0] = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+        for (int c = 0; c < QN; c++) {
+          const u32x4 none = {0u, 0u, 0u, 0u};
+          q[i][k][c] = __builtin_bit_cast(bf16x8, side == c ? w : none);
+        }
       } else {
         float v[8];
 #pragma unroll
@@ -272,9 +288,12 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
 #pragma unroll
     for (int i = 0; i < TILE; i++)
 #pragma unroll
-      for (int k = 0; k < KS; k++)
-        drop[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, raise), q[i][k][0],
-                                                             f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+      for (int k = 0; k < KS; k++) {
+        drop[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < QN; c++)
+          drop[i][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, raise), q[i][k][c], drop[i][k], 0, 0, 0);
+      }
   }
 
   f32x4 acc[TILE][NV];
@@ -286,42 +305,55 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
     for (int n = 0; n < NV; n++) acc[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // ---- this workgroup's keys, a block of 32 per wave at a time
-  const int share = ((end + a.splits - 1) / a.splits + BLOCK * WAVES - 1) / (BLOCK * WAVES) * (BLOCK * WAVES);
+  // ---- this workgroup's keys, BLOCKS blocks of 32 per wave at a time
+  constexpr int STEP = BLOCK * BLOCKS;
+  const int share = ((end + a.splits - 1) / a.splits + STEP * WAVES - 1) / (STEP * WAVES) * (STEP * WAVES);
   const int from = split * share, to = from + share < end ? from + share : end;
   const int64_t base = unit * a.capacity;
   const uint8_t* K = a.codes[0] + base * ROW;
   const uint8_t* V = a.codes[1] + base * ROW;
   const bf16_t* KSC = a.scales[0] + base * G;
   const bf16_t* VSC = a.scales[1] + base * G;
-  for (int s0 = from + wave * BLOCK; s0 < to; s0 += WAVES * BLOCK) {
-    uint32_t kw[2][KW], vw[8][VW], ks[2][2 * G], vs[2][2 * G];
-    const uint8_t* key_rows = K + (int64_t)s0 * ROW;
-    const uint8_t* value_rows = V + (int64_t)s0 * ROW;
+  for (int s0 = from + wave * STEP; s0 < to; s0 += WAVES * STEP) {
+    uint32_t kw[BLOCKS][2][KW], vw[BLOCKS][8][VW], ks[2][2 * G], vs[2][2 * G];
     const bf16_t* key_scales = KSC + (int64_t)s0 * G;
     const bf16_t* value_scales = VSC + (int64_t)s0 * G;
+    // the last block may stand alone: then it is taken twice, and no row sees the second's keys (end <= s0 + 32)
+    const bool both = s0 + BLOCK < to;
+    const int own = both ? BLOCK * side : 0;
+#pragma unroll
+    for (int c = 0; c < BLOCKS; c++) {
+      const uint8_t* key_rows = K + (int64_t)(s0 + (c && both ? BLOCK : 0)) * ROW;
+#pragma unroll
+      for (int u = 0; u < 2; u++) load_key<BITS, DP>(key_rows, (uint32_t)((16 * u + r) * ROW), g, kw[c][u]);
+    }
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      load_key<BITS, DP>(key_rows, (uint32_t)((16 * u + r) * ROW), g, kw[u]);
 #pragma unroll
       for (int n = 0; n < 2 * G; n++) {
-        ks[u][n] = global_load<uint32_t>(key_scales + (uint32_t)((16 * u + 4 * g) * G + 2 * n));
-        vs[u][n] = global_load<uint32_t>(value_scales + (uint32_t)((16 * u + 4 * g) * G + 2 * n));
+        ks[u][n] = global_load<uint32_t>(key_scales + (uint32_t)((own + 16 * u + 4 * g) * G + 2 * n));
+        vs[u][n] = global_load<uint32_t>(value_scales + (uint32_t)((own + 16 * u + 4 * g) * G + 2 * n));
       }
     }
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-      load_value<BITS, DP>(value_rows, (uint32_t)((16 * (j >> 2) + 4 * g + (j & 3)) * ROW), r, vw[j]);
+    for (int c = 0; c < BLOCKS; c++) {
+      const uint8_t* value_rows = V + (int64_t)(s0 + (c && both ? BLOCK : 0)) * ROW;
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        load_value<BITS, DP>(value_rows, (uint32_t)((16 * (j >> 2) + 4 * g + (j & 3)) * ROW), r, vw[c][j]);
+    }
     __builtin_amdgcn_sched_barrier(0);  // all of a block's loads are in flight before the first is waited for
     if constexpr (RAISED) {  // the halves of two keys' dwords beside each other
 #pragma unroll
-      for (int j = 0; j < 8; j += 2)
+      for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-        for (int n = 0; n < VW; n++) {
-          const uint32_t lo = __builtin_amdgcn_perm(vw[j + 1][n], vw[j][n], 0x05040100u);
-          vw[j + 1][n] = __builtin_amdgcn_perm(vw[j + 1][n], vw[j][n], 0x07060302u);
-          vw[j][n] = lo;
-        }
+        for (int j = 0; j < 8; j += 2)
+#pragma unroll
+          for (int n = 0; n < VW; n++) {
+            const uint32_t lo = __builtin_amdgcn_perm(vw[c][j + 1][n], vw[c][j][n], 0x05040100u);
+            vw[c][j + 1][n] = __builtin_amdgcn_perm(vw[c][j + 1][n], vw[c][j][n], 0x07060302u);
+            vw[c][j][n] = lo;
+          }
     }
 
     // scores, before the factor that makes them powers of two
@@ -337,12 +369,13 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
           else dot[i][n] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        const bf16x8 key = key_operand<BITS, RAISED>(kw[u], k);
+      for (int ck = 0; ck < BLOCKS * KS; ck++) {
+        const int c = ck / KS, k = ck % KS;
+        const bf16x8 key = key_operand<BITS, RAISED>(kw[c][u], k);
 #pragma unroll
         for (int i = 0; i < TILE; i++)
 #pragma unroll
-          for (int n = 0; n < QP; n++)
+          for (int n = BLOCKS > 1 ? c : 0; n < (BLOCKS > 1 ? c + 1 : QP); n++)
             dot[i][G == 1 ? 0 : k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key, q[i][k][n], dot[i][G == 1 ? 0 : k], 0, 0, 0);
       }
 #pragma unroll
@@ -359,14 +392,14 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
         }
       }
     }
-    if (s0 + BLOCK > least) {  // the block has keys that some row does not see
+    if (s0 + STEP > least) {  // the block has keys that some row does not see
 #pragma unroll
       for (int i = 0; i < TILE; i++)
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
           for (int e = 0; e < 4; e++)
-            if (s0 + 16 * u + 4 * g + e >= limit[i]) score[i][u][e] = -INFINITY;
+            if (s0 + BLOCK * side + 16 * u + 4 * g + e >= limit[i]) score[i][u][e] = -INFINITY;
     }
     // probabilities relative to the row's running maximum
     float p[TILE][8];
@@ -399,12 +432,12 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) x[j] = p[i][j] * scale_at(vs[j >> 2], (j & 3) * G + n);
-        if (s0 + BLOCK > least) {  // 0 for what the row does not see, whatever its scale
+        if (s0 + STEP > least) {  // 0 for what the row does not see, whatever its scale
 #pragma unroll
           for (int j = 0; j < 8; j++)
-            if (s0 + 16 * (j >> 2) + 4 * g + (j & 3) >= limit[i]) x[j] = 0.f;
+            if (s0 + BLOCK * side + 16 * (j >> 2) + 4 * g + (j & 3) >= limit[i]) x[j] = 0.f;
         }
-        if constexpr (SPREAD > 1) {  // part number r / ROWS alone
+        if constexpr (SPREAD > 1) {  // the column's part alone
           u32x4 w;
 #pragma unroll
           for (int n2 = 0; n2 < PP; n2++) {
@@ -412,26 +445,35 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
             for (int e = 0; e < 4; e++) {
               w[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
               if (n2 + 1 < PP) {
-                const float more = r / ROWS > n2 ? 1.f : 0.f;
+                const float more = part > n2 ? 1.f : 0.f;
                 x[2 * e] = __builtin_fmaf(-more, __uint_as_float(w[e] << 16), x[2 * e]);
                 x[2 * e + 1] = __builtin_fmaf(-more, __uint_as_float(w[e] & 0xffff0000u), x[2 * e + 1]);
               }
             }
           }
-          if (r / ROWS >= PP) w = u32x4{0u, 0u, 0u, 0u};  // more columns than parts
+          if (COPIES > PP && part >= PP) w = u32x4{0u, 0u, 0u, 0u};  // more columns than parts
           weights[i][0] = __builtin_bit_cast(bf16x8, w);
         } else {
           split_bf16<PP>(x, weights[i]);
         }
       }
+      bf16x8 sided[BLOCKS];  // the weights of a block's columns, 0 in the other's
+      if constexpr (BLOCKS > 1) {
+        const u32x4 none = {0u, 0u, 0u, 0u}, w = __builtin_bit_cast(u32x4, weights[0][0]);
+#pragma unroll
+        for (int c = 0; c < BLOCKS; c++) sided[c] = __builtin_bit_cast(bf16x8, side == c ? w : none);
+      }
 #pragma unroll
       for (int v = n * (NV / G); v < (n + 1) * (NV / G); v++) {
-        const bf16x8 value = value_operand<BITS, RAISED, VW>(vw, v);
 #pragma unroll
-        for (int i = 0; i < TILE; i++)
+        for (int c = 0; c < BLOCKS; c++) {
+          const bf16x8 value = value_operand<BITS, RAISED, VW>(vw[c], v);
 #pragma unroll
-          for (int n2 = 0; n2 < (SPREAD > 1 ? 1 : PP); n2++)
-            acc[i][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, weights[i][n2], acc[i][v], 0, 0, 0);
+          for (int i = 0; i < TILE; i++)
+#pragma unroll
+            for (int n2 = 0; n2 < (SPREAD > 1 ? 1 : PP); n2++)
+              acc[i][v] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value, BLOCKS > 1 ? sided[c] : weights[i][n2], acc[i][v], 0, 0, 0);
+        }
         if constexpr (RAISED) {  // block by block: the sums never hold more than a block's excess
           const u32x4 raise = {RAISE, RAISE, RAISE, RAISE};
 #pragma unroll
@@ -454,17 +496,24 @@ __global__ void __launch_bounds__(WAVES * 64) attend(AttendArgs a) {
     __syncthreads();
     if (g == 0) tops[wave][r] = top[i], sums[wave][r] = sum[i];
     __syncthreads();
-    float most = tops[0][r];
+    float most = LOWEST;
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) most = fmaxf(most, tops[w][r]);
+    for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) most = fmaxf(most, tops[w][r % ROWS + c * SIDE]);
     const float fade = __builtin_amdgcn_exp2f(top[i] - most);
     // thread c % 16 = row r' of the products, c / 16 = column
     const int channel_row = threadIdx.x & 15, column = threadIdx.x >> 4, row = column % ROWS;
-    float whole = 0.f, high = tops[0][row];
+    float whole = 0.f, high = LOWEST;
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) high = fmaxf(high, tops[w][row]);
+    for (int c = 0; c < BLOCKS; c++)
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) whole += sums[w][row] * __builtin_amdgcn_exp2f(tops[w][row] - high);
+      for (int w = 0; w < WAVES; w++) high = fmaxf(high, tops[w][row + c * SIDE]);
+#pragma unroll
+    for (int c = 0; c < BLOCKS; c++)
+#pragma unroll
+      for (int w = 0; w < WAVES; w++)
+        whole += sums[w][row + c * SIDE] * __builtin_amdgcn_exp2f(tops[w][row + c * SIDE] - high);
     const int64_t at = row0 + i * ROWS + row, t = at / a.group;
     const bool writes = column < ROWS && at < rows;
     if (sees(at) == 0) whole = 0.f;  // not a query, or one without keys: zero
@@ -558,10 +607,11 @@ __global__ void __launch_bounds__(64) attend_join(AttendArgs a, int tile_rows) {
 template <class T, int BITS, int DP>
 int attend_width(const AttendArgs& a, const AttendPlan& p, hipStream_t stream) {
   const dim3 grid((unsigned)(a.units * p.tiles * p.splits)), block(WAVES * 64);
-  constexpr int SPREAD = sizeof(T) == 2 ? 2 : 4;
-  if (p.spread > 1) {
-    hipLaunchKernelGGL((attend<T, BITS, DP, 1, SPREAD>), grid, block, 0, stream, a);
-  } else if constexpr (sizeof(T) == 4 && DP > 128) {
+  if (p.spread == 4) {
+    hipLaunchKernelGGL((attend<T, BITS, DP, 1, 4, sizeof(T) == 2 && DP <= 128 ? 2 : 1>), grid, block, 0, stream, a);
+  } else if (p.spread == 2) {
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((attend<T, BITS, DP, 1, 2>), grid, block, 0, stream, a);
+  } else if constexpr (one_tile(sizeof(T), BITS, DP)) {
     hipLaunchKernelGGL((attend<T, BITS, DP, 1, 1>), grid, block, 0, stream, a);
   } else {
     if constexpr (sizeof(T) == 2 && DP <= 128) {

@@ -5,23 +5,29 @@
 
 namespace {
 
-// Workgroups wanted in a launch of 256 CUs: four for each where a tile has few
-// rows and the keys are what is read (32 sequences of up to 16000 keys, 8 bits:
-// 149 us, 156 with two, 152 with twelve; 16 of up to 8000, 4 bits: 42, 40 and 57),
-// one where it has many, whose sums a split row writes and reads again (512 new
+// Workgroups wanted in a launch of 256 CUs.  Where a tile has few rows, and the keys
+// are what is read: two for each, which run together (16 sequences of up to 7000
+// keys, 4 bits, 128 channels: 31 us, 35 with four, 41 with six); four, which even
+// out sequences of different lengths, where a range keeps LONG_RANGE keys all the
+// same (32 of up to 14000, 8 bits: 120 us, 132 with two, 128 with six).  Where it
+// has many rows, whose sums a split one writes and reads again: one (512 new
 // positions over 3500: 63 us, 79 with two, 96 with four).
-constexpr int64_t FEW_ROWS = 1024, MANY_ROWS = 256;
+constexpr int64_t FEW_ROWS = 512, MANY_ROWS = 256, LONG_RANGE = 2048;
 
-AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype) {
+AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int bits,
+                   int dtype) {
   AttendPlan p;
   const int64_t rows = fresh * (heads / kv_heads);
   p.pitch = (int)cache_pitch(dim);
-  p.spread = dtype == BF16 ? (rows <= 8 ? 2 : 1) : rows <= 4 ? 4 : 1;
-  p.tile = p.spread > 1 || (dtype == F32 && p.pitch > 128) ? 1 : dtype == F32 || p.pitch > 128 || rows <= 32 ? 2 : 4;
+  p.spread = rows <= 4 ? 4 : dtype == BF16 && rows <= 8 ? 2 : 1;
+  p.tile = p.spread > 1 || one_tile(dtype == BF16 ? 2 : 4, bits, p.pitch) ? 1 : dtype == F32 || p.pitch > 128 || rows <= 32 ? 2 : 4;
   p.rows = 16 / p.spread * p.tile;
   p.tiles = (rows + p.rows - 1) / p.rows;
-  const int64_t units = batch * kv_heads * p.tiles, most = (longest + WAVES * BLOCK - 1) / (WAVES * BLOCK);
+  const int64_t units = batch * kv_heads * p.tiles;
+  const int64_t step = WAVES * BLOCK * (dtype == BF16 && p.spread == 4 && p.pitch <= 128 ? 2 : 1);
+  const int64_t most = (longest + step - 1) / step;
   p.splits = ((p.spread > 1 ? FEW_ROWS : MANY_ROWS) + units - 1) / units;
+  if (p.spread > 1 && longest / ((2 * FEW_ROWS + units - 1) / units) >= LONG_RANGE) p.splits = (2 * FEW_ROWS + units - 1) / units;
   if (p.splits > most) p.splits = most;
   if (p.splits > 256) p.splits = 256;
   if (p.splits < 1) p.splits = 1;
@@ -41,8 +47,13 @@ bool sizes_ok(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int
 extern "C" size_t qutai_amd_attention_quantized_workspace_size(int64_t batch, int64_t fresh, int64_t heads,
                                                                int64_t kv_heads, int64_t dim, int64_t longest, int dtype) {
   if (!sizes_ok(batch, fresh, heads, kv_heads, dim, longest, dtype) || batch == 0 || fresh == 0) return 0;
-  const AttendPlan p = plan_of(batch, fresh, heads, kv_heads, dim, longest, dtype);
-  return p.splits > 1 ? (size_t)slots_of(p, batch * kv_heads) * (p.pitch + 2) * sizeof(float) : 0;
+  size_t need = 0;
+  for (const int bits : {8, 4}) {
+    const AttendPlan p = plan_of(batch, fresh, heads, kv_heads, dim, longest, bits, dtype);
+    const size_t own = p.splits > 1 ? (size_t)slots_of(p, batch * kv_heads) * (p.pitch + 2) * sizeof(float) : 0;
+    need = own > need ? own : need;
+  }
+  return need;
 }
 
 extern "C" int qutai_amd_attention_quantized(const void* q, const void* key_codes, const void* key_scales,
@@ -60,7 +71,7 @@ extern "C" int qutai_amd_attention_quantized(const void* q, const void* key_code
   if (!q || !key_codes || !key_scales || !value_codes || !value_scales || !out) return QA_EINVAL;
   if ((uintptr_t)key_codes % 16 || (uintptr_t)value_codes % 16 || (uintptr_t)key_scales % 4 || (uintptr_t)value_scales % 4)
     return QA_EINVAL;
-  const AttendPlan p = plan_of(batch, fresh, heads, kv_heads, dim, longest, dtype);
+  const AttendPlan p = plan_of(batch, fresh, heads, kv_heads, dim, longest, bits, dtype);
   const int64_t units = batch * kv_heads;
   if (units * p.tiles * p.splits >= (1ll << 24)) return QA_EINVAL;  // workgroups of 256 threads, below 2^32
   const int64_t slots = slots_of(p, units);
