@@ -31,8 +31,8 @@
 // then runs without an exchange between lanes or a rescaling of the sums.
 //
 // Bound by HBM with 8 bits and few rows: 32 sequences of up to 16000 keys, 32 heads
-// of 128 over 8, 0.67 GB: 131 us (5.1 TB/s; a wave per query and head 9072), and 5 to
-// join.  Bound by vector operations with 4 bits (16 of up to 8000 keys, 92 MB: 43 us)
+// of 128 over 8, 0.67 GB: 129 us (5.2 TB/s; a wave per query and head 9072), and 5 to
+// join.  Bound by vector operations with 4 bits (16 of up to 8000 keys, 92 MB: 34 us)
 // and with many rows, where the softmax of a block costs more than its codes (512
 // new positions over 3500, 16 heads of 64 over 4: 62 us for 7.4 GFLOP).
 #pragma once
@@ -70,6 +70,11 @@ struct AttendPlan {
 // Two tiles of such rows do not fit in registers (4 bits, bf16, 256 channels, 512 new positions over 3000: 324 us
 // with one, 490 with two; 8 bits 198 and 158).
 constexpr bool one_tile(int item, int bits, int pitch) { return item == 4 ? pitch > 128 : bits == 4 && pitch == 256; }
+
+// Blocks of keys beside each other in a tile of four rows or fewer: two, but for wide
+// rows of 8 bits, whose operands then leave no room for a second wave (16 sequences
+// of up to 7000 keys, 192 channels: 54 us, one 50; 4 bits: 57 and 71).
+constexpr int blocks_of(int item, int bits, int pitch) { return item == 2 && (pitch <= 128 || bits == 4) ? 2 : 1; }
 
 template <class T> struct Parts;
 template <> struct Parts<bf16_t> { static constexpr int Q = 1, P = 2; };
@@ -608,7 +613,7 @@ template <class T, int BITS, int DP>
 int attend_width(const AttendArgs& a, const AttendPlan& p, hipStream_t stream) {
   const dim3 grid((unsigned)(a.units * p.tiles * p.splits)), block(WAVES * 64);
   if (p.spread == 4) {
-    hipLaunchKernelGGL((attend<T, BITS, DP, 1, 4, sizeof(T) == 2 && DP <= 128 ? 2 : 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((attend<T, BITS, DP, 1, 4, blocks_of(sizeof(T), BITS, DP)>), grid, block, 0, stream, a);
   } else if (p.spread == 2) {
     if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((attend<T, BITS, DP, 1, 2>), grid, block, 0, stream, a);
   } else if constexpr (one_tile(sizeof(T), BITS, DP)) {

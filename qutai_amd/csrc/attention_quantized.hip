@@ -3,6 +3,8 @@
 // attention_quantized.h).
 #include "attention_quantized.h"
 
+#include <initializer_list>
+
 namespace {
 
 // Workgroups wanted in a launch of 256 CUs.  Where a tile has few rows, and the keys
@@ -17,14 +19,15 @@ constexpr int64_t FEW_ROWS = 512, MANY_ROWS = 256, LONG_RANGE = 2048;
 AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int bits,
                    int dtype) {
   AttendPlan p;
+  const int item = dtype == BF16 ? 2 : 4;
   const int64_t rows = fresh * (heads / kv_heads);
   p.pitch = (int)cache_pitch(dim);
   p.spread = rows <= 4 ? 4 : dtype == BF16 && rows <= 8 ? 2 : 1;
-  p.tile = p.spread > 1 || one_tile(dtype == BF16 ? 2 : 4, bits, p.pitch) ? 1 : dtype == F32 || p.pitch > 128 || rows <= 32 ? 2 : 4;
+  p.tile = p.spread > 1 || one_tile(item, bits, p.pitch) ? 1 : dtype == F32 || p.pitch > 128 || rows <= 32 ? 2 : 4;
   p.rows = 16 / p.spread * p.tile;
   p.tiles = (rows + p.rows - 1) / p.rows;
   const int64_t units = batch * kv_heads * p.tiles;
-  const int64_t step = WAVES * BLOCK * (dtype == BF16 && p.spread == 4 && p.pitch <= 128 ? 2 : 1);
+  const int64_t step = WAVES * BLOCK * (p.spread == 4 ? blocks_of(item, bits, p.pitch) : 1);
   const int64_t most = (longest + step - 1) / step;
   p.splits = ((p.spread > 1 ? FEW_ROWS : MANY_ROWS) + units - 1) / units;
   if (p.spread > 1 && longest / ((2 * FEW_ROWS + units - 1) / units) >= LONG_RANGE) p.splits = (2 * FEW_ROWS + units - 1) / units;

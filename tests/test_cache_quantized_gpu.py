@@ -235,6 +235,24 @@ def test_attention_matches_float64(dtype, bits, batch, heads, kv_heads, dim, pas
         check_attention(download(out.storage).reshape(q.shape), q, k, v, starts, counts, dim ** -0.5, dtype, bits)
 
 
+PAIRS = [("bfloat16", 8, 64), ("bfloat16", 4, 64), ("bfloat16", 4, 128), ("bfloat16", 8, 128), ("bfloat16", 4, 256),
+         ("bfloat16", 8, 192), ("float32", 8, 64)]
+
+
+@pytest.mark.parametrize("dtype,bits,dim", PAIRS)
+@pytest.mark.parametrize("heads,new", [(3, 1), (1, 4), (2, 2)])
+def test_sequences_that_end_around_blocks_and_pairs_of_them(dtype, bits, dim, heads, new):
+    """Four rows or fewer: two blocks of 32 keys beside each other, the second of
+    which may hold nothing, at a split's end and at the capacity's."""
+    past = (0, 30, 31, 32, 33, 62, 63, 64, 65, 95, 96, 97, 255, 256, 287, 288, 289, 511, 512 - new)
+    test_attention_matches_float64(dtype, bits, len(past), heads, 1, dim, past, new)
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 256), (4, 200), (8, 256)])
+def test_many_rows_of_wide_heads(bits, dim):
+    test_attention_matches_float64("bfloat16", bits, 2, 4, 2, dim, (70, 129), 37)
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_what_lies_behind_a_sequence_does_not_leak(bits):
     """Scales of NaN and infinity behind the visible positions, and a poisoned
