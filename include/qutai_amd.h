@@ -508,8 +508,9 @@ int qutai_amd_cache_dequantize(const void* key_codes, const void* key_scales, co
  * longest bounds the positions that any sequence sees (it decides how the work is
  * split, not what is computed).  Scores, probabilities and sums are fp32, the
  * cache's values those its codes stand for.  workspace:
- * qutai_amd_attention_quantized_workspace_size bytes; too small a one is
- * QA_EWORKSPACE.  capacity is a multiple of 32 (at most 2^30; what lies behind a
+ * qutai_amd_attention_quantized_workspace_size bytes for the call's own longest
+ * (the size may grow from any length to the next, and never falls: one workspace for
+ * the largest serves all); too small a one is QA_EWORKSPACE.  capacity is a multiple of 32 (at most 2^30; what lies behind a
  * sequence's last position may be anything), the scales are 4-byte aligned;
  * batch x fresh x heads at most 2^25; scale lies between 1e-30 and 1e30. */
 int qutai_amd_attention_quantized(const void* q, const void* key_codes, const void* key_scales,

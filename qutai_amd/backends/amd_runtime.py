@@ -412,9 +412,10 @@ class Runtime:
         return need
 
     def attention_workspace(self, batch, fresh, heads, kv_heads, dim, longest, dtype):
-        """qutai_amd_attention_quantized_workspace_size, asked once for each plan:
-        the longest sequence counts in blocks of 128 positions."""
-        key = (batch, fresh, heads, kv_heads, dim, (longest + 127) // 128, dtype)
+        """qutai_amd_attention_quantized_workspace_size, asked once for the same
+        arguments (the layers of a decode step share them): the plan may change at
+        any length, so the length itself is part of the key."""
+        key = (batch, fresh, heads, kv_heads, dim, longest, dtype)
         need = self._attention_workspaces.get(key)
         if need is None:
             if len(self._attention_workspaces) >= 4096:

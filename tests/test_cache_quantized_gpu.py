@@ -304,6 +304,27 @@ def test_rows_beyond_four_gigabytes(bits):
     check_attention(out, q, *read(cache), (2,), (1,), 1 / 16, "bfloat16", bits)
 
 
+@pytest.mark.parametrize("bits,dtype", [(8, "bfloat16"), (4, "bfloat16"), (8, "float32")])
+def test_decoding_over_the_length_at_which_the_split_changes(bits, dtype):
+    """512 (sequence, head) pairs, one position at a time past 4096 keys, from
+    where on each takes twice the ranges."""
+    rng = np.random.default_rng(15)
+    batch, kv_heads, dim, past = 64, 8, 8, 4094
+    cache = QuantizedKVCache(4100, bits=bits)
+    old = [rng.standard_normal((batch, past, kv_heads, dim), dtype=np.float32) for _ in range(2)]
+    cache.append(*(as_tensor(x, dtype) for x in old), (past,) + tuple(range(past - 63, past)))
+    starts = cache.lengths
+    steps = []
+    for _ in range(4):
+        cache.append(*(as_tensor(rng.standard_normal((batch, 1, kv_heads, dim)), dtype) for _ in range(2)))
+        q = stored(rng.standard_normal((batch, 1, 2 * kv_heads, dim)) * 2, dtype)
+        steps.append((q, download(cache.attend(as_tensor(q, dtype)).storage).reshape(q.shape)))
+    some = [0, 1, 30, 63]
+    k, v = (x[some] for x in read(cache))
+    for i, (q, out) in enumerate(steps):
+        check_attention(out[some], q[some], k, v, [starts[b] + i for b in some], (1,) * 4, dim ** -0.5, dtype, bits)
+
+
 def test_no_new_positions_and_counts_of_the_library():
     """An append of nothing; counts above the new positions and below none, as the
     library's callers may pass them."""

@@ -207,6 +207,36 @@ def test_a_refused_first_append_settles_nothing(new, counts):
     assert cache.codes is None and cache.lengths == () and cache.length == 0
 
 
+def around_changes_of_plan():
+    """Lengths before, at and behind each multiple of 2048 (where ranges of keys
+    change) and every length around a power of two, in order."""
+    lengths = set(range(300))
+    for n in range(2048, 66000, 2048):
+        lengths.update(range(n - 140, n + 3, 1 if n & (n - 1) == 0 else 20), (n - 1, n, n + 1))
+    return sorted(lengths)
+
+
+@built
+@pytest.mark.parametrize("dtype", [0, 5])
+@pytest.mark.parametrize("sequences,heads,kv_heads,dim", [(8, 16, 8, 64), (16, 32, 8, 128), (32, 32, 8, 128), (40, 32, 8, 128),
+                                                          (64, 32, 8, 128), (128, 16, 4, 64), (128, 32, 8, 32), (1, 16, 4, 256)])
+def test_a_growing_cache_never_keeps_too_small_a_workspace(sequences, heads, kv_heads, dim, dtype):
+    """The size that the runtime keeps, while the longest sequence grows over
+    every change of plan and shrinks again, against the library's own, which
+    never falls where the length grows."""
+    runtime = object.__new__(amd_runtime.Runtime)
+    runtime._closed, runtime._attention_workspaces = True, {}
+    runtime.lib = amd_runtime.load_library()
+    size = runtime.lib.qutai_amd_attention_quantized_workspace_size
+    lengths = around_changes_of_plan()
+    for longest in (*lengths, *reversed(lengths)):
+        for new in (1, 2):
+            arguments = sequences, new, heads, kv_heads, dim, longest, dtype
+            assert runtime.attention_workspace(*arguments) >= size(*arguments), arguments
+    sizes = [size(sequences, 1, heads, kv_heads, dim, longest, dtype) for longest in lengths]
+    assert sizes == sorted(sizes)
+
+
 # ---- sampling ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("change", [
