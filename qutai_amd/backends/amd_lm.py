@@ -566,6 +566,19 @@ def _cache_positions(cache, *arrays):
             raise ValueError("a cache's positions and counts are one int64 per sequence")
 
 
+def cache_rows(keys, values, batch, new, kv_heads, dim, *, key_column=0, key_row=None, value_column=0, value_row=None):
+    """(key_row, value_row) of new keys and values that ``cache_quantize`` takes
+    for a cache of these sizes; ValueError where it does not take them."""
+    width = kv_heads * dim
+    key_row, value_row = (width if row is None else row for row in (key_row, value_row))
+    if new < 0 or keys.dtype != values.dtype or keys.dtype not in ("bfloat16", "float32"):
+        raise ValueError("cached keys and values are bfloat16 or float32, of one dtype")
+    for x, column, row in ((keys, key_column, key_row), (values, value_column, value_row)):
+        if column < 0 or column + width > row or x.size < batch * new * row:
+            raise ValueError("keys and values need new positions of kv_heads * dim values for every sequence")
+    return key_row, value_row
+
+
 def cache_quantize(cache, keys, values, new, *, start=0, starts=None, counts=None, key_column=0, key_row=None,
                    value_column=0, value_row=None):
     """Quantise ``new`` positions of every sequence into ``cache`` from position
@@ -574,15 +587,10 @@ def cache_quantize(cache, keys, values, new, *, start=0, starts=None, counts=Non
     the capacity).  keys and values are [batch][new][kv_heads][dim], or columns
     key_column .. (value_column ..) of wider matrices of key_row (value_row)
     elements per position."""
-    width, positions = cache.kv_heads * cache.dim, cache.batch * new
-    key_row, value_row = (width if row is None else row for row in (key_row, value_row))
-    if new < 0 or keys.dtype != values.dtype or keys.dtype not in ("bfloat16", "float32"):
-        raise ValueError("cached keys and values are bfloat16 or float32, of one dtype")
-    for x, column, row in ((keys, key_column, key_row), (values, value_column, value_row)):
-        if column < 0 or column + width > row or x.size < positions * row:
-            raise ValueError("keys and values need new positions of kv_heads * dim values for every sequence")
+    key_row, value_row = cache_rows(keys, values, cache.batch, new, cache.kv_heads, cache.dim, key_column=key_column,
+                                    key_row=key_row, value_column=value_column, value_row=value_row)
     _cache_positions(cache, starts, counts)
-    if positions:
+    if new:
         item = _TYPES[keys.dtype][1]
         cache.key_codes.runtime.call(
             "qutai_amd_cache_quantize", keys.ptr + key_column * item, values.ptr + value_column * item,

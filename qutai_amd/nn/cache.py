@@ -124,6 +124,8 @@ class QuantizedKVCache:
         lengths = tuple(n + m for n, m in zip(self.lengths or (0,) * batch, counts))
         if max(lengths) > self.capacity:
             raise ValueError("the cache's capacity is exceeded")
+        if self.codes is None:  # (cache_quantize checks them too, but behind reserve)
+            amd_lm.cache_rows(keys, values, batch, new, kv_heads, dim, **columns)
         self.reserve(batch, kv_heads, dim)  # last: a refused call settles nothing
         start, starts = self.positions()
         held = None if min(counts) == new else amd.storage(counts, dtype="int64")

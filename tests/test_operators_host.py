@@ -207,6 +207,21 @@ def test_a_refused_first_append_settles_nothing(new, counts):
     assert cache.codes is None and cache.lengths == () and cache.length == 0
 
 
+@pytest.mark.parametrize("keys, values, columns", [
+    (fake(96, "float64"), fake(96, "float64"), {}), (fake(96, "int64"), fake(96, "int64"), {}),
+    (fake(96, "float32"), fake(96, "bfloat16"), {}), (fake(95, "float32"), fake(96, "float32"), {}),
+    (fake(96, "float32"), fake(96, "float32"), dict(key_row=15)), (fake(96, "float32"), fake(96, "float32"), dict(value_column=1)),
+    (fake(96, "float32"), fake(96, "float32"), dict(value_column=-1, value_row=17)),
+])
+def test_a_first_append_of_wrong_rows_settles_nothing(keys, values, columns, monkeypatch):
+    reserved = []
+    monkeypatch.setattr(amd_lm, "QuantizedCache", lambda *sizes: reserved.append(sizes) or fake_cache())
+    cache = QuantizedKVCache(4)
+    with pytest.raises(ValueError):
+        cache.append_rows(keys, values, 2, 3, 2, 8, **columns)
+    assert not reserved and cache.codes is None and cache.lengths == ()
+
+
 def around_changes_of_plan():
     """Lengths before, at and behind each multiple of 2048 (where ranges of keys
     change) and every length around a power of two, in order."""
