@@ -24,7 +24,7 @@ from ..backends import amd
 from ..core.context import set_recording
 from ..core.tensor import Tensor
 from .config import Config
-from ..nn.cache import QuantizedKVCache
+from ..nn.cache import QuantizedKVCache, unchanged_on_failure
 from .layers import Block, Projection, RMSNorm, backend, embed, linear, projection_loss, sample, scaled, unpack
 from .recompute import checkpoint
 
@@ -126,7 +126,8 @@ class Decoder:
     def decode(self, tokens, caches, counts=None):
         """Logits (batch, vocab) that follow the last of ``tokens`` (batch, new),
         the positions behind those that ``caches`` hold; of sequence b only the
-        first counts[b] are there, at least one.  Nothing is recorded."""
+        first counts[b] are there, at least one.  Nothing is recorded; a call
+        that fails leaves the caches as they were."""
         ids, (batch, new) = self._tokens(tokens)
         caches = tuple(caches)
         counts = (new,) * batch if counts is None else tuple(counts)
@@ -138,7 +139,7 @@ class Decoder:
         limit = min(self.config.max_seq_len, *(c.capacity for c in caches))
         if any(n + m > limit for n, m in zip(held, counts)):
             raise ValueError("the positions exceed max_seq_len or the caches' capacity")
-        with set_recording(False):
+        with set_recording(False), unchanged_on_failure(*caches):
             hidden = embed(ids, self.embedding.weight, (batch, new))
             for block, cache in zip(self.blocks, caches):
                 hidden = block.decode(hidden, cache, None if min(counts) == new else counts)

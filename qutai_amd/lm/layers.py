@@ -21,6 +21,7 @@ from ..backends.precision import matmul_precision, set_matmul_precision
 from ..core.context import is_recording
 from ..core.grad import DeferredGradient, owned, record
 from ..core.tensor import Tensor
+from ..nn.cache import unchanged_on_failure
 
 
 def backend(value):
@@ -459,7 +460,11 @@ class GQA:
         """The block over new positions of (batch, new, width) alone: their keys
         and values are appended to ``cache`` (a QuantizedKVCache; of sequence b
         the first counts[b] where given) and they attend over all that it holds.
-        Nothing is recorded."""
+        Nothing is recorded; a call that fails leaves the cache as it was."""
+        with unchanged_on_failure(cache):
+            return self._decode(x, cache, counts)
+
+    def _decode(self, x, cache, counts):
         b = backend(x)
         batch, new, width = x.shape
         weights = (self.q.weight, self.k.weight, self.v.weight)

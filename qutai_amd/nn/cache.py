@@ -107,6 +107,15 @@ class QuantizedKVCache:
         elif (batch, kv_heads, dim) != (self.codes.batch, self.codes.kv_heads, self.codes.dim):
             raise ValueError("new keys and values must match the cache in batch, heads and head size")
 
+    def state(self):
+        """What the cache holds now, for ``restore``."""
+        return self.codes, self.lengths, self._base, self._stored, self._shift, self._last
+
+    def restore(self, state):
+        """Back to an earlier ``state``: the positions appended since are forgotten
+        (those that were truncated since are not there again)."""
+        self.codes, self.lengths, self._base, self._stored, self._shift, self._last = state
+
     def append(self, keys, values, counts=None):
         """Quantise new positions (batch, new, kv_heads, dim) behind those each
         sequence has; of sequence b only the first ``counts[b]`` where given."""
@@ -126,10 +135,11 @@ class QuantizedKVCache:
             raise ValueError("the cache's capacity is exceeded")
         if self.codes is None:  # (cache_quantize checks them too, but behind reserve)
             amd_lm.cache_rows(keys, values, batch, new, kv_heads, dim, **columns)
-        self.reserve(batch, kv_heads, dim)  # last: a refused call settles nothing
-        start, starts = self.positions()
-        held = None if min(counts) == new else amd.storage(counts, dtype="int64")
-        amd_lm.cache_quantize(self.codes, keys, values, new, start=start, starts=starts, counts=held, **columns)
+        with unchanged_on_failure(self):
+            self.reserve(batch, kv_heads, dim)
+            start, starts = self.positions()
+            held = None if min(counts) == new else amd.storage(counts, dtype="int64")
+            amd_lm.cache_quantize(self.codes, keys, values, new, start=start, starts=starts, counts=held, **columns)
         self._set_lengths(lengths)
         self._last = new, start, starts, held
 
@@ -167,3 +177,19 @@ class QuantizedKVCache:
             return
         self._set_lengths(self._per_sequence(lengths, self.lengths, "lengths"))
         self._last = None
+
+
+class unchanged_on_failure:
+    """Context in which quantised caches are appended to: where it raises they
+    are as they were before, so that the call may be made again."""
+
+    def __init__(self, *caches):
+        self.states = [(cache, cache.state()) for cache in caches]
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, kind, value, traceback):
+        if kind is not None:
+            for cache, state in self.states:
+                cache.restore(state)

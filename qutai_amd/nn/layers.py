@@ -30,7 +30,7 @@ from ..core import operations
 from ..core.context import set_recording
 from ..core.grad import owned, record
 from ..core.tensor import Tensor, _result, matmul
-from .cache import KVCache, QuantizedKVCache  # noqa: F401 - the reference exposes KVCache beside the layers
+from .cache import KVCache, QuantizedKVCache, unchanged_on_failure  # noqa: F401 - the reference exposes KVCache beside the layers
 
 
 def _tensor(data, like):
@@ -173,8 +173,9 @@ class MultiHeadAttention(Attention):
             queries, keys, values = (layer(tensor) for layer in (self.query, self.key, self.value))
             if isinstance(cache, QuantizedKVCache):
                 shape = (*queries.shape[:2], self.heads, queries.shape[2] // self.heads)
-                cache.append(keys.reshape(shape), values.reshape(shape))
-                return self.output(cache.attend(queries.reshape(shape)).reshape(queries.shape))
+                with unchanged_on_failure(cache):
+                    cache.append(keys.reshape(shape), values.reshape(shape))
+                    return self.output(cache.attend(queries.reshape(shape)).reshape(queries.shape))
             keys, values = cache.update(self._split(keys), self._split(values))
             batch, length, features = tensor.shape
             total, dim = keys.shape[2:]

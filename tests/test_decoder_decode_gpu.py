@@ -4,8 +4,10 @@ against a float64 forward pass that reads the values the caches hold."""
 import numpy as np
 import pytest
 
-from qutai_amd.backends import amd
+from qutai_amd import Tensor
+from qutai_amd.backends import amd, amd_lm
 from qutai_amd.lm import Config, Decoder, autocast, sample
+from qutai_amd.nn import MultiHeadAttention, QuantizedKVCache
 from tests.helpers import download, stored, upload
 from tests.test_cache_quantized_gpu import held
 
@@ -152,6 +154,56 @@ def test_generate_samples_what_decode_gives():
     logits = model.decode([p + [0] * (4 - len(p)) for p in prompts], model.caches(), [4, 1, 2])
     assert [row[0] for row in greedy] == download(logits.storage).reshape(3, 61).argmax(1).tolist()
     assert model.generate([[1]], 0) == [[]]
+
+
+@pytest.mark.parametrize("failing", [0, 1])
+def test_a_step_that_failed_can_be_made_again(failing, monkeypatch):
+    """The attention of a block raises: the caches hold what they did, and the
+    same call then gives the logits of a run without the failure."""
+    model, rng = build(True), np.random.default_rng(7)
+    steps = [rng.integers(0, 61, (2, new)).tolist() for new in (4, 1)]
+    whole = model.caches()
+    expected = [model.decode(tokens, whole).storage.to_array() for tokens in steps]
+    caches, attention = model.caches(), amd_lm.attention_quantized
+    for tokens, logits in zip(steps, expected):
+        held, calls = [(c.lengths, c.codes) for c in caches], []
+
+        def fail(*arguments, **options):
+            calls.append(None)
+            if len(calls) > failing:
+                raise RuntimeError("no memory left")
+            return attention(*arguments, **options)
+
+        with monkeypatch.context() as patch:
+            patch.setattr(amd_lm, "attention_quantized", fail)
+            with pytest.raises(RuntimeError):
+                model.decode(tokens, caches)
+        assert [(c.lengths, c.codes) for c in caches] == held
+        assert model.decode(tokens, caches).storage.to_array() == logits
+
+
+def test_layers_that_fail_append_nothing(monkeypatch):
+    layer, heads = build(True, layers=1).blocks[0].attn, MultiHeadAttention(32, 4, causal=True, seed=1)
+    x = Tensor(upload(np.random.default_rng(2).standard_normal((2, 3, 32)), "float32"), shape=(2, 3, 32))
+    calls = (lambda cache: layer.decode(x, cache), lambda cache: heads(x, cache=cache))
+
+    def fail(*arguments, **options):
+        raise RuntimeError("no memory left")
+
+    for call in calls:
+        small = QuantizedKVCache(2)
+        with pytest.raises(ValueError):
+            call(small)  # too many positions: no batch or heads are settled
+        assert small.codes is None and small.lengths == ()
+        cache, whole = QuantizedKVCache(8), QuantizedKVCache(8)
+        expected = [call(whole).storage.to_array() for _ in range(2)]
+        for held, result in zip(((), (3, 3)), expected):
+            with monkeypatch.context() as patch:
+                patch.setattr(amd_lm, "attention_quantized", fail)
+                with pytest.raises(RuntimeError):
+                    call(cache)
+            assert cache.lengths == held
+            assert call(cache).storage.to_array() == result
 
 
 def test_refusals():

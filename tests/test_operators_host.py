@@ -3,11 +3,12 @@ Python checks, and the C entry points' own (stand-in pointers that are never
 followed)."""
 from itertools import count
 from pathlib import Path
+from types import SimpleNamespace
 
 import pytest
 
 from qutai_amd.backends import amd, amd_lm, amd_runtime
-from qutai_amd.lm import Config
+from qutai_amd.lm import Config, decoder
 from qutai_amd.nn import QuantizedKVCache
 
 LIBRARY = Path(__file__).resolve().parent.parent / "qutai_amd" / "libqutai_amd.so"
@@ -220,6 +221,63 @@ def test_a_first_append_of_wrong_rows_settles_nothing(keys, values, columns, mon
     with pytest.raises(ValueError):
         cache.append_rows(keys, values, 2, 3, 2, 8, **columns)
     assert not reserved and cache.codes is None and cache.lengths == ()
+
+
+def stand_in(batch, kv_heads, dim, capacity, bits):
+    return SimpleNamespace(batch=batch, kv_heads=kv_heads, dim=dim, capacity=capacity, bits=bits)
+
+
+def test_an_append_that_the_library_refuses_changes_nothing(monkeypatch):
+    refuse = []
+    monkeypatch.setattr(amd_lm, "QuantizedCache", stand_in)
+
+    def quantize(*arguments, **options):
+        if refuse:
+            raise ValueError("refused")
+
+    monkeypatch.setattr(amd_lm, "cache_quantize", quantize)
+    rows = fake(2 * 3 * 2 * 8, "float32")
+    cache = QuantizedKVCache(32)
+    refuse.append(True)
+    with pytest.raises(ValueError):
+        cache.append_rows(rows, rows, 2, 3, 2, 8)
+    assert cache.codes is None and cache.lengths == () and cache.length == 0
+    refuse.clear()
+    cache.append_rows(rows, rows, 1, 3, 2, 8)  # other sizes than those refused
+    refuse.append(True)
+    with pytest.raises(ValueError):
+        cache.append_rows(rows, rows, 1, 3, 2, 8)
+    assert cache.lengths == (3,) and cache._last[:2] == (3, 0)
+
+
+@pytest.mark.parametrize("failing", [0, 1, 2])
+def test_a_decode_step_that_fails_leaves_the_caches(failing, monkeypatch):
+    """Three blocks, of which one raises behind its append."""
+    monkeypatch.setattr(amd_lm, "QuantizedCache", stand_in)
+    monkeypatch.setattr(amd_lm, "cache_quantize", lambda *arguments, **options: None)
+    monkeypatch.setattr(decoder, "embed", lambda ids, weight, shape: None)
+    rows = fake(2 * 3 * 2 * 8, "float32")
+
+    class FailingBlock:
+        fails = False
+
+        def decode(self, hidden, cache, counts):
+            cache.append_rows(rows, rows, 2, 3, 2, 8)
+            if self.fails:
+                raise RuntimeError("out of memory")
+
+    model = object.__new__(decoder.Decoder)
+    model.config, model.blocks = Config(max_seq_len=16, n_layers=3), [FailingBlock() for _ in range(3)]
+    model.embedding = SimpleNamespace(weight=None)
+    caches = model.caches()
+    model.blocks[failing].fails = True
+    for held in ((), (5, 5)):
+        with pytest.raises(RuntimeError):
+            model.decode([[1, 2, 3], [4, 5, 6]], caches)
+        assert all(c.lengths == held and (c.codes is None) == (held == ()) for c in caches)
+        for c in caches:
+            c.append_rows(rows, rows, 2, 3, 2, 8)
+            c.append_rows(rows, rows, 2, 2, 2, 8)
 
 
 def around_changes_of_plan():
