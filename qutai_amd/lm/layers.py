@@ -18,7 +18,7 @@ from math import prod, sqrt
 
 from ..backends import amd, amd_lm
 from ..backends.precision import matmul_precision, set_matmul_precision
-from ..core.context import is_recording
+from ..core.context import is_recording, set_recording
 from ..core.grad import DeferredGradient, owned, record
 from ..core.tensor import Tensor
 from ..nn.cache import unchanged_on_failure
@@ -461,7 +461,7 @@ class GQA:
         and values are appended to ``cache`` (a QuantizedKVCache; of sequence b
         the first counts[b] where given) and they attend over all that it holds.
         Nothing is recorded; a call that fails leaves the cache as it was."""
-        with unchanged_on_failure(cache):
+        with set_recording(False), unchanged_on_failure(cache):
             return self._decode(x, cache, counts)
 
     def _decode(self, x, cache, counts):
@@ -523,10 +523,12 @@ class Block:
         return self(x)[0]
 
     def decode(self, x, cache, counts=None):
-        """The block over new positions, attending over ``cache`` (GQA.decode)."""
-        x = residual_add(x, self.attn.decode(self.attn_norm(x), cache, counts))
-        y = self.ffn(self.ffn_norm(x))
-        return residual_add(x, y[0] if self.is_moe else y)
+        """The block over new positions, attending over ``cache`` (GQA.decode);
+        nothing is recorded, and a call that fails leaves the cache as it was."""
+        with set_recording(False), unchanged_on_failure(cache):
+            x = residual_add(x, self.attn.decode(self.attn_norm(x), cache, counts))
+            y = self.ffn(self.ffn_norm(x))
+            return residual_add(x, y[0] if self.is_moe else y)
 
     def packed(self, x):
         return pack(*self(x))

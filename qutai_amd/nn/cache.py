@@ -61,7 +61,8 @@ class QuantizedKVCache:
     """Keys and values of up to ``capacity`` positions per sequence, in codes of
     ``bits`` 8 (a scale per head and position) or 4 (a scale per 32 channels of
     it).  Sequences may have different lengths.  Its memory is allocated by the
-    first ``append``, which settles batch, heads and head width."""
+    first ``append``, which settles batch, heads and head width.  It serves
+    inference: what is appended, attended and read has no graph."""
 
     def __init__(self, capacity, *, bits=8):
         if type(capacity) is not int or capacity <= 0 or bits not in (8, 4):
@@ -147,7 +148,7 @@ class QuantizedKVCache:
         """Causal attention of the last ``append``'s positions over everything
         cached: queries (batch, new, heads, dim), heads a multiple of the
         cached ones; the result has their shape and dtype, and is zero at the
-        positions that ``counts`` left out."""
+        positions that ``counts`` left out.  Nothing is recorded."""
         if self._last is None:
             raise ValueError("attend follows an append: its queries are the positions appended last")
         new, start, starts, counts = self._last

@@ -206,6 +206,27 @@ def test_layers_that_fail_append_nothing(monkeypatch):
             assert call(cache).storage.to_array() == result
 
 
+@pytest.mark.parametrize("cast", [False, True])
+@pytest.mark.parametrize("ffn", ["dense", "moe"])
+def test_decoding_layers_record_nothing(ffn, cast):
+    """GQA.decode and Block.decode called by themselves, with parameters and an
+    input that require gradients; recording is on again behind them."""
+    from contextlib import nullcontext
+
+    block = build(True, ffn, layers=1).blocks[0]
+    rng = np.random.default_rng(2)
+    with autocast() if cast else nullcontext():
+        for layer in (block.attn, block):
+            x = Tensor(upload(rng.standard_normal((2, 3, 32)), "float32"), shape=(2, 3, 32), requires_grad=True)
+            cache = QuantizedKVCache(8)
+            y = layer.decode(x, cache)
+            assert cache.lengths == (3, 3) and not y.requires_grad and y.parents == () and y.backward_rule is None
+            attended = cache.attend(Tensor(upload(rng.standard_normal((2, 3, 4, 8)), "float32"), shape=(2, 3, 4, 8),
+                                           requires_grad=True))
+            assert not attended.requires_grad
+            assert block.attn_norm(x).requires_grad
+
+
 def test_refusals():
     model = build(True)
     caches = model.caches()
