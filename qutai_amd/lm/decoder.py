@@ -133,6 +133,8 @@ class Decoder:
         counts = (new,) * batch if counts is None else tuple(counts)
         if len(caches) != len(self.blocks) or len(counts) != batch or any(type(n) is not int or not 1 <= n <= new for n in counts):
             raise ValueError("decode takes a cache for each block and a count of 1 to new positions for each sequence")
+        if len({id(c) for c in caches}) != len(caches):
+            raise ValueError("every block needs a cache of its own")
         held = caches[0].lengths or (0,) * batch
         if any((c.lengths or (0,) * batch) != held for c in caches) or len(held) != batch:
             raise ValueError("the caches hold other sequences than the tokens'")

@@ -280,6 +280,20 @@ def test_a_decode_step_that_fails_leaves_the_caches(failing, monkeypatch):
             c.append_rows(rows, rows, 2, 2, 2, 8)
 
 
+def test_blocks_do_not_share_a_cache(monkeypatch):
+    """One cache for two blocks: each would append behind the other's positions."""
+    monkeypatch.setattr(amd_lm, "QuantizedCache", stand_in)
+    appended = []
+    monkeypatch.setattr(decoder, "embed", lambda ids, weight, shape: None)
+    model = object.__new__(decoder.Decoder)
+    model.config, model.embedding = Config(max_seq_len=16, n_layers=2), SimpleNamespace(weight=None)
+    model.blocks = [SimpleNamespace(decode=lambda hidden, cache, counts: appended.append(cache))] * 2
+    cache = model.caches()[0]
+    with pytest.raises(ValueError, match="of its own"):
+        model.decode([[1, 2]], (cache, cache))
+    assert not appended
+
+
 def around_changes_of_plan():
     """Lengths before, at and behind each multiple of 2048 (where ranges of keys
     change) and every length around a power of two, in order."""
