@@ -639,7 +639,7 @@ def attention_quantized(cache, q, new, heads, *, start=0, starts=None, counts=No
         runtime.call("qutai_amd_attention_quantized", q.ptr, cache.key_codes.ptr, cache.key_scales.ptr,
                      cache.value_codes.ptr, cache.value_scales.ptr, out.ptr, amd._p(starts), amd._p(counts), start,
                      cache.batch, new, heads, cache.kv_heads, cache.dim, cache.capacity, longest, cache.bits,
-                     dtype, float(scale), cache.workspace.ptr, cache.workspace.nbytes)
+                     dtype, float(scale), cache.workspace.ptr, cache.workspace.nbytes, mfma=True)
     return out
 
 

@@ -341,6 +341,16 @@ def test_no_new_positions_and_counts_of_the_library():
     check_attention(download(out).reshape(q.shape), q, *read(cache), (0, 0, 0), (6, 0, 4), 32 ** -0.5, "float32")
 
 
+@pytest.mark.parametrize("dtype,bits,dim", [("bfloat16", 8, 64), ("float32", 4, 256), ("bfloat16", 4, 5)])
+def test_attention_counts_as_a_launch_on_the_matrix_cores(dtype, bits, dim):
+    cache, runtime = QuantizedKVCache(8, bits=bits), amd.get_runtime()
+    x = as_tensor(np.ones((1, 2, 1, dim)), dtype)
+    cache.append(x, x)
+    before = runtime.mfma_launches
+    cache.attend(x)
+    assert runtime.mfma_launches == before + 1
+
+
 def test_the_same_call_gives_the_same_bits():
     rng = np.random.default_rng(3)
     cache = QuantizedKVCache(4000)
