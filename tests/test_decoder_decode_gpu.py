@@ -256,3 +256,37 @@ def test_quantised_values_are_those_of_the_keys():
     # what the codes stand for lies on the codes' own grid: quantised again it moves by half a step at most
     for x, y in zip((keys, values), again):
         assert np.abs(x - y).max() <= 0.51 * np.abs(x).max() / 126
+
+
+@pytest.mark.parametrize("qk_norm,bits", [(True, 8), (True, 4), (False, 8), (False, 4)])
+def test_the_first_block_caches_the_codes_of_its_keys_and_values(qk_norm, bits):
+    """What the first block's cache holds against the definition's codes of its
+    normed and rotated keys and of its values, computed in float64 from the
+    embedding's rows.  The kernel's fp32 keys and values are 34 roundings of 2^-24
+    off at most, of sums some five times a row's largest value: 0.003 of a step of
+    1/127 on either side of a border, so that some 0.3% of the codes (and, with a
+    scale's 2^-8, as many scales) may be the next one's."""
+    model = build(qk_norm)
+    c, p = model.config, Reference(model).p
+    rng, caches = np.random.default_rng(4), model.caches(bits=bits)
+    kept = [[] for _ in range(3)]
+    for counts in ((25, 9, 17), (1, 1, 1), (13, 14, 2)):
+        tokens = rng.integers(0, 61, (3, max(counts))).tolist()
+        model.decode(tokens, caches, counts)
+        for row, new, n in zip(kept, tokens, counts):
+            row += new[:n]
+    read = [download(x.storage).reshape(x.shape) for x in caches[0].read()]
+    changed = total = 0
+    for b, tokens in enumerate(kept):
+        y = norm(p["embedding.weight"][tokens], p["blocks.0.attn_norm.weight"], c.norm_eps)
+        k, v = ((y @ p[f"blocks.0.attn.{n}.weight"].T).reshape(len(tokens), c.n_kv_heads, -1) for n in "kv")
+        if qk_norm:
+            k = norm(k, p["blocks.0.attn.k_norm.weight"], c.norm_eps)
+        k = turned(k, np.arange(len(tokens)), c.rope_theta)
+        for got, x in zip(read, (k, v)):
+            got, expected = got[b, :, :len(tokens)].transpose(1, 0, 2), held(x, bits)
+            # one step of a scale that is 2^-7 too large at most
+            step = np.abs(x).max(-1, keepdims=True) * (1 + 2.0 ** -6) / (127 if bits == 8 else 7)
+            assert (np.abs(got - expected) <= step).all()
+            changed, total = changed + (got != expected).sum(), total + x.size
+    assert changed <= 0.02 * total
