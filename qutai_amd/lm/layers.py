@@ -240,6 +240,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, heads, kv_heads, theta, eps, offset=0
     kv_heads*dim), weights of dim values each, and their rotary embedding in
     one launch; (q, k), recorded."""
     b = backend(q)
+    if q.ndim != 3 or heads <= 0 or q.shape[2] % heads or k.shape != (*q.shape[:2], kv_heads * (q.shape[2] // heads)):
+        raise ValueError("qk_norm_rope takes q (batch, time, heads*dim) and k (batch, time, kv_heads*dim)")
     batch, time, features = q.shape
     dims = (batch, time, heads, kv_heads, features // heads, theta, eps)
     values = b.qk_norm_rope(q.storage, k.storage, q_weight.storage, k_weight.storage, *dims, offset=offset)

@@ -2,13 +2,15 @@
 Python checks, and the C entry points' own (stand-in pointers that are never
 followed)."""
 from itertools import count
+from math import prod
 from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
 
+from qutai_amd import Tensor
 from qutai_amd.backends import amd, amd_lm, amd_runtime
-from qutai_amd.lm import Config, decoder
+from qutai_amd.lm import Config, decoder, qk_norm_rope
 from qutai_amd.nn import QuantizedKVCache
 
 LIBRARY = Path(__file__).resolve().parent.parent / "qutai_amd" / "libqutai_amd.so"
@@ -47,6 +49,19 @@ def qk_call(**change):
 def test_qk_norm_rope_refuses(change):
     with pytest.raises(ValueError):
         qk_call(**change)
+
+
+@pytest.mark.parametrize("q,k,heads,kv_heads", [
+    ((2, 3, 32), (1, 6, 16), 4, 2), ((2, 3, 32), (3, 2, 16), 4, 2), ((2, 3, 32), (2, 3, 16), 4, 4), ((2, 3, 32), (2, 3, 24), 4, 2),
+    ((2, 3, 32), (2, 6, 16), 4, 2), ((2, 3, 34), (2, 3, 16), 4, 2), ((6, 32), (6, 16), 4, 2), ((2, 3, 32), (6, 16), 4, 2),
+    ((2, 3, 32), (2, 3, 16), 0, 2),
+])
+def test_recorded_qk_norm_rope_refuses_other_shapes(q, k, heads, kv_heads):
+    """Keys of as many values in other sequences or positions among them, which
+    would be turned by the positions of the queries."""
+    q, k, *weights = (Tensor(fake(prod(shape), "float32"), shape=shape) for shape in (q, k, (8,), (8,)))
+    with pytest.raises(ValueError, match="qk_norm_rope takes q"):
+        qk_norm_rope(q, k, *weights, heads, kv_heads, 1e4, 1e-6)
 
 
 def test_qk_norm_rope_backward_refuses():
