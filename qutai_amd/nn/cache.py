@@ -134,13 +134,18 @@ class QuantizedKVCache:
         lengths = tuple(n + m for n, m in zip(self.lengths or (0,) * batch, counts))
         if max(lengths) > self.capacity:
             raise ValueError("the cache's capacity is exceeded")
-        if self.codes is None:  # (cache_quantize checks them too, but behind reserve)
+        first = self.codes is None
+        if first:  # (cache_quantize checks them too, but behind reserve)
             amd_lm.cache_rows(keys, values, batch, new, kv_heads, dim, **columns)
-        with unchanged_on_failure(self):
+        try:
             self.reserve(batch, kv_heads, dim)
             start, starts = self.positions()
             held = None if min(counts) == new else amd.storage(counts, dtype="int64")
             amd_lm.cache_quantize(self.codes, keys, values, new, start=start, starts=starts, counts=held, **columns)
+        except BaseException:
+            if first:  # a refused call settles nothing
+                self.codes, self.lengths = None, ()
+            raise
         self._set_lengths(lengths)
         self._last = new, start, starts, held
 
