@@ -108,13 +108,13 @@ class QuantizedKVCache:
         elif (batch, kv_heads, dim) != (self.codes.batch, self.codes.kv_heads, self.codes.dim):
             raise ValueError("new keys and values must match the cache in batch, heads and head size")
 
-    def state(self):
-        """What the cache holds now, for ``restore``."""
+    def _state(self):
+        """What the cache holds now, for ``_restore``."""
         return self.codes, self.lengths, self._base, self._stored, self._shift, self._last
 
-    def restore(self, state):
-        """Back to an earlier ``state``: the positions appended since are forgotten
-        (those that were truncated since are not there again)."""
+    def _restore(self, state):
+        """Back to an earlier ``_state``, behind which there were appends alone:
+        positions truncated in between may have been written again."""
         self.codes, self.lengths, self._base, self._stored, self._shift, self._last = state
 
     def append(self, keys, values, counts=None):
@@ -190,7 +190,7 @@ class unchanged_on_failure:
     are as they were before, so that the call may be made again."""
 
     def __init__(self, *caches):
-        self.states = [(cache, cache.state()) for cache in caches]
+        self.states = [(cache, cache._state()) for cache in caches]
 
     def __enter__(self):
         return self
@@ -198,4 +198,4 @@ class unchanged_on_failure:
     def __exit__(self, kind, value, traceback):
         if kind is not None:
             for cache, state in self.states:
-                cache.restore(state)
+                cache._restore(state)
