@@ -416,7 +416,7 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * one wider matrix; q_out and k_out are contiguous.  Either side may be absent
  * (0 heads, NULL pointers).  dtype QA_F32 or QA_BF16 for rows and outputs; the
  * norm, the angles' sine and cosine and the products are fp32, the angles'
- * reduction fp64.  batch x time is below 2^31.  Outputs share no memory with inputs.  The unfused form is
+ * reduction fp64 (the reduced angle is rounded to fp32: at most pi 2^-24 off).  batch x time is below 2^31.  Outputs share no memory with inputs.  The unfused form is
  * qutai_amd_rms_norm per head and qutai_amd_rope_rows. */
 int qutai_amd_qk_norm_rope(const void* q, const void* k, const float* q_weight, const float* k_weight, void* q_out,
                            void* k_out, const int64_t* starts, int64_t offset, int64_t batch, int64_t time,
@@ -449,10 +449,13 @@ int64_t qutai_amd_qk_norm_rope_workspace(int64_t dim);
  * among the kept tokens goes to probabilities (fp32).  Temperature 0 takes the
  * largest logit, the lowest index of equal ones, with probability 1.  A NaN
  * counts as -inf; a row of nothing else gives token -1 with probability 0; beside
- * +inf every finite logit weighs nothing.  Weights and their sums are 64-bit.
+ * +inf every finite logit weighs nothing.  Weights and their sums are 64-bit; the
+ * sums that top_p compares count weights in units of 2^-45 of the largest (2^-42 in
+ * 2^20 tokens).
  * Each parameter is one number, or where its pointer is not NULL one per row
  * (there a temperature that is not above 0 counts as 0, a top_k below 1, a top_p
- * of 1 and more and a min_p below 0 as no filter, a min_p above 1 as 1).  A token
+ * of 1 and more and a min_p below 0 as no filter, a min_p above 1 as 1; a NaN is a
+ * temperature of 0, no top_p, a min_p of 1).  A token
  * that weighs less than 2^-100 of the largest is never taken. */
 int qutai_amd_sample(const void* logits, const void* uniforms, int64_t* tokens, float* probabilities, int64_t rows,
                      int64_t vocab, const float* temperatures, double temperature, const int64_t* top_ks,
@@ -480,12 +483,13 @@ int qutai_amd_attention_cached(const void* q, const void* k, const void* v, void
  * bits 8: a scale per row, codes -127 .. 127; bits 4: a scale per 32 channels,
  * codes -7 .. 7.  A scale is the smallest bfloat16 from 2^-100 up whose product
  * with 127 (7) reaches the group's largest magnitude; a code is x / scale rounded
- * to nearest, ties to even, and stands for code x scale (exact in fp32).  A group
- * with an infinity or NaN stands for NaN.  key_codes and value_codes (16-byte
+ * to nearest, ties to even, and stands for code x scale (exact in fp32; with bits 4
+ * a magnitude above 3.396e38 may stand for infinity).  A group with an infinity or
+ * NaN stands for NaN.  key_codes and value_codes (16-byte
  * aligned) hold qutai_amd_cache_pitch(dim) x bits / 8 bytes for each cached
  * position, in an order of the library's own; key_scales and value_scales one
  * bfloat16 (bits 8) or pitch / 32 of them (bits 4).  batch x fresh x kv_heads
- * below 2^25. */
+ * at most 2^25. */
 int qutai_amd_cache_quantize(const void* keys, const void* values, void* key_codes, void* key_scales,
                              void* value_codes, void* value_scales, const int64_t* starts, const int64_t* counts,
                              int64_t start, int64_t batch, int64_t fresh, int64_t kv_heads, int64_t dim,
@@ -512,7 +516,8 @@ int qutai_amd_cache_dequantize(const void* key_codes, const void* key_scales, co
  * (the size may grow from any length to the next, and never falls: one workspace for
  * the largest serves all); too small a one is QA_EWORKSPACE.  capacity is a multiple of 32 (at most 2^30; what lies behind a
  * sequence's last position may be anything), the scales are 4-byte aligned;
- * batch x fresh x heads at most 2^25; scale lies between 1e-30 and 1e30. */
+ * batch x fresh x heads at most 2^25, batch x kv_heads 2^22; scale lies between 1e-30
+ * and 1e30.  Sums of values up to 1e27 in magnitude stay within fp32. */
 int qutai_amd_attention_quantized(const void* q, const void* key_codes, const void* key_scales,
                                   const void* value_codes, const void* value_scales, void* out, const int64_t* starts,
                                   const int64_t* counts, int64_t start, int64_t batch, int64_t fresh, int64_t heads,

@@ -24,17 +24,19 @@
 // parts (BLOCKS = 2) half of the columns belong to a second block of keys: zeros in
 // the operands keep the other block's products out, and what is done with the scores
 // and the probabilities is done for both blocks at once (16 sequences of up to 8000
-// keys, 4 bits: 43 us with one, 37 with two).
+// keys, 4 bits, ranges joined: 42 us with one, 35 with two).
 //
 // The running maximum of a row is only raised when a score exceeds it by 2^8
 // (in powers of two): fp32 holds the sums all the same, and nearly every block
-// then runs without an exchange between lanes or a rescaling of the sums.
+// then runs without an exchange between lanes or a rescaling of the sums.  (So a
+// weight is 2^8 at most: sums of up to 2^30 values of 1e27 stay within fp32.)
 //
 // Bound by HBM with 8 bits and few rows: 32 sequences of up to 16000 keys, 32 heads
-// of 128 over 8, 0.67 GB: 129 us (5.2 TB/s; a wave per query and head 9072), and 5 to
-// join.  Bound by vector operations with 4 bits (16 of up to 8000 keys, 92 MB: 34 us)
+// of 128 over 8, 0.67 GB: 128 to 131 us (5.1 TB/s; a wave per query and head 9072), and
+// 5 to join.  Bound by vector operations with 4 bits (16 of up to 8000 keys, 92 MB: 34 us,
+// and 4 to join)
 // and with many rows, where the softmax of a block costs more than its codes (512
-// new positions over 3500, 16 heads of 64 over 4: 62 us for 7.4 GFLOP).
+// new positions over 3500, 16 heads of 64 over 4: 63 us for 7.4 GFLOP).
 #pragma once
 #include <type_traits>
 

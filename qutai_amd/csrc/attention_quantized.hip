@@ -14,6 +14,12 @@ namespace {
 // same (32 of up to 14000, 8 bits: 120 us, 132 with two, 128 with six).  Where it
 // has many rows, whose sums a split one writes and reads again: one (512 new
 // positions over 3500: 63 us, 79 with two, 96 with four).
+// Few rows are those that share a tile (bf16 8 and fewer, fp32 4).  From there to
+// some 32 rows the keys of a long cache bound a call as before, and it would gain
+// from the ranges of few rows, which it does not get: 32 sequences of up to 14000, 8
+// bits, bf16, 8 kv heads of 128: 129 us with 8 rows, 200 with 9 to 17, 209 with 32 (150
+// to 157, and 167); 16 of up to 8000, 4 bits: 43 with 8, 82 with 9 (71); fp32, 16 of
+// up to 7000, 8 bits: 41 with 4, 64 to 69 with 5 to 17 (62 to 68), 73 with 32 (76).
 constexpr int64_t FEW_ROWS = 512, MANY_ROWS = 256, LONG_RANGE = 2048;
 
 AttendPlan plan_of(int64_t batch, int64_t fresh, int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int bits,

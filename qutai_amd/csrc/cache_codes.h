@@ -3,8 +3,9 @@
 // A group of channels -- the row where codes have 8 bits, 32 channels where they
 // have 4 -- shares a scale: the smallest bfloat16 s >= 2^-100 with M s >= the
 // group's largest magnitude, M = 127 or 7; a code is x / s rounded to nearest,
-// ties to even, and stands for code * s, a product that fp32 holds exactly.  A
-// group with an infinity or NaN has the scale NaN (and codes 0).
+// ties to even, and stands for code * s, a product that fp32 holds exactly (but
+// where M = 7 and a magnitude lies above 3.396e38: 7 s is then beyond fp32, infinity).
+// A group with an infinity or NaN has the scale NaN (and codes 0).
 //
 // Rows are padded to a pitch P of channels (zeros).  Eight bits: a byte per
 // channel, in order.  Four bits: nibbles of code + 8 in the order in which the

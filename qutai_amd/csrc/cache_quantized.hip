@@ -24,7 +24,7 @@ struct WriteArgs {
   const int64_t* starts;
   const int64_t* counts;
   int64_t start, capacity;
-  uint32_t fresh, heads, rows;  // rows: batch x fresh x heads, below 2^25
+  uint32_t fresh, heads, rows;  // rows: batch x fresh x heads, at most 2^25
   int dim, pitch, vector;
 };
 
@@ -239,8 +239,8 @@ extern "C" int qutai_amd_cache_quantize(const void* keys, const void* values, vo
     return QA_EINVAL;
   if (start < -(1ll << 40) || start > (1ll << 40)) return QA_EINVAL;
   if (batch == 0 || fresh == 0) return QA_OK;
-  const int64_t most = 1ll << 28;  // rows: below 2^32 threads in a launch, 64 lanes to a row at most, and keys and values
-  if (fresh > most / batch || batch * fresh > most / kv_heads / 8 || (int64_t)capacity * kv_heads > (1ll << 44) / batch)
+  const int64_t most = 1ll << 25;  // rows: 32 lanes each at most, a lane has two or four: 2^30 threads for keys and values
+  if (fresh > most / batch || batch * fresh > most / kv_heads || (int64_t)capacity * kv_heads > (1ll << 44) / batch)
     return QA_EINVAL;
   for (const int64_t row : {key_row, value_row})
     if (batch * fresh > (1ll << 60) / row) return QA_EINVAL;

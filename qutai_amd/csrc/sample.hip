@@ -16,8 +16,11 @@
 //  top_k: the k-th largest of the threads' maxima (two each) bounds the k-th largest logit
 //  from below; the few logits from there on go into a list in LDS, where the
 //  threshold is found.
-//  top_p: weights in bins of 1/32 of a power of two, whose sums are 64-bit integers
-//  (weight times 2^45, or less for very large vocabularies): exact in any order.
+//  top_p: weights in bins of 1/32 of a power of two, whose sums are 64-bit integers:
+//  the same in any order.  They count each weight in units of 2^-45 of the largest
+//  (2^-42 in 2^20 tokens), so the prefix may end one token off where a sum of more
+//  bits lies within the roundings of its goal, and a top_p within some 2^-29 of 1 leaves
+//  out tokens that weigh less than half a unit.
 //  The logits of the bin that the prefix ends in go into the list.
 // A list is searched digit by digit of its keys (bits in an order of unsigned
 // integers), from histograms, a short one by comparing all with all.  Where it

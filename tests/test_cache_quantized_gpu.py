@@ -288,6 +288,37 @@ def test_large_scores_and_scales():
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+def test_the_largest_magnitudes(bits):
+    """fp32's largest number: 8 bits hold it; with 4 bits 7 times the scale that
+    holds what lies above 3.396e38 is beyond fp32, and infinity."""
+    most = float(np.finfo(np.float32).max)
+    x = np.zeros((1, 3, 1, 32), dtype=np.float32)
+    x[0, :, 0, 3] = most, 3.3961e38, -3.39e38
+    cache = QuantizedKVCache(3, bits=bits)
+    cache.append(as_tensor(x, "float32"), as_tensor(x, "float32"))
+    exact = held(x, bits)
+    expected = np.where(np.abs(exact) > most, np.copysign(np.inf, exact), exact).transpose(0, 2, 1, 3)
+    assert all(np.array_equal(got, expected) for got in read(cache))
+    assert np.isfinite(expected).all() == (bits == 8) and np.isfinite(expected[0, 0, 1:]).all()
+
+
+@pytest.mark.parametrize("dtype,bits", [("float32", 8), ("float32", 4), ("bfloat16", 8), ("bfloat16", 4)])
+def test_sums_of_large_values_stay_in_range(dtype, bits):
+    """Values of 1e27, keys whose scores rise by less than 2^8 along the sequence,
+    so that weights above 1 are summed."""
+    rng = np.random.default_rng(16)
+    k, v = np.zeros((1, 3000, 1, 32)), 1e27 * (1 - 0.2 * rng.random((1, 3000, 1, 32)))
+    k[..., 0] = np.linspace(0, 30, 3000)[None, :, None]
+    cache = QuantizedKVCache(3000, bits=bits)
+    cache.append(as_tensor(k[:, :2999], dtype), as_tensor(v[:, :2999], dtype))
+    cache.append(as_tensor(k[:, 2999:], dtype), as_tensor(v[:, 2999:], dtype))
+    q = np.zeros((1, 1, 2, 32))
+    q[..., 0] = 1.0
+    out = download(cache.attend(as_tensor(q, dtype)).storage).reshape(q.shape)
+    check_attention(out, q, *read(cache), (2999,), (1,), 32 ** -0.5, dtype, bits)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
 def test_rows_beyond_four_gigabytes(bits):
     """The last heads' codes lie behind the 32-bit offsets."""
     rng = np.random.default_rng(10)

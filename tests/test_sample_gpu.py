@@ -171,3 +171,16 @@ def test_no_rows():
     empty = amd.AMDStorage(0, "float32")
     tokens, probabilities = amd_lm.sample(empty, empty, 0, 10)
     assert tokens.size == 0 and probabilities.size == 0 and tokens.dtype == "int64"
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_parameters_of_rows_that_are_not_numbers(dtype):
+    """NaN: a temperature of 0, no top_p, a min_p of 1."""
+    rng = np.random.default_rng(3)
+    logits, nan = stored(rng.standard_normal((6, 40)), dtype), float("nan")
+    given = dict(temperature=[nan, 1.0, 1.0, nan, 0.7, 1.0], top_p=[1.0, nan, 1.0, nan, 0.4, 2.0], min_p=[0.0, 0.0, nan, nan, -1.0, 3.0])
+    meant = dict(temperature=[0.0, 1.0, 1.0, 0.0, 0.7, 1.0], top_p=[1.0, 1.0, 1.0, 1.0, 0.4, 1.0], min_p=[0.0, 0.0, 1.0, 1.0, 0.0, 1.0])
+    results = [amd_lm.sample(upload(logits, dtype), upload(np.full(6, 0.6), "float32"), 6, 40,
+                             **{n: upload(np.array(v), "float32") for n, v in p.items()}) for p in (given, meant)]
+    assert all(a.to_array() == b.to_array() for a, b in zip(*results))
+    assert list(download(results[0][0])[[0, 2, 3, 5]]) == list(logits[[0, 2, 3, 5]].argmax(1))
