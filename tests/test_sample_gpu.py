@@ -184,3 +184,18 @@ def test_parameters_of_rows_that_are_not_numbers(dtype):
                              **{n: upload(np.array(v), "float32") for n, v in p.items()}) for p in (given, meant)]
     assert all(a.to_array() == b.to_array() for a, b in zip(*results))
     assert list(download(results[0][0])[[0, 2, 3, 5]]) == list(logits[[0, 2, 3, 5]].argmax(1))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [4097, 140000])
+def test_infinities_and_ties_in_long_rows(dtype, vocab):
+    """+inf in a few places and in more than top_k keeps, NaN in a third, and all
+    logits alike, in rows longer than the list of candidates and than the registers."""
+    rng = np.random.default_rng(vocab)
+    rows = rng.standard_normal((4, vocab)) * 3
+    rows[0, rng.integers(0, vocab, 3)] = np.inf
+    rows[1, rng.integers(0, vocab, 900)] = np.inf
+    rows[2, ::3] = np.nan
+    rows[3] = -7.25
+    for setting in (dict(), dict(top_k=5), dict(top_k=700, top_p=0.4), dict(top_p=0.5), dict(min_p=1.0), dict(temperature=0.0)):
+        check(rows, rng.random(4), dtype, **setting)
