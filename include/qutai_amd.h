@@ -405,6 +405,72 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
                             int64_t heads, int64_t kv_heads, int64_t time, int64_t dim, int dtype, int layout,
                             double scale, int causal, void* stream);
 
+/* Attention among the tokens of each of several sequences of different lengths
+ * that lie one behind the other in one matrix of tokens, as
+ * qutai_amd_attention_fwd of each alone (causal != 0: a token sees its sequence up
+ * to itself).  q, k and v rows start q_row, k_row and v_row elements after the
+ * previous token's (columns of wider matrices), heads `dim` elements after each
+ * other; out is contiguous [tokens][heads][dim], lse fp32 [tokens][heads].  `tiles`
+ * (device, int64 triples) says which rows the workgroups take, `tile_rows` each
+ * and in this order: the sequence's first token, its length, and the tile's first
+ * row in it, a multiple of tile_rows; tiles cover every row once.  tile_rows is
+ * what qutai_amd_attention_packed_rows returns for the call's sizes, `longest`
+ * sequence, scale and pass (0: forward, 1: the backward's query tiles, 2: its key
+ * tiles); aligned: every pointer and pitch is a multiple of 16 bytes.  Rows in no
+ * tile are left as they are.  dtype QA_F32 or QA_BF16, dim up to 256. */
+int64_t qutai_amd_attention_packed_rows(int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype,
+                                        int aligned, double scale, int pass);
+int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
+                                   double scale, int causal, void* stream);
+/* Its gradients: grad is that of out (contiguous), out and lse the forward's; dq,
+ * dk and dv rows start dq_row, dk_row and dv_row elements after each other; delta
+ * is scratch, fp32 [tokens][heads].  Every gradient is summed in a fixed order. */
+int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                   const float* lse, void* dq, void* dk, void* dv, float* delta,
+                                   const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
+                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
+                                   int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
+                                   void* stream);
+
+/* The first `rotary` channels (even) of every query and key head turned by their
+ * token's position: pair i (channels 2i and 2i+1, or with half != 0 i and i +
+ * rotary/2) by p * turns[i] whole turns (`turns` is HOST memory, rotary/2 fp64
+ * values), times `magnitude`; inverse != 0 turns back (the gradient).  p is
+ * positions[token] (device), or offset + t + starts[b] where it is NULL (starts may
+ * be NULL).  Rows of q, k and of the results start q_row, k_row, q_out_row and
+ * k_out_row elements after the previous token's; results may be in place of the
+ * inputs.  Either side may be absent (0 heads).  dtype QA_F32 or QA_BF16; angles
+ * are reduced in fp64, one rounding at the end. */
+int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, const double* turns,
+                     const int64_t* positions, const int64_t* starts, int64_t offset, int64_t batch, int64_t time,
+                     int64_t heads, int64_t kv_heads, int64_t dim, int64_t rotary, int64_t q_row, int64_t k_row,
+                     int64_t q_out_row, int64_t k_out_row, int half, double magnitude, int inverse, int dtype,
+                     void* stream);
+
+/* One AdamW step over `count` tensors.  `tensors` is HOST memory, eight int64 each:
+ * addresses of the parameter, its gradient, its first and second moments and its
+ * moments' exponents (8 bits only), its values, its dtype (QA_F32 or QA_BF16, the
+ * gradient's too) and a number that tells it from the others (8 bits: part of what
+ * decides how its codes are rounded, with `seed` and `step`).  bits 32: moments are
+ * fp32.  bits 8: one byte a value, and two exponents (int8, first and second) for
+ * every 256 values; zeros stand for zeros.
+ *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
+ *   p' = p (1 - rate weight_decay) - rate m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
+ * With max_norm > 0 gradients are scaled to that norm over all tensors where they
+ * exceed it, the norm goes to `norm` (fp64, device, may be NULL), a norm that is not
+ * finite leaves everything as it is, and `workspace` holds at least
+ * qutai_amd_adamw_workspace fp64 values. */
+int64_t qutai_amd_adamw_workspace(const int64_t* tensors, int64_t count);
+int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate, double beta1, double beta2,
+                    double eps, double weight_decay, int64_t step, uint64_t seed, double max_norm, double* workspace,
+                    int64_t workspace_values, double* norm, void* stream);
+/* The values that `count` moments of 8 bits stand for. */
+int qutai_amd_adamw_moments(const void* first, const void* second, const void* exponents, float* first_out,
+                            float* second_out, int64_t count, void* stream);
+
 /* RMSNorm of every query and key head and the rotation of its position, in one
  * launch: for each row x of `dim` values (even, at most 256) of [batch][time]
  * positions and heads (kv_heads) heads,

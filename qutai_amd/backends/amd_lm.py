@@ -667,6 +667,114 @@ def attention_backward(gradient, q, k, v, out, lse, batch, time, heads, kv_heads
     return dq, dk, dv
 
 
+def _packed_places(q, k, v, packing, heads, kv_heads, dim, places):
+    """Pointers and pitches of the q, k and v rows of a packed call, which it
+    checks, and whether all of them are whole 16-byte chunks."""
+    if len({q.dtype, k.dtype, v.dtype}) != 1 or q.dtype not in ("bfloat16", "float32"):
+        raise ValueError("attention takes q, k, v of one dtype, bfloat16 or float32")
+    if not 0 < dim <= 256 or kv_heads <= 0 or heads <= 0 or heads % kv_heads:
+        raise ValueError("attention needs 0 < head dimension <= 256 and heads divisible by kv_heads")
+    sides = ((q, heads, *places[0]), (k, kv_heads, *places[1]), (v, kv_heads, *places[2]))
+    found = [_qk_rows(x, packing.total, n, dim, column, row, q.dtype) for x, n, column, row in sides]
+    item = _TYPES[q.dtype][1]
+    return found, all(at % 16 == 0 and row * item % 16 == 0 for at, row in found) and dim * item % 16 == 0
+
+
+def _packed_tail(packing, *blocks):
+    """Zeros in the rows behind the last sequence of contiguous results."""
+    if packing.used < packing.total:
+        for x in blocks:
+            if x is not None:
+                width = x.size // packing.total
+                start = packing.used * width
+                x.runtime.call("qutai_amd_fill", x.ptr + start * _TYPES[x.dtype][1], x.size - start, 0.0, code(x.dtype))
+
+
+def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, scale=None, q_column=0, q_row=None,
+                     k_column=0, k_row=None, v_column=0, v_row=None, rest=False):
+    """(out, lse float32) of attention among the tokens of each sequence of a
+    ``packing`` (an ``lm.Packing``): as ``attention``, with the sequences one
+    behind the other in the rows of q, k and v, which may be columns q_column ..
+    of matrices of q_row elements per token (and so on).  out is contiguous
+    [total][heads][dim], lse [total][heads]; rows behind the last sequence are
+    zero.  With ``rest`` also what out's rounding left, for the backward (None
+    where there is none)."""
+    ((q_at, q_row), (k_at, k_row), (v_at, v_row)), whole = _packed_places(
+        q, k, v, packing, heads, kv_heads, dim, ((q_column, q_row), (k_column, k_row), (v_column, v_row)))
+    runtime, dtype = get_runtime(), code(q.dtype)
+    out, lse = AMDStorage(packing.total * heads * dim, q.dtype), AMDStorage(packing.total * heads, "float32")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if packing.used:
+        rows = runtime.lib.qutai_amd_attention_packed_rows(heads, kv_heads, dim, packing.longest, dtype, int(whole), scale, 0)
+        tiles, count = packing.tiles(rows, "end" if causal else "length")
+        runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, tiles.ptr, count, rows, heads,
+                     kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
+                     mfma=_on_matrix_cores(q.dtype, dim))
+    _packed_tail(packing, out, lse)
+    return (out, lse, None) if rest else (out, lse)
+
+
+def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_heads, dim, *, causal=True, scale=None,
+                              q_column=0, q_row=None, k_column=0, k_row=None, v_column=0, v_row=None, rest=None,
+                              into=None):
+    """(dq, dk, dv) of ``attention_packed``: its operands and options, its out, lse
+    and rest, and the contiguous gradient of out.  The results are contiguous, or
+    with ``into`` (a storage laid out as the one matrix that q, k and v are columns
+    of) its columns q_column .., k_column .., v_column ...; every one is summed in
+    a fixed order.  Rows behind the last sequence are zero."""
+    places = ((q_column, q_row), (k_column, k_row), (v_column, v_row))
+    ((q_at, q_row), (k_at, k_row), (v_at, v_row)), whole = _packed_places(q, k, v, packing, heads, kv_heads, dim, places)
+    total = packing.total
+    if gradient.dtype != q.dtype or out.dtype != q.dtype or lse.dtype != "float32":
+        raise ValueError("attention backward needs gradient/out of the activations' dtype and a float32 lse")
+    if gradient.size != total * heads * dim or out.size != gradient.size or lse.size != total * heads:
+        raise ValueError("gradient/out/lse sizes do not match (total, heads, dim)")
+    if rest is not None and (rest.dtype != q.dtype or rest.size != out.size):
+        raise ValueError("rest is what attention_packed returned beside out")
+    if into is None:
+        results = tuple(AMDStorage(total * n * dim, q.dtype) for n in (heads, kv_heads, kv_heads))
+        targets = [(x.ptr, n * dim) for x, n in zip(results, (heads, kv_heads, kv_heads))]
+    else:
+        row, spans = q_row, sorted((column, column + n * dim) for (column, _), n in zip(places, (heads, kv_heads, kv_heads)))
+        if not q_row == k_row == v_row or any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("into holds the gradients in separate columns of one row")
+        for x in (gradient, q, k, v, out):
+            if into.ptr < x.ptr + x.nbytes and x.ptr < into.ptr + into.nbytes:
+                raise ValueError("into must not share memory with an input")
+        results = (into,) * 3
+        targets = [_qk_rows(into, total, n, dim, column, row, q.dtype)
+                   for (column, _), n in zip(places, (heads, kv_heads, kv_heads))]
+    whole = whole and all(at % 16 == 0 and row * _TYPES[q.dtype][1] % 16 == 0
+                          for at, row in (*targets, (gradient.ptr, 0), (out.ptr, 0)))
+    runtime, dtype = get_runtime(), code(q.dtype)
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if packing.used:
+        delta = AMDStorage(total * heads, "float32")
+        q_rows, k_rows = (runtime.lib.qutai_amd_attention_packed_rows(heads, kv_heads, dim, packing.longest, dtype,
+                                                                      int(whole), scale, n) for n in (1, 2))
+        q_tiles, q_count = packing.tiles(q_rows, "end" if causal else "length")
+        k_tiles, k_count = packing.tiles(k_rows, "start" if causal else "length")
+        runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, lse.ptr,
+                     *(at for at, _ in targets), delta.ptr, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count, k_rows,
+                     heads, kv_heads, dim, q_row, k_row, v_row, *(row for _, row in targets), dtype, scale,
+                     int(bool(causal)), mfma=_on_matrix_cores(q.dtype, dim))
+    if into is None:
+        _packed_tail(packing, *results)
+    elif packing.used < total:
+        tail = total - packing.used
+        for (at, row), n in zip(targets, (heads, kv_heads, kv_heads)):
+            _zero_columns(into, at, tail, packing.used, row, n * dim)
+    return results
+
+
+def _zero_columns(block, at, rows, first, row, width):
+    """Zeros in ``rows`` rows from ``first`` on of the columns that start at
+    address ``at`` of a matrix of ``row`` elements per row."""
+    zeros = amd.full(rows * width, 0.0, dtype=block.dtype)
+    column = (at - block.ptr) // _TYPES[block.dtype][1]
+    amd._copy_strided(zeros, block, (rows, width), (width, 1), (row, 1), source_offset=0, target_offset=first * row + column)
+
+
 # ---- decoder glue (the rest of a Decoder.loss step) ---------------------------------
 
 def _acc_dtype(dtype):
@@ -926,6 +1034,107 @@ def qk_norm_rope_backward(gq, gk, q, k, q_weight, k_weight, batch, time, heads, 
                  kv_heads, dim, q_step, k_step, dq_step, dk_step, float(theta), float(eps), code(dtype),
                  amd._p(workspace), need)
     return dq, dk, dwq, dwk
+
+
+def rotary(q, k, rotary, batch, time, heads, kv_heads, dim, *, positions=None, offset=0, starts=None, inverse=False,
+           q_column=0, q_row=None, k_column=0, k_row=None, out=None, out_row=None, out_q_column=0, out_k_column=None):
+    """(q, k) with the first channels of every head turned by their tokens'
+    positions as ``rotary`` (an ``lm.Rotary``) says, in one launch; ``inverse``
+    turns back, which is the gradient.  Token t of sequence b is at positions[b *
+    time + t] (int64 storage of one per token), or at offset + t plus starts[b]
+    (int64 storage of one per sequence).  q and k are columns q_column .. and
+    k_column .. of matrices of q_row (k_row) elements per token.  The results are
+    contiguous [batch][time][heads][dim], or with ``out`` its columns out_q_column
+    .. and out_k_column .. (out_row elements per token; ``out`` may be the matrix
+    that q and k are columns of, if they are the same columns).  0 heads leave a
+    side out (its result is None)."""
+    if rotary.dim != dim or min(batch, time, heads, kv_heads) < 0 or heads + kv_heads == 0:
+        raise ValueError("rotary turns query or key heads of its own width")
+    if inverse not in (False, True) or offset != int(offset):
+        raise ValueError("inverse is True or False, the offset an integer")
+    tokens = batch * time
+    if positions is not None and (starts is not None or offset or positions.dtype != "int64" or positions.size != tokens):
+        raise ValueError("positions hold one int64 for every token, without offset and starts")
+    if starts is not None and (starts.dtype != "int64" or starts.size != batch):
+        raise ValueError("starts holds one int64 position per sequence")
+    dtype = (q if heads else k).dtype
+    if dtype not in ("bfloat16", "float32"):
+        raise ValueError("rotary takes bfloat16 or float32 rows")
+    sides = ((q, heads, q_column, q_row, out_q_column),
+             (k, kv_heads, k_column, k_row, heads * dim if out_k_column is None else out_k_column))
+    sources = [_qk_rows(x, tokens, n, dim, column, row, dtype) for x, n, column, row, _ in sides]
+    if out is not None:
+        targets = [_qk_rows(out, tokens, n, dim, column, out_row, dtype) for _, n, _, _, column in sides]
+        for (x, n, *_), source, target in zip(sides, sources, targets):
+            if n and source != target and out.ptr < x.ptr + x.nbytes and x.ptr < out.ptr + out.nbytes:
+                raise ValueError("out shares memory with an input that is not in its place")
+        (q_to, q_out), (k_to, k_out) = targets
+        item = _TYPES[dtype][1]
+        if heads and kv_heads and (q_out != k_out or not (q_to + heads * dim * item <= k_to
+                                                          or k_to + kv_heads * dim * item <= q_to)):
+            raise ValueError("out holds q's and k's results in separate columns of one row")
+        results = tuple(out if n else None for n in (heads, kv_heads))
+    else:
+        results = tuple(AMDStorage(tokens * n * dim, dtype) if n else None for n in (heads, kv_heads))
+        (q_to, q_out), (k_to, k_out) = ((amd._p(x), n * dim) for x, n in zip(results, (heads, kv_heads)))
+    (q_at, q_step), (k_at, k_step) = sources
+    if tokens:
+        get_runtime().call("qutai_amd_rotary", q_at, k_at, q_to, k_to, rotary.turns, amd._p(positions), amd._p(starts),
+                           offset, batch, time, heads, kv_heads, dim, rotary.rotary_dim, q_step, k_step, q_out, k_out,
+                           int(rotary.layout == "half"), rotary.magnitude, int(inverse), code(dtype))
+    return results
+
+
+class AdamWMoments:
+    """Device memory of one tensor's moments: fp32, or 8-bit codes and an exponent
+    for every 256 values of each, laid out by the library."""
+
+    def __init__(self, size, bits):
+        self.size, self.bits = size, bits
+        if bits == 32:
+            self.first, self.second = (amd.full(size, 0.0, dtype="float32") for _ in range(2))
+            self.exponents = None
+        else:  # bytes, as whole int64 words of zeros
+            self.first, self.second = (amd.full((size + 7) // 8, 0, dtype="int64") for _ in range(2))
+            self.exponents = amd.full((2 * ((size + 255) // 256) + 7) // 8, 0, dtype="int64")
+
+    def storages(self):
+        return (self.first, self.second) if self.exponents is None else (self.first, self.second, self.exponents)
+
+    def values(self):
+        """(first, second) as fp32 storages."""
+        if self.bits == 32:
+            return self.first, self.second
+        out = AMDStorage(self.size, "float32"), AMDStorage(self.size, "float32")
+        if self.size:
+            out[0].runtime.call("qutai_amd_adamw_moments", self.first.ptr, self.second.ptr, self.exponents.ptr,
+                                out[0].ptr, out[1].ptr, self.size)
+        return out
+
+
+def adamw(tensors, bits, lr, beta1, beta2, eps, weight_decay, step, *, seed=0, max_norm=None):
+    """One AdamW step (its ``step``-th, from 1) over ``tensors``: tuples of a
+    parameter's storage, its gradient's, its AdamWMoments and the number that
+    tells it from the others where 8-bit codes are rounded.  Parameters and moments
+    are changed in place.  With ``max_norm`` returns the fp64 storage that holds
+    the norm of all gradients, else None."""
+    table = array("q")
+    for p, g, moments, index in tensors:
+        if p.dtype not in ("bfloat16", "float32") or g.dtype != p.dtype or not p.size == g.size == moments.size \
+                or moments.bits != bits:
+            raise ValueError("adamw takes float32 or bfloat16 parameters with gradients and moments of their size")
+        table.extend((p.ptr, g.ptr, moments.first.ptr, moments.second.ptr, amd._p(moments.exponents), p.size,
+                      code(p.dtype), index))
+    runtime, count, address = get_runtime(), len(tensors), table.buffer_info()[0]
+    norm = workspace = None
+    if max_norm is not None:  # the step writes it if any gradient has a value
+        norm = AMDStorage(1, "float64") if any(p.size for p, *_ in tensors) else amd.full(1, 0.0, dtype="float64")
+        workspace = AMDStorage(runtime.lib.qutai_amd_adamw_workspace(address, count), "float64")
+    if count:
+        runtime.call("qutai_amd_adamw", address, count, bits, lr, beta1, beta2, eps, weight_decay, step, seed,
+                     0.0 if max_norm is None else max_norm, amd._p(workspace), 0 if workspace is None else workspace.size,
+                     amd._p(norm))
+    return norm
 
 
 def copy_rows(source, rows, width, *, column=0, row=None, out=None, out_column=0, out_row=None):

@@ -158,7 +158,7 @@ struct AttnStage {
   bool lo[Tile::ITEMS], hi[Tile::ITEMS];
   Raw8<F32> raw[Tile::ITEMS];
 
-  __device__ __forceinline__ void plan(int tid, int64_t stride, int D) {
+  __device__ __forceinline__ void plan(int tid, int64_t x_stride, int64_t y_stride, int D) {
 #pragma unroll
     for (int j = 0; j < Tile::ITEMS; j++) {
       const int idx = tid + 256 * j, q = idx % (Tile::KB * Tile::CK);
@@ -166,15 +166,19 @@ struct AttnStage {
       row[j] = r;
       lo[j] = 8 * c < D;
       hi[j] = 8 * c + 4 < D;
-      off[j] = (uint32_t)((r * stride + 8 * c) * ES);
+      const bool second = idx / (Tile::KB * Tile::CK);  // wave-uniform
+      off[j] = (uint32_t)((r * (second ? y_stride : x_stride) + 8 * c) * ES);
       lds[j] = (idx / (Tile::KB * Tile::CK)) * Tile::NX * Tile::PLANE + r * Tile::PITCH + ((c ^ Tile::swz(r)) * 8);
     }
   }
-  __device__ __forceinline__ void fetch(const char* x, const char* y, int64_t stride, int left, int wave) {
-    const int64_t bytes = Tile::KB * stride * ES;
-    const uint32_t n = bytes > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)bytes;
-    const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(x), 0, n, 0x00020000);
-    const auto ry = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(y), 0, n, 0x00020000);
+  __device__ __forceinline__ void fetch(const char* x, const char* y, int64_t x_stride, int64_t y_stride, int left,
+                                        int wave) {
+    const auto bytes = [](int64_t stride) {
+      const int64_t n = Tile::KB * stride * ES;
+      return n > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)n;
+    };
+    const auto rx = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(x), 0, bytes(x_stride), 0x00020000);
+    const auto ry = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(y), 0, bytes(y_stride), 0x00020000);
 #pragma unroll
     for (int j = 0; j < Tile::ITEMS; j++) {
       const bool in = row[j] < left;
@@ -259,19 +263,12 @@ __device__ __forceinline__ float log2_of(float lse, float& lo) {
   return hi;
 }
 
-template <bool F32, int DP>
-__global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) attention_fwd_mma(AttnGenArgs p) {
-  typedef AttnTile<F32, DP> Tile;
-  typedef AttnStage<F32, DP> Stage;
-  typedef typename std::conditional<F32, float, bf16_t>::type T_;
-  constexpr int KB = Tile::KB, QPB = 128, ES = F32 ? 4 : 2;
-  __shared__ __attribute__((aligned(16))) bf16_t tiles[2 * Tile::NX * Tile::PLANE];  // [K, V][plane]
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
-  const int T = (int)p.time, D = (int)p.dim;
-  const int blocks_q = (T + QPB - 1) / QPB;
-  // causal: the longest query blocks of every head first; otherwise one
-  // head's blocks on one XCD (as the D = 64 kernels)
-  int bh, qblk;
+// The (b, h) and query block of a workgroup.  Causal: the longest query blocks of
+// every head first; otherwise one head's blocks on one XCD (as the D = 64 kernels).
+template <class T, int ROWS>
+__device__ __forceinline__ void place_queries(const AttnGenArgs& p, int& b, int& h, int& qblk) {
+  const int blocks_q = ((int)p.time + ROWS - 1) / ROWS;
+  int bh;
   if (p.causal) {
     const int nbh = (int)(p.batch * p.heads);
     bh = uniform32((int)blockIdx.x % nbh);
@@ -281,8 +278,59 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
     bh = uniform32(pid / blocks_q);
     qblk = uniform32(pid % blocks_q);
   }
+  b = bh / (int)p.heads;
+  h = bh % (int)p.heads;
+}
+// Packed: the tiles come in their order of work, the heads of one tile together.
+template <class T, int ROWS>
+__device__ __forceinline__ void place_queries(AttnPackedArgs& p, int& b, int& h, int& qblk) {
+  const int heads = (int)p.heads, tile = uniform32((int)blockIdx.x / heads);
+  b = 0;
+  h = uniform32((int)blockIdx.x % heads);
+  qblk = enter_sequence<T>(p, tile) / ROWS;
+}
+
+// The (b, kv head), key block and query head of the group (of nsplit) of a workgroup.
+template <class T, int ROWS>
+__device__ __forceinline__ void place_keys(const AttnGenArgs& p, int nsplit, int& b, int& kvh, int& kblk, int& gsel) {
+  const int blocks_k = ((int)p.time + ROWS - 1) / ROWS;
+  int bkh;
+  if (p.causal) {  // the first keys see the most queries and start first
+    const int nbh = (int)(p.batch * p.kv_heads) * nsplit, id = (int)blockIdx.x % nbh;
+    bkh = uniform32(id / nsplit);
+    gsel = uniform32(id % nsplit);
+    kblk = uniform32((int)blockIdx.x / nbh);
+  } else {
+    const int pid = uniform32(xcd_remap(blockIdx.x, gridDim.x)), rest = pid % (blocks_k * nsplit);
+    bkh = uniform32(pid / (blocks_k * nsplit));
+    kblk = uniform32(rest / nsplit);
+    gsel = uniform32(rest % nsplit);
+  }
+  b = bkh / (int)p.kv_heads;
+  kvh = bkh % (int)p.kv_heads;
+}
+template <class T, int ROWS>
+__device__ __forceinline__ void place_keys(AttnPackedArgs& p, int nsplit, int& b, int& kvh, int& kblk, int& gsel) {
+  const int all = (int)p.kv_heads * nsplit, id = (int)blockIdx.x % all;
+  b = 0;
+  kvh = uniform32(id / nsplit);
+  gsel = uniform32(id % nsplit);
+  kblk = enter_sequence<T>(p, uniform32((int)blockIdx.x / all)) / ROWS;
+}
+
+template <bool F32, int DP, class Args = AttnGenArgs>
+__global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) attention_fwd_mma(Args p) {
+  typedef AttnTile<F32, DP> Tile;
+  typedef AttnStage<F32, DP> Stage;
+  typedef typename std::conditional<F32, float, bf16_t>::type T_;
+  constexpr int KB = Tile::KB, QPB = 128, ES = F32 ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) bf16_t tiles[2 * Tile::NX * Tile::PLANE];  // [K, V][plane]
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
+  int b, h, qblk;
+  place_queries<T_, QPB>(p, b, h, qblk);
+  const int T = (int)p.time, D = (int)p.dim;
   const int wg_q0 = qblk * QPB, q0 = uniform32(wg_q0 + wave * 32);
-  const int b = bh / (int)p.heads, h = bh % (int)p.heads, kvh = h / (int)(p.heads / p.kv_heads);
+  const int kvh = h / (int)(p.heads / p.kv_heads);
   const int64_t kbase = b * p.kb + kvh * p.kh;
   const char* K = uniform_ptr((const char*)p.k + kbase * ES);
   const char* V = uniform_ptr((const char*)p.v + kbase * ES);
@@ -305,10 +353,11 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
   const int nkb_w = p.causal ? min(nkb, (q0 + 32 + KB - 1) / KB) : nkb;
   const int n_full = min(nkb_w, (p.causal ? min(T, q0 + 1) : T) / KB);
   Stage stage;
-  stage.plan(tid, p.kt, D);
+  const int64_t vt = value_pitch(p);
+  stage.plan(tid, p.kt, vt, D);
   auto fetch = [&](int kbk) {
-    const int64_t at = (int64_t)kbk * KB * p.kt * ES;
-    stage.fetch(K + at, V + at, p.kt, T - kbk * KB, wave);
+    const int64_t at = (int64_t)kbk * KB * ES;
+    stage.fetch(K + at * p.kt, V + at * vt, p.kt, vt, T - kbk * KB, wave);
   };
   // block kbk into LDS (every wave has read the previous one), the next one
   // into registers
@@ -396,7 +445,7 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
   }
   if (t < T) {
     const float inv = Tile::SUM / total;
-    const int64_t at = b * p.qb + h * p.qh + (int64_t)t * p.qt;
+    const int64_t at = b * p.qb + h * p.qh + (int64_t)t * out_pitch(p);
 #pragma unroll
     for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
@@ -414,28 +463,19 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
 // a query that sees one key (or nearly so) is what O and V leave: an exact zero
 // for bf16.  With delta in fp32 fmas, the two sums' roundings stayed: 1.0% of
 // the bf16 dQ of 40 causal queries of 128 were not float64's rounded, 0.02% now.
-template <bool F32, int DP>
-__global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) attention_bwd_dq_mma(AttnGenArgs p) {
+template <bool F32, int DP, class Args = AttnGenArgs>
+__global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) attention_bwd_dq_mma(Args p) {
   typedef AttnTile<F32, DP> Tile;
   typedef AttnStage<F32, DP> Stage;
   typedef typename std::conditional<F32, float, bf16_t>::type T_;
   constexpr int KB = Tile::KB, QPB = 128, ES = F32 ? 4 : 2;
   __shared__ __attribute__((aligned(16))) bf16_t tiles[2 * Tile::NX * Tile::PLANE];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
+  int b, h, qblk;
+  place_queries<T_, QPB>(p, b, h, qblk);
   const int T = (int)p.time, D = (int)p.dim;
-  const int blocks_q = (T + QPB - 1) / QPB;
-  int bh, qblk;
-  if (p.causal) {
-    const int nbh = (int)(p.batch * p.heads);
-    bh = uniform32((int)blockIdx.x % nbh);
-    qblk = uniform32(blocks_q - 1 - (int)blockIdx.x / nbh);
-  } else {
-    const int pid = uniform32(xcd_remap(blockIdx.x, gridDim.x));
-    bh = uniform32(pid / blocks_q);
-    qblk = uniform32(pid % blocks_q);
-  }
   const int wg_q0 = qblk * QPB, q0 = uniform32(wg_q0 + wave * 32);
-  const int b = bh / (int)p.heads, h = bh % (int)p.heads, kvh = h / (int)(p.heads / p.kv_heads);
+  const int kvh = h / (int)(p.heads / p.kv_heads);
   const int64_t qbase = b * p.qb + h * p.qh, kbase = b * p.kb + kvh * p.kh;
   const char* K = uniform_ptr((const char*)p.k + kbase * ES);
   const char* V = uniform_ptr((const char*)p.v + kbase * ES);
@@ -448,10 +488,10 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
     own_rows<F32, DP>(p.q, qbase + q0 * p.qt, p.qt, col, t < T, half, D, raw);
 #pragma unroll
     for (int s = 0; s < Tile::S; s++) raw[s].parts(qf[s]);
-    own_rows<F32, DP>(p.g, qbase + q0 * p.qt, p.qt, col, t < T, half, D, raw);
+    own_rows<F32, DP>(p.g, qbase + q0 * out_pitch(p), out_pitch(p), col, t < T, half, D, raw);
 #pragma unroll
     for (int s = 0; s < Tile::S; s++) raw[s].parts(gf[s]);
-    own_rows<F32, DP>(p.o, qbase + q0 * p.qt, p.qt, col, t < T, half, D, raw);
+    own_rows<F32, DP>(p.o, qbase + q0 * out_pitch(p), out_pitch(p), col, t < T, half, D, raw);
     f32x16 og = {}, og_lo = {};  // O dO^T of the wave's queries, whose diagonal is delta
 #pragma unroll
     for (int s = 0; s < Tile::S; s++) {
@@ -478,10 +518,11 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
   const int nkb_w = p.causal ? min(nkb, (q0 + 32 + KB - 1) / KB) : nkb;
   const int n_full = min(nkb_w, (p.causal ? min(T, q0 + 1) : T) / KB);
   Stage stage;
-  stage.plan(tid, p.kt, D);
+  const int64_t vt = value_pitch(p);
+  stage.plan(tid, p.kt, vt, D);
   auto fetch = [&](int kbk) {
-    const int64_t at = (int64_t)kbk * KB * p.kt * ES;
-    stage.fetch(K + at, V + at, p.kt, T - kbk * KB, wave);
+    const int64_t at = (int64_t)kbk * KB * ES;
+    stage.fetch(K + at * p.kt, V + at * vt, p.kt, vt, T - kbk * KB, wave);
   };
   auto advance = [&](int kbk) {
     __syncthreads();
@@ -542,7 +583,7 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
     return;
   }
   if (t < T) {
-    const int64_t at = qbase + (int64_t)t * p.qt;
+    const int64_t at = qbase + (int64_t)t * dq_pitch(p);
 #pragma unroll
     for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
@@ -563,8 +604,8 @@ __global__ void __launch_bounds__(256, F32 && DP > 64 || DP > 128 ? 1 : 2) atten
 // 637 us, about twice that with both and their spills).
 enum KeySide { KEYS_BOTH, KEYS_DK, KEYS_DV };
 
-template <bool F32, int DP, KeySide SIDE>
-__global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attention_bwd_dkv_mma(AttnGenArgs p) {
+template <bool F32, int DP, KeySide SIDE, class Args = AttnGenArgs>
+__global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attention_bwd_dkv_mma(Args p) {
   typedef AttnTile<F32, DP> Tile;
   typedef AttnStage<F32, DP> Stage;
   typedef typename std::conditional<F32, float, bf16_t>::type T_;
@@ -572,24 +613,12 @@ __global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attent
   __shared__ __attribute__((aligned(16))) bf16_t tiles[2 * Tile::NX * Tile::PLANE];  // [Q, dO][plane]
   __shared__ __attribute__((aligned(16))) float stats[3][KB];  // lse log2(e) and its rounding error, delta as dS
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
+  const int group = (int)(p.heads / p.kv_heads);
+  int b, kvh, kblk, gsel;
+  place_keys<T_, KPB>(p, p.split ? group : 1, b, kvh, kblk, gsel);
   const int T = (int)p.time, D = (int)p.dim;
-  const int blocks_k = (T + KPB - 1) / KPB;
-  const int group = (int)(p.heads / p.kv_heads), nsplit = p.split ? group : 1;
-  int bkh, kblk, gsel;
-  if (p.causal) {  // the first keys see the most queries and start first
-    const int nbh = (int)(p.batch * p.kv_heads) * nsplit, id = (int)blockIdx.x % nbh;
-    bkh = uniform32(id / nsplit);
-    gsel = uniform32(id % nsplit);
-    kblk = uniform32((int)blockIdx.x / nbh);
-  } else {
-    const int pid = uniform32(xcd_remap(blockIdx.x, gridDim.x)), rest = pid % (blocks_k * nsplit);
-    bkh = uniform32(pid / (blocks_k * nsplit));
-    kblk = uniform32(rest / nsplit);
-    gsel = uniform32(rest % nsplit);
-  }
   const int g_lo = p.split ? gsel : 0, g_hi = p.split ? gsel + 1 : group;
   const int k0 = uniform32(kblk * KPB), kw = uniform32(k0 + wave * 32);
-  const int b = bkh / (int)p.kv_heads, kvh = bkh % (int)p.kv_heads;
   const int64_t kbase = b * p.kb + kvh * p.kh;
   const int key = kw + col;
 
@@ -599,7 +628,7 @@ __global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attent
     own_rows<F32, DP>(p.k, kbase + kw * p.kt, p.kt, col, key < T, half, D, raw);
 #pragma unroll
     for (int s = 0; s < Tile::S; s++) raw[s].parts(kf[s]);
-    own_rows<F32, DP>(p.v, kbase + kw * p.kt, p.kt, col, key < T, half, D, raw);
+    own_rows<F32, DP>(p.v, kbase + kw * value_pitch(p), value_pitch(p), col, key < T, half, D, raw);
 #pragma unroll
     for (int s = 0; s < Tile::S; s++) raw[s].parts(vf[s]);
   }
@@ -614,12 +643,14 @@ __global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attent
   const int nq = qs0 < T ? (T - qs0 + KB - 1) / KB : 0;
   const int iterations = nq * (g_hi - g_lo);
   Stage stage;
-  stage.plan(tid, p.qt, D);
+  const int64_t ot = out_pitch(p);
+  stage.plan(tid, p.qt, ot, D);
   float lse_next = 0.f, delta_next = 0.f;  // of query tid of the block in flight (tid < KB)
   auto fetch = [&](int it) {
     const int h = kvh * group + g_lo + it / nq, qs = qs0 + (it % nq) * KB;
-    const int64_t at = (b * p.qb + h * p.qh + (int64_t)qs * p.qt) * ES;
-    stage.fetch(uniform_ptr((const char*)p.q + at), uniform_ptr((const char*)p.g + at), p.qt, T - qs, wave);
+    const int64_t head = b * p.qb + h * p.qh;
+    stage.fetch(uniform_ptr((const char*)p.q + (head + (int64_t)qs * p.qt) * ES),
+                uniform_ptr((const char*)p.g + (head + (int64_t)qs * ot) * ES), p.qt, ot, T - qs, wave);
     if (tid < KB) {
       const bool in = qs + tid < T;
       const int64_t li = b * p.lb + h * p.lh + (int64_t)(in ? qs + tid : 0) * p.lt;
@@ -727,7 +758,8 @@ __global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attent
     return;
   }
   if (key < T) {
-    const int64_t at = kbase + (int64_t)key * p.kt;
+    const int64_t part = kbase + (int64_t)key * part_pitch(p);
+    const int64_t at_k = kbase + (int64_t)key * dk_pitch(p), at_v = kbase + (int64_t)key * dv_pitch(p);
 #pragma unroll
     for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
@@ -737,14 +769,14 @@ __global__ void __launch_bounds__(256, F32 && DP > 32 || DP > 64 ? 1 : 2) attent
         if constexpr (DK) {
           const f32x16& y = dkt[db];
           const f32x4 x = {y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]};
-          if (p.split) global_store(p.part_k + gsel * p.part_stride + at + d, x * Tile::SUM);
-          else put4<F32>(p.dk, at + d, x * (p.scale * Tile::SUM));
+          if (p.split) global_store(p.part_k + gsel * p.part_stride + part + d, x * Tile::SUM);
+          else put4<F32>(p.dk, at_k + d, x * (p.scale * Tile::SUM));
         }
         if constexpr (DV) {
           const f32x16& y = dvt[db];
           const f32x4 x = {y[4 * g], y[4 * g + 1], y[4 * g + 2], y[4 * g + 3]};
-          if (p.split) global_store(p.part_v + gsel * p.part_stride + at + d, x * Tile::SUM);
-          else put4<F32>(p.dv, at + d, x * Tile::SUM);
+          if (p.split) global_store(p.part_v + gsel * p.part_stride + part + d, x * Tile::SUM);
+          else put4<F32>(p.dv, at_v + d, x * Tile::SUM);
         }
       }
   }

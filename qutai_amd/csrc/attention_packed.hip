@@ -1,0 +1,205 @@
+// Attention of sequences of different lengths that lie one behind the other in
+// one matrix of tokens: C ABI `qutai_amd_attention_packed_fwd`, `_bwd`, `_rows`,
+// `_bwd_workspace_size`.
+//
+//   forward:  S = scale Q K^T over a sequence's own (causal: no later) keys,
+//             O = softmax(S) V, lse = log sum exp S
+//   backward: P = exp(S - lse), dV = P^T dO, dP = dO V^T, delta = rowsum(dO O),
+//             dS = P (dP - delta), dQ = scale dS K, dK = scale dS^T Q.
+//
+// The caller's tile tables say which rows of which sequence a workgroup takes, in
+// the order in which the workgroups start; every tile lies in one sequence, so
+// padding costs no work and no mask but a sequence's own end is needed.
+#include <algorithm>
+#include <type_traits>
+
+#include "attention_rows.h"
+#include "attention_mma.h"
+
+namespace {
+
+constexpr int64_t MMA_ROWS = 128;  // queries or keys of a workgroup of the matrix kernels
+
+template <class T>
+__global__ void __launch_bounds__(GEN_WAVES * 64) packed_fwd_rows(AttnPackedArgs p) {
+  int b, h, blk;
+  place_queries<T, GEN_WAVES>(p, b, h, blk);
+  const int t = blk * GEN_WAVES + uniform32(threadIdx.x >> 6);
+  if (t < p.time) fwd_row<T>(p, b, h, t, threadIdx.x & 63);
+}
+template <class T>
+__global__ void __launch_bounds__(GEN_WAVES * 64) packed_bwd_q_rows(AttnPackedArgs p) {
+  int b, h, blk;
+  place_queries<T, GEN_WAVES>(p, b, h, blk);
+  const int t = blk * GEN_WAVES + uniform32(threadIdx.x >> 6);
+  if (t < p.time) bwd_q_row<T>(p, b, h, t, threadIdx.x & 63);
+}
+template <class T>
+__global__ void __launch_bounds__(GEN_WAVES * 64) packed_bwd_kv_rows(AttnPackedArgs p) {
+  int b, kvh, blk, gsel;
+  place_keys<T, GEN_WAVES>(p, 1, b, kvh, blk, gsel);
+  const int t = blk * GEN_WAVES + uniform32(threadIdx.x >> 6);
+  if (t < p.time) bwd_kv_row<T>(p, b, kvh, t, threadIdx.x & 63, 0, (int)(p.heads / p.kv_heads));
+}
+
+enum Pass { FORWARD, QUERIES, KEYS };
+
+template <bool F32, int DP>
+void launch_mma(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
+  const dim3 grid(blocks), block(256);
+  if (pass == FORWARD) hipLaunchKernelGGL((attention_fwd_mma<F32, DP, AttnPackedArgs>), grid, block, 0, stream, a);
+  else if (pass == QUERIES)
+    hipLaunchKernelGGL((attention_bwd_dq_mma<F32, DP, AttnPackedArgs>), grid, block, 0, stream, a);
+  else if constexpr (DP > 128) {
+    hipLaunchKernelGGL((attention_bwd_dkv_mma<F32, DP, KEYS_DV, AttnPackedArgs>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((attention_bwd_dkv_mma<F32, DP, KEYS_DK, AttnPackedArgs>), grid, block, 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((attention_bwd_dkv_mma<F32, DP, KEYS_BOTH, AttnPackedArgs>), grid, block, 0, stream, a);
+  }
+}
+
+template <class T>
+void launch_rows(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
+  const dim3 grid(blocks), block(GEN_WAVES * 64);
+  if (pass == FORWARD) hipLaunchKernelGGL(packed_fwd_rows<T>, grid, block, 0, stream, a);
+  else if (pass == QUERIES) hipLaunchKernelGGL(packed_bwd_q_rows<T>, grid, block, 0, stream, a);
+  else hipLaunchKernelGGL(packed_bwd_kv_rows<T>, grid, block, 0, stream, a);
+}
+
+// Whether the matrix kernels take rows of this type and width (of whole 16-byte chunks).
+bool mma_fits(int dtype, int64_t dim) { return dtype == BF16 ? dim % 8 == 0 && dim <= 256 : dim % 4 == 0 && dim <= 128; }
+
+// One pass over the tiles of `rows` rows each; blocks of each tile: heads of its side.
+hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, const int64_t* tiles, int64_t count, int64_t rows,
+                  int64_t blocks, hipStream_t stream) {
+  if (!count) return hipSuccess;
+  a.tiles = tiles;
+  const unsigned n = (unsigned)(count * blocks);
+  if (rows == GEN_WAVES) {
+    if (dtype == BF16) launch_rows<bf16_t>(pass, a, n, stream);
+    else launch_rows<float>(pass, a, n, stream);
+  } else if (dtype == BF16) {
+    if (a.dim <= 32) launch_mma<false, 32>(pass, a, n, stream);
+    else if (a.dim <= 64) launch_mma<false, 64>(pass, a, n, stream);
+    else if (a.dim <= 96) launch_mma<false, 96>(pass, a, n, stream);
+    else if (a.dim <= 128) launch_mma<false, 128>(pass, a, n, stream);
+    else launch_mma<false, 256>(pass, a, n, stream);
+  } else {
+    if (a.dim <= 32) launch_mma<true, 32>(pass, a, n, stream);
+    else if (a.dim <= 64) launch_mma<true, 64>(pass, a, n, stream);
+    else if (a.dim <= 96) launch_mma<true, 96>(pass, a, n, stream);
+    else launch_mma<true, 128>(pass, a, n, stream);
+  }
+  return hipGetLastError();
+}
+
+// What forward and backward share: sizes, scale, pitches.  rows: of a tile.
+int set_packed(AttnPackedArgs& a, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
+               int64_t v_row, int dtype, double scale, int causal, std::initializer_list<int64_t> tile_rows) {
+  if ((dtype != BF16 && dtype != F32) || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1 << 16) return QA_EINVAL;
+  if (dim <= 0 || dim > 256 || !(scale > 0.0) || scale > 1e30) return QA_EINVAL;
+  if (q_row < heads * dim || k_row < kv_heads * dim || v_row < kv_heads * dim) return QA_EINVAL;
+  if (std::max({q_row, k_row, v_row, heads * dim}) > 1 << 22) return QA_EINVAL;  // 64 rows within a buffer descriptor
+  for (int64_t rows : tile_rows) {
+    if (rows != GEN_WAVES && rows != MMA_ROWS) return QA_EINVAL;
+    if (rows == MMA_ROWS && (!mma_fits(dtype, dim) || scale < 0x1p-50)) return QA_EINVAL;
+  }
+  a.batch = 1;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.dim = dim;
+  a.qh = a.kh = dim;
+  a.qt = q_row;
+  a.kt = k_row;
+  a.vt = v_row;
+  a.ot = heads * dim;
+  a.lh = 1;
+  a.lt = heads;
+  a.scale = (float)scale;
+  const double log2 = scale * 1.4426950408889634 * (dtype == F32 ? 0x1p-48 : 1.0);
+  a.scale_log2 = (float)log2;
+  a.scale_log2_lo = (float)(log2 - (double)a.scale_log2);
+  a.causal = causal ? 1 : 0;
+  return QA_OK;
+}
+
+bool whole(std::initializer_list<const void*> pointers, std::initializer_list<int64_t> pitches, int dtype) {
+  for (int64_t pitch : pitches)
+    if (pitch * (dtype == F32 ? 4 : 2) % 16) return false;
+  return aligned16(pointers);
+}
+
+// Workgroups of 256 threads that a launch can hold.
+bool grid_fits(int64_t tiles, int64_t blocks) { return tiles >= 0 && tiles <= ((1ll << 24) - 1) / blocks; }
+
+}  // namespace
+
+extern "C" {
+
+int64_t qutai_amd_attention_packed_rows(int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype,
+                                        int aligned, double scale, int pass) {
+  if ((dtype != BF16 && dtype != F32) || dim <= 0 || dim > 256 || pass < 0 || pass > 2 || heads <= 0 || kv_heads <= 0)
+    return 0;
+  if (!aligned || !mma_fits(dtype, dim) || scale < 0x1p-50 || longest <= (pass == FORWARD ? 2 : 4)) return GEN_WAVES;
+  return MMA_ROWS;
+}
+
+int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
+                                   double scale, int causal, void* stream) {
+  AttnPackedArgs a = {};
+  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {tile_rows});
+  if (status != QA_OK) return status;
+  if (!grid_fits(tile_count, heads)) return QA_EINVAL;
+  if (!tile_count) return QA_OK;
+  if (!q || !k || !v || !out || !lse || !tiles) return QA_EINVAL;
+  if (tile_rows != GEN_WAVES && !whole({q, k, v, out}, {q_row, k_row, v_row}, dtype)) return QA_EINVAL;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.dq = out;
+  a.dqt = a.ot;
+  a.lse = lse;
+  return (int)launch(FORWARD, dtype, a, tiles, tile_count, tile_rows, heads, (hipStream_t)stream);
+}
+
+int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                   const float* lse, void* dq, void* dk, void* dv, float* delta,
+                                   const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
+                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t heads,
+                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
+                                   int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
+                                   void* stream) {
+  AttnPackedArgs a = {};
+  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {query_rows, key_rows});
+  if (status != QA_OK) return status;
+  if (dq_row < heads * dim || dk_row < kv_heads * dim || dv_row < kv_heads * dim) return QA_EINVAL;
+  if (std::max({dq_row, dk_row, dv_row}) > 1 << 22) return QA_EINVAL;
+  if (!grid_fits(query_count, heads) || !grid_fits(key_count, kv_heads)) return QA_EINVAL;
+  if (!query_count && !key_count) return QA_OK;
+  if (!grad || !q || !k || !v || !out || !dq || !dk || !dv || !lse || !delta || !query_tiles || !key_tiles)
+    return QA_EINVAL;
+  if ((query_rows != GEN_WAVES || key_rows != GEN_WAVES) &&
+      !whole({grad, q, k, v, out, dq, dk, dv}, {q_row, k_row, v_row, dq_row, dk_row, dv_row}, dtype))
+    return QA_EINVAL;
+  a.g = grad;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.o = out;
+  a.lse = const_cast<float*>(lse);
+  a.delta = delta;
+  a.dq = dq;
+  a.dk = dk;
+  a.dv = dv;
+  a.dqt = dq_row;
+  a.dkt = dk_row;
+  a.dvt = dv_row;
+  // the query pass writes delta, which the key pass reads
+  const hipError_t e = launch(QUERIES, dtype, a, query_tiles, query_count, query_rows, heads, (hipStream_t)stream);
+  if (e != hipSuccess) return (int)e;
+  return (int)launch(KEYS, dtype, a, key_tiles, key_count, key_rows, kv_heads, (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -38,6 +38,49 @@ struct AttnGenArgs {
   int64_t part_stride;
 };
 
+// Sequences of different lengths, one behind the other in rows of tokens (b = 0):
+// a workgroup's tile is (start of its sequence, the sequence's length, first row
+// in it), and q, k, v and their gradients may be columns of wider matrices.
+struct AttnPackedArgs : AttnGenArgs {
+  const int64_t* tiles;
+  int64_t vt, ot, dqt, dkt, dvt;  // elements from row to row of v, of out and its gradient, and of dq, dk, dv
+};
+
+// Elements from row to row, where a packed call's differ from the others'.
+__device__ __forceinline__ int64_t value_pitch(const AttnGenArgs& p) { return p.kt; }
+__device__ __forceinline__ int64_t out_pitch(const AttnGenArgs& p) { return p.qt; }
+__device__ __forceinline__ int64_t dq_pitch(const AttnGenArgs& p) { return p.qt; }
+__device__ __forceinline__ int64_t dk_pitch(const AttnGenArgs& p) { return p.kt; }
+__device__ __forceinline__ int64_t dv_pitch(const AttnGenArgs& p) { return p.kt; }
+__device__ __forceinline__ int64_t part_pitch(const AttnGenArgs& p) { return p.kt; }
+__device__ __forceinline__ int64_t value_pitch(const AttnPackedArgs& p) { return p.vt; }
+__device__ __forceinline__ int64_t out_pitch(const AttnPackedArgs& p) { return p.ot; }
+__device__ __forceinline__ int64_t dq_pitch(const AttnPackedArgs& p) { return p.dqt; }
+__device__ __forceinline__ int64_t dk_pitch(const AttnPackedArgs& p) { return p.dkt; }
+__device__ __forceinline__ int64_t dv_pitch(const AttnPackedArgs& p) { return p.dvt; }
+__device__ __forceinline__ int64_t part_pitch(const AttnPackedArgs& p) { return p.kv_heads * p.dim; }
+
+// The arguments of tile `tile`'s sequence alone; returns the tile's first row in it.
+template <class T>
+__device__ __forceinline__ int enter_sequence(AttnPackedArgs& p, int64_t tile) {
+  const int64_t start = uniform64(p.tiles[3 * tile]);
+  p.time = uniform64(p.tiles[3 * tile + 1]);
+  const auto at = [&](const void* x, int64_t pitch) { return (const void*)((const T*)x + start * pitch); };
+  p.q = at(p.q, p.qt);
+  p.k = at(p.k, p.kt);
+  p.v = at(p.v, p.vt);
+  p.g = at(p.g, p.ot);
+  p.o = at(p.o, p.ot);
+  p.dq = const_cast<void*>(at(p.dq, p.dqt));
+  p.dk = const_cast<void*>(at(p.dk, p.dkt));
+  p.dv = const_cast<void*>(at(p.dv, p.dvt));
+  if (p.lse) p.lse += start * p.lt;
+  p.delta += start * p.lt;
+  p.part_k += start * part_pitch(p);
+  p.part_v += start * part_pitch(p);
+  return uniform32((int)p.tiles[3 * tile + 2]);
+}
+
 template <class T> __device__ __forceinline__ float ld(const void* p, int64_t i);
 template <> __device__ __forceinline__ float ld<float>(const void* p, int64_t i) { return ((const float*)p)[i]; }
 template <> __device__ __forceinline__ float ld<bf16_t>(const void* p, int64_t i) {
@@ -66,10 +109,11 @@ __device__ __forceinline__ void gen_row(const AttnGenArgs& p, int64_t row, int64
 }
 
 // Output and lse of query t of (b, h).
-template <class T>
-__device__ __forceinline__ void fwd_row(const AttnGenArgs& p, int64_t b, int64_t h, int64_t t, int lane) {
+template <class T, class Args>
+__device__ __forceinline__ void fwd_row(const Args& p, int64_t b, int64_t h, int64_t t, int lane) {
   const int64_t kvh = h / (p.heads / p.kv_heads);
   const int64_t qi = b * p.qb + h * p.qh + t * p.qt, kbase = b * p.kb + kvh * p.kh;
+  const int64_t oi = b * p.qb + h * p.qh + t * out_pitch(p);
   const int D = (int)p.dim;
   float qv[4], acc[4];
 #pragma unroll
@@ -81,7 +125,7 @@ __device__ __forceinline__ void fwd_row(const AttnGenArgs& p, int64_t b, int64_t
   float m = -INFINITY, l = 0.f;
   const int64_t end = p.causal ? t + 1 : p.time;
   for (int64_t s = 0; s < end; s++) {
-    const int64_t ki = kbase + s * p.kt;
+    const int64_t ki = kbase + s * p.kt, vi = kbase + s * value_pitch(p);
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -95,7 +139,7 @@ __device__ __forceinline__ void fwd_row(const AttnGenArgs& p, int64_t b, int64_t
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int d = lane + 64 * j;
-      acc[j] = acc[j] * alpha + (d < D ? pr * ld<T>(p.v, ki + d) : 0.f);
+      acc[j] = acc[j] * alpha + (d < D ? pr * ld<T>(p.v, vi + d) : 0.f);
     }
     m = m_new;
   }
@@ -103,16 +147,17 @@ __device__ __forceinline__ void fwd_row(const AttnGenArgs& p, int64_t b, int64_t
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const int d = lane + 64 * j;
-    if (d < D) st<T>(p.dq, qi + d, acc[j] * inv);
+    if (d < D) st<T>(p.dq, oi + d, acc[j] * inv);
   }
   if (p.lse && lane == 0) p.lse[b * p.lb + h * p.lh + t * p.lt] = m + __logf(l);
 }
 
 // dQ and delta of query t of (b, h).
-template <class T>
-__device__ __forceinline__ void bwd_q_row(const AttnGenArgs& p, int64_t b, int64_t h, int64_t t, int lane) {
+template <class T, class Args>
+__device__ __forceinline__ void bwd_q_row(const Args& p, int64_t b, int64_t h, int64_t t, int lane) {
   const int64_t kvh = h / (p.heads / p.kv_heads);
   const int64_t qi = b * p.qb + h * p.qh + t * p.qt, kbase = b * p.kb + kvh * p.kh;
+  const int64_t oi = b * p.qb + h * p.qh + t * out_pitch(p), di = b * p.qb + h * p.qh + t * dq_pitch(p);
   const int64_t li = b * p.lb + h * p.lh + t * p.lt;
   const int D = (int)p.dim;
   float qv[4], gv[4], acc[4], dl = 0.f;
@@ -120,8 +165,8 @@ __device__ __forceinline__ void bwd_q_row(const AttnGenArgs& p, int64_t b, int64
   for (int j = 0; j < 4; j++) {
     const int d = lane + 64 * j;
     qv[j] = d < D ? ld<T>(p.q, qi + d) : 0.f;
-    gv[j] = d < D ? ld<T>(p.g, qi + d) : 0.f;
-    dl += d < D ? gv[j] * ld<T>(p.o, qi + d) : 0.f;
+    gv[j] = d < D ? ld<T>(p.g, oi + d) : 0.f;
+    dl += d < D ? gv[j] * ld<T>(p.o, oi + d) : 0.f;
     acc[j] = 0.f;
   }
   dl = wave_sum(dl);
@@ -129,14 +174,14 @@ __device__ __forceinline__ void bwd_q_row(const AttnGenArgs& p, int64_t b, int64
   const float lse = p.lse[li];
   const int64_t end = p.causal ? t + 1 : p.time;
   for (int64_t s = 0; s < end; s++) {
-    const int64_t ki = kbase + s * p.kt;
+    const int64_t ki = kbase + s * p.kt, vi = kbase + s * value_pitch(p);
     float dot = 0.f, dp = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int d = lane + 64 * j;
       if (d < D) {
         dot += qv[j] * ld<T>(p.k, ki + d);
-        dp += gv[j] * ld<T>(p.v, ki + d);
+        dp += gv[j] * ld<T>(p.v, vi + d);
       }
     }
     const float pr = __expf(wave_sum(dot) * p.scale - lse);
@@ -150,16 +195,16 @@ __device__ __forceinline__ void bwd_q_row(const AttnGenArgs& p, int64_t b, int64
 #pragma unroll
   for (int j = 0; j < 4; j++) {
     const int d = lane + 64 * j;
-    if (d < D) st<T>(p.dq, qi + d, acc[j]);
+    if (d < D) st<T>(p.dq, di + d, acc[j]);
   }
 }
 
 // dK and dV of key s of (b, kvh), summed over the query heads [g_lo, g_hi) of
 // its group (p.split: head g_lo's unscaled partials).
-template <class T>
-__device__ __forceinline__ void bwd_kv_row(const AttnGenArgs& p, int64_t b, int64_t kvh, int64_t s, int lane,
+template <class T, class Args>
+__device__ __forceinline__ void bwd_kv_row(const Args& p, int64_t b, int64_t kvh, int64_t s, int lane,
                                            int g_lo, int g_hi) {
-  const int64_t ki = b * p.kb + kvh * p.kh + s * p.kt;
+  const int64_t head = b * p.kb + kvh * p.kh, ki = head + s * p.kt, vi = head + s * value_pitch(p);
   const int64_t group = p.heads / p.kv_heads;
   const int D = (int)p.dim;
   const float scale = p.split ? 1.f : p.scale;
@@ -168,12 +213,13 @@ __device__ __forceinline__ void bwd_kv_row(const AttnGenArgs& p, int64_t b, int6
   for (int j = 0; j < 4; j++) {
     const int d = lane + 64 * j;
     kv_[j] = d < D ? ld<T>(p.k, ki + d) : 0.f;
-    vv[j] = d < D ? ld<T>(p.v, ki + d) : 0.f;
+    vv[j] = d < D ? ld<T>(p.v, vi + d) : 0.f;
     ak[j] = av[j] = 0.f;
   }
   for (int64_t h = kvh * group + g_lo; h < kvh * group + g_hi; h++) {
     for (int64_t t = p.causal ? s : 0; t < p.time; t++) {
       const int64_t qi = b * p.qb + h * p.qh + t * p.qt;
+      const int64_t oi = b * p.qb + h * p.qh + t * out_pitch(p);
       const int64_t li = b * p.lb + h * p.lh + t * p.lt;
       float dot = 0.f, dp = 0.f;
 #pragma unroll
@@ -181,7 +227,7 @@ __device__ __forceinline__ void bwd_kv_row(const AttnGenArgs& p, int64_t b, int6
         const int d = lane + 64 * j;
         if (d < D) {
           dot += ld<T>(p.q, qi + d) * kv_[j];
-          dp += ld<T>(p.g, qi + d) * vv[j];
+          dp += ld<T>(p.g, oi + d) * vv[j];
         }
       }
       const float pr = __expf(wave_sum(dot) * p.scale - p.lse[li]);
@@ -191,7 +237,7 @@ __device__ __forceinline__ void bwd_kv_row(const AttnGenArgs& p, int64_t b, int6
         const int d = lane + 64 * j;
         if (d < D) {
           ak[j] += ds * ld<T>(p.q, qi + d);
-          av[j] += pr * ld<T>(p.g, qi + d);
+          av[j] += pr * ld<T>(p.g, oi + d);
         }
       }
     }
@@ -201,11 +247,11 @@ __device__ __forceinline__ void bwd_kv_row(const AttnGenArgs& p, int64_t b, int6
     const int d = lane + 64 * j;
     if (d < D) {
       if (p.split) {
-        p.part_k[g_lo * p.part_stride + ki + d] = ak[j];
-        p.part_v[g_lo * p.part_stride + ki + d] = av[j];
+        p.part_k[g_lo * p.part_stride + head + s * part_pitch(p) + d] = ak[j];
+        p.part_v[g_lo * p.part_stride + head + s * part_pitch(p) + d] = av[j];
       } else {
-        st<T>(p.dk, ki + d, ak[j]);
-        st<T>(p.dv, ki + d, av[j]);
+        st<T>(p.dk, head + s * dk_pitch(p) + d, ak[j]);
+        st<T>(p.dv, head + s * dv_pitch(p) + d, av[j]);
       }
     }
   }

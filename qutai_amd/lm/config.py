@@ -1,11 +1,14 @@
 """Decoder configuration (src/qutai/lm/config.py:5-71): the same fields,
-defaults, validation and parameter-count formula, and ``qk_norm``: an RMSNorm of
-every query and key head before its rotation, off by default."""
+defaults, validation and parameter-count formula, ``qk_norm``: an RMSNorm of
+every query and key head before its rotation, off by default, and the rotary
+positions' ``rope_layout``, ``rope_dim`` (the channels of a head that are turned) and
+``rope_scaling`` (lm.Rotary), those of the reference by default."""
 from __future__ import annotations
 
 from dataclasses import asdict, dataclass
 from math import isfinite
 
+from .rotary import Rotary
 
 @dataclass
 class Config:
@@ -25,6 +28,9 @@ class Config:
     aux_loss_coef: float = 0.01
     activation_checkpointing: bool = True
     qk_norm: bool = False
+    rope_layout: str = "interleaved"
+    rope_dim: int | None = None
+    rope_scaling: dict | None = None
 
     def __post_init__(self):
         sizes = (self.vocab_size, self.n_layers, self.d_model, self.n_heads, self.n_kv_heads, self.d_ff,
@@ -45,13 +51,24 @@ class Config:
             raise ValueError("qk_norm must be True or False")
         if self.norm_eps <= 0 or self.rope_theta <= 0 or self.aux_loss_coef < 0:
             raise ValueError("norm_eps and rope_theta must be positive, aux_loss_coef non-negative")
+        self.rotary()
+
+    def rotary(self):
+        """The Rotary of a block's heads; None where it is the reference's: pairs
+        (2i, 2i+1) of the whole head at rope_theta's frequencies."""
+        head = self.d_model // self.n_heads
+        if (self.rope_layout, self.rope_dim, self.rope_scaling) == ("interleaved", None, None):
+            return None
+        return Rotary(head, self.rope_theta, rotary_dim=self.rope_dim, layout=self.rope_layout,
+                      scaling=self.rope_scaling)
 
     def to_dict(self):
-        """The fields as a dict; qk_norm only where it is set, so that a
-        configuration without it is the reference's."""
+        """The fields as a dict; qk_norm and the rope's options only where they are
+        set, so that a configuration without them is the reference's."""
         fields = asdict(self)
-        if not self.qk_norm:
-            del fields["qk_norm"]
+        for name, default in (("qk_norm", False), ("rope_layout", "interleaved"), ("rope_dim", None), ("rope_scaling", None)):
+            if fields[name] == default:
+                del fields[name]
         return fields
 
     def parameter_counts(self):

@@ -17,6 +17,7 @@ from __future__ import annotations
 
 from array import array
 from bisect import bisect_left
+from functools import partial
 from itertools import chain
 from random import Random
 
@@ -25,6 +26,7 @@ from ..core.context import set_recording
 from ..core.tensor import Tensor
 from .config import Config
 from ..nn.cache import QuantizedKVCache, unchanged_on_failure
+from .packing import Packing
 from .layers import Block, Projection, RMSNorm, backend, embed, linear, projection_loss, sample, scaled, unpack
 from .recompute import checkpoint
 
@@ -92,19 +94,21 @@ class Decoder:
             return self._hidden(tokens, train=train)
 
     def _hidden(self, tokens, *, train=True):
-        ids, shape = self._tokens(tokens)
+        return self._blocks(*self._tokens(tokens), train)
+
+    def _blocks(self, ids, shape, train, packing=None):
         hidden = embed(ids, self.embedding.weight, shape)
         auxiliary = []
         for block in self.blocks:
             if train and self.config.activation_checkpointing:
                 if block.is_moe:
-                    hidden, aux = unpack(checkpoint(block.packed, hidden, parameters=block.parameters()),
-                                         hidden.shape)
+                    function = partial(block.packed, packing=packing)
+                    hidden, aux = unpack(checkpoint(function, hidden, parameters=block.parameters()), hidden.shape)
                 else:
-                    hidden = checkpoint(block.hidden, hidden, parameters=block.parameters())
+                    hidden = checkpoint(partial(block.hidden, packing=packing), hidden, parameters=block.parameters())
                     aux = Tensor(amd.full(1, 0.0, dtype=hidden.dtype), shape=())
             else:
-                hidden, aux = block(hidden)
+                hidden, aux = block(hidden, packing)
             auxiliary.append(aux)
         total = auxiliary[0]
         for value in auxiliary[1:]:
@@ -185,14 +189,7 @@ class Decoder:
         _, shape = self._tokens(tokens)
         if shape[1] < 2:
             raise ValueError("next-token training needs at least two positions")
-        labels = tokens if labels is None else labels
-        label_rows = [row if isinstance(row, (list, tuple)) else list(row) for row in labels]
-        if len(label_rows) != shape[0] or any(len(row) != shape[1] for row in label_rows):
-            raise ValueError("labels must have the shape of tokens")
-        ordered = sorted(_int_array(chain.from_iterable(label_rows)))
-        first = bisect_left(ordered, -99)  # first label above the ignore id
-        if ordered[0] < -100 or ordered[-1] >= self.config.vocab_size or (first < len(ordered) and ordered[first] < 0):
-            raise ValueError("labels must be vocabulary ids or -100")
+        label_rows = self._labels(tokens if labels is None else labels, [shape[1]] * shape[0])
         with set_recording(train):
             prepared = backend(self.embedding.weight).prepare_labels(
                 _int_array(chain.from_iterable(row[1:] for row in label_rows)))
@@ -202,3 +199,42 @@ class Decoder:
             aux = self.last_auxiliary_loss.to(dtype=self.last_lm_loss.dtype)
             return self.last_lm_loss + scaled(aux, self.config.aux_loss_coef)
 
+    def _labels(self, labels, lengths):
+        """The labels as rows of these lengths; ValueError where they are not, or
+        hold anything but vocabulary ids and -100."""
+        rows = [row if isinstance(row, (list, tuple)) else list(row) for row in labels]
+        if [len(row) for row in rows] != list(lengths):
+            raise ValueError("labels must have the shape of tokens")
+        ordered = sorted(_int_array(chain.from_iterable(rows)))
+        first = bisect_left(ordered, -99)  # first label above the ignore id
+        if ordered[0] < -100 or ordered[-1] >= self.config.vocab_size or (first < len(ordered) and ordered[first] < 0):
+            raise ValueError("labels must be vocabulary ids or -100")
+        return rows
+
+    def loss_packed(self, sequences, labels=None, *, train=True, chunk_size=128):
+        """``loss`` of sequences of different lengths (lists of ids, each no longer
+        than max_seq_len), which lie one behind the other in one row of tokens: no
+        padding, no token sees another sequence, and positions start at 0 in each.
+        The mean runs over the predictions of all sequences (a sequence's last token
+        predicts nothing); labels have the sequences' shape, -100 is ignored."""
+        if chunk_size <= 0:
+            raise ValueError("chunk_size must be positive")
+        rows = [row if isinstance(row, (list, tuple)) else list(row) for row in sequences]
+        if not rows or any(not 1 <= len(row) <= self.config.max_seq_len for row in rows):
+            raise ValueError("packed sequences hold one token at least and no more than max_seq_len")
+        if sum(map(len, rows)) < 2:
+            raise ValueError("next-token training needs at least two positions")
+        ids = _int_array(chain.from_iterable(rows))
+        if min(ids) < 0 or max(ids) >= self.config.vocab_size:
+            raise ValueError("token id outside the vocabulary")
+        label_rows = self._labels(rows if labels is None else labels, map(len, rows))
+        # the token before a sequence's first predicts nothing
+        targets = [list(chain.from_iterable((-100, *row[1:]) for row in label_rows))]
+        packing = Packing(map(len, rows))
+        with set_recording(train):
+            prepared = backend(self.embedding.weight).prepare_labels(_int_array(targets[0][1:]))
+            hidden = self._blocks(ids, (1, packing.total), train, packing)
+            self.last_lm_loss = projection_loss(hidden, self.embedding.weight, targets, chunk_size,
+                                                prepared_labels=prepared)
+            aux = self.last_auxiliary_loss.to(dtype=self.last_lm_loss.dtype)
+            return self.last_lm_loss + scaled(aux, self.config.aux_loss_coef)

@@ -22,6 +22,7 @@ from ..core.context import is_recording, set_recording
 from ..core.grad import DeferredGradient, owned, record
 from ..core.tensor import Tensor
 from ..nn.cache import unchanged_on_failure
+from .rotary import Rotary
 
 
 def backend(value):
@@ -235,29 +236,54 @@ def rope(x, heads, theta, offset=0):
                   lambda g: (b.rope(g, *dims, inverse=True),))
 
 
-def qk_norm_rope(q, k, q_weight, k_weight, heads, kv_heads, theta, eps, offset=0):
+def qk_norm_rope(q, k, q_weight, k_weight, heads, kv_heads, theta, eps, offset=0, *, positions=None):
     """RMSNorm of every head of q (batch, time, heads*dim) and k (batch, time,
     kv_heads*dim), weights of dim values each, and their rotary embedding in
-    one launch; (q, k), recorded."""
+    one launch; (q, k), recorded.  ``positions`` (an int64 storage of one for every
+    token) takes the place of offset + the token's number."""
     b = backend(q)
     if q.ndim != 3 or heads <= 0 or q.shape[2] % heads or k.shape != (*q.shape[:2], kv_heads * (q.shape[2] // heads)):
         raise ValueError("qk_norm_rope takes q (batch, time, heads*dim) and k (batch, time, kv_heads*dim)")
     batch, time, features = q.shape
+    if positions is not None:  # every token a sequence of its own
+        batch, time = batch * time, 1
     dims = (batch, time, heads, kv_heads, features // heads, theta, eps)
-    values = b.qk_norm_rope(q.storage, k.storage, q_weight.storage, k_weight.storage, *dims, offset=offset)
+    where = dict(offset=offset, starts=positions)
+    values = b.qk_norm_rope(q.storage, k.storage, q_weight.storage, k_weight.storage, *dims, **where)
 
     def query_gradients(g):
         dq, _, dweight, _ = b.qk_norm_rope_backward(g, None, q.storage, None, q_weight.storage, None, batch, time, heads,
-                                                    0, *dims[4:], offset=offset)
+                                                    0, *dims[4:], **where)
         return owned(dq), owned(dweight)
 
     def key_gradients(g):
         _, dk, _, dweight = b.qk_norm_rope_backward(None, g, None, k.storage, None, k_weight.storage, batch, time, 0,
-                                                    kv_heads, *dims[4:], offset=offset)
+                                                    kv_heads, *dims[4:], **where)
         return owned(dk), owned(dweight)
 
     return (record(Tensor(values[0], shape=q.shape), (q, q_weight), query_gradients),
             record(Tensor(values[1], shape=k.shape), (k, k_weight), key_gradients))
+
+
+def rotary(q, k, heads, kv_heads, turns, *, positions=None, offset=0):
+    """The rotary positions that ``turns`` (a Rotary of the heads' width) says of q
+    (batch, time, heads*dim) and k (batch, time, kv_heads*dim), one launch; (q, k),
+    recorded.  ``positions``: an int64 storage of one for every token, else offset +
+    the token's number."""
+    b = backend(q)
+    if q.ndim != 3 or heads <= 0 or q.shape[2] % heads or k.shape != (*q.shape[:2], kv_heads * (q.shape[2] // heads)):
+        raise ValueError("rotary takes q (batch, time, heads*dim) and k (batch, time, kv_heads*dim)")
+    batch, time, features = q.shape
+    dim, where = features // heads, dict(positions=positions, offset=offset)
+    values = b.rotary(q.storage, k.storage, turns, batch, time, heads, kv_heads, dim, **where)
+
+    def back(g, side):
+        n = [0, 0]
+        n[side] = (heads, kv_heads)[side]
+        return owned(b.rotary(*((None, g) if side else (g, None)), turns, batch, time, *n, dim, **where, inverse=True)[side])
+
+    return (record(Tensor(values[0], shape=q.shape), (q,), lambda g: (back(g, 0),)),
+            record(Tensor(values[1], shape=k.shape), (k,), lambda g: (back(g, 1),)))
 
 
 def silu_mul(gate, up):
@@ -444,19 +470,32 @@ class GQA:
         self.heads, self.kv_heads, self.theta = config.n_heads, config.n_kv_heads, config.rope_theta
         self.q_norm, self.k_norm = (RMSNorm(width // config.n_heads, config.norm_eps, device=device, dtype=dtype)
                                     if getattr(config, "qk_norm", False) else None for _ in range(2))
+        # None: pairs (2i, 2i+1) of the whole head at theta's frequencies
+        self.turns = config.rotary() if hasattr(config, "rotary") else None
 
-    def __call__(self, x):
+    def __call__(self, x, packing=None):
+        """The block over (batch, time, width); with a ``packing`` over its sequences
+        in one row of tokens."""
         weights = (self.q.weight, self.k.weight, self.v.weight)
         norms = () if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight)
         if _stacked_qkv(x, *weights):
             return self.out(gqa_attention(x, *weights, self.heads, self.kv_heads, self.theta, *norms,
-                                          **({"eps": self.q_norm.eps} if norms else {})))
-        if norms:
-            q, k = qk_norm_rope(self.q(x), self.k(x), *norms, self.heads, self.kv_heads, self.theta, self.q_norm.eps)
-        else:
-            q = rope(self.q(x), self.heads, self.theta)
-            k = rope(self.k(x), self.kv_heads, self.theta)
-        return self.out(attention(q, k, self.v(x), self.heads, self.kv_heads))
+                                          **({"eps": self.q_norm.eps} if norms else {}), turns=self.turns,
+                                          packing=packing))
+        q, k, sizes = self.q(x), self.k(x), (self.heads, self.kv_heads)
+        positions, turns = None if packing is None else packing.positions, self.turns
+        if norms and turns is not None:  # at position 0 the norm's launch turns nothing
+            nowhere = amd.full(x.size // x.shape[-1], 0, dtype="int64")
+            q, k = qk_norm_rope(q, k, *norms, *sizes, self.theta, self.q_norm.eps, positions=nowhere)
+        elif norms:
+            q, k = qk_norm_rope(q, k, *norms, *sizes, self.theta, self.q_norm.eps, positions=positions)
+        elif turns is None and packing is None:
+            q, k = rope(q, self.heads, self.theta), rope(k, self.kv_heads, self.theta)
+        elif turns is None:
+            turns = Rotary(q.shape[2] // self.heads, self.theta)
+        if turns is not None:
+            q, k = rotary(q, k, *sizes, turns, positions=positions)
+        return self.out(attention(q, k, self.v(x), *sizes, packing))
 
     def decode(self, x, cache, counts=None):
         """The block over new positions of (batch, new, width) alone: their keys
@@ -476,15 +515,25 @@ class GQA:
         offset, starts = cache.positions()
         norms = (None, None) if self.q_norm is None else (self.q_norm.weight.storage, self.k_norm.weight.storage)
         dims = (*norms, batch, new, self.heads, self.kv_heads, head, self.theta)
-        options = dict(offset=offset, starts=starts, **({} if self.q_norm is None else {"eps": self.q_norm.eps}))
+        options = dict(offset=offset, starts=starts)
         if _stacked_qkv(x, *weights):
             qkv, row = _stacked_product(x, *weights)
-            q, k = b.qk_norm_rope(qkv, qkv, *dims, **options, q_row=row, k_column=q_width, k_row=row)
+            q = k = qkv
+            columns = dict(q_row=row, k_column=q_width, k_row=row)
             v, place = qkv, dict(value_column=q_width + kv_width, value_row=row)
         else:
-            projected = [linear(x, w).storage for w in weights]
-            q, k = b.qk_norm_rope(*projected[:2], *dims, **options)
-            v, place = projected[2], {}
+            q, k, v = (linear(x, w).storage for w in weights)
+            columns, place = {}, {}
+        if self.q_norm is not None:
+            options["eps"] = self.q_norm.eps
+        if self.turns is None:
+            q, k = b.qk_norm_rope(q, k, *dims, **options, **columns)
+        else:
+            if self.q_norm is not None:  # at position 0 its launch turns nothing
+                q, k = b.qk_norm_rope(q, k, *norms, rows, 1, *dims[4:], eps=self.q_norm.eps, **columns)
+                columns = {}
+            q, k = b.rotary(q, k, self.turns, batch, new, self.heads, self.kv_heads, head, offset=offset, starts=starts,
+                            **columns)
         cache.append_rows(k, v, batch, new, self.kv_heads, head, counts, **place)
         mixed = cache.attend(Tensor(q, shape=(batch, new, self.heads, head)))
         return self.out(Tensor(mixed.storage, shape=(batch, new, q_width)))
@@ -512,8 +561,8 @@ class Block:
         else:
             self.ffn = SwiGLU(config.d_model, config.d_ff, device=device, dtype=dtype, seed=ffn_seed, std=down_std)
 
-    def __call__(self, x):
-        x = residual_add(x, self.attn(self.attn_norm(x)))
+    def __call__(self, x, packing=None):
+        x = residual_add(x, self.attn(self.attn_norm(x), packing))
         if self.is_moe:
             y, aux = self.ffn(self.ffn_norm(x))
         else:
@@ -521,8 +570,8 @@ class Block:
             aux = Tensor(amd.full(1, 0.0, dtype=x.dtype), shape=())
         return residual_add(x, y), aux
 
-    def hidden(self, x):
-        return self(x)[0]
+    def hidden(self, x, packing=None):
+        return self(x, packing)[0]
 
     def decode(self, x, cache, counts=None):
         """The block over new positions, attending over ``cache`` (GQA.decode);
@@ -532,8 +581,8 @@ class Block:
             y = self.ffn(self.ffn_norm(x))
             return residual_add(x, y[0] if self.is_moe else y)
 
-    def packed(self, x):
-        return pack(*self(x))
+    def packed(self, x, packing=None):
+        return pack(*self(x, packing))
 
     def parameters(self):
         return (*self.attn_norm.parameters(), *self.ffn_norm.parameters(), *self.attn.parameters(),
@@ -680,12 +729,26 @@ def attention_products(q, k, v, *, scale=None):
     return Tensor(out, shape=(groups, time, dim)), Tensor(probs, shape=(groups, time, time))
 
 
-def attention(q, k, v, heads, kv_heads):
+def attention(q, k, v, heads, kv_heads, packing=None):
     """Causal grouped-query attention on (batch, time, heads*64) tensors in the
     lm layout (src/qutai/lm/layers.py:119-130): fused forward (the T x T
-    scores are never stored) and fused backward recorded for autograd."""
+    scores are never stored) and fused backward recorded for autograd.  With a
+    ``packing`` batch is 1 and the row holds its sequences one behind the other:
+    a token sees its own alone."""
     b = backend(q)
     batch, time, features = q.shape
+    if packing is not None:
+        if (batch, time) != (1, packing.total):
+            raise ValueError("a packing's sequences lie in one row of its total tokens")
+        dims = (packing, heads, kv_heads, features // heads)
+        stores = (q.storage, k.storage, v.storage)
+        keep = is_recording() and any(x.requires_grad for x in (q, k, v))
+        out, lse, *rest = b.attention_packed(*stores, *dims, rest=keep)
+
+        def backward(g):
+            return tuple(map(owned, b.attention_packed_backward(g, *stores, out, lse, *dims, rest=rest[0])))
+
+        return record(Tensor(out, shape=q.shape), (q, k, v), backward)
     dims = (batch, time, heads, kv_heads, features // heads)
     out, lse = b.attention(q.storage, k.storage, v.storage, *dims)
     return record(Tensor(out, shape=q.shape), (q, k, v),
@@ -704,19 +767,26 @@ def _stacked_qkv(x, wq, wk, wv):
     return _bf16_path(x, wq) and activation_dtype(x, wq) == "bfloat16"
 
 
-def _stacked_product(x, wq, wk, wv):
-    """(x [Wq; Wk; Wv]^T in bf16, columns of a row) of the bf16 path."""
-    width, rows = x.shape[-1], x.size // x.shape[-1]
-    total = wq.shape[0] + 2 * wk.shape[0]
-    ws = amd.AMDStorage(total * width, "bfloat16")
+def _stacked_weights(wq, wk, wv):
+    """[Wq; Wk; Wv] rounded to bf16 into one block."""
+    width = wq.shape[1]
+    ws = amd.AMDStorage((wq.shape[0] + 2 * wk.shape[0]) * width, "bfloat16")
     start = 0
     for w in (wq, wk, wv):
         amd.cast_into(amd.view(ws, start * width, w.size), w.storage)
         start += w.shape[0]
+    return ws
+
+
+def _stacked_product(x, wq, wk, wv):
+    """(x [Wq; Wk; Wv]^T in bf16, columns of a row) of the bf16 path."""
+    width, rows = x.shape[-1], x.size // x.shape[-1]
+    total = wq.shape[0] + 2 * wk.shape[0]
+    ws = _stacked_weights(wq, wk, wv)
     return backend(x).gemm(_bf16_input(x), ws, rows, width, total, transpose_right=True, out_dtype="bfloat16"), total
 
 
-def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=None, *, eps=1e-6):
+def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=None, *, eps=1e-6, turns=None, packing=None):
     """RoPE(x Wq^T), RoPE(x Wk^T), x Wv^T and causal grouped-query attention
     as one recorded op: GQA up to its out projection (src/qutai/lm/layers.py:
     317-350 with rope 108-116 and attention 119-130) on the bf16 path.  The
@@ -730,7 +800,11 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=Non
     gradient sums its three terms in one accumulator where the separate
     projections add three rounded products.  With norm weights q_norm and k_norm
     (of a head's width) every head is normed before its rotation, in the pass
-    that reads the product's columns; the product is then kept for the backward."""
+    that reads the product's columns; the product is then kept for the backward.
+    ``turns`` (a Rotary) takes the place of theta's rotation; with a ``packing`` the
+    row of tokens holds its sequences, and q, k and v stay columns of the product."""
+    if turns is not None or packing is not None:
+        return _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turns, packing)
     b = backend(x)
     batch, time, width = x.shape
     rows = batch * time
@@ -739,9 +813,7 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=Non
     head = dq // heads
     precision = matmul_precision()
     xs = _bf16_input(x)
-    ws = amd.AMDStorage(total * width, "bfloat16")
-    for w, start in ((wq, 0), (wk, dq), (wv, dq + dkv)):
-        amd.cast_into(amd.view(ws, start * width, w.size), w.storage)
+    ws = _stacked_weights(wq, wk, wv)
     qkv = b.gemm(xs, ws, rows, width, total, transpose_right=True, out_dtype="bfloat16")
     v = b.copy_rows(qkv, rows, dkv, column=dq + dkv, row=total)
     if q_norm is None:
@@ -768,6 +840,83 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=Non
             else:
                 dnorms = tuple(map(owned, b.qk_norm_rope_backward(gq, gk, qkv, qkv, *norm_dims, **columns, out=d)[2:]))
             b.copy_rows(gv, rows, dkv, out=d, out_column=dq + dkv, out_row=total)
+            dx = None
+            if x.requires_grad:
+                dx = (ProductGradient(b, d, ws, rows, total, width, precision) if x.dtype == "float32"
+                      else b.gemm(d, ws, rows, total, width, out_dtype=x.dtype))
+            dws = (None, None, None)
+            if wq.requires_grad or wk.requires_grad or wv.requires_grad:
+                dw = b.gemm(d, xs, total, rows, width, transpose_left=True, out_dtype=wq.dtype)
+                dws = tuple(owned(amd.view(dw, start * width, w.size)) if w.requires_grad else None
+                            for w, start in ((wq, 0), (wk, dq), (wv, dq + dkv)))
+        return (dx, *dws, *dnorms)
+
+    return record(Tensor(out, shape=(batch, time, dq)), parents, backward)
+
+
+def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turns, packing):
+    """gqa_attention with a Rotary or over packed sequences.  The heads are turned
+    in the product's own columns; normed heads, whose product the backward needs,
+    go to new rows (the norm's launch turns them too, but by a Rotary's turns, which
+    take a launch of their own)."""
+    b = backend(x)
+    batch, time, width = x.shape
+    if packing is not None and (batch, time) != (1, packing.total):
+        raise ValueError("a packing's sequences lie in one row of its total tokens")
+    rows, dq, dkv = batch * time, wq.shape[0], wk.shape[0]
+    total, head = dq + 2 * dkv, dq // heads
+    precision = matmul_precision()
+    xs = _bf16_input(x)
+    ws = _stacked_weights(wq, wk, wv)
+    qkv = b.gemm(xs, ws, rows, width, total, transpose_right=True, out_dtype="bfloat16")
+    positions = None if packing is None else packing.positions
+    columns = dict(q_row=total, k_column=dq, k_row=total)
+    into = dict(out_row=total, out_k_column=dq)
+    if turns is None and q_norm is None:
+        turns = Rotary(head, theta)
+    turned = (turns, batch, time, heads, kv_heads, head)
+    if q_norm is None:
+        q, k = b.rotary(qkv, qkv, *turned, positions=positions, **columns, out=qkv, **into)
+        parents = (x, wq, wk, wv)
+    else:  # a position for each token: 0 turns nothing
+        starts = positions if turns is None else None
+        norm_dims = (q_norm.storage, k_norm.storage, *((batch, time) if turns is None and packing is None else (rows, 1)),
+                     heads, kv_heads, head, theta, eps)
+        q, k = b.qk_norm_rope(qkv, qkv, *norm_dims, **columns, starts=starts)
+        if turns is not None:
+            for side, block in ((0, q), (1, k)):
+                n = (0, kv_heads) if side else (heads, 0)
+                b.rotary(q, k, turns, batch, time, *n, head, positions=positions, out=block, out_k_column=0)
+        parents = (x, wq, wk, wv, q_norm, k_norm)
+    if packing is not None:
+        place = dict(v_column=dq + dkv, v_row=total, **(columns if q_norm is None else {}))
+        dims = (packing, heads, kv_heads, head)
+        out, lse, rest = b.attention_packed(q, k, qkv, *dims, **place, rest=True)
+    else:
+        if q_norm is None:
+            q, k = (b.copy_rows(qkv, rows, n, column=c, row=total) for n, c in ((dq, 0), (dkv, dq)))
+        v = b.copy_rows(qkv, rows, dkv, column=dq + dkv, row=total)
+        dims = (batch, time, heads, kv_heads, head)
+        out, lse = b.attention(q, k, v, *dims)
+
+    def backward(g):
+        with set_matmul_precision(precision):
+            d = amd.AMDStorage(rows * total, "bfloat16")
+            dnorms = ()
+            if packing is not None and q_norm is None:
+                b.attention_packed_backward(g, q, k, qkv, out, lse, *dims, **place, rest=rest, into=d)
+            else:
+                gq, gk, gv = (b.attention_packed_backward(g, q, k, qkv, out, lse, *dims, **place, rest=rest)
+                              if packing is not None else b.attention_backward(g, q, k, v, out, lse, *dims))
+                b.copy_rows(gv, rows, dkv, out=d, out_column=dq + dkv, out_row=total)
+            if q_norm is None:
+                source, where = ((d, d), columns) if packing is not None else ((gq, gk), {})
+                b.rotary(*source, *turned, positions=positions, inverse=True, **where, out=d, **into)
+            else:
+                if turns is not None:
+                    gq, gk = b.rotary(gq, gk, *turned, positions=positions, inverse=True)
+                dnorms = tuple(map(owned, b.qk_norm_rope_backward(gq, gk, qkv, qkv, *norm_dims, **columns, starts=starts,
+                                                                  out=d)[2:]))
             dx = None
             if x.requires_grad:
                 dx = (ProductGradient(b, d, ws, rows, total, width, precision) if x.dtype == "float32"

@@ -1,0 +1,97 @@
+"""AdamW over the tensors of a model, in a few launches whatever their number."""
+from __future__ import annotations
+
+from array import array
+from math import isfinite
+
+from .backends import amd, amd_lm
+from .core.tensor import Tensor
+
+
+class AdamW:
+    """``step()`` applies the gradients of ``parameters`` (float32 or bfloat16
+    Tensors; those without a ``grad`` are left as they are):
+
+        m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2
+        p' = p (1 - lr weight_decay) - lr m' / (1 - beta1^t) / (sqrt(v' / (1 - beta2^t)) + eps)
+
+    ``bits`` 32 holds the moments in fp32, 8 in codes of 8 bits with an exponent
+    for every 256 values, rounded up or down by chance (``seed``: the same run
+    gives the same bits).  With ``max_norm`` gradients whose norm over all tensors
+    exceeds it are scaled down to it, and a step whose norm is not finite changes
+    nothing; ``norm()`` is the last step's.  ``lr`` may be changed between steps."""
+
+    def __init__(self, parameters, lr=1e-3, *, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, max_norm=None,
+                 seed=0):
+        parameters = tuple(dict.fromkeys(parameters))
+        if not parameters or any(not isinstance(p, Tensor) or p.device != "amd" or p.dtype not in ("float32", "bfloat16")
+                                 for p in parameters):
+            raise ValueError("AdamW takes float32 or bfloat16 Tensors of the amd device")
+        if bits not in (8, 32) or type(seed) is not int or not 0 <= seed < 1 << 32:
+            raise ValueError("moments have 8 or 32 bits, the seed is an integer below 2^32")
+        if len(betas) != 2 or any(not 0 <= b < 1 for b in betas) or not 0 < eps < float("inf"):
+            raise ValueError("betas lie in [0, 1), eps is positive")
+        if max_norm is not None and not 0 < max_norm < float("inf"):
+            raise ValueError("max_norm is a positive number")
+        self.parameters, self.lr, self.betas, self.eps = parameters, lr, tuple(map(float, betas)), eps
+        self.weight_decay, self.bits, self.max_norm, self.seed = weight_decay, bits, max_norm, seed
+        self.steps = 0
+        self._state = tuple(amd_lm.AdamWMoments(p.size, bits) for p in parameters)
+        self._norm = None
+
+    def step(self):
+        rate, decay = float(self.lr), float(self.weight_decay)
+        if not (isfinite(rate) and rate >= 0 and isfinite(decay) and decay >= 0):
+            raise ValueError("lr and weight_decay are numbers of 0 or more")
+        pairs = []
+        for index, (p, state) in enumerate(zip(self.parameters, self._state)):
+            if p.grad is None:
+                continue
+            if p.size != state.size or p.grad.dtype != p.dtype or p.grad.size != p.size:
+                raise ValueError("a gradient has its parameter's size and dtype, and a parameter keeps its size")
+            pairs.append((p.storage, p.grad.storage, state, index))
+        norm = amd_lm.adamw(pairs, self.bits, rate, *self.betas, self.eps, decay, self.steps + 1, seed=self.seed,
+                            max_norm=self.max_norm)
+        self.steps += 1
+        self._norm = norm
+
+    def norm(self):
+        """The norm of all gradients of the last step, before it was cut (waits
+        for the device); None without max_norm or before a step."""
+        return None if self._norm is None else self._norm.tolist()[0]
+
+    def zero_grad(self):
+        for p in self.parameters:
+            p.zero_grad()
+
+    def _of(self, parameter):
+        for p, state in zip(self.parameters, self._state):
+            if p is parameter:
+                return state
+        raise ValueError("the optimizer does not hold this parameter")
+
+    def moments(self, parameter):
+        """(first, second) moments of one parameter as float32 Tensors: its own
+        where they are held in 32 bits, the values that its codes stand for in 8."""
+        state = self._of(parameter)
+        return tuple(Tensor(x, shape=parameter.shape) for x in state.values())
+
+    def state_dict(self):
+        """Plain values (host arrays) from which ``load_state_dict`` goes on with
+        the same bits."""
+        return {"steps": self.steps, "bits": self.bits, "seed": self.seed,
+                "moments": [[x.to_array() for x in state.storages()] for state in self._state]}
+
+    def load_state_dict(self, state):
+        moments = state["moments"]
+        if state["bits"] != self.bits or len(moments) != len(self._state) or type(state["steps"]) is not int \
+                or state["steps"] < 0:
+            raise ValueError("the state is of another optimizer")
+        for own, given in zip(self._state, moments):
+            if len(given) != len(own.storages()) or any(len(x) != len(g) for x, g in zip(own.storages(), given)):
+                raise ValueError("the state's moments have other sizes")
+        for own, given in zip(self._state, moments):
+            for x, values in zip(own.storages(), given):
+                if len(x):
+                    x.runtime.upload(x.ptr, array(values.typecode, values))
+        self.steps, self.seed = state["steps"], state["seed"]
