@@ -704,14 +704,17 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
     runtime, dtype = get_runtime(), code(q.dtype)
     out, lse = AMDStorage(packing.total * heads * dim, q.dtype), AMDStorage(packing.total * heads, "float32")
     scale = dim ** -0.5 if scale is None else float(scale)
+    left = None
     if packing.used:
         rows = runtime.lib.qutai_amd_attention_packed_rows(heads, kv_heads, dim, packing.longest, dtype, int(whole), scale, 0)
         tiles, count = packing.tiles(rows, "end" if causal else "length")
-        runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, tiles.ptr, count, rows, heads,
+        if rest and rows > 4 and q.dtype == "bfloat16" and dim <= 128:
+            left = AMDStorage(out.size, q.dtype)
+        runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count, rows, heads,
                      kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
                      mfma=_on_matrix_cores(q.dtype, dim))
-    _packed_tail(packing, out, lse)
-    return (out, lse, None) if rest else (out, lse)
+    _packed_tail(packing, out, lse, left)
+    return (out, lse, left) if rest else (out, lse)
 
 
 def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_heads, dim, *, causal=True, scale=None,
@@ -738,7 +741,7 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
         row, spans = q_row, sorted((column, column + n * dim) for (column, _), n in zip(places, (heads, kv_heads, kv_heads)))
         if not q_row == k_row == v_row or any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("into holds the gradients in separate columns of one row")
-        for x in (gradient, q, k, v, out):
+        for x in (gradient, q, k, v, out, *(() if rest is None else (rest,))):
             if into.ptr < x.ptr + x.nbytes and x.ptr < into.ptr + into.nbytes:
                 raise ValueError("into must not share memory with an input")
         results = (into,) * 3
@@ -754,7 +757,7 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
                                                                       int(whole), scale, n) for n in (1, 2))
         q_tiles, q_count = packing.tiles(q_rows, "end" if causal else "length")
         k_tiles, k_count = packing.tiles(k_rows, "start" if causal else "length")
-        runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, lse.ptr,
+        runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
                      *(at for at, _ in targets), delta.ptr, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count, k_rows,
                      heads, kv_heads, dim, q_row, k_row, v_row, *(row for _, row in targets), dtype, scale,
                      int(bool(causal)), mfma=_on_matrix_cores(q.dtype, dim))

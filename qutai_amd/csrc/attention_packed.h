@@ -1,0 +1,582 @@
+// Attention of packed bf16 sequences with heads of up to 128 channels (multiples
+// of 8) on the matrix cores, forward and backward.
+//
+// A wave takes 32 queries of one head (forward, dQ) or 32 keys of one kv head (dK,
+// dV); the other side streams through LDS in blocks of 64 rows, copied with
+// buffer_load ... lds into a ring of two stages while the block before is worked
+// on.  Scores are computed transposed (S^T = K Q^T with v_mfma_f32_32x32x16_bf16),
+// so that a lane holds one query, the softmax's maximum and sum are its own (and
+// its partner lane's), and the probabilities are the next product's operand as they
+// stand.
+//
+// The waves of a workgroup share the stream.  They take the query heads of one kv
+// head first and consecutive blocks of 32 queries after that: with four heads to a
+// kv head a tile is 64 queries of four heads instead of 256 of one.  Short documents
+// then fill tiles (70 documents of 10 to 1024 tokens: 291 tiles of 64 instead of 110
+// of 256, of which a third is padding), and causal waves of a tile end their work
+// within two blocks of each other.
+//
+// Roundings to fewer bits: the probabilities and dS go into the second products as
+// bf16 (2^-8 of each, of random sign, as their other operand has; the normaliser
+// sums them in fp32), everything else stays fp32 until a result is stored.  out's
+// own rounding is returned as a second bf16 (`rest`), from which the backward sums
+// delta = dO . (out + rest): documents of a few tokens would otherwise see that
+// rounding as an error of all their dS (1.2 times the error of dQ and dK).
+//
+// A wave whose sums hold an infinity or NaN (its operands did, masked or not)
+// computes its rows again one at a time (attention_rows.h), where what is masked is
+// not read.
+#pragma once
+#include "attention_rows.h"
+#include "attention_mma.h"
+
+namespace {
+
+// Heads of a kv head that share a workgroup of NW waves: the largest power of two.
+constexpr int packed_heads(int64_t heads, int64_t kv_heads, int waves) {
+  int n = 1;
+  while (2 * n <= waves && heads / kv_heads % (2 * n) == 0) n *= 2;
+  return n;
+}
+
+template <int DP>
+struct PackedTile {
+  static constexpr int S = DP / 16, DB = DP / 32;  // MFMA k-steps over d, 32-wide d blocks
+  static constexpr int PC = DP / 8;                // 16-byte chunks of a row
+  typedef AttnTile<false, DP> Base;
+  static_assert(Base::PITCH == DP, "rows lie without gaps");
+
+  // Copies of a block of ROWS rows by NW waves: chunk (j * NW + wave) * 64 + lane of
+  // the block, at c ^ swz(r) of row r.
+  template <int ROWS, int NW>
+  struct Copy {
+    static constexpr int N = ROWS * PC / 64 / NW;
+    static_assert(N * NW * 64 == ROWS * PC, "whole copies");
+    uint32_t off[N];
+    int row[N];
+    __device__ __forceinline__ void plan(int64_t pitch, int D, int wave, int lane) {
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const int at = (j * NW + wave) * 64 + lane, r = at / PC, c = (at % PC) ^ Base::swz(r);
+        row[j] = r;
+        off[j] = (uint32_t)((r * pitch + 8 * c) * 2) | (8 * c < D ? 0u : ATTN_OOB);
+      }
+    }
+    // rows at or beyond `left` and channels at or beyond D arrive as zeros
+    __device__ __forceinline__ void issue(bf16_t* to, const bf16_t* from, int64_t pitch, int left, int wave) const {
+      const u32x4 r = lds_rsrc(from, ROWS * pitch * 2);
+#pragma unroll
+      for (int j = 0; j < N; j++)
+        lds_load16(r, reinterpret_cast<char*>(to) + (j * NW + wave) * 1024, off[j] | (row[j] < left ? 0u : ATTN_OOB));
+    }
+  };
+
+  // The wave's own 32 rows as operands: lane = row col, d = 16 s + 8 half + [0, 8).
+  __device__ static __forceinline__ void own(const void* base, int64_t first, int64_t pitch, int left, int D, int col,
+                                             int half, bf16x8 (&f)[S]) {
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<bf16_t*>(uniform_ptr((const bf16_t*)base + first)), 0, (uint32_t)(32 * pitch * 2), 0x00020000);
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      const int d = 16 * s + 8 * half;
+      const uint32_t off = (uint32_t)((col * pitch + d) * 2) | (col < left && d < D ? 0u : ATTN_OOB);
+      f[s] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    }
+  }
+
+  __device__ static __forceinline__ bf16x8 rows(const bf16_t* x, int r, int s, int half) {
+    bf16x8 f[1];
+    Base::rows(x, r, s, half, f);
+    return f[0];
+  }
+  __device__ static __forceinline__ bf16x8 columns(const bf16_t* x, int db, int rb, int lane) {
+    bf16x8 f[1];
+    Base::columns(x, db, rb, lane, f);
+    return f[0];
+  }
+};
+
+__device__ __forceinline__ bf16x8 rounded(const float* v) {
+  const u32x4 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+  return __builtin_bit_cast(bf16x8, w);
+}
+
+// The tile, heads and rows of a wave of a query tile.
+struct PackedPlace {
+  int h, kvh, first, q0;  // first row of the tile, of the wave
+};
+template <int NW>
+__device__ __forceinline__ PackedPlace enter_queries(AttnPackedArgs& p, int wave) {
+  const int pack = p.pack, subs = (int)p.heads / pack;
+  const int tile = uniform32((int)blockIdx.x / subs), h0 = uniform32((int)blockIdx.x % subs) * pack;
+  PackedPlace at;
+  at.first = enter_sequence<bf16_t>(p, tile);
+  at.h = uniform32(h0 + wave % pack);
+  at.kvh = uniform32(h0 / (int)(p.heads / p.kv_heads));
+  at.q0 = uniform32(at.first + wave / pack * 32);
+  return at;
+}
+
+// The 32 keys from row 32 mb of the block on, for the wave's queries.  lim (MASK):
+// the keys of the block that the lane's query sees, less 4 half.
+template <int DP, bool MASK>
+__device__ __forceinline__ void packed_attend(const bf16_t* sk, const bf16_t* sv, const bf16x8 (&qf)[DP / 16],
+                                              f32x16 (&o)[DP / 32], float& m, float& l, int lim, float c, int lane,
+                                              int mb) {
+  typedef PackedTile<DP> Tile;
+  const int half = lane >> 5, col = lane & 31;
+  f32x16 sc = {};
+#pragma unroll
+  for (int s = 0; s < Tile::S; s++)
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, 32 * mb + col, s, half), qf[s], sc, 0, 0, 0);
+  if constexpr (MASK) {
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (32 * mb + 8 * (e >> 2) + (e & 3) >= lim) sc[e] = -INFINITY;
+  }
+  float peak = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < 16; e++) peak = fmaxf(peak, sc[e]);
+  // the reference point m moves only for a maximum more than 2^8 above it
+  const float cand = pair_max(peak) * c;
+  const bool grow = cand > m + 8.f;
+  if (__builtin_amdgcn_ballot_w64(grow)) {
+    if (grow) {
+      const float alpha = __builtin_amdgcn_exp2f(m - cand);
+      m = cand;
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[db][e] *= alpha;
+    }
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+  bf16x8 pf[2];
+#pragma unroll
+  for (int st = 0; st < 2; st++) {
+    float pv[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * st + e], c, -ref));
+      sum += pv[e];
+    }
+    pf[st] = rounded(pv);
+  }
+  l += sum;
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+    for (int st = 0; st < 2; st++)
+      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sv, db, 32 * mb + 16 * st, lane), pf[st], o[db], 0, 0, 0);
+}
+
+// Four consecutive channels of a result row, and of what its rounding left.
+__device__ __forceinline__ void put_rest(void* base, int64_t at, const f32x4& v, const u32x2& stored) {
+  const f32x4 kept = {__uint_as_float(stored[0] << 16), __uint_as_float(stored[0] & 0xffff0000u),
+                      __uint_as_float(stored[1] << 16), __uint_as_float(stored[1] & 0xffff0000u)};
+  const f32x4 left = v - kept;
+  global_store((bf16_t*)base + at, u32x2{pack_bf16x2(left[0], left[1]), pack_bf16x2(left[2], left[3])});
+}
+
+template <int DP, int NW>
+__global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_fwd(AttnPackedArgs p) {
+  typedef PackedTile<DP> Tile;
+  constexpr int KB = 64;
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * DP];  // [stage][K, V]
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
+  const PackedPlace at = enter_queries<NW>(p, wave);
+  const int T = (int)p.time, D = (int)p.dim, q0 = at.q0, t = q0 + col, tile_rows = NW / p.pack * 32;
+  const bf16_t* K = uniform_ptr((const bf16_t*)p.k + at.kvh * p.kh);
+  const bf16_t* V = uniform_ptr((const bf16_t*)p.v + at.kvh * p.kh);
+
+  bf16x8 qf[Tile::S];
+  Tile::own(p.q, at.h * p.qh + (int64_t)q0 * p.qt, p.qt, T - q0, D, col, half, qf);
+  typename Tile::template Copy<KB, NW> ck, cv;
+  ck.plan(p.kt, D, wave, lane);
+  cv.plan(p.vt, D, wave, lane);
+  auto issue = [&](int kbk) {
+    const int64_t kv0 = (int64_t)kbk * KB;
+    ck.issue(&lds[kbk & 1][0][0], K + kv0 * p.kt, p.kt, T - kbk * KB, wave);
+    cv.issue(&lds[kbk & 1][1][0], V + kv0 * p.vt, p.vt, T - kbk * KB, wave);
+  };
+
+  f32x16 o[Tile::DB];
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++) o[db] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  const float c = p.scale_log2;
+  // blocks of which the wave's queries see every key, halves of blocks of which they
+  // see some, blocks of which they see none (the copies' and barriers' order is kept)
+  const int nkb = ((p.causal ? min(at.first + tile_rows, T) : T) + KB - 1) / KB;
+  const int seen = q0 >= T ? 0 : p.causal ? min(q0 + 32, T) : T;
+  const int n_full = min(seen, p.causal ? q0 + 1 : T) / KB;
+  auto advance = [&](int kbk) {  // wait for a block, start the next one's copies
+    wait_vmcnt<0>();
+    asm volatile("s_barrier" ::: "memory");
+    if (kbk + 1 < nkb) issue(kbk + 1);
+  };
+  if (nkb > 0) issue(0);
+  int kbk = 0;
+  for (; kbk < n_full; kbk++) {
+    advance(kbk);
+    packed_attend<DP, false>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, o, m, l, 0, c, lane, 0);
+    packed_attend<DP, false>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, o, m, l, 0, c, lane, 1);
+  }
+  for (; kbk * KB < seen; kbk++) {
+    advance(kbk);
+    const int kv0 = kbk * KB, lim = min(T - kv0, p.causal ? t - kv0 + 1 : KB) - 4 * half;
+#pragma unroll 1
+    for (int mb = 0; mb < 2 && kv0 + 32 * mb < seen; mb++)
+      packed_attend<DP, true>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, o, m, l, lim, c, lane, mb);
+  }
+  for (; kbk < nkb; kbk++) advance(kbk);
+
+  const float total = pair_sum(l);
+  const float bad = not_finite(o) + total * 0.f + m * 0.f;
+  if (__builtin_amdgcn_ballot_w64(t < T && !(bad == 0.f))) {
+    for (int i = 0; i < 32 && q0 + i < T; i++) {
+      fwd_row<bf16_t>(p, 0, at.h, q0 + i, lane);
+      if (p.rest)
+        for (int d = lane; d < D; d += 64) ((bf16_t*)p.rest)[at.h * p.qh + (int64_t)(q0 + i) * p.ot + d] = 0;
+    }
+    return;
+  }
+  if (t < T) {
+    const float inv = 1.f / total;
+    const int64_t to = at.h * p.qh + (int64_t)t * p.ot;
+#pragma unroll
+    for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = 32 * db + 8 * g + 4 * half;
+        if (d >= D) continue;
+        const f32x4 v = f32x4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]} * inv;
+        const u32x2 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        global_store((bf16_t*)p.dq + to + d, w);
+        if (p.rest) put_rest(p.rest, to + d, v, w);
+      }
+    if (half == 0) p.lse[at.h + t * p.lt] = (m + __log2f(total)) * 0.6931471805599453f;
+  }
+}
+
+// dQ of the wave's queries, and delta; K and V stream.
+template <int DP, bool MASK>
+__device__ __forceinline__ void packed_dq_step(const bf16_t* sk, const bf16_t* sv, const bf16x8 (&qf)[DP / 16],
+                                               const bf16x8 (&gf)[DP / 16], float lse2, float dl,
+                                               f32x16 (&dqt)[DP / 32], int lim, float c, int lane, int mb) {
+  typedef PackedTile<DP> Tile;
+  const int half = lane >> 5, col = lane & 31;
+  f32x16 sc = {}, dp = {};
+#pragma unroll
+  for (int s = 0; s < Tile::S; s++) {
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, 32 * mb + col, s, half), qf[s], sc, 0, 0, 0);
+    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sv, 32 * mb + col, s, half), gf[s], dp, 0, 0, 0);
+  }
+  bf16x8 dsf[2];
+#pragma unroll
+  for (int st = 0; st < 2; st++) {
+    float ds[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int e = 8 * st + i;
+      float x = sc[e];
+      if constexpr (MASK)
+        if (32 * mb + 8 * (e >> 2) + (e & 3) >= lim) x = -INFINITY;
+      ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, -lse2)) * (dp[e] - dl);
+    }
+    dsf[st] = rounded(ds);
+  }
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+    for (int st = 0; st < 2; st++)
+      dqt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sk, db, 32 * mb + 16 * st, lane), dsf[st], dqt[db], 0, 0, 0);
+}
+
+template <int DP, int NW>
+__global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnPackedArgs p) {
+  typedef PackedTile<DP> Tile;
+  constexpr int KB = 64;
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * DP];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
+  const PackedPlace at = enter_queries<NW>(p, wave);
+  const int T = (int)p.time, D = (int)p.dim, q0 = at.q0, t = q0 + col, tile_rows = NW / p.pack * 32;
+  const bf16_t* K = uniform_ptr((const bf16_t*)p.k + at.kvh * p.kh);
+  const bf16_t* V = uniform_ptr((const bf16_t*)p.v + at.kvh * p.kh);
+  const int64_t head = at.h * p.qh;
+
+  bf16x8 qf[Tile::S], gf[Tile::S];
+  float dl = 0.f, lse2 = 0.f;
+  {
+    Tile::own(p.g, head + (int64_t)q0 * p.ot, p.ot, T - q0, D, col, half, gf);
+    // delta: the diagonal of O dO^T, summed as dP is, so that a query that sees one
+    // key leaves what O and V leave, and of the rest
+    f32x16 og = {};
+    Tile::own(p.o, head + (int64_t)q0 * p.ot, p.ot, T - q0, D, col, half, qf);
+#pragma unroll
+    for (int s = 0; s < Tile::S; s++) og = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[s], gf[s], og, 0, 0, 0);
+    if (p.rest) {
+      Tile::own(p.rest, head + (int64_t)q0 * p.ot, p.ot, T - q0, D, col, half, qf);
+#pragma unroll
+      for (int s = 0; s < Tile::S; s++) og = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[s], gf[s], og, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (8 * (e >> 2) + 4 * half + (e & 3) == col) dl = og[e];
+    dl = pair_sum(dl);
+    const int64_t li = at.h + (int64_t)t * p.lt;
+    if (t < T) lse2 = p.lse[li] * LOG2E;
+    if (t < T && half == 0) p.delta[li] = dl;
+    Tile::own(p.q, head + (int64_t)q0 * p.qt, p.qt, T - q0, D, col, half, qf);
+  }
+  typename Tile::template Copy<KB, NW> ck, cv;
+  ck.plan(p.kt, D, wave, lane);
+  cv.plan(p.vt, D, wave, lane);
+  auto issue = [&](int kbk) {
+    const int64_t kv0 = (int64_t)kbk * KB;
+    ck.issue(&lds[kbk & 1][0][0], K + kv0 * p.kt, p.kt, T - kbk * KB, wave);
+    cv.issue(&lds[kbk & 1][1][0], V + kv0 * p.vt, p.vt, T - kbk * KB, wave);
+  };
+  f32x16 dqt[Tile::DB];
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++) dqt[db] = f32x16{};
+  const float c = p.scale_log2;
+  const int nkb = ((p.causal ? min(at.first + tile_rows, T) : T) + KB - 1) / KB;
+  const int seen = q0 >= T ? 0 : p.causal ? min(q0 + 32, T) : T;
+  const int n_full = min(seen, p.causal ? q0 + 1 : T) / KB;
+  auto advance = [&](int kbk) {
+    wait_vmcnt<0>();
+    asm volatile("s_barrier" ::: "memory");
+    if (kbk + 1 < nkb) issue(kbk + 1);
+  };
+  if (nkb > 0) issue(0);
+  int kbk = 0;
+  for (; kbk < n_full; kbk++) {
+    advance(kbk);
+#pragma unroll 1
+    for (int mb = 0; mb < 2; mb++)
+      packed_dq_step<DP, false>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, gf, lse2, dl, dqt, 0, c, lane, mb);
+  }
+  for (; kbk * KB < seen; kbk++) {
+    advance(kbk);
+    const int kv0 = kbk * KB, lim = min(T - kv0, p.causal ? t - kv0 + 1 : KB) - 4 * half;
+#pragma unroll 1
+    for (int mb = 0; mb < 2 && kv0 + 32 * mb < seen; mb++)
+      packed_dq_step<DP, true>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, gf, lse2, dl, dqt, lim, c, lane, mb);
+  }
+  for (; kbk < nkb; kbk++) advance(kbk);
+
+  if (__builtin_amdgcn_ballot_w64(t < T && !(not_finite(dqt) + dl * 0.f == 0.f))) {
+    for (int i = 0; i < 32 && q0 + i < T; i++) bwd_q_row<bf16_t>(p, 0, at.h, q0 + i, lane);
+    return;
+  }
+  if (t < T) {
+    const int64_t to = head + (int64_t)t * p.dqt;
+#pragma unroll
+    for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = 32 * db + 8 * g + 4 * half;
+        if (d < D)
+          put4<false>(p.dq, to + d, f32x4{dqt[db][4 * g], dqt[db][4 * g + 1], dqt[db][4 * g + 2], dqt[db][4 * g + 3]} * p.scale);
+      }
+  }
+}
+
+// A key tile: 4 waves of 32 keys; QB: rows of a streamed block.  Two sums of 128
+// channels and K and V of the wave's keys do not fit 256 registers beside the scores
+// (97 of them spilled): there V stays in LDS, for 8 reads more beside 32 products,
+// and blocks of 32 rows leave room for two workgroups on a CU.
+template <int DP>
+struct PackedKeys {
+  static constexpr int NW = 4, ROWS = NW * 32, QB = DP > 64 ? 32 : 64;
+  static constexpr bool V_IN_LDS = DP > 64;
+  static constexpr int VF = V_IN_LDS ? 1 : DP / 16;
+};
+
+// dK and dV of the wave's 32 keys: 32 queries from row 32 mb of the streamed block
+// on.  Element e of a score block: query 32 mb + 8 (e / 4) + 4 half + e % 4, key col.
+// One product after the other, so that dK's and dV's sums, the wave's K and V and
+// one block of scores and dP are all that lives.
+template <int DP, bool MASK>
+__device__ __forceinline__ void packed_dkv_step(const bf16_t* sq, const bf16_t* sg, const float* slse, const float* sdl,
+                                                const bf16x8 (&kf)[DP / 16], const bf16x8 (&vf)[PackedKeys<DP>::VF],
+                                                const bf16_t* sv, int own, f32x16 (&dkt)[DP / 32], f32x16 (&dvt)[DP / 32], int end, int before,
+                                                float c, int lane, int mb) {
+  typedef PackedTile<DP> Tile;
+  const int half = lane >> 5, col = lane & 31;
+  f32x16 sc = {};
+#pragma unroll
+  for (int s = 0; s < Tile::S; s++)
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sq, 32 * mb + col, s, half), kf[s], sc, 0, 0, 0);
+  if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+  float pr[16];
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const f32x4 l4 = *reinterpret_cast<const f32x4*>(slse + 32 * mb + 8 * j + 4 * half);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      float x = sc[4 * j + i];
+      if constexpr (MASK) {
+        const int q = 32 * mb + 8 * j + 4 * half + i;
+        if (q >= end || q < before) x = -INFINITY;  // before: of a causal key
+      }
+      pr[4 * j + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, c, l4[i]));  // slse holds -lse log2(e)
+    }
+  }
+  bf16x8 w[2] = {rounded(pr), rounded(pr + 8)};
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+    for (int st = 0; st < 2; st++)
+      dvt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sg, db, 32 * mb + 16 * st, lane), w[st], dvt[db], 0, 0, 0);
+  if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+  f32x16 dp = {};
+#pragma unroll
+  for (int s = 0; s < Tile::S; s++)
+    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sg, 32 * mb + col, s, half),
+                                                 PackedKeys<DP>::V_IN_LDS ? Tile::rows(sv, own, s, half)
+                                                                          : vf[PackedKeys<DP>::V_IN_LDS ? 0 : s],
+                                                 dp, 0, 0, 0);
+  if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const f32x4 d4 = *reinterpret_cast<const f32x4*>(sdl + 32 * mb + 8 * j + 4 * half);
+#pragma unroll
+    for (int i = 0; i < 4; i++) pr[4 * j + i] *= dp[4 * j + i] - d4[i];
+  }
+  w[0] = rounded(pr);
+  w[1] = rounded(pr + 8);
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+    for (int st = 0; st < 2; st++)
+      dkt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sq, db, 32 * mb + 16 * st, lane), w[st], dkt[db], 0, 0, 0);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(256, 2) packed_bwd_dkv(AttnPackedArgs p) {
+  typedef PackedTile<DP> Tile;
+  constexpr int NW = PackedKeys<DP>::NW, QB = PackedKeys<DP>::QB;
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][QB * DP];     // [stage][Q, dO]
+  __shared__ __attribute__((aligned(16))) float stats[2][2][QB];         // [stage][-lse log2(e), delta]
+  constexpr bool V_IN_LDS = PackedKeys<DP>::V_IN_LDS;
+  __shared__ __attribute__((aligned(16))) bf16_t own_v[V_IN_LDS ? NW * 32 * DP : 8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
+  const int group = (int)(p.heads / p.kv_heads), nsplit = p.split ? group : 1;
+  int b, kvh, blk, gsel;
+  place_keys<bf16_t, 1>(p, nsplit, b, kvh, blk, gsel);
+  const int T = (int)p.time, D = (int)p.dim, k0 = blk, kw = uniform32(k0 + wave * 32), key = kw + col;
+  const int g_lo = p.split ? gsel : 0, g_hi = p.split ? gsel + 1 : group;
+
+  bf16x8 kf[Tile::S], vf[PackedKeys<DP>::VF];
+  Tile::own(p.k, kvh * p.kh + (int64_t)kw * p.kt, p.kt, T - kw, D, col, half, kf);
+  if constexpr (V_IN_LDS) {  // there before the first block is, whose wait and barrier cover it
+    typename Tile::template Copy<NW * 32, NW> cv;
+    cv.plan(p.vt, D, wave, lane);
+    cv.issue(own_v, uniform_ptr((const bf16_t*)p.v + kvh * p.kh + (int64_t)k0 * p.vt), p.vt, T - k0, wave);
+  } else {
+    Tile::own(p.v, kvh * p.kh + (int64_t)kw * p.vt, p.vt, T - kw, D, col, half, vf);
+  }
+  f32x16 dkt[Tile::DB], dvt[Tile::DB];
+#pragma unroll
+  for (int db = 0; db < Tile::DB; db++) dkt[db] = dvt[db] = f32x16{};
+
+  const int qs0 = p.causal ? k0 : 0, nq = (T - qs0 + QB - 1) / QB, iterations = nq * (g_hi - g_lo);
+  typename Tile::template Copy<QB, NW> cq, cg;
+  cq.plan(p.qt, D, wave, lane);
+  cg.plan(p.ot, D, wave, lane);
+  float next = 0.f;  // waves 0 and 1: the lane's row of the block in flight, lse and delta
+  auto issue = [&](int it, int h, int qs) {
+    const int stage = it & 1;
+    cq.issue(&lds[stage][0][0], uniform_ptr((const bf16_t*)p.q + h * p.qh + (int64_t)qs * p.qt), p.qt, T - qs, wave);
+    cg.issue(&lds[stage][1][0], uniform_ptr((const bf16_t*)p.g + h * p.qh + (int64_t)qs * p.ot), p.ot, T - qs, wave);
+    if (wave < 2 && lane < QB) {
+      const float* from = wave ? p.delta : p.lse;
+      next = qs + lane < T ? from[h + (int64_t)(qs + lane) * p.lt] : 0.f;
+    }
+  };
+  // wait for a block, start the copies of the next one: of the same head, or the
+  // first of the next
+  auto advance = [&](int it, int h, int qi) {
+    wait_vmcnt<0>();
+    if (wave < 2 && lane < QB) {
+      stats[it & 1][wave][lane] = wave ? next : -next * LOG2E;
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): in LDS before the barrier
+    }
+    asm volatile("s_barrier" ::: "memory");
+    if (it + 1 < iterations) {
+      const bool wrap = qi + 1 == nq;
+      issue(it + 1, wrap ? h + 1 : h, qs0 + (wrap ? 0 : qi + 1) * QB);
+    }
+  };
+  // steps of 32 queries, per head: before every key of the wave (causal; skipped),
+  // on the diagonal (masked), with every pair visible, at the sequence's end (masked),
+  // behind it (skipped)
+  constexpr int HB = QB / 32;
+  const int steps = nq * HB, rows = T - qs0;
+  auto clamped = [&](int x, int lo) { return x < lo ? lo : x > steps ? steps : x; };
+  const bool none = kw >= T;
+  const int skipped = none ? steps : p.causal ? clamped((kw - qs0) / 32, 0) : 0;
+  const int diagonal = none ? steps : clamped(p.causal ? skipped + 1 : 0, skipped);
+  const int tail = none ? steps : clamped(rows / 32, diagonal);
+  const int end = none ? steps : clamped((rows + 31) / 32, tail);
+  if (iterations > 0) issue(0, kvh * group + g_lo, qs0);
+  int it = -1;
+  for (int h = kvh * group + g_lo; h < kvh * group + g_hi; h++) {
+    auto enter = [&](int st) {
+      if (st % HB == 0) advance(++it, h, st / HB);
+    };
+    auto step = [&](int st, auto mask) {
+      const int qi = st / HB, qs = qs0 + qi * QB;
+      packed_dkv_step<DP, decltype(mask)::value>(&lds[it & 1][0][0], &lds[it & 1][1][0], &stats[it & 1][0][0],
+                                                 &stats[it & 1][1][0], kf, vf, own_v, 32 * wave + col, dkt, dvt, T - qs,
+                                                 p.causal ? key - qs : -1, p.scale_log2, lane, st % HB);
+    };
+    int st = 0;
+    for (; st < skipped; st++) enter(st);
+    for (; st < diagonal; st++) {
+      enter(st);
+      step(st, std::true_type{});
+    }
+    for (; st < tail; st++) {
+      enter(st);
+      step(st, std::false_type{});
+    }
+    for (; st < end; st++) {
+      enter(st);
+      step(st, std::true_type{});
+    }
+    for (; st < steps; st++) enter(st);
+  }
+
+  const bool bad = key < T && !(not_finite(dkt) + not_finite(dvt) == 0.f);
+  if (__builtin_amdgcn_ballot_w64(bad)) {
+    for (int i = 0; i < 32 && kw + i < T; i++) bwd_kv_row<bf16_t>(p, 0, kvh, kw + i, lane, g_lo, g_hi);
+    return;
+  }
+  if (key < T) {
+    const int64_t head = kvh * p.kh, part = gsel * p.part_stride + head + (int64_t)key * part_pitch(p);
+    const int64_t to_k = head + (int64_t)key * p.dkt, to_v = head + (int64_t)key * p.dvt;
+#pragma unroll
+    for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = 32 * db + 8 * g + 4 * half;
+        if (d >= D) continue;
+        const f32x4 x = {dkt[db][4 * g], dkt[db][4 * g + 1], dkt[db][4 * g + 2], dkt[db][4 * g + 3]};
+        const f32x4 y = {dvt[db][4 * g], dvt[db][4 * g + 1], dvt[db][4 * g + 2], dvt[db][4 * g + 3]};
+        if (p.split) {
+          global_store(p.part_k + part + d, x);
+          global_store(p.part_v + part + d, y);
+        } else {
+          put4<false>(p.dk, to_k + d, x * p.scale);
+          put4<false>(p.dv, to_v + d, y);
+        }
+      }
+  }
+}
+
+}  // namespace

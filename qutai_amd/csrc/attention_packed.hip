@@ -9,16 +9,20 @@
 //
 // The caller's tile tables say which rows of which sequence a workgroup takes, in
 // the order in which the workgroups start; every tile lies in one sequence, so
-// padding costs no work and no mask but a sequence's own end is needed.
+// padding costs no work and no mask but a sequence's own end is needed.  bf16 heads of
+// up to 128 channels take the kernels of attention_packed.h, fp32 and wider heads those
+// that keep fp32 values in bf16 parts (attention_mma.h), rows that are not whole
+// 16-byte chunks and sequences of a few tokens one wave per row (attention_rows.h).
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 
-#include "attention_rows.h"
-#include "attention_mma.h"
+#include "attention_packed.h"
 
 namespace {
 
-constexpr int64_t MMA_ROWS = 128;  // queries or keys of a workgroup of the matrix kernels
+constexpr int64_t MMA_ROWS = 128;  // queries or keys of a workgroup of attention_mma.h's kernels
+constexpr int WAVES = 8;           // of a workgroup of attention_packed.h's query kernels
 
 template <class T>
 __global__ void __launch_bounds__(GEN_WAVES * 64) packed_fwd_rows(AttnPackedArgs p) {
@@ -43,6 +47,13 @@ __global__ void __launch_bounds__(GEN_WAVES * 64) packed_bwd_kv_rows(AttnPackedA
 }
 
 enum Pass { FORWARD, QUERIES, KEYS };
+
+template <int DP>
+void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
+  if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+  else if (pass == QUERIES) hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+  else hipLaunchKernelGGL((packed_bwd_dkv<DP>), dim3(blocks), dim3(256), 0, stream, a);
+}
 
 template <bool F32, int DP>
 void launch_mma(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
@@ -69,20 +80,33 @@ void launch_rows(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_
 // Whether the matrix kernels take rows of this type and width (of whole 16-byte chunks).
 bool mma_fits(int dtype, int64_t dim) { return dtype == BF16 ? dim % 8 == 0 && dim <= 256 : dim % 4 == 0 && dim <= 128; }
 
-// One pass over the tiles of `rows` rows each; blocks of each tile: heads of its side.
+bool packed_fits(int dtype, int64_t dim) { return dtype == BF16 && dim % 8 == 0 && dim <= 128; }
+
+// Workgroups of a tile: heads of its side, less those that share one.
+int64_t groups_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim, int64_t rows) {
+  if (pass == KEYS) return kv_heads;
+  return rows != GEN_WAVES && packed_fits(dtype, dim) ? heads / packed_heads(heads, kv_heads, WAVES) : heads;
+}
+
+// Rows of a tile of the matrix kernels.
+int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim) {
+  if (!packed_fits(dtype, dim)) return MMA_ROWS;
+  return pass == KEYS ? PackedKeys<64>::ROWS : WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
+}
+
+// One pass over the tiles of `rows` rows each.
 hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, const int64_t* tiles, int64_t count, int64_t rows,
-                  int64_t blocks, hipStream_t stream) {
+                  hipStream_t stream) {
   if (!count) return hipSuccess;
   a.tiles = tiles;
-  const unsigned n = (unsigned)(count * blocks);
+  a.pack = packed_heads(a.heads, a.kv_heads, WAVES);
+  const unsigned n = (unsigned)(count * groups_of(pass, dtype, a.heads, a.kv_heads, a.dim, rows));
   if (rows == GEN_WAVES) {
     if (dtype == BF16) launch_rows<bf16_t>(pass, a, n, stream);
     else launch_rows<float>(pass, a, n, stream);
   } else if (dtype == BF16) {
-    if (a.dim <= 32) launch_mma<false, 32>(pass, a, n, stream);
-    else if (a.dim <= 64) launch_mma<false, 64>(pass, a, n, stream);
-    else if (a.dim <= 96) launch_mma<false, 96>(pass, a, n, stream);
-    else if (a.dim <= 128) launch_mma<false, 128>(pass, a, n, stream);
+    if (a.dim <= 64) launch_packed<64>(pass, a, n, stream);
+    else if (a.dim <= 128) launch_packed<128>(pass, a, n, stream);
     else launch_mma<false, 256>(pass, a, n, stream);
   } else {
     if (a.dim <= 32) launch_mma<true, 32>(pass, a, n, stream);
@@ -95,14 +119,14 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, const int64_t* tiles, 
 
 // What forward and backward share: sizes, scale, pitches.  rows: of a tile.
 int set_packed(AttnPackedArgs& a, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
-               int64_t v_row, int dtype, double scale, int causal, std::initializer_list<int64_t> tile_rows) {
+               int64_t v_row, int dtype, double scale, int causal, std::initializer_list<std::pair<Pass, int64_t>> tiles) {
   if ((dtype != BF16 && dtype != F32) || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1 << 16) return QA_EINVAL;
   if (dim <= 0 || dim > 256 || !(scale > 0.0) || scale > 1e30) return QA_EINVAL;
   if (q_row < heads * dim || k_row < kv_heads * dim || v_row < kv_heads * dim) return QA_EINVAL;
   if (std::max({q_row, k_row, v_row, heads * dim}) > 1 << 22) return QA_EINVAL;  // 64 rows within a buffer descriptor
-  for (int64_t rows : tile_rows) {
-    if (rows != GEN_WAVES && rows != MMA_ROWS) return QA_EINVAL;
-    if (rows == MMA_ROWS && (!mma_fits(dtype, dim) || scale < 0x1p-50)) return QA_EINVAL;
+  for (const auto& [pass, rows] : tiles) {
+    if (rows == GEN_WAVES) continue;
+    if (rows != rows_of(pass, dtype, heads, kv_heads, dim) || !mma_fits(dtype, dim) || scale < 0x1p-50) return QA_EINVAL;
   }
   a.batch = 1;
   a.heads = heads;
@@ -129,8 +153,8 @@ bool whole(std::initializer_list<const void*> pointers, std::initializer_list<in
   return aligned16(pointers);
 }
 
-// Workgroups of 256 threads that a launch can hold.
-bool grid_fits(int64_t tiles, int64_t blocks) { return tiles >= 0 && tiles <= ((1ll << 24) - 1) / blocks; }
+// Workgroups of 512 threads that a launch can hold.
+bool grid_fits(int64_t tiles, int64_t blocks) { return tiles >= 0 && tiles <= ((1ll << 23) - 1) / blocks; }
 
 }  // namespace
 
@@ -138,41 +162,45 @@ extern "C" {
 
 int64_t qutai_amd_attention_packed_rows(int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype,
                                         int aligned, double scale, int pass) {
-  if ((dtype != BF16 && dtype != F32) || dim <= 0 || dim > 256 || pass < 0 || pass > 2 || heads <= 0 || kv_heads <= 0)
+  if ((dtype != BF16 && dtype != F32) || dim <= 0 || dim > 256 || pass < 0 || pass > 2 || heads <= 0 || kv_heads <= 0 ||
+      heads % kv_heads)
     return 0;
   if (!aligned || !mma_fits(dtype, dim) || scale < 0x1p-50 || longest <= (pass == FORWARD ? 2 : 4)) return GEN_WAVES;
-  return MMA_ROWS;
+  return rows_of((Pass)pass, dtype, heads, kv_heads, dim);
 }
 
-int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse,
+int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
                                    const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t heads,
                                    int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
                                    double scale, int causal, void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {tile_rows});
+  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
   if (status != QA_OK) return status;
   if (!grid_fits(tile_count, heads)) return QA_EINVAL;
+  if (rest && (tile_rows == GEN_WAVES || !packed_fits(dtype, dim))) return QA_EINVAL;
   if (!tile_count) return QA_OK;
   if (!q || !k || !v || !out || !lse || !tiles) return QA_EINVAL;
-  if (tile_rows != GEN_WAVES && !whole({q, k, v, out}, {q_row, k_row, v_row}, dtype)) return QA_EINVAL;
+  if (tile_rows != GEN_WAVES && !whole({q, k, v, out, rest ? rest : out}, {q_row, k_row, v_row}, dtype)) return QA_EINVAL;
   a.q = q;
   a.k = k;
   a.v = v;
   a.dq = out;
   a.dqt = a.ot;
   a.lse = lse;
-  return (int)launch(FORWARD, dtype, a, tiles, tile_count, tile_rows, heads, (hipStream_t)stream);
+  a.rest = rest;
+  return (int)launch(FORWARD, dtype, a, tiles, tile_count, tile_rows, (hipStream_t)stream);
 }
 
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                   const float* lse, void* dq, void* dk, void* dv, float* delta,
+                                   const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
                                    const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
                                    const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t heads,
                                    int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
                                    int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
                                    void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {query_rows, key_rows});
+  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
+                                {{QUERIES, query_rows}, {KEYS, key_rows}});
   if (status != QA_OK) return status;
   if (dq_row < heads * dim || dk_row < kv_heads * dim || dv_row < kv_heads * dim) return QA_EINVAL;
   if (std::max({dq_row, dk_row, dv_row}) > 1 << 22) return QA_EINVAL;
@@ -181,13 +209,14 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
   if (!grad || !q || !k || !v || !out || !dq || !dk || !dv || !lse || !delta || !query_tiles || !key_tiles)
     return QA_EINVAL;
   if ((query_rows != GEN_WAVES || key_rows != GEN_WAVES) &&
-      !whole({grad, q, k, v, out, dq, dk, dv}, {q_row, k_row, v_row, dq_row, dk_row, dv_row}, dtype))
+      !whole({grad, q, k, v, out, rest ? rest : out, dq, dk, dv}, {q_row, k_row, v_row, dq_row, dk_row, dv_row}, dtype))
     return QA_EINVAL;
   a.g = grad;
   a.q = q;
   a.k = k;
   a.v = v;
   a.o = out;
+  a.rest = query_rows == GEN_WAVES || !packed_fits(dtype, dim) ? nullptr : const_cast<void*>(rest);
   a.lse = const_cast<float*>(lse);
   a.delta = delta;
   a.dq = dq;
@@ -197,9 +226,9 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
   a.dkt = dk_row;
   a.dvt = dv_row;
   // the query pass writes delta, which the key pass reads
-  const hipError_t e = launch(QUERIES, dtype, a, query_tiles, query_count, query_rows, heads, (hipStream_t)stream);
+  const hipError_t e = launch(QUERIES, dtype, a, query_tiles, query_count, query_rows, (hipStream_t)stream);
   if (e != hipSuccess) return (int)e;
-  return (int)launch(KEYS, dtype, a, key_tiles, key_count, key_rows, kv_heads, (hipStream_t)stream);
+  return (int)launch(KEYS, dtype, a, key_tiles, key_count, key_rows, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -44,6 +44,8 @@ struct AttnGenArgs {
 struct AttnPackedArgs : AttnGenArgs {
   const int64_t* tiles;
   int64_t vt, ot, dqt, dkt, dvt;  // elements from row to row of v, of out and its gradient, and of dq, dk, dv
+  void* rest;                     // what out's rounding left, or null
+  int pack;                       // query heads of a kv head that share a workgroup
 };
 
 // Elements from row to row, where a packed call's differ from the others'.
@@ -74,7 +76,8 @@ __device__ __forceinline__ int enter_sequence(AttnPackedArgs& p, int64_t tile) {
   p.dq = const_cast<void*>(at(p.dq, p.dqt));
   p.dk = const_cast<void*>(at(p.dk, p.dkt));
   p.dv = const_cast<void*>(at(p.dv, p.dvt));
-  if (p.lse) p.lse += start * p.lt;
+  if (p.rest) p.rest = const_cast<void*>(at(p.rest, p.ot));
+  p.lse += start * p.lt;
   p.delta += start * p.lt;
   p.part_k += start * part_pitch(p);
   p.part_v += start * part_pitch(p);

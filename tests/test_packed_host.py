@@ -205,7 +205,6 @@ def test_c_entry_points_refuse():
     def forward(**change):
         a = dict(q=p, k=p, v=p, out=p, lse=p, rest=None, tiles=p, count=2, rows=128, heads=4, kv=2, dim=64, qr=256, kr=128,
                  vr=128, dtype=5, scale=0.125, causal=1, stream=None)
-        del a["rest"]
         a.update(change)
         return library.qutai_amd_attention_packed_fwd(*a.values())
 
@@ -215,7 +214,8 @@ def test_c_entry_points_refuse():
     for change in wrong:
         assert forward(**change) == EINVAL, change
     assert forward(count=0) == 0
-    for dtype, dim, rows in ((5, 20, 4), (0, 160, 4)):
+    assert forward(rest=p, dim=136, qr=544, kr=272, vr=272) == EINVAL and forward(rest=p, rows=4) == EINVAL
+    for dtype, dim, rows in ((5, 20, 4), (0, 160, 4), (0, 64, 128), (5, 64, 128)):
         assert library.qutai_amd_attention_packed_rows(4, 2, dim, 1000, dtype, 1, 0.1, 0) == rows
     assert library.qutai_amd_attention_packed_rows(4, 2, 64, 1000, 5, 0, 0.1, 0) == 4
     assert library.qutai_amd_attention_packed_rows(4, 2, 64, 1000, 4, 1, 0.1, 0) == 0
