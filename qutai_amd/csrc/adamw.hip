@@ -32,7 +32,9 @@ namespace {
 
 constexpr int THREADS = 256, BLOCK = 256;     // BLOCK: values that share an exponent
 constexpr int CHUNK = 4096;                   // values of a workgroup's turn
+constexpr int TURNS = CHUNK / (4 * THREADS);  // a thread takes 4 values, and 4 more a thousand on
 constexpr int TENSORS = 48;                   // of a launch: their records fit the kernel's arguments
+constexpr int GROUPS = 2048;                  // workgroups of a launch at most: eight for a CU
 constexpr int NORM_GROUPS = 1024;             // partial sums of a launch
 constexpr int NOT_FINITE = 127;
 
@@ -45,7 +47,7 @@ struct Tensor {
   int64_t count;
   uint32_t chunks;  // of the tensors before it in this launch
   uint32_t key;     // of its rounding
-  int bf16, whole;  // whole: 16-byte aligned
+  int bf16, whole;  // whole: every address is a multiple of 16 bytes
 };
 
 struct StepArgs {
@@ -76,15 +78,66 @@ __device__ __forceinline__ int tensor_of(const Args& a, uint32_t c) {
     if (a.t[mid].chunks <= c) lo = mid;
     else hi = mid;
   }
-  return lo;
+  return uniform32(lo);
 }
 
-__device__ __forceinline__ float get(const void* x, int64_t i, int bf16) {
-  return bf16 ? bf16_to_f32(((const bf16_t*)x)[i]) : ((const float*)x)[i];
+// Four values from index i on, and back: at once where `whole` (i a multiple of 4),
+// else one by one, those at or beyond `end` left out.
+template <class T>
+__device__ __forceinline__ f32x4 get4(const void* x, int64_t i, int64_t end, bool whole) {
+  const T* p = (const T*)x + i;
+  f32x4 v = {};
+  if (whole) {
+    if constexpr (sizeof(T) == 4) {
+      v = global_load_nt<f32x4>(p);
+    } else {
+      const u32x2 w = global_load_nt<u32x2>(p);
+      v = f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16),
+                __uint_as_float(w[1] & 0xffff0000u)};
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (i + j < end) {
+        if constexpr (sizeof(T) == 4) v[j] = p[j];
+        else v[j] = bf16_to_f32(p[j]);
+      }
+  }
+  return v;
 }
-__device__ __forceinline__ void put(void* x, int64_t i, float v, int bf16) {
-  if (bf16) ((bf16_t*)x)[i] = f32_to_bf16(v);
-  else ((float*)x)[i] = v;
+template <class T>
+__device__ __forceinline__ void put4(void* x, int64_t i, int64_t end, bool whole, const f32x4& v) {
+  T* p = (T*)x + i;
+  if (whole) {
+    if constexpr (sizeof(T) == 4) global_store_nt(p, v);
+    else global_store_nt(p, u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])});
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (i + j < end) {
+        if constexpr (sizeof(T) == 4) p[j] = v[j];
+        else p[j] = f32_to_bf16(v[j]);
+      }
+  }
+}
+__device__ __forceinline__ uint32_t get_codes(const void* x, int64_t i, int64_t end, bool whole) {
+  const uint8_t* p = (const uint8_t*)x + i;
+  if (whole) return global_load_nt<uint32_t>(p);
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    if (i + j < end) w |= (uint32_t)p[j] << 8 * j;
+  return w;
+}
+__device__ __forceinline__ void put_codes(void* x, int64_t i, int64_t end, bool whole, uint32_t w) {
+  uint8_t* p = (uint8_t*)x + i;
+  if (whole) {
+    global_store_nt(p, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (i + j < end) p[j] = (uint8_t)(w >> 8 * j);
+  }
 }
 
 // Sum over a workgroup, the same in every thread; the order is fixed.
@@ -97,22 +150,35 @@ __device__ __forceinline__ double group_sum(double x, double* shared) {
   return (shared[0] + shared[1]) + (shared[2] + shared[3]);
 }
 
+template <class T>
+__device__ __forceinline__ void square_sum(const Tensor& t, int64_t start, int64_t end, double& sum) {
+  f32x4 g[TURNS];
+  const int64_t i = start + 4 * threadIdx.x;
+#pragma unroll
+  for (int u = 0; u < TURNS; u++) {
+    const int64_t at = i + 4 * THREADS * u;
+    g[u] = get4<T>(t.g, at, end, t.whole && at + 4 <= end);
+  }
+#pragma unroll
+  for (int u = 0; u < TURNS; u++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) sum = fma((double)g[u][j], (double)g[u][j], sum);
+}
+
 __global__ void __launch_bounds__(THREADS) adamw_norm(NormArgs a) {
   __shared__ double shared[4];
   double sum = 0.0;
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
     const Tensor& t = a.t[tensor_of(a, c)];
     const int64_t start = (int64_t)(c - t.chunks) * CHUNK, end = min(t.count, start + CHUNK);
-    for (int64_t i = start + threadIdx.x; i < end; i += THREADS) {
-      const double g = get(t.g, i, t.bf16);
-      sum += g * g;
-    }
+    if (t.bf16) square_sum<bf16_t>(t, start, end, sum);
+    else square_sum<float>(t, start, end, sum);
   }
   sum = group_sum(sum, shared);
   if (threadIdx.x == 0) a.partial[blockIdx.x] = sum;
 }
 
-__device__ __forceinline__ uint32_t mixed(uint32_t x) {
+__host__ __device__ __forceinline__ uint32_t mixed(uint32_t x) {
   x ^= x >> 15;
   x *= 0xBB67AE85u;
   x ^= x >> 13;
@@ -139,15 +205,126 @@ __device__ __forceinline__ uint32_t coded(double magnitude, int least, uint32_t 
   return (uint32_t)(mine - least) * 8 + (uint32_t)(ldexp(magnitude, 3 - mine) + (double)bits * 0x1p-16);
 }
 
+// Maximum over a wave, the same in every lane: within rows of 16 lanes by
+// data-parallel moves, across them by exchanges of rows and halves.
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));   // lanes 1 0 3 2
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));   // lanes 2 3 0 1
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));  // half a row, reversed
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));  // a row, reversed
+  const auto rows = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max((uint32_t)rows[0], (uint32_t)rows[1]);
+  const auto halves = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return max((uint32_t)halves[0], (uint32_t)halves[1]);
+}
+
+// The 256 values from `base` on by a wave, four to a lane.
+template <class T>
+struct Block8 {
+  f32x4 p, g;
+  uint32_t m, v;
+  int e1, e2;
+  __device__ __forceinline__ void load(const Tensor& t, int64_t base, int64_t end, int lane) {
+    const int64_t i = base + 4 * lane;
+    const bool whole = t.whole && i + 4 <= end;
+    g = get4<T>(t.g, i, end, whole);
+    p = get4<T>(t.p, i, end, whole);
+    m = get_codes(t.m, i, end, whole);
+    v = get_codes(t.v, i, end, whole);
+    if (base < end) {  // the wave's own block alone writes them
+      e1 = t.e[base / BLOCK * 2];
+      e2 = t.e[base / BLOCK * 2 + 1];
+    }
+  }
+  __device__ __forceinline__ void step(const StepArgs& a, const Tensor& t, int64_t base, int64_t end, int lane, double factor) {
+#pragma clang fp contract(off)
+    if (base >= end) return;
+    const int64_t i = base + 4 * lane;
+    const bool whole = t.whole && i + 4 <= end;
+    double m1[4], v1[4];
+    uint32_t most1 = 0, most2 = 0;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) x = max(x, (uint32_t)__shfl_xor((int)x, o));
-  return x;
+    for (int j = 0; j < 4; j++) {
+      const uint32_t c1 = m >> 8 * j & 255, c2 = v >> 8 * j & 255;
+      float m0 = decoded(c1 & 127, e1 - 14), v0 = decoded(c2, e2 - 30);
+      m0 = __uint_as_float(__float_as_uint(m0) | (c1 & 128) << 24);
+      if (e1 == NOT_FINITE) m0 = NAN;
+      if (e2 == NOT_FINITE) v0 = NAN;
+      const double gj = (double)g[j] * factor;
+      m1[j] = a.b1 * (double)m0 + a.b1_rest * gj;
+      v1[j] = a.b2 * (double)v0 + a.b2_rest * (gj * gj);
+      // values behind the end are zeros, unless the block's exponent says NaN
+      most1 = max(most1, high_word(m1[j]) & 0x7fffffffu);
+      most2 = max(most2, high_word(v1[j]) & 0x7fffffffu);
+    }
+    const int E1 = block_exponent(wave_max(most1)), E2 = block_exponent(wave_max(most2));
+    uint32_t codes1 = 0, codes2 = 0;
+    f32x4 p1;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint32_t bits = mixed((uint32_t)(i + j) * 0x9E3779B9u + t.key);
+      if (E1 != NOT_FINITE) codes1 |= (coded(fabs(m1[j]), E1 - 14, bits & 0xffff) | (m1[j] < 0.0 ? 128u : 0u)) << 8 * j;
+      if (E2 != NOT_FINITE) {
+        const uint32_t c2 = coded(v1[j], E2 - 30, bits >> 16);
+        codes2 |= (c2 == 0 && v1[j] > 0.0 ? 1u : c2) << 8 * j;
+      }
+      const float update = (float)m1[j] / (sqrtf((float)v1[j]) * a.root + a.eps);
+      p1[j] = p[j] * a.keep - a.rate * update;
+    }
+    put_codes(t.m, i, end, whole, codes1);
+    put_codes(t.v, i, end, whole, codes2);
+    put4<T>(t.p, i, end, whole, p1);
+    if (lane == 0) {
+      t.e[base / BLOCK * 2] = (int8_t)E1;
+      t.e[base / BLOCK * 2 + 1] = (int8_t)E2;
+    }
+  }
+};
+
+template <class T>
+__device__ __forceinline__ void step8(const StepArgs& a, const Tensor& t, int64_t start, int64_t end, double factor) {
+  const int lane = threadIdx.x & 63, wave = uniform32(threadIdx.x >> 6);
+  constexpr int N = CHUNK / BLOCK / (THREADS / 64);  // blocks of a wave, whose loads go out together
+  Block8<T> b[N];
+#pragma unroll
+  for (int u = 0; u < N; u++) b[u].load(t, start + (u * (THREADS / 64) + wave) * BLOCK, end, lane);
+#pragma unroll
+  for (int u = 0; u < N; u++) b[u].step(a, t, start + (u * (THREADS / 64) + wave) * BLOCK, end, lane, factor);
+}
+
+template <class T>
+__device__ __forceinline__ void step32(const StepArgs& a, const Tensor& t, int64_t start, int64_t end, double factor) {
+#pragma clang fp contract(off)
+  const float f = (float)factor, b1 = (float)a.b1, r1 = (float)a.b1_rest, b2 = (float)a.b2, r2 = (float)a.b2_rest;
+  f32x4 g[TURNS], p[TURNS], m[TURNS], v[TURNS];
+#pragma unroll
+  for (int u = 0; u < TURNS; u++) {
+    const int64_t i = start + 4 * (threadIdx.x + THREADS * u);
+    const bool whole = t.whole && i + 4 <= end;
+    g[u] = get4<T>(t.g, i, end, whole);
+    p[u] = get4<T>(t.p, i, end, whole);
+    m[u] = get4<float>(t.m, i, end, whole);
+    v[u] = get4<float>(t.v, i, end, whole);
+  }
+#pragma unroll
+  for (int u = 0; u < TURNS; u++) {
+    const int64_t i = start + 4 * (threadIdx.x + THREADS * u);
+    const bool whole = t.whole && i + 4 <= end;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float gj = g[u][j] * f;
+      m[u][j] = b1 * m[u][j] + r1 * gj;
+      v[u][j] = b2 * v[u][j] + r2 * (gj * gj);
+      p[u][j] = p[u][j] * a.keep - a.rate * (m[u][j] / (sqrtf(v[u][j]) * a.root + a.eps));
+    }
+    put4<float>(t.m, i, end, whole, m[u]);
+    put4<float>(t.v, i, end, whole, v[u]);
+    put4<T>(t.p, i, end, whole, p[u]);
+  }
 }
 
 template <bool EIGHT>
 __global__ void __launch_bounds__(THREADS) adamw_step(StepArgs a) {
-#pragma clang fp contract(off)
   __shared__ double shared[4];
   double factor = 1.0;
   if (a.partial) {
@@ -162,57 +339,11 @@ __global__ void __launch_bounds__(THREADS) adamw_step(StepArgs a) {
     const Tensor& t = a.t[tensor_of(a, c)];
     const int64_t start = (int64_t)(c - t.chunks) * CHUNK, end = min(t.count, start + CHUNK);
     if constexpr (EIGHT) {
-      const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-      for (int64_t base = start + wave * BLOCK; base < end; base += 4 * BLOCK) {
-        int8_t* e = t.e + base / BLOCK * 2;
-        const int e1 = e[0], e2 = e[1];
-        double m[4], v[4];
-        uint32_t most1 = 0, most2 = 0;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int64_t i = base + lane * 4 + j;
-          m[j] = v[j] = 0.0;
-          if (i >= end) continue;
-          const uint32_t c1 = ((const uint8_t*)t.m)[i], c2 = ((const uint8_t*)t.v)[i];
-          float m0 = decoded(c1 & 127, e1 - 14), v0 = decoded(c2, e2 - 30);
-          if (c1 & 128) m0 = -m0;
-          if (e1 == NOT_FINITE) m0 = NAN;
-          if (e2 == NOT_FINITE) v0 = NAN;
-          const double g = (double)get(t.g, i, t.bf16) * factor;
-          m[j] = a.b1 * (double)m0 + a.b1_rest * g;
-          v[j] = a.b2 * (double)v0 + a.b2_rest * (g * g);
-          most1 = max(most1, high_word(m[j]) & 0x7fffffffu);
-          most2 = max(most2, high_word(v[j]) & 0x7fffffffu);
-        }
-        const int E1 = block_exponent(wave_max(most1)), E2 = block_exponent(wave_max(most2));
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int64_t i = base + lane * 4 + j;
-          if (i >= end) continue;
-          const uint32_t bits = mixed((uint32_t)i * 0x9E3779B9u + t.key);
-          uint32_t c1 = 0, c2 = 0;
-          if (E1 != NOT_FINITE) c1 = coded(fabs(m[j]), E1 - 14, bits & 0xffff) | (m[j] < 0.0 ? 128 : 0);
-          if (E2 != NOT_FINITE) {
-            c2 = coded(v[j], E2 - 30, bits >> 16);
-            if (c2 == 0 && v[j] > 0.0) c2 = 1;
-          }
-          ((uint8_t*)t.m)[i] = (uint8_t)c1;
-          ((uint8_t*)t.v)[i] = (uint8_t)c2;
-          const float p = get(t.p, i, t.bf16);
-          const float step = (float)m[j] / (sqrtf((float)v[j]) * a.root + a.eps);
-          put(t.p, i, p * a.keep - a.rate * step, t.bf16);
-        }
-        if (lane == 0) e[0] = (int8_t)E1, e[1] = (int8_t)E2;
-      }
+      if (t.bf16) step8<bf16_t>(a, t, start, end, factor);
+      else step8<float>(a, t, start, end, factor);
     } else {
-      const float f = (float)factor, b1 = (float)a.b1, r1 = (float)a.b1_rest, b2 = (float)a.b2, r2 = (float)a.b2_rest;
-      for (int64_t i = start + threadIdx.x; i < end; i += THREADS) {
-        const float g = get(t.g, i, t.bf16) * f, p = get(t.p, i, t.bf16);
-        const float m = b1 * ((const float*)t.m)[i] + r1 * g, v = b2 * ((const float*)t.v)[i] + r2 * (g * g);
-        ((float*)t.m)[i] = m;
-        ((float*)t.v)[i] = v;
-        put(t.p, i, p * a.keep - a.rate * (m / (sqrtf(v) * a.root + a.eps)), t.bf16);
-      }
+      if (t.bf16) step32<bf16_t>(a, t, start, end, factor);
+      else step32<float>(a, t, start, end, factor);
     }
   }
 }
@@ -227,18 +358,17 @@ __global__ void __launch_bounds__(THREADS) adamw_moments(const uint8_t* m, const
   }
 }
 
-// Records of up to TENSORS tensors from `first` on; returns how many tensors
-// they took (those without values among them), or a negative status.
+// Records of up to TENSORS tensors from `first` on; returns how many tensors they
+// took (those without values among them).
 template <class Args>
-int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, int bits, uint32_t key, bool gradients_only) {
+int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, uint32_t key) {
   a.n = 0;
   a.chunks = 0;
   int64_t i = first;
   for (; i < count && a.n < TENSORS; i++) {
     const int64_t* r = tensors + 8 * i;
-    const int64_t values = r[5];
-    if (values == 0) continue;
-    const int64_t chunks = (values + CHUNK - 1) / CHUNK;
+    if (r[5] == 0) continue;
+    const int64_t chunks = (r[5] + CHUNK - 1) / CHUNK;
     if (a.chunks + chunks > 0x7fffffff) break;
     Tensor& t = a.t[a.n++];
     t.p = (void*)r[0];
@@ -246,27 +376,14 @@ int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, int 
     t.m = (void*)r[2];
     t.v = (void*)r[3];
     t.e = (int8_t*)r[4];
-    t.count = values;
+    t.count = r[5];
     t.chunks = a.chunks;
     t.bf16 = r[6] == BF16;
     t.whole = (r[0] | r[1] | r[2] | r[3]) % 16 == 0;
-    uint32_t x = key + (uint32_t)r[7];
-    x ^= x >> 15;
-    x *= 0xBB67AE85u;
-    x ^= x >> 13;
-    x *= 0x6A09E667u;
-    t.key = x ^ (x >> 16);
+    t.key = mixed(key + (uint32_t)r[7]);
     a.chunks += (uint32_t)chunks;
   }
   return i - first;
-}
-
-uint32_t host_mixed(uint32_t x) {
-  x ^= x >> 15;
-  x *= 0xBB67AE85u;
-  x ^= x >> 13;
-  x *= 0x6A09E667u;
-  return x ^ (x >> 16);
 }
 
 int64_t launches(const int64_t* tensors, int64_t count) {
@@ -316,7 +433,7 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
     NormArgs a = {};
     int64_t at = 0;
     for (int64_t first = 0; first < count;) {
-      first += take(a, tensors, first, count, bits, 0, true);
+      first += take(a, tensors, first, count, 0);
       if (!a.n) continue;
       a.partial = workspace + at * NORM_GROUPS;
       at++;
@@ -342,11 +459,11 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
     a.partials = (int)parts;
     a.norm = norm;
   }
-  const uint32_t key = host_mixed(host_mixed((uint32_t)seed) + (uint32_t)step);
+  const uint32_t key = mixed(mixed((uint32_t)seed) + (uint32_t)step);
   for (int64_t first = 0; first < count;) {
-    first += take(a, tensors, first, count, bits, key, false);
+    first += take(a, tensors, first, count, key);
     if (!a.n) continue;
-    const dim3 grid(std::min<uint32_t>(a.chunks, 2048));
+    const dim3 grid(std::min<uint32_t>(a.chunks, GROUPS));
     if (bits == 8) hipLaunchKernelGGL(adamw_step<true>, grid, dim3(THREADS), 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(adamw_step<false>, grid, dim3(THREADS), 0, (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();
