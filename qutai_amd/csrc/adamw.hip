@@ -200,9 +200,21 @@ __device__ __forceinline__ int block_exponent(uint32_t most) {
   return e > NOT_FINITE - 1 ? NOT_FINITE : e < -64 ? -64 : e;
 }
 
+// The code of a magnitude: in steps of an eighth of its binade (of the lowest one
+// where it lies below), with 16 bits of a step's rest; those bits decide with `bits`
+// whether it is rounded up.
 __device__ __forceinline__ uint32_t coded(double magnitude, int least, uint32_t bits) {
-  const int mine = max((int)(high_word(magnitude) >> 20) - 1023, least);
-  return (uint32_t)(mine - least) * 8 + (uint32_t)(ldexp(magnitude, 3 - mine) + (double)bits * 0x1p-16);
+  const int mine = max((int)(high_word(magnitude) >> 20 & 0x7ff) - 1023, least);
+  return (uint32_t)(mine - least) * 8 + (((uint32_t)ldexp(magnitude, 19 - mine) + bits) >> 16);
+}
+
+// What a code's float of the same fields is multiplied by to be its value: a code's
+// exponent and fraction, put into the lowest exponent bits and highest fraction bits of
+// a float, are the code's value times 2^-126 / 2^L, the lowest binade's (whose codes
+// are subnormal floats) included.
+__device__ __forceinline__ double code_scale(int exponent, int below) {
+  if (exponent == NOT_FINITE) return NAN;
+  return __longlong_as_double((int64_t)(exponent - below + 126 + 1023) << 52);
 }
 
 // Maximum over a wave, the same in every lane: within rows of 16 lanes by
@@ -237,40 +249,40 @@ struct Block8 {
     }
   }
   __device__ __forceinline__ void step(const StepArgs& a, const Tensor& t, int64_t base, int64_t end, int lane, double factor) {
-#pragma clang fp contract(off)
     if (base >= end) return;
     const int64_t i = base + 4 * lane;
     const bool whole = t.whole && i + 4 <= end;
     double m1[4], v1[4];
     uint32_t most1 = 0, most2 = 0;
+    // a product with a power of two is exact, so the decay may take it
+    const double d1 = a.b1 * code_scale(uniform32(e1), 14), d2 = a.b2 * code_scale(uniform32(e2), 30);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const uint32_t c1 = m >> 8 * j & 255, c2 = v >> 8 * j & 255;
-      float m0 = decoded(c1 & 127, e1 - 14), v0 = decoded(c2, e2 - 30);
-      m0 = __uint_as_float(__float_as_uint(m0) | (c1 & 128) << 24);
-      if (e1 == NOT_FINITE) m0 = NAN;
-      if (e2 == NOT_FINITE) v0 = NAN;
+#pragma clang fp contract(off)
+      const uint32_t c1 = m >> 8 * j, c2 = v >> 8 * j;
+      const float m0 = __uint_as_float((c1 & 127) << 20 | (c1 & 128) << 24), v0 = __uint_as_float((c2 & 255) << 20);
       const double gj = (double)g[j] * factor;
-      m1[j] = a.b1 * (double)m0 + a.b1_rest * gj;
-      v1[j] = a.b2 * (double)v0 + a.b2_rest * (gj * gj);
+      m1[j] = d1 * (double)m0 + a.b1_rest * gj;
+      v1[j] = d2 * (double)v0 + a.b2_rest * (gj * gj);
       // values behind the end are zeros, unless the block's exponent says NaN
       most1 = max(most1, high_word(m1[j]) & 0x7fffffffu);
       most2 = max(most2, high_word(v1[j]) & 0x7fffffffu);
     }
-    const int E1 = block_exponent(wave_max(most1)), E2 = block_exponent(wave_max(most2));
+    const int E1 = uniform32(block_exponent(wave_max(most1))), E2 = uniform32(block_exponent(wave_max(most2)));
     uint32_t codes1 = 0, codes2 = 0;
     f32x4 p1;
+    const uint32_t seed = (uint32_t)i * 0x9E3779B9u + t.key;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const uint32_t bits = mixed((uint32_t)(i + j) * 0x9E3779B9u + t.key);
-      if (E1 != NOT_FINITE) codes1 |= (coded(fabs(m1[j]), E1 - 14, bits & 0xffff) | (m1[j] < 0.0 ? 128u : 0u)) << 8 * j;
-      if (E2 != NOT_FINITE) {
-        const uint32_t c2 = coded(v1[j], E2 - 30, bits >> 16);
-        codes2 |= (c2 == 0 && v1[j] > 0.0 ? 1u : c2) << 8 * j;
-      }
-      const float update = (float)m1[j] / (sqrtf((float)v1[j]) * a.root + a.eps);
-      p1[j] = p[j] * a.keep - a.rate * update;
+      const uint32_t bits = mixed(seed + j * 0x9E3779B9u);
+      codes1 |= (coded(fabs(m1[j]), E1 - 14, bits & 0xffff) | (high_word(m1[j]) >> 24 & 128)) << 8 * j;
+      codes2 |= max(coded(v1[j], E2 - 30, bits >> 16), v1[j] > 0.0 ? 1u : 0u) << 8 * j;
+      // the hardware's fp64 root holds fp32's bits for every value that fp64 holds
+      const float root = (float)__builtin_amdgcn_sqrt(v1[j]);
+      p1[j] = fmaf(p[j], a.keep, -a.rate * (float)m1[j] * __builtin_amdgcn_rcpf(fmaf(root, a.root, a.eps)));
     }
+    if (E1 == NOT_FINITE) codes1 = 0;
+    if (E2 == NOT_FINITE) codes2 = 0;
     put_codes(t.m, i, end, whole, codes1);
     put_codes(t.v, i, end, whole, codes2);
     put4<T>(t.p, i, end, whole, p1);
