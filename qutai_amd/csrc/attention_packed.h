@@ -39,12 +39,57 @@ constexpr int packed_heads(int64_t heads, int64_t kv_heads, int waves) {
   return n;
 }
 
+typedef __attribute__((address_space(3))) const char* lds_bytes;
+__device__ __forceinline__ lds_bytes lds_at(const void* x) {
+  return (lds_bytes)(lds_ptr_t)const_cast<void*>(x);
+}
+
 template <int DP>
 struct PackedTile {
   static constexpr int S = DP / 16, DB = DP / 32;  // MFMA k-steps over d, 32-wide d blocks
   static constexpr int PC = DP / 8;                // 16-byte chunks of a row
-  typedef AttnTile<false, DP> Base;
-  static_assert(Base::PITCH == DP, "rows lie without gaps");
+  static constexpr int ROW = DP * 2;               // bytes
+
+  // Chunk c of row r lies at c ^ swz(r).  16 rows' same chunk (a read of 16 lanes) and 4
+  // rows' 64 bytes (a transposed read of 32) fall into different banks, and rows 16
+  // apart are swizzled alike, so that a lane's addresses in a tile differ by constants.
+  __device__ static __forceinline__ int swz(int r) {
+    if constexpr (PC == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
+    else return (r & 3) << 2 | (r >> 2 & 3);
+  }
+
+  // A lane's byte offsets in a tile: of its 16 bytes of row col (row fragments: the
+  // 32 s bytes of k-step s are a xor of the chunk), and of its 8 bytes of the two rows of
+  // a transposed read (the 64 db bytes of a d block too).
+  struct Lane {
+    uint32_t row, c0, c1;
+    __device__ __forceinline__ void plan(int lane) {
+      const int half = lane >> 5, col = lane & 31, g = lane >> 4, i = lane & 15;
+      const int r0 = 4 * (g >> 1) + (i >> 2), r1 = r0 + 8, c = 2 * (g & 1) + ((i & 3) >> 1), b = 8 * (i & 1);
+      row = col * ROW + (half ^ swz(col)) * 16;
+      c0 = r0 * ROW + (c ^ swz(r0)) * 16 + b;
+      c1 = r1 * ROW + (c ^ swz(r1)) * 16 + b;
+    }
+    // The same in the other stage of the ring, BYTES (a power of two) away.
+    template <int BYTES>
+    __device__ __forceinline__ void flip() {
+      row ^= BYTES, c0 ^= BYTES, c1 ^= BYTES;
+    }
+  };
+  // Row fragment: row rb + col, d = 16 s + 8 half + [0, 8), of the tile at x.
+  __device__ static __forceinline__ bf16x8 rows(lds_bytes x, const Lane& l, int rb, int s) {
+    typedef __attribute__((address_space(3))) const bf16x8* ptr;
+    return *(ptr)(x + (l.row ^ (32 * s)) + rb * ROW);
+  }
+  // Transposed fragment: rows = d columns 32 db + [0, 32), k = tile rows
+  // rb + {4 half + [0, 4), 8 + ...}, the order of an MFMA result's elements.
+  __device__ static __forceinline__ bf16x8 columns(lds_bytes x, const Lane& l, int db, int rb) {
+    typedef __attribute__((address_space(3))) i16x4* ptr;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(x + (l.c0 ^ (64 * db)) + rb * ROW));
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(x + (l.c1 ^ (64 * db)) + rb * ROW));
+    const i16x8 w = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(bf16x8, w);
+  }
 
   // Copies of a block of ROWS rows by NW waves: chunk (j * NW + wave) * 64 + lane of
   // the block, at c ^ swz(r) of row r.
@@ -57,7 +102,7 @@ struct PackedTile {
     __device__ __forceinline__ void plan(int64_t pitch, int D, int wave, int lane) {
 #pragma unroll
       for (int j = 0; j < N; j++) {
-        const int at = (j * NW + wave) * 64 + lane, r = at / PC, c = (at % PC) ^ Base::swz(r);
+        const int at = (j * NW + wave) * 64 + lane, r = at / PC, c = (at % PC) ^ swz(r);
         row[j] = r;
         off[j] = (uint32_t)((r * pitch + 8 * c) * 2) | (8 * c < D ? 0u : ATTN_OOB);
       }
@@ -82,17 +127,6 @@ struct PackedTile {
       const uint32_t off = (uint32_t)((col * pitch + d) * 2) | (col < left && d < D ? 0u : ATTN_OOB);
       f[s] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
     }
-  }
-
-  __device__ static __forceinline__ bf16x8 rows(const bf16_t* x, int r, int s, int half) {
-    bf16x8 f[1];
-    Base::rows(x, r, s, half, f);
-    return f[0];
-  }
-  __device__ static __forceinline__ bf16x8 columns(const bf16_t* x, int db, int rb, int lane) {
-    bf16x8 f[1];
-    Base::columns(x, db, rb, lane, f);
-    return f[0];
   }
 };
 
@@ -120,15 +154,14 @@ __device__ __forceinline__ PackedPlace enter_queries(AttnPackedArgs& p, int wave
 // The 32 keys from row 32 mb of the block on, for the wave's queries.  lim (MASK):
 // the keys of the block that the lane's query sees, less 4 half.
 template <int DP, bool MASK>
-__device__ __forceinline__ void packed_attend(const bf16_t* sk, const bf16_t* sv, const bf16x8 (&qf)[DP / 16],
-                                              f32x16 (&o)[DP / 32], float& m, float& l, int lim, float c, int lane,
-                                              int mb) {
+__device__ __forceinline__ void packed_attend(lds_bytes sk, lds_bytes sv, const typename PackedTile<DP>::Lane& at,
+                                              const bf16x8 (&qf)[DP / 16], f32x16 (&o)[DP / 32], float& m, float& l,
+                                              int lim, float c, int mb) {
   typedef PackedTile<DP> Tile;
-  const int half = lane >> 5, col = lane & 31;
   f32x16 sc = {};
 #pragma unroll
   for (int s = 0; s < Tile::S; s++)
-    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, 32 * mb + col, s, half), qf[s], sc, 0, 0, 0);
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, at, 32 * mb, s), qf[s], sc, 0, 0, 0);
   if constexpr (MASK) {
 #pragma unroll
     for (int e = 0; e < 16; e++)
@@ -169,7 +202,7 @@ __device__ __forceinline__ void packed_attend(const bf16_t* sk, const bf16_t* sv
   for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
     for (int st = 0; st < 2; st++)
-      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sv, db, 32 * mb + 16 * st, lane), pf[st], o[db], 0, 0, 0);
+      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sv, at, db, 32 * mb + 16 * st), pf[st], o[db], 0, 0, 0);
 }
 
 // Four consecutive channels of a result row, and of what its rounding left.
@@ -218,18 +251,23 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_fwd(AttnPack
     if (kbk + 1 < nkb) issue(kbk + 1);
   };
   if (nkb > 0) issue(0);
+  constexpr int STAGE = 2 * KB * DP * 2;
+  typename Tile::Lane in;  // in the stage of block kbk
+  in.plan(lane);
+  const lds_bytes sk = lds_at(&lds[0][0][0]), sv = lds_at(&lds[0][1][0]);
   int kbk = 0;
   for (; kbk < n_full; kbk++) {
     advance(kbk);
-    packed_attend<DP, false>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, o, m, l, 0, c, lane, 0);
-    packed_attend<DP, false>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, o, m, l, 0, c, lane, 1);
+    packed_attend<DP, false>(sk, sv, in, qf, o, m, l, 0, c, 0);
+    packed_attend<DP, false>(sk, sv, in, qf, o, m, l, 0, c, 1);
+    in.template flip<STAGE>();
   }
   for (; kbk * KB < seen; kbk++) {
     advance(kbk);
     const int kv0 = kbk * KB, lim = min(T - kv0, p.causal ? t - kv0 + 1 : KB) - 4 * half;
 #pragma unroll 1
-    for (int mb = 0; mb < 2 && kv0 + 32 * mb < seen; mb++)
-      packed_attend<DP, true>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, o, m, l, lim, c, lane, mb);
+    for (int mb = 0; mb < 2 && kv0 + 32 * mb < seen; mb++) packed_attend<DP, true>(sk, sv, in, qf, o, m, l, lim, c, mb);
+    in.template flip<STAGE>();
   }
   for (; kbk < nkb; kbk++) advance(kbk);
 
@@ -263,16 +301,15 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_fwd(AttnPack
 
 // dQ of the wave's queries, and delta; K and V stream.
 template <int DP, bool MASK>
-__device__ __forceinline__ void packed_dq_step(const bf16_t* sk, const bf16_t* sv, const bf16x8 (&qf)[DP / 16],
-                                               const bf16x8 (&gf)[DP / 16], float lse2, float dl,
-                                               f32x16 (&dqt)[DP / 32], int lim, float c, int lane, int mb) {
+__device__ __forceinline__ void packed_dq_step(lds_bytes sk, lds_bytes sv, const typename PackedTile<DP>::Lane& at,
+                                               const bf16x8 (&qf)[DP / 16], const bf16x8 (&gf)[DP / 16], float lse2,
+                                               float dl, f32x16 (&dqt)[DP / 32], int lim, float c, int mb) {
   typedef PackedTile<DP> Tile;
-  const int half = lane >> 5, col = lane & 31;
   f32x16 sc = {}, dp = {};
 #pragma unroll
   for (int s = 0; s < Tile::S; s++) {
-    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, 32 * mb + col, s, half), qf[s], sc, 0, 0, 0);
-    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sv, 32 * mb + col, s, half), gf[s], dp, 0, 0, 0);
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, at, 32 * mb, s), qf[s], sc, 0, 0, 0);
+    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sv, at, 32 * mb, s), gf[s], dp, 0, 0, 0);
   }
   bf16x8 dsf[2];
 #pragma unroll
@@ -292,7 +329,7 @@ __device__ __forceinline__ void packed_dq_step(const bf16_t* sk, const bf16_t* s
   for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
     for (int st = 0; st < 2; st++)
-      dqt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sk, db, 32 * mb + 16 * st, lane), dsf[st], dqt[db], 0, 0, 0);
+      dqt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sk, at, db, 32 * mb + 16 * st), dsf[st], dqt[db], 0, 0, 0);
 }
 
 template <int DP, int NW>
@@ -352,19 +389,24 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnP
     if (kbk + 1 < nkb) issue(kbk + 1);
   };
   if (nkb > 0) issue(0);
+  constexpr int STAGE = 2 * KB * DP * 2;
+  typename Tile::Lane in;  // in the stage of block kbk
+  in.plan(lane);
+  const lds_bytes sk = lds_at(&lds[0][0][0]), sv = lds_at(&lds[0][1][0]);
   int kbk = 0;
   for (; kbk < n_full; kbk++) {
     advance(kbk);
 #pragma unroll 1
-    for (int mb = 0; mb < 2; mb++)
-      packed_dq_step<DP, false>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, gf, lse2, dl, dqt, 0, c, lane, mb);
+    for (int mb = 0; mb < 2; mb++) packed_dq_step<DP, false>(sk, sv, in, qf, gf, lse2, dl, dqt, 0, c, mb);
+    in.template flip<STAGE>();
   }
   for (; kbk * KB < seen; kbk++) {
     advance(kbk);
     const int kv0 = kbk * KB, lim = min(T - kv0, p.causal ? t - kv0 + 1 : KB) - 4 * half;
 #pragma unroll 1
     for (int mb = 0; mb < 2 && kv0 + 32 * mb < seen; mb++)
-      packed_dq_step<DP, true>(&lds[kbk & 1][0][0], &lds[kbk & 1][1][0], qf, gf, lse2, dl, dqt, lim, c, lane, mb);
+      packed_dq_step<DP, true>(sk, sv, in, qf, gf, lse2, dl, dqt, lim, c, mb);
+    in.template flip<STAGE>();
   }
   for (; kbk < nkb; kbk++) advance(kbk);
 
@@ -391,7 +433,7 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnP
 // and blocks of 32 rows leave room for two workgroups on a CU.
 template <int DP>
 struct PackedKeys {
-  static constexpr int NW = 4, ROWS = NW * 32, QB = DP > 64 ? 32 : 64;
+  static constexpr int QB = DP > 64 ? 32 : 64;
   static constexpr bool V_IN_LDS = DP > 64;
   static constexpr int VF = V_IN_LDS ? 1 : DP / 16;
 };
@@ -401,16 +443,16 @@ struct PackedKeys {
 // One product after the other, so that dK's and dV's sums, the wave's K and V and
 // one block of scores and dP are all that lives.
 template <int DP, bool MASK>
-__device__ __forceinline__ void packed_dkv_step(const bf16_t* sq, const bf16_t* sg, const float* slse, const float* sdl,
-                                                const bf16x8 (&kf)[DP / 16], const bf16x8 (&vf)[PackedKeys<DP>::VF],
-                                                const bf16_t* sv, int own, f32x16 (&dkt)[DP / 32], f32x16 (&dvt)[DP / 32], int end, int before,
-                                                float c, int lane, int mb) {
+__device__ __forceinline__ void packed_dkv_step(lds_bytes sq, lds_bytes sg, const typename PackedTile<DP>::Lane& at,
+                                                const float* slse, const float* sdl, const bf16x8 (&kf)[DP / 16],
+                                                const bf16x8 (&vf)[PackedKeys<DP>::VF], lds_bytes sv,
+                                                const typename PackedTile<DP>::Lane& own, f32x16 (&dkt)[DP / 32], f32x16 (&dvt)[DP / 32], int end, int before,
+                                                float c, int half, int mb) {
   typedef PackedTile<DP> Tile;
-  const int half = lane >> 5, col = lane & 31;
   f32x16 sc = {};
 #pragma unroll
   for (int s = 0; s < Tile::S; s++)
-    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sq, 32 * mb + col, s, half), kf[s], sc, 0, 0, 0);
+    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sq, at, 32 * mb, s), kf[s], sc, 0, 0, 0);
   if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
   float pr[16];
 #pragma unroll
@@ -431,13 +473,13 @@ __device__ __forceinline__ void packed_dkv_step(const bf16_t* sq, const bf16_t* 
   for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
     for (int st = 0; st < 2; st++)
-      dvt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sg, db, 32 * mb + 16 * st, lane), w[st], dvt[db], 0, 0, 0);
+      dvt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sg, at, db, 32 * mb + 16 * st), w[st], dvt[db], 0, 0, 0);
   if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
   f32x16 dp = {};
 #pragma unroll
   for (int s = 0; s < Tile::S; s++)
-    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sg, 32 * mb + col, s, half),
-                                                 PackedKeys<DP>::V_IN_LDS ? Tile::rows(sv, own, s, half)
+    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sg, at, 32 * mb, s),
+                                                 PackedKeys<DP>::V_IN_LDS ? Tile::rows(sv, own, 0, s)
                                                                           : vf[PackedKeys<DP>::V_IN_LDS ? 0 : s],
                                                  dp, 0, 0, 0);
   if constexpr (DP > 64) __builtin_amdgcn_sched_barrier(0);
@@ -453,30 +495,34 @@ __device__ __forceinline__ void packed_dkv_step(const bf16_t* sq, const bf16_t* 
   for (int db = 0; db < Tile::DB; db++)
 #pragma unroll
     for (int st = 0; st < 2; st++)
-      dkt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sq, db, 32 * mb + 16 * st, lane), w[st], dkt[db], 0, 0, 0);
+      dkt[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sq, at, db, 32 * mb + 16 * st), w[st], dkt[db], 0, 0, 0);
 }
 
-template <int DP>
-__global__ void __launch_bounds__(256, 2) packed_bwd_dkv(AttnPackedArgs p) {
+// SPLIT sets of KW waves take the query heads of a group in turns, each with a stream
+// of its own, and add up their sums at the end in the order of the sets.
+template <int DP, int KW, int SPLIT>
+__global__ void __launch_bounds__(KW * SPLIT * 64, 2) packed_bwd_dkv(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
-  constexpr int NW = PackedKeys<DP>::NW, QB = PackedKeys<DP>::QB;
-  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][QB * DP];     // [stage][Q, dO]
-  __shared__ __attribute__((aligned(16))) float stats[2][2][QB];         // [stage][-lse log2(e), delta]
+  constexpr int QB = PackedKeys<DP>::QB;
   constexpr bool V_IN_LDS = PackedKeys<DP>::V_IN_LDS;
-  __shared__ __attribute__((aligned(16))) bf16_t own_v[V_IN_LDS ? NW * 32 * DP : 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
-  const int group = (int)(p.heads / p.kv_heads), nsplit = p.split ? group : 1;
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][SPLIT][2][QB * DP];  // [stage][set][Q, dO]
+  __shared__ __attribute__((aligned(16))) float stats[2][SPLIT][2][QB];      // [stage][set][-lse log2(e), delta]
+  __shared__ __attribute__((aligned(16))) bf16_t own_v[V_IN_LDS ? KW * 32 * DP : 8];
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+  const int set = uniform32(tid >> 6) / KW, wave = uniform32(tid >> 6) % KW;
+  const int group = (int)(p.heads / p.kv_heads);
   int b, kvh, blk, gsel;
-  place_keys<bf16_t, 1>(p, nsplit, b, kvh, blk, gsel);
+  place_keys<bf16_t, 1>(p, 1, b, kvh, blk, gsel);
   const int T = (int)p.time, D = (int)p.dim, k0 = blk, kw = uniform32(k0 + wave * 32), key = kw + col;
-  const int g_lo = p.split ? gsel : 0, g_hi = p.split ? gsel + 1 : group;
 
   bf16x8 kf[Tile::S], vf[PackedKeys<DP>::VF];
   Tile::own(p.k, kvh * p.kh + (int64_t)kw * p.kt, p.kt, T - kw, D, col, half, kf);
   if constexpr (V_IN_LDS) {  // there before the first block is, whose wait and barrier cover it
-    typename Tile::template Copy<NW * 32, NW> cv;
-    cv.plan(p.vt, D, wave, lane);
-    cv.issue(own_v, uniform_ptr((const bf16_t*)p.v + kvh * p.kh + (int64_t)k0 * p.vt), p.vt, T - k0, wave);
+    if (set == 0) {
+      typename Tile::template Copy<KW * 32, KW> cv;
+      cv.plan(p.vt, D, wave, lane);
+      cv.issue(own_v, uniform_ptr((const bf16_t*)p.v + kvh * p.kh + (int64_t)k0 * p.vt), p.vt, T - k0, wave);
+    }
   } else {
     Tile::own(p.v, kvh * p.kh + (int64_t)kw * p.vt, p.vt, T - kw, D, col, half, vf);
   }
@@ -484,32 +530,34 @@ __global__ void __launch_bounds__(256, 2) packed_bwd_dkv(AttnPackedArgs p) {
 #pragma unroll
   for (int db = 0; db < Tile::DB; db++) dkt[db] = dvt[db] = f32x16{};
 
-  const int qs0 = p.causal ? k0 : 0, nq = (T - qs0 + QB - 1) / QB, iterations = nq * (g_hi - g_lo);
-  typename Tile::template Copy<QB, NW> cq, cg;
+  // every set makes the same iterations, whose barriers all waves share: heads
+  // kvh group + set + SPLIT g (SPLIT divides the group)
+  const int qs0 = p.causal ? k0 : 0, nq = (T - qs0 + QB - 1) / QB, iterations = nq * (group / SPLIT);
+  typename Tile::template Copy<QB, KW> cq, cg;
   cq.plan(p.qt, D, wave, lane);
   cg.plan(p.ot, D, wave, lane);
-  float next = 0.f;  // waves 0 and 1: the lane's row of the block in flight, lse and delta
+  float next = 0.f;  // a set's waves 0 and 1: the lane's row of the block in flight, lse and delta
   auto issue = [&](int it, int h, int qs) {
-    const int stage = it & 1;
-    cq.issue(&lds[stage][0][0], uniform_ptr((const bf16_t*)p.q + h * p.qh + (int64_t)qs * p.qt), p.qt, T - qs, wave);
-    cg.issue(&lds[stage][1][0], uniform_ptr((const bf16_t*)p.g + h * p.qh + (int64_t)qs * p.ot), p.ot, T - qs, wave);
+    bf16_t* to = &lds[it & 1][set][0][0];
+    cq.issue(to, uniform_ptr((const bf16_t*)p.q + h * p.qh + (int64_t)qs * p.qt), p.qt, T - qs, wave);
+    cg.issue(to + QB * DP, uniform_ptr((const bf16_t*)p.g + h * p.qh + (int64_t)qs * p.ot), p.ot, T - qs, wave);
     if (wave < 2 && lane < QB) {
       const float* from = wave ? p.delta : p.lse;
       next = qs + lane < T ? from[h + (int64_t)(qs + lane) * p.lt] : 0.f;
     }
   };
   // wait for a block, start the copies of the next one: of the same head, or the
-  // first of the next
+  // first of the set's next
   auto advance = [&](int it, int h, int qi) {
     wait_vmcnt<0>();
     if (wave < 2 && lane < QB) {
-      stats[it & 1][wave][lane] = wave ? next : -next * LOG2E;
+      stats[it & 1][set][wave][lane] = wave ? next : -next * LOG2E;
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): in LDS before the barrier
     }
     asm volatile("s_barrier" ::: "memory");
     if (it + 1 < iterations) {
       const bool wrap = qi + 1 == nq;
-      issue(it + 1, wrap ? h + 1 : h, qs0 + (wrap ? 0 : qi + 1) * QB);
+      issue(it + 1, wrap ? h + SPLIT : h, qs0 + (wrap ? 0 : qi + 1) * QB);
     }
   };
   // steps of 32 queries, per head: before every key of the wave (causal; skipped),
@@ -523,23 +571,44 @@ __global__ void __launch_bounds__(256, 2) packed_bwd_dkv(AttnPackedArgs p) {
   const int diagonal = none ? steps : clamped(p.causal ? skipped + 1 : 0, skipped);
   const int tail = none ? steps : clamped(rows / 32, diagonal);
   const int end = none ? steps : clamped((rows + 31) / 32, tail);
-  if (iterations > 0) issue(0, kvh * group + g_lo, qs0);
+  if (iterations > 0) issue(0, kvh * group + set, qs0);
+  constexpr int STAGE = SPLIT * 2 * QB * DP * 2;
+  typename Tile::Lane in, own;  // in the stage of block `it`, in the wave's rows of V
+  in.plan(lane);
+  own = in;
+  own.row += wave * 32 * Tile::ROW;
+  in.template flip<STAGE>();  // as every block's entry does
+  const lds_bytes sq = lds_at(&lds[0][set][0][0]), sg = lds_at(&lds[0][set][1][0]), sv = lds_at(own_v);
   int it = -1;
-  for (int h = kvh * group + g_lo; h < kvh * group + g_hi; h++) {
+  for (int h = kvh * group + set; h < kvh * group + group; h += SPLIT) {
     auto enter = [&](int st) {
-      if (st % HB == 0) advance(++it, h, st / HB);
+      if (st % HB == 0) {
+        advance(++it, h, st / HB);
+        in.template flip<STAGE>();
+      }
     };
     auto step = [&](int st, auto mask) {
       const int qi = st / HB, qs = qs0 + qi * QB;
-      packed_dkv_step<DP, decltype(mask)::value>(&lds[it & 1][0][0], &lds[it & 1][1][0], &stats[it & 1][0][0],
-                                                 &stats[it & 1][1][0], kf, vf, own_v, 32 * wave + col, dkt, dvt, T - qs,
-                                                 p.causal ? key - qs : -1, p.scale_log2, lane, st % HB);
+      packed_dkv_step<DP, decltype(mask)::value>(sq, sg, in, &stats[it & 1][set][0][0], &stats[it & 1][set][1][0], kf, vf,
+                                                 sv, own, dkt, dvt, T - qs, p.causal ? key - qs : -1, p.scale_log2,
+                                                 half, st % HB);
     };
     int st = 0;
     for (; st < skipped; st++) enter(st);
     for (; st < diagonal; st++) {
       enter(st);
       step(st, std::true_type{});
+    }
+    if constexpr (HB > 1) {  // whole blocks, whose two steps overlap
+      for (; st < tail && st % HB; st++) {
+        enter(st);
+        step(st, std::false_type{});
+      }
+      for (; st + HB <= tail; st += HB) {
+        enter(st);
+        step(st, std::false_type{});
+        step(st + 1, std::false_type{});
+      }
     }
     for (; st < tail; st++) {
       enter(st);
@@ -552,13 +621,35 @@ __global__ void __launch_bounds__(256, 2) packed_bwd_dkv(AttnPackedArgs p) {
     for (; st < steps; st++) enter(st);
   }
 
+  if constexpr (SPLIT > 1) {
+    // set s hands its sums to set 0 through the stages, 16 channels of dK and dV a turn
+    // (4 KiB a wave), in the lanes that hold them
+    static_assert(sizeof(lds) >= KW * 64 * 2 * 16 * sizeof(float), "a turn's sums fit the stages");
+    f32x16* sums = reinterpret_cast<f32x16*>(&lds[0][0][0][0]) + (wave * 64 + lane) * 2;
+#pragma unroll
+    for (int from = 1; from < SPLIT; from++)
+#pragma unroll
+      for (int db = 0; db < Tile::DB; db++) {
+        __syncthreads();
+        if (set == from) {
+          sums[0] = dkt[db];
+          sums[1] = dvt[db];
+        }
+        __syncthreads();
+        if (set == 0) {
+          dkt[db] += sums[0];
+          dvt[db] += sums[1];
+        }
+      }
+    if (set) return;
+  }
   const bool bad = key < T && !(not_finite(dkt) + not_finite(dvt) == 0.f);
   if (__builtin_amdgcn_ballot_w64(bad)) {
-    for (int i = 0; i < 32 && kw + i < T; i++) bwd_kv_row<bf16_t>(p, 0, kvh, kw + i, lane, g_lo, g_hi);
+    for (int i = 0; i < 32 && kw + i < T; i++) bwd_kv_row<bf16_t>(p, 0, kvh, kw + i, lane, 0, group);
     return;
   }
   if (key < T) {
-    const int64_t head = kvh * p.kh, part = gsel * p.part_stride + head + (int64_t)key * part_pitch(p);
+    const int64_t head = kvh * p.kh;
     const int64_t to_k = head + (int64_t)key * p.dkt, to_v = head + (int64_t)key * p.dvt;
 #pragma unroll
     for (int db = 0; db < Tile::DB; db++)
@@ -568,13 +659,8 @@ __global__ void __launch_bounds__(256, 2) packed_bwd_dkv(AttnPackedArgs p) {
         if (d >= D) continue;
         const f32x4 x = {dkt[db][4 * g], dkt[db][4 * g + 1], dkt[db][4 * g + 2], dkt[db][4 * g + 3]};
         const f32x4 y = {dvt[db][4 * g], dvt[db][4 * g + 1], dvt[db][4 * g + 2], dvt[db][4 * g + 3]};
-        if (p.split) {
-          global_store(p.part_k + part + d, x);
-          global_store(p.part_v + part + d, y);
-        } else {
-          put4<false>(p.dk, to_k + d, x * p.scale);
-          put4<false>(p.dv, to_v + d, y);
-        }
+        put4<false>(p.dk, to_k + d, x * p.scale);
+        put4<false>(p.dv, to_v + d, y);
       }
   }
 }

@@ -48,11 +48,22 @@ __global__ void __launch_bounds__(GEN_WAVES * 64) packed_bwd_kv_rows(AttnPackedA
 
 enum Pass { FORWARD, QUERIES, KEYS };
 
+int key_split(int64_t heads, int64_t kv_heads, int64_t dim) {
+  const int64_t group = heads / kv_heads;
+  return dim > 64 ? 1 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+}
+
 template <int DP>
 void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
   if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
   else if (pass == QUERIES) hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
-  else hipLaunchKernelGGL((packed_bwd_dkv<DP>), dim3(blocks), dim3(256), 0, stream, a);
+  else if constexpr (DP == 64) {
+    if (key_split(a.heads, a.kv_heads, a.dim) == 4)
+      hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 2>), dim3(blocks), dim3(256), 0, stream, a);
+    else if (key_split(a.heads, a.kv_heads, a.dim) == 2)
+      hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 2>), dim3(blocks), dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), dim3(256), 0, stream, a);
+  } else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), dim3(256), 0, stream, a);
 }
 
 template <bool F32, int DP>
@@ -91,7 +102,7 @@ int64_t groups_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t
 // Rows of a tile of the matrix kernels.
 int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim) {
   if (!packed_fits(dtype, dim)) return MMA_ROWS;
-  return pass == KEYS ? PackedKeys<64>::ROWS : WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
+  return pass == KEYS ? (key_split(heads, kv_heads, dim) == 4 ? 64 : 128) : WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
 }
 
 // One pass over the tiles of `rows` rows each.
