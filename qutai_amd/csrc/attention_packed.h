@@ -151,25 +151,33 @@ __device__ __forceinline__ PackedPlace enter_queries(AttnPackedArgs& p, int wave
   return at;
 }
 
-// The 32 keys from row 32 mb of the block on, for the wave's queries.  lim (MASK):
-// the keys of the block that the lane's query sees, less 4 half.
-template <int DP, bool MASK>
+// HALVES times 32 keys from row 32 mb of the block on, for the wave's queries: all
+// scores first, so that the later halves' products overlap the first half's
+// exponentials.  lim (MASK): the keys of the block that the lane's query sees, less 4 half.
+template <int DP, int HALVES, bool MASK>
 __device__ __forceinline__ void packed_attend(lds_bytes sk, lds_bytes sv, const typename PackedTile<DP>::Lane& at,
                                               const bf16x8 (&qf)[DP / 16], f32x16 (&o)[DP / 32], float& m, float& l,
                                               int lim, float c, int mb) {
   typedef PackedTile<DP> Tile;
-  f32x16 sc = {};
-#pragma unroll
-  for (int s = 0; s < Tile::S; s++)
-    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, at, 32 * mb, s), qf[s], sc, 0, 0, 0);
-  if constexpr (MASK) {
-#pragma unroll
-    for (int e = 0; e < 16; e++)
-      if (32 * mb + 8 * (e >> 2) + (e & 3) >= lim) sc[e] = -INFINITY;
-  }
+  f32x16 sc[HALVES];
   float peak = -INFINITY;
 #pragma unroll
-  for (int e = 0; e < 16; e++) peak = fmaxf(peak, sc[e]);
+  for (int n = 0; n < HALVES; n++) {
+    sc[n] = f32x16{};
+#pragma unroll
+    for (int s = 0; s < Tile::S; s++)
+      sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::rows(sk, at, 32 * (mb + n), s), qf[s], sc[n], 0, 0, 0);
+  }
+#pragma unroll
+  for (int n = 0; n < HALVES; n++) {
+    if constexpr (MASK) {
+#pragma unroll
+      for (int e = 0; e < 16; e++)
+        if (32 * (mb + n) + 8 * (e >> 2) + (e & 3) >= lim) sc[n][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++) peak = fmaxf(peak, sc[n][e]);
+  }
   // the reference point m moves only for a maximum more than 2^8 above it
   const float cand = pair_max(peak) * c;
   const bool grow = cand > m + 8.f;
@@ -186,23 +194,26 @@ __device__ __forceinline__ void packed_attend(lds_bytes sk, lds_bytes sv, const 
   }
   const float ref = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
-  bf16x8 pf[2];
 #pragma unroll
-  for (int st = 0; st < 2; st++) {
-    float pv[8];
+  for (int n = 0; n < HALVES; n++) {
+    bf16x8 pf[2];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * st + e], c, -ref));
-      sum += pv[e];
+    for (int st = 0; st < 2; st++) {
+      float pv[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * st + e], c, -ref));
+        sum += pv[e];
+      }
+      pf[st] = rounded(pv);
     }
-    pf[st] = rounded(pv);
+#pragma unroll
+    for (int db = 0; db < Tile::DB; db++)
+#pragma unroll
+      for (int st = 0; st < 2; st++)
+        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sv, at, db, 32 * (mb + n) + 16 * st), pf[st], o[db], 0, 0, 0);
   }
   l += sum;
-#pragma unroll
-  for (int db = 0; db < Tile::DB; db++)
-#pragma unroll
-    for (int st = 0; st < 2; st++)
-      o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(Tile::columns(sv, at, db, 32 * mb + 16 * st), pf[st], o[db], 0, 0, 0);
 }
 
 // Four consecutive channels of a result row, and of what its rounding left.
@@ -213,10 +224,9 @@ __device__ __forceinline__ void put_rest(void* base, int64_t at, const f32x4& v,
   global_store((bf16_t*)base + at, u32x2{pack_bf16x2(left[0], left[1]), pack_bf16x2(left[2], left[3])});
 }
 
-template <int DP, int NW>
-__global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_fwd(AttnPackedArgs p) {
+template <int DP, int NW, int KB>
+__global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : KB == 32 ? 3 : 2) packed_fwd(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
-  constexpr int KB = 64;
   __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * DP];  // [stage][K, V]
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
   const PackedPlace at = enter_queries<NW>(p, wave);
@@ -258,15 +268,14 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_fwd(AttnPack
   int kbk = 0;
   for (; kbk < n_full; kbk++) {
     advance(kbk);
-    packed_attend<DP, false>(sk, sv, in, qf, o, m, l, 0, c, 0);
-    packed_attend<DP, false>(sk, sv, in, qf, o, m, l, 0, c, 1);
+    packed_attend<DP, KB / 32, false>(sk, sv, in, qf, o, m, l, 0, c, 0);
     in.template flip<STAGE>();
   }
   for (; kbk * KB < seen; kbk++) {
     advance(kbk);
     const int kv0 = kbk * KB, lim = min(T - kv0, p.causal ? t - kv0 + 1 : KB) - 4 * half;
 #pragma unroll 1
-    for (int mb = 0; mb < 2 && kv0 + 32 * mb < seen; mb++) packed_attend<DP, true>(sk, sv, in, qf, o, m, l, lim, c, mb);
+    for (int mb = 0; mb < KB / 32 && kv0 + 32 * mb < seen; mb++) packed_attend<DP, 1, true>(sk, sv, in, qf, o, m, l, lim, c, mb);
     in.template flip<STAGE>();
   }
   for (; kbk < nkb; kbk++) advance(kbk);

@@ -22,7 +22,7 @@
 namespace {
 
 constexpr int64_t MMA_ROWS = 128;  // queries or keys of a workgroup of attention_mma.h's kernels
-constexpr int WAVES = 8;           // of a workgroup of attention_packed.h's query kernels
+constexpr int WAVES = 4;           // of a workgroup of attention_packed.h's query kernels
 
 template <class T>
 __global__ void __launch_bounds__(GEN_WAVES * 64) packed_fwd_rows(AttnPackedArgs p) {
@@ -55,7 +55,7 @@ int key_split(int64_t heads, int64_t kv_heads, int64_t dim) {
 
 template <int DP>
 void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
-  if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+  if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP == 64 ? 64 : 32>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
   else if (pass == QUERIES) hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
   else if constexpr (DP == 64) {
     if (key_split(a.heads, a.kv_heads, a.dim) == 4)
