@@ -414,18 +414,18 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * (device, int64 triples) says which rows the workgroups take, `tile_rows` each
  * and in this order: the sequence's first token, its length, and the tile's first
  * row in it, a multiple of tile_rows; tiles cover every row once.  tile_rows is
- * what qutai_amd_attention_packed_rows returns for the call's sizes, `longest`
- * sequence, scale and pass (0: forward, 1: the backward's query tiles, 2: its key
+ * what qutai_amd_attention_packed_rows returns for the call's `tokens` (of all
+ * `sequences`), `longest` sequence, sizes, scale and pass (0: forward, 1: the backward's query tiles, 2: its key
  * tiles); aligned: every pointer and pitch is a multiple of 16 bytes.  rest (NULL, or
  * bf16 laid out as out; bf16 with dim up to 128 and tile_rows above 4) receives what
  * out's rounding left, for the backward.  Rows in no tile are left as they are.
  * dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up to 128 rounds probabilities and dS
  * to bf16 for their products, the others keep fp32's bits. */
-int64_t qutai_amd_attention_packed_rows(int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype,
-                                        int aligned, double scale, int pass);
+int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads,
+                                        int64_t dim, int dtype, int aligned, double scale, int pass);
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
-                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t heads,
-                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
+                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens, int64_t sequences,
+                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
                                    double scale, int causal, void* stream);
 /* Its gradients: grad is that of out (contiguous), out, lse and rest (or NULL) the
  * forward's; dq,
@@ -434,8 +434,8 @@ int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, 
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                    const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
                                    const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
-                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t heads,
-                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
+                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
+                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
                                    int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
                                    void* stream);
 

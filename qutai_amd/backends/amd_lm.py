@@ -706,12 +706,12 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
     scale = dim ** -0.5 if scale is None else float(scale)
     left = None
     if packing.used:
-        rows = runtime.lib.qutai_amd_attention_packed_rows(heads, kv_heads, dim, packing.longest, dtype, int(whole), scale, 0)
+        rows = runtime.lib.qutai_amd_attention_packed_rows(*packing.extent, heads, kv_heads, dim, dtype, int(whole), scale, 0)
         tiles, count = packing.tiles(rows, "end" if causal else "length")
         if rest and rows > 4 and q.dtype == "bfloat16" and dim <= 128:
             left = AMDStorage(out.size, q.dtype)
-        runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count, rows, heads,
-                     kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
+        runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count, rows,
+                     *packing.extent[:2], heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
                      mfma=_on_matrix_cores(q.dtype, dim))
     _packed_tail(packing, out, lse, left)
     return (out, lse, left) if rest else (out, lse)
@@ -753,13 +753,13 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
     scale = dim ** -0.5 if scale is None else float(scale)
     if packing.used:
         delta = AMDStorage(total * heads, "float32")
-        q_rows, k_rows = (runtime.lib.qutai_amd_attention_packed_rows(heads, kv_heads, dim, packing.longest, dtype,
-                                                                      int(whole), scale, n) for n in (1, 2))
+        q_rows, k_rows = (runtime.lib.qutai_amd_attention_packed_rows(*packing.extent, heads, kv_heads, dim, dtype, int(whole), scale,
+                                                                      n) for n in (1, 2))
         q_tiles, q_count = packing.tiles(q_rows, "end" if causal else "length")
         k_tiles, k_count = packing.tiles(k_rows, "start" if causal else "length")
         runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
                      *(at for at, _ in targets), delta.ptr, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count, k_rows,
-                     heads, kv_heads, dim, q_row, k_row, v_row, *(row for _, row in targets), dtype, scale,
+                     *packing.extent[:2], heads, kv_heads, dim, q_row, k_row, v_row, *(row for _, row in targets), dtype, scale,
                      int(bool(causal)), mfma=_on_matrix_cores(q.dtype, dim))
     if into is None:
         _packed_tail(packing, *results)

@@ -48,22 +48,47 @@ __global__ void __launch_bounds__(GEN_WAVES * 64) packed_bwd_kv_rows(AttnPackedA
 
 enum Pass { FORWARD, QUERIES, KEYS };
 
-int key_split(int64_t heads, int64_t kv_heads, int64_t dim) {
+// How a workgroup of the key pass is cut: waves of 32 keys each, and sets of them
+// that share the group's query heads.
+struct KeyShape {
+  int waves, sets;
+};
+
+// `tiles` bounds the key tiles from above (of 64 rows, for each kv head).  Many of
+// them: as many workgroups as fit a CU (registers allow two waves of each SIMD).  Few:
+// a workgroup is a CU's only one, four sets of waves take a head each, and the longest
+// tile ends in a quarter of the time.  Measured, us: 16384 tokens of up to 1024, 16
+// heads over 4 of 64, {2, 2} 76, {4, 2} 92-99, {2, 4} 114, {4, 1} 155; one of 2000, 8
+// over 2 of 64, {2, 2} 103, {2, 4} 76; 16000 of up to 6000, 32 over 8 of 128, {4, 1}
+// 1866, {4, 2} 1993 (an older form of both); 8000 of up to 2000, 16 over 4 of 96,
+// {4, 1} 398, {2, 4} 177; 8000 of up to 8, 16 over 4 of 64, {2, 2} 157, {2, 4} 335.
+KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles) {
   const int64_t group = heads / kv_heads;
-  return dim > 64 ? 1 : group % 4 == 0 ? 4 : group % 2 == 0 ? 2 : 1;
+  const bool few = tiles * kv_heads < 2 * cu_count() * (dim > 64 ? 2 : 1);
+  if (few && group % 4 == 0) return {2, 4};
+  if (dim <= 64) return group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
+  return few && group % 2 == 0 ? KeyShape{4, 2} : KeyShape{4, 1};
 }
 
+int64_t key_tiles_of(int64_t tokens, int64_t sequences) { return tokens / 64 + std::min(sequences, tokens); }
+
 template <int DP>
-void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
+void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape shape, hipStream_t stream) {
   if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP == 64 ? 64 : 32>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
   else if (pass == QUERIES) hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
-  else if constexpr (DP == 64) {
-    if (key_split(a.heads, a.kv_heads, a.dim) == 4)
-      hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 2>), dim3(blocks), dim3(256), 0, stream, a);
-    else if (key_split(a.heads, a.kv_heads, a.dim) == 2)
-      hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 2>), dim3(blocks), dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), dim3(256), 0, stream, a);
-  } else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), dim3(256), 0, stream, a);
+  else {
+    const auto [waves, sets] = shape;
+    const dim3 block(waves * sets * 64);
+    if constexpr (DP == 64) {
+      if (sets == 4) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 4>), dim3(blocks), block, 0, stream, a);
+      else if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 2>), dim3(blocks), block, 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 1>), dim3(blocks), block, 0, stream, a);
+    } else {
+      if (sets == 4) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 4>), dim3(blocks), block, 0, stream, a);
+      else if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 2>), dim3(blocks), block, 0, stream, a);
+      else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), block, 0, stream, a);
+    }
+  }
 }
 
 template <bool F32, int DP>
@@ -100,14 +125,14 @@ int64_t groups_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t
 }
 
 // Rows of a tile of the matrix kernels.
-int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim) {
+int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim, int64_t key_tiles) {
   if (!packed_fits(dtype, dim)) return MMA_ROWS;
-  return pass == KEYS ? (key_split(heads, kv_heads, dim) == 4 ? 64 : 128) : WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
+  return pass == KEYS ? 32 * key_shape(heads, kv_heads, dim, key_tiles).waves : WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
 }
 
 // One pass over the tiles of `rows` rows each.
-hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, const int64_t* tiles, int64_t count, int64_t rows,
-                  hipStream_t stream) {
+hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, const int64_t* tiles, int64_t count,
+                  int64_t rows, hipStream_t stream) {
   if (!count) return hipSuccess;
   a.tiles = tiles;
   a.pack = packed_heads(a.heads, a.kv_heads, WAVES);
@@ -116,8 +141,9 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, const int64_t* tiles, 
     if (dtype == BF16) launch_rows<bf16_t>(pass, a, n, stream);
     else launch_rows<float>(pass, a, n, stream);
   } else if (dtype == BF16) {
-    if (a.dim <= 64) launch_packed<64>(pass, a, n, stream);
-    else if (a.dim <= 128) launch_packed<128>(pass, a, n, stream);
+    const KeyShape shape = key_shape(a.heads, a.kv_heads, a.dim, key_tiles);
+    if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, stream);
+    else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, stream);
     else launch_mma<false, 256>(pass, a, n, stream);
   } else {
     if (a.dim <= 32) launch_mma<true, 32>(pass, a, n, stream);
@@ -129,15 +155,16 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, const int64_t* tiles, 
 }
 
 // What forward and backward share: sizes, scale, pitches.  rows: of a tile.
-int set_packed(AttnPackedArgs& a, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
+int set_packed(AttnPackedArgs& a, int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
                int64_t v_row, int dtype, double scale, int causal, std::initializer_list<std::pair<Pass, int64_t>> tiles) {
   if ((dtype != BF16 && dtype != F32) || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1 << 16) return QA_EINVAL;
+  if (tokens < 0 || tokens >= 1ll << 31 || sequences < 0) return QA_EINVAL;
   if (dim <= 0 || dim > 256 || !(scale > 0.0) || scale > 1e30) return QA_EINVAL;
   if (q_row < heads * dim || k_row < kv_heads * dim || v_row < kv_heads * dim) return QA_EINVAL;
   if (std::max({q_row, k_row, v_row, heads * dim}) > 1 << 22) return QA_EINVAL;  // 64 rows within a buffer descriptor
   for (const auto& [pass, rows] : tiles) {
     if (rows == GEN_WAVES) continue;
-    if (rows != rows_of(pass, dtype, heads, kv_heads, dim) || !mma_fits(dtype, dim) || scale < 0x1p-50) return QA_EINVAL;
+    if (rows != rows_of(pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences)) || !mma_fits(dtype, dim) || scale < 0x1p-50) return QA_EINVAL;
   }
   a.batch = 1;
   a.heads = heads;
@@ -171,21 +198,28 @@ bool grid_fits(int64_t tiles, int64_t blocks) { return tiles >= 0 && tiles <= ((
 
 extern "C" {
 
-int64_t qutai_amd_attention_packed_rows(int64_t heads, int64_t kv_heads, int64_t dim, int64_t longest, int dtype,
-                                        int aligned, double scale, int pass) {
+int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads,
+                                        int64_t dim, int dtype, int aligned, double scale, int pass) {
   if ((dtype != BF16 && dtype != F32) || dim <= 0 || dim > 256 || pass < 0 || pass > 2 || heads <= 0 || kv_heads <= 0 ||
-      heads % kv_heads)
+      heads % kv_heads || tokens < 0 || tokens >= 1ll << 31 || sequences < 0)
     return 0;
-  if (!aligned || !mma_fits(dtype, dim) || scale < 0x1p-50 || longest <= (pass == FORWARD ? 2 : 4)) return GEN_WAVES;
-  return rows_of((Pass)pass, dtype, heads, kv_heads, dim);
+  if (!aligned || !mma_fits(dtype, dim) || scale < 0x1p-50) return GEN_WAVES;
+  // Tiles of sequences of a few tokens are mostly empty.  8000 tokens, us, tiles and one
+  // wave per row: bf16, 16 heads over 4 of 64, sequences of up to 4, forward 73 and 80; of
+  // up to 8, forward 49 and 91, dQ 58 and 104, dK and dV 157 and 70; fp32 of up to 8, 371 and
+  // 89, 582 and 101, 646 and 69, of up to 16 194 and 117, 307 and 130, 332 and 104, of up to
+  // 32 82 and 202, 132 and 217, 144 and 197.
+  const int64_t few = packed_fits(dtype, dim) ? (pass == KEYS ? 8 : 0) : 20;
+  if (longest <= few) return GEN_WAVES;
+  return rows_of((Pass)pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences));
 }
 
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
-                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t heads,
-                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
+                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens, int64_t sequences,
+                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
                                    double scale, int causal, void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
+  const int status = set_packed(a, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
   if (status != QA_OK) return status;
   if (!grid_fits(tile_count, heads)) return QA_EINVAL;
   if (rest && (tile_rows == GEN_WAVES || !packed_fits(dtype, dim))) return QA_EINVAL;
@@ -199,18 +233,18 @@ int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, 
   a.dqt = a.ot;
   a.lse = lse;
   a.rest = rest;
-  return (int)launch(FORWARD, dtype, a, tiles, tile_count, tile_rows, (hipStream_t)stream);
+  return (int)launch(FORWARD, dtype, a, key_tiles_of(tokens, sequences), tiles, tile_count, tile_rows, (hipStream_t)stream);
 }
 
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                    const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
                                    const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
-                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t heads,
-                                   int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
+                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
+                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
                                    int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
                                    void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
+  const int status = set_packed(a, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
                                 {{QUERIES, query_rows}, {KEYS, key_rows}});
   if (status != QA_OK) return status;
   if (dq_row < heads * dim || dk_row < kv_heads * dim || dv_row < kv_heads * dim) return QA_EINVAL;
@@ -237,9 +271,9 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
   a.dkt = dk_row;
   a.dvt = dv_row;
   // the query pass writes delta, which the key pass reads
-  const hipError_t e = launch(QUERIES, dtype, a, query_tiles, query_count, query_rows, (hipStream_t)stream);
+  const hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), query_tiles, query_count, query_rows, (hipStream_t)stream);
   if (e != hipSuccess) return (int)e;
-  return (int)launch(KEYS, dtype, a, key_tiles, key_count, key_rows, (hipStream_t)stream);
+  return (int)launch(KEYS, dtype, a, key_tiles_of(tokens, sequences), key_tiles, key_count, key_rows, (hipStream_t)stream);
 }
 
 }  // extern "C"

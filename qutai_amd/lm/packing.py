@@ -26,6 +26,7 @@ class Packing:
         if type(self.total) is not int or self.total < self.used or self.total >= 1 << 31:
             raise ValueError("total is at least the sum of lengths, below 2^31")
         self.longest = max(lengths, default=0)
+        self.extent = self.used, len(lengths), self.longest  # what the kernels' shapes are chosen by
         self._positions, self._tiles = None, {}
 
     @property

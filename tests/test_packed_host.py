@@ -203,22 +203,22 @@ def test_c_entry_points_refuse():
     assert turn(batch=0) == 0
 
     def forward(**change):
-        a = dict(q=p, k=p, v=p, out=p, lse=p, rest=None, tiles=p, count=2, rows=128, heads=4, kv=2, dim=64, qr=256, kr=128,
+        a = dict(q=p, k=p, v=p, out=p, lse=p, rest=None, tiles=p, count=2, rows=64, tokens=200, sequences=3, heads=4, kv=2, dim=64, qr=256, kr=128,
                  vr=128, dtype=5, scale=0.125, causal=1, stream=None)
         a.update(change)
         return library.qutai_amd_attention_packed_fwd(*a.values())
 
     wrong = (dict(heads=3), dict(kv=0), dict(dim=0), dict(dim=264), dict(qr=255), dict(kr=127), dict(vr=64), dict(dtype=4),
              dict(scale=0.0), dict(scale=float("nan")), dict(rows=100), dict(rows=0), dict(q=None), dict(lse=None),
-             dict(tiles=None), dict(count=-1), dict(count=1 << 40), dict(q=p + 2), dict(qr=1 << 30), dict(dim=20))
+             dict(tiles=None), dict(count=-1), dict(count=1 << 40), dict(tokens=-1), dict(sequences=-1), dict(tokens=1 << 31), dict(q=p + 2), dict(qr=1 << 30), dict(dim=20))
     for change in wrong:
         assert forward(**change) == EINVAL, change
     assert forward(count=0) == 0
     assert forward(rest=p, dim=136, qr=544, kr=272, vr=272) == EINVAL and forward(rest=p, rows=4) == EINVAL
-    for dtype, dim, rows in ((5, 20, 4), (0, 160, 4), (0, 64, 128), (5, 64, 128)):
-        assert library.qutai_amd_attention_packed_rows(4, 2, dim, 1000, dtype, 1, 0.1, 0) == rows
-    assert library.qutai_amd_attention_packed_rows(4, 2, 64, 1000, 5, 0, 0.1, 0) == 4
-    assert library.qutai_amd_attention_packed_rows(4, 2, 64, 1000, 4, 1, 0.1, 0) == 0
+    for dtype, dim, rows in ((5, 20, 4), (0, 160, 4), (0, 64, 128), (5, 64, 64)):
+        assert library.qutai_amd_attention_packed_rows(50000, 9, 1000, 4, 2, dim, dtype, 1, 0.1, 0) == rows
+    assert library.qutai_amd_attention_packed_rows(50000, 9, 1000, 4, 2, 64, 5, 0, 0.1, 0) == 4
+    assert library.qutai_amd_attention_packed_rows(50000, 9, 1000, 4, 2, 64, 4, 1, 0.1, 0) == 0
 
     row = (ctypes.c_int64 * 8)(p, p, p, p, p, 8, 0, 0)
 
