@@ -466,8 +466,8 @@ int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, con
  * With max_norm > 0 gradients are scaled to that norm over all tensors where they
  * exceed it, the norm goes to `norm` (fp64, device, may be NULL), a norm that is not
  * finite leaves everything as it is, and `workspace` holds at least
- * qutai_amd_adamw_workspace fp64 values. */
-int64_t qutai_amd_adamw_workspace(const int64_t* tensors, int64_t count);
+ * qutai_amd_adamw_workspace(tensors, values in all of them) fp64 values. */
+int64_t qutai_amd_adamw_workspace(int64_t count, int64_t values);
 int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate, double beta1, double beta2,
                     double eps, double weight_decay, int64_t step, uint64_t seed, double max_norm, double* workspace,
                     int64_t workspace_values, double* norm, void* stream);

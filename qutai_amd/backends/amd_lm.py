@@ -706,8 +706,7 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
     scale = dim ** -0.5 if scale is None else float(scale)
     left = None
     if packing.used:
-        rows = runtime.lib.qutai_amd_attention_packed_rows(*packing.extent, heads, kv_heads, dim, dtype, int(whole), scale, 0)
-        tiles, count = packing.tiles(rows, "end" if causal else "length")
+        tiles, count, rows = packing.plan(0, heads, kv_heads, dim, dtype, whole, scale, causal)
         if rest and rows > 4 and q.dtype == "bfloat16" and dim <= 128:
             left = AMDStorage(out.size, q.dtype)
         runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count, rows,
@@ -753,10 +752,8 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
     scale = dim ** -0.5 if scale is None else float(scale)
     if packing.used:
         delta = AMDStorage(total * heads, "float32")
-        q_rows, k_rows = (runtime.lib.qutai_amd_attention_packed_rows(*packing.extent, heads, kv_heads, dim, dtype, int(whole), scale,
-                                                                      n) for n in (1, 2))
-        q_tiles, q_count = packing.tiles(q_rows, "end" if causal else "length")
-        k_tiles, k_count = packing.tiles(k_rows, "start" if causal else "length")
+        (q_tiles, q_count, q_rows), (k_tiles, k_count, k_rows) = (
+            packing.plan(n, heads, kv_heads, dim, dtype, whole, scale, causal) for n in (1, 2))
         runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
                      *(at for at, _ in targets), delta.ptr, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count, k_rows,
                      *packing.extent[:2], heads, kv_heads, dim, q_row, k_row, v_row, *(row for _, row in targets), dtype, scale,
@@ -1100,6 +1097,7 @@ class AdamWMoments:
         else:  # bytes, as whole int64 words of zeros
             self.first, self.second = (amd.full((size + 7) // 8, 0, dtype="int64") for _ in range(2))
             self.exponents = amd.full((2 * ((size + 255) // 256) + 7) // 8, 0, dtype="int64")
+        self.pointers = self.first.ptr, self.second.ptr, amd._p(self.exponents)
 
     def storages(self):
         return (self.first, self.second) if self.exponents is None else (self.first, self.second, self.exponents)
@@ -1115,29 +1113,39 @@ class AdamWMoments:
         return out
 
 
-def adamw(tensors, bits, lr, beta1, beta2, eps, weight_decay, step, *, seed=0, max_norm=None):
+def adamw_workspace(count, values):
+    """What ``adamw`` needs to cut the norm of up to ``count`` gradients of
+    ``values`` values: (partial sums, the norm), fp64 storages."""
+    return AMDStorage(get_runtime().lib.qutai_amd_adamw_workspace(count, values), "float64"), amd.full(1, 0.0, dtype="float64")
+
+
+def adamw(tensors, bits, lr, beta1, beta2, eps, weight_decay, step, *, seed=0, max_norm=None, workspace=None):
     """One AdamW step (its ``step``-th, from 1) over ``tensors``: tuples of a
     parameter's storage, its gradient's, its AdamWMoments and the number that
     tells it from the others where 8-bit codes are rounded.  Parameters and moments
-    are changed in place.  With ``max_norm`` returns the fp64 storage that holds
-    the norm of all gradients, else None."""
-    table = array("q")
+    are changed in place.  With ``max_norm`` returns the fp64 storage that holds the
+    norm of all gradients, else None; ``workspace``: an ``adamw_workspace`` of as
+    many tensors and values at least, which this step alone uses meanwhile."""
+    rows, values = [], 0
     for p, g, moments, index in tensors:
-        if p.dtype not in ("bfloat16", "float32") or g.dtype != p.dtype or not p.size == g.size == moments.size \
-                or moments.bits != bits:
+        dtype, size = p.dtype, p._size
+        if dtype not in _ADAMW_CODES or g.dtype != dtype or not size == g._size == moments.size or moments.bits != bits:
             raise ValueError("adamw takes float32 or bfloat16 parameters with gradients and moments of their size")
-        table.extend((p.ptr, g.ptr, moments.first.ptr, moments.second.ptr, amd._p(moments.exponents), p.size,
-                      code(p.dtype), index))
-    runtime, count, address = get_runtime(), len(tensors), table.buffer_info()[0]
-    norm = workspace = None
-    if max_norm is not None:  # the step writes it if any gradient has a value
-        norm = AMDStorage(1, "float64") if any(p.size for p, *_ in tensors) else amd.full(1, 0.0, dtype="float64")
-        workspace = AMDStorage(runtime.lib.qutai_amd_adamw_workspace(address, count), "float64")
-    if count:
-        runtime.call("qutai_amd_adamw", address, count, bits, lr, beta1, beta2, eps, weight_decay, step, seed,
-                     0.0 if max_norm is None else max_norm, amd._p(workspace), 0 if workspace is None else workspace.size,
-                     amd._p(norm))
+        rows += (p.ptr, g.ptr, *moments.pointers, size, _ADAMW_CODES[dtype], index)
+        values += size
+    table, partial, norm = array("q", rows), None, None
+    if max_norm is not None:
+        partial, norm = adamw_workspace(len(rows) // 8, values) if workspace is None else workspace
+        if not values:
+            norm = amd.full(1, 0.0, dtype="float64")
+    if values:
+        get_runtime().call("qutai_amd_adamw", table.buffer_info()[0], len(rows) // 8, bits, lr, beta1, beta2, eps,
+                           weight_decay, step, seed, max_norm or 0.0, None if partial is None else partial.ptr,
+                           0 if partial is None else partial.size, None if norm is None else norm.ptr)
     return norm
+
+
+_ADAMW_CODES = {name: code(name) for name in ("float32", "bfloat16")}
 
 
 def copy_rows(source, rows, width, *, column=0, row=None, out=None, out_column=0, out_row=None):

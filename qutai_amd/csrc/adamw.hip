@@ -69,16 +69,15 @@ struct NormArgs {
   Tensor t[TENSORS];
 };
 
-// The record that holds chunk c.
+// The record that holds chunk c: the last whose first chunk is not behind it.
+// `starts`: lane i's is record i's first chunk.
 template <class Args>
-__device__ __forceinline__ int tensor_of(const Args& a, uint32_t c) {
-  int lo = 0, hi = a.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.t[mid].chunks <= c) lo = mid;
-    else hi = mid;
-  }
-  return uniform32(lo);
+__device__ __forceinline__ uint32_t starts_of(const Args& a) {
+  const int lane = threadIdx.x & 63;
+  return lane < a.n ? a.t[lane].chunks : 0xffffffffu;
+}
+__device__ __forceinline__ int tensor_of(uint32_t starts, uint32_t c) {
+  return __builtin_popcountll(__builtin_amdgcn_ballot_w64(starts <= c)) - 1;
 }
 
 // Four values from index i on, and back: at once where `whole` (i a multiple of 4),
@@ -168,8 +167,9 @@ __device__ __forceinline__ void square_sum(const Tensor& t, int64_t start, int64
 __global__ void __launch_bounds__(THREADS) adamw_norm(NormArgs a) {
   __shared__ double shared[4];
   double sum = 0.0;
+  const uint32_t starts = starts_of(a);
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const Tensor& t = a.t[tensor_of(a, c)];
+    const Tensor& t = a.t[tensor_of(starts, c)];
     const int64_t start = (int64_t)(c - t.chunks) * CHUNK, end = min(t.count, start + CHUNK);
     if (t.bf16) square_sum<bf16_t>(t, start, end, sum);
     else square_sum<float>(t, start, end, sum);
@@ -338,6 +338,7 @@ __device__ __forceinline__ void step32(const StepArgs& a, const Tensor& t, int64
 template <bool EIGHT>
 __global__ void __launch_bounds__(THREADS) adamw_step(StepArgs a) {
   __shared__ double shared[4];
+  const uint32_t starts = starts_of(a);
   double factor = 1.0;
   if (a.partial) {
     double sum = 0.0;
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(THREADS) adamw_step(StepArgs a) {
     factor = norm > a.max_norm ? a.max_norm / norm : 1.0;
   }
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
-    const Tensor& t = a.t[tensor_of(a, c)];
+    const Tensor& t = a.t[tensor_of(starts, c)];
     const int64_t start = (int64_t)(c - t.chunks) * CHUNK, end = min(t.count, start + CHUNK);
     if constexpr (EIGHT) {
       if (t.bf16) step8<bf16_t>(a, t, start, end, factor);
@@ -398,26 +399,22 @@ int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, uint
   return i - first;
 }
 
-int64_t launches(const int64_t* tensors, int64_t count) {
-  int64_t n = 0, chunks = 0, launched = 0;
-  for (int64_t i = 0; i < count; i++) {
-    const int64_t values = tensors[8 * i + 5], c = (values + CHUNK - 1) / CHUNK;
-    if (values == 0) continue;
-    if (n == TENSORS || chunks + c > 0x7fffffff) launched++, n = 0, chunks = 0;
-    n++;
-    chunks += c;
-  }
-  return launched + (n > 0);
+// Launches that any `tensors` tensors of `values` values need at most: one ends with
+// TENSORS of them, or with 2^30 chunks at least.
+int64_t launches(int64_t tensors, int64_t values) {
+  return (tensors + TENSORS - 1) / TENSORS + (values / CHUNK + tensors >> 30);
 }
 
-bool valid(const int64_t* tensors, int64_t count, int bits, bool gradients_only) {
-  if (count < 0 || (count && !tensors)) return false;
+bool valid(const int64_t* tensors, int64_t count, int bits, int64_t& values) {
+  values = 0;
+  if (count < 0 || count > 1 << 24 || (count && !tensors)) return false;
   for (int64_t i = 0; i < count; i++) {
     const int64_t* r = tensors + 8 * i;
     if (r[5] < 0 || r[5] > (1ll << 42) || (r[6] != F32 && r[6] != BF16)) return false;
     if (r[5] == 0) continue;
+    values += r[5];
+    if (values > 1ll << 48) return false;
     if (!r[1] || r[1] % (r[6] == BF16 ? 2 : 4)) return false;
-    if (gradients_only) continue;
     if (!r[0] || r[0] % (r[6] == BF16 ? 2 : 4) || !r[2] || !r[3]) return false;
     if (bits == 8 ? !r[4] : r[2] % 4 || r[3] % 4) return false;
   }
@@ -428,29 +425,29 @@ bool valid(const int64_t* tensors, int64_t count, int bits, bool gradients_only)
 
 extern "C" {
 
-int64_t qutai_amd_adamw_workspace(const int64_t* tensors, int64_t count) {
-  return valid(tensors, count, 32, true) ? launches(tensors, count) * NORM_GROUPS : 0;
+int64_t qutai_amd_adamw_workspace(int64_t count, int64_t values) {
+  return count < 0 || count > 1 << 24 || values < 0 || values > 1ll << 48 ? 0 : launches(count, values) * NORM_GROUPS;
 }
 
 int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate, double beta1, double beta2,
                     double eps, double weight_decay, int64_t step, uint64_t seed, double max_norm, double* workspace,
                     int64_t workspace_values, double* norm, void* stream) {
-  if ((bits != 8 && bits != 32) || !valid(tensors, count, bits, false)) return QA_EINVAL;
+  int64_t values;
+  if ((bits != 8 && bits != 32) || !valid(tensors, count, bits, values)) return QA_EINVAL;
   if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0) || step < 1) return QA_EINVAL;
   if (!(rate >= 0.0) || !(rate < 1e30) || !(weight_decay >= 0.0) || !(weight_decay < 1e30) || !(max_norm >= 0.0))
     return QA_EINVAL;
-  const int64_t parts = launches(tensors, count) * NORM_GROUPS;
-  if (max_norm > 0.0 && parts && (!workspace || (uintptr_t)workspace % 8 || workspace_values < parts)) return QA_EWORKSPACE;
-  if (max_norm > 0.0 && parts) {
+  int64_t parts = 0;
+  if (max_norm > 0.0 && values) {
+    if (!workspace || (uintptr_t)workspace % 8 || workspace_values < launches(count, values) * NORM_GROUPS) return QA_EWORKSPACE;
     NormArgs a = {};
-    int64_t at = 0;
     for (int64_t first = 0; first < count;) {
       first += take(a, tensors, first, count, 0);
       if (!a.n) continue;
-      a.partial = workspace + at * NORM_GROUPS;
-      at++;
-      // every partial sum is written: workgroups without a chunk write 0
-      hipLaunchKernelGGL(adamw_norm, dim3(NORM_GROUPS), dim3(THREADS), 0, (hipStream_t)stream, a);
+      a.partial = workspace + parts;
+      const unsigned groups = std::min<uint32_t>(a.chunks, NORM_GROUPS);
+      parts += groups;
+      hipLaunchKernelGGL(adamw_norm, dim3(groups), dim3(THREADS), 0, (hipStream_t)stream, a);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return (int)e;
     }
@@ -466,7 +463,7 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
   a.root = (float)(1.0 / __builtin_sqrt(c2));
   a.eps = (float)eps;
   a.max_norm = max_norm;
-  if (max_norm > 0.0 && parts) {
+  if (parts) {
     a.partial = workspace;
     a.partials = (int)parts;
     a.norm = norm;

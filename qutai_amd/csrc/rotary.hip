@@ -23,6 +23,7 @@ using namespace qa;
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int64_t CACHED = 128 << 20;  // bytes of results that stay in the memory-side cache (256 MB)
 
 struct RotaryArgs {
   const void* x[2];  // queries, keys
@@ -34,47 +35,48 @@ struct RotaryArgs {
   int heads[2], dim, rotary;
   int pair_lanes, lanes, slots;  // lanes of a token that turn pairs, all of its lanes, lanes that share its heads
   float magnitude, sign;
+  bool past;  // results are stored past the caches
   double turns[128];
 };
 
+// N elements at once: 16 or 8 bytes, or one.  Inputs are read once, past the caches;
+// results stay there for the attention that reads them next, unless (`past`) they do
+// not fit: 336 MB of them take 123 us past the caches and 133 through them.
 template <class T, int N>
 __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
-  if constexpr (sizeof(T) * N == 16) {
-    const u32x4 w = global_load<u32x4>(p);
+  if constexpr (N == 1) {
+    if constexpr (sizeof(T) == 4) v[0] = p[0];
+    else v[0] = bf16_to_f32(p[0]);
+  } else {
+    typedef uint32_t words __attribute__((__vector_size__(sizeof(T) * N)));
+    const words w = global_load_nt<words>(p);
 #pragma unroll
     for (int e = 0; e < N; e++) {
       if constexpr (sizeof(T) == 4) v[e] = __uint_as_float(w[e]);
       else v[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      if constexpr (sizeof(T) == 4) v[e] = p[e];
-      else v[e] = bf16_to_f32(p[e]);
-    }
   }
 }
 template <class T, int N>
-__device__ __forceinline__ void store(T* p, const float (&v)[N]) {
-  if constexpr (sizeof(T) * N == 16) {
-    u32x4 w;
+__device__ __forceinline__ void store(T* p, const float (&v)[N], bool past) {
+  if constexpr (N == 1) {
+    if constexpr (sizeof(T) == 4) p[0] = v[0];
+    else p[0] = f32_to_bf16(v[0]);
+  } else {
+    typedef uint32_t words __attribute__((__vector_size__(sizeof(T) * N)));
+    words w;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < (int)(sizeof(T) * N / 4); e++) {
       if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(v[e]);
       else w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
     }
-    global_store(p, w);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; e++) {
-      if constexpr (sizeof(T) == 4) p[e] = v[e];
-      else p[e] = f32_to_bf16(v[e]);
-    }
+    if (past) global_store_nt(p, w);
+    else global_store(p, w);
   }
 }
 
-// V elements of T at a time: 16 bytes, or one where widths, pitches or
-// addresses are not whole chunks.
+// V elements of T at a time: 16 or 8 bytes, or one where widths, pitches or addresses
+// are no whole chunks of that.
 template <class T, int V, bool HALF>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(RotaryArgs a) {
   const int64_t id = (int64_t)blockIdx.x * THREADS + threadIdx.x;
@@ -134,8 +136,8 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(RotaryArgs a) {
         for (int e = 0; e < V; e++) u[e] = y[e], w[e] = y[V + e];
       }
     }
-    store<T, V>(out + first, u);
-    if (both) store<T, V>(out + second, w);
+    store<T, V>(out + first, u, a.past);
+    if (both) store<T, V>(out + second, w, a.past);
   }
 }
 
@@ -169,14 +171,14 @@ extern "C" int qutai_amd_rotary(const void* q, const void* k, void* q_out, void*
   const int64_t n[2] = {heads, kv_heads}, rows[2] = {q_row, k_row}, out_rows[2] = {q_out_row, k_out_row};
   const void* x[2] = {q, k};
   void* out[2] = {q_out, k_out};
-  const int64_t item = dtype == F32 ? 4 : 2, chunk = 16 / item;
-  bool whole = rotary % (2 * chunk) == 0 && dim % chunk == 0;
+  const int64_t item = dtype == F32 ? 4 : 2;
+  int64_t odd = 0;  // what has to be whole chunks, or'd
   for (int i = 0; i < 2; i++) {
     if (!n[i]) continue;
     if (rows[i] < n[i] * dim || out_rows[i] < n[i] * dim || rows[i] > (1ll << 40) || out_rows[i] > (1ll << 40))
       return QA_EINVAL;
     if (batch * time && (!x[i] || !out[i])) return QA_EINVAL;
-    whole &= (uintptr_t)x[i] % 16 == 0 && (uintptr_t)out[i] % 16 == 0 && rows[i] % chunk == 0 && out_rows[i] % chunk == 0;
+    odd |= (int64_t)(uintptr_t)x[i] | (int64_t)(uintptr_t)out[i] | rows[i] * item | out_rows[i] * item;
     a.x[i] = x[i];
     a.out[i] = out[i];
     a.x_row[i] = rows[i];
@@ -193,10 +195,19 @@ extern "C" int qutai_amd_rotary(const void* q, const void* k, void* q_out, void*
   a.rotary = (int)rotary;
   a.magnitude = (float)magnitude;
   a.sign = inverse ? -1.f : 1.f;
+  a.past = a.tokens * (heads + kv_heads) * dim * item > CACHED;
   for (int64_t i = 0; i < rotary / 2; i++) a.turns[i] = turns[i];
   const hipStream_t s = (hipStream_t)stream;
   hipError_t e;
-  if (dtype == F32) e = whole ? launch<float, 4>(a, half, s) : launch<float, 1>(a, half, s);
-  else e = whole ? launch<bf16_t, 8>(a, half, s) : launch<bf16_t, 1>(a, half, s);
+  odd |= rotary / 2 * item | dim * item;
+  if (dtype == F32) {
+    if (odd % 16 == 0) e = launch<float, 4>(a, half, s);
+    else if (odd % 8 == 0) e = launch<float, 2>(a, half, s);
+    else e = launch<float, 1>(a, half, s);
+  } else {
+    if (odd % 16 == 0) e = launch<bf16_t, 8>(a, half, s);
+    else if (odd % 8 == 0) e = launch<bf16_t, 4>(a, half, s);
+    else e = launch<bf16_t, 1>(a, half, s);
+  }
   return e == hipErrorInvalidValue ? QA_EINVAL : (int)e;
 }

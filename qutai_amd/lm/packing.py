@@ -6,6 +6,7 @@ from array import array
 from itertools import accumulate, chain
 
 from ..backends import amd
+from ..backends.amd_runtime import get_runtime
 
 
 class Packing:
@@ -27,7 +28,7 @@ class Packing:
             raise ValueError("total is at least the sum of lengths, below 2^31")
         self.longest = max(lengths, default=0)
         self.extent = self.used, len(lengths), self.longest  # what the kernels' shapes are chosen by
-        self._positions, self._tiles = None, {}
+        self._positions, self._tiles, self._plans = None, {}, {}
 
     @property
     def positions(self):
@@ -36,6 +37,17 @@ class Packing:
             places.extend([0] * (self.total - self.used))
             self._positions = amd.storage(places, dtype="int64")
         return self._positions
+
+    def plan(self, number, heads, kv_heads, dim, dtype, whole, scale, causal):
+        """(tiles, count, rows of a tile) of pass ``number`` of attention (forward,
+        queries of the backward, its keys) of these sizes; asked of the library once."""
+        key = number, heads, kv_heads, dim, dtype, whole, scale, bool(causal)
+        found = self._plans.get(key)
+        if found is None:
+            rows = get_runtime().lib.qutai_amd_attention_packed_rows(*self.extent, heads, kv_heads, dim, dtype, int(whole),
+                                                                     scale, number)
+            found = self._plans[key] = (*self.tiles(rows, "length" if not causal else "start" if number == 2 else "end"), rows)
+        return found
 
     def tiles(self, rows, longest_first):
         """(storage, count): for every tile of ``rows`` tokens of a sequence its

@@ -37,21 +37,18 @@ class AdamW:
         self.weight_decay, self.bits, self.max_norm, self.seed = weight_decay, bits, max_norm, seed
         self.steps = 0
         self._state = tuple(amd_lm.AdamWMoments(p.size, bits) for p in parameters)
+        self._workspace = (None if max_norm is None else
+                           amd_lm.adamw_workspace(len(parameters), sum(p.size for p in parameters)))
         self._norm = None
 
     def step(self):
         rate, decay = float(self.lr), float(self.weight_decay)
         if not (isfinite(rate) and rate >= 0 and isfinite(decay) and decay >= 0):
             raise ValueError("lr and weight_decay are numbers of 0 or more")
-        pairs = []
-        for index, (p, state) in enumerate(zip(self.parameters, self._state)):
-            if p.grad is None:
-                continue
-            if p.size != state.size or p.grad.dtype != p.dtype or p.grad.size != p.size:
-                raise ValueError("a gradient has its parameter's size and dtype, and a parameter keeps its size")
-            pairs.append((p.storage, p.grad.storage, state, index))
-        norm = amd_lm.adamw(pairs, self.bits, rate, *self.betas, self.eps, decay, self.steps + 1, seed=self.seed,
-                            max_norm=self.max_norm)
+        tensors = [(p.storage, p.grad.storage, state, index)
+                   for index, (p, state) in enumerate(zip(self.parameters, self._state)) if p.grad is not None]
+        norm = amd_lm.adamw(tensors, self.bits, rate, *self.betas, self.eps, decay, self.steps + 1, seed=self.seed,
+                            max_norm=self.max_norm, workspace=self._workspace)
         self.steps += 1
         self._norm = norm
 

@@ -167,7 +167,7 @@ def test_adamw_step_refusals(monkeypatch):
     monkeypatch.setattr(amd_lm, "AdamWMoments", lambda size, bits: SimpleNamespace(size=size, bits=bits))
     p = parameter()
     optimizer = AdamW([p])
-    for grad in (fake(7, "float32"), fake(8, "bfloat16")):
+    for grad in (fake(7, "float32"), fake(8, "bfloat16")):  # other sizes, other types
         p.grad = Tensor(grad, shape=(grad.size,))
         with pytest.raises(ValueError):
             optimizer.step()
@@ -238,5 +238,6 @@ def test_c_entry_points_refuse():
         assert step(**change) == EINVAL, change
     assert step(max_norm=1.0) == EWORKSPACE
     assert step(values=(0, 0, 0, 0, 0, 0, 0, 0)) == 0 and step(count=0) == 0
+    assert library.qutai_amd_adamw_workspace(-1, 8) == 0 and library.qutai_amd_adamw_workspace(49, 8) == 2048
     assert library.qutai_amd_adamw_moments(p, p, None, p, p, 8, None) == EINVAL
     assert library.qutai_amd_adamw_moments(p, p, p, p, p, -1, None) == EINVAL
