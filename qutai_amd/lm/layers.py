@@ -891,7 +891,8 @@ def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turn
     if packing is not None:
         place = dict(v_column=dq + dkv, v_row=total, **(columns if q_norm is None else {}))
         dims = (packing, heads, kv_heads, head)
-        out, lse, rest = b.attention_packed(q, k, qkv, *dims, **place, rest=True)
+        keep = is_recording() and any(t.requires_grad for t in parents)
+        out, lse, *rest = b.attention_packed(q, k, qkv, *dims, **place, rest=keep)
     else:
         if q_norm is None:
             q, k = (b.copy_rows(qkv, rows, n, column=c, row=total) for n, c in ((dq, 0), (dkv, dq)))
@@ -904,9 +905,9 @@ def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turn
             d = amd.AMDStorage(rows * total, "bfloat16")
             dnorms = ()
             if packing is not None and q_norm is None:
-                b.attention_packed_backward(g, q, k, qkv, out, lse, *dims, **place, rest=rest, into=d)
+                b.attention_packed_backward(g, q, k, qkv, out, lse, *dims, **place, rest=rest[0], into=d)
             else:
-                gq, gk, gv = (b.attention_packed_backward(g, q, k, qkv, out, lse, *dims, **place, rest=rest)
+                gq, gk, gv = (b.attention_packed_backward(g, q, k, qkv, out, lse, *dims, **place, rest=rest[0])
                               if packing is not None else b.attention_backward(g, q, k, v, out, lse, *dims))
                 b.copy_rows(gv, rows, dkv, out=d, out_column=dq + dkv, out_row=total)
             if q_norm is None:

@@ -39,7 +39,14 @@ CASES = [
     ("bfloat16", [140, 20], 2, 1, 256, False, False),
     ("bfloat16", [9, 30], 2, 1, 20, True, True),
     ("bfloat16", [9, 30], 2, 1, 7, False, False),
+    ("bfloat16", [90, 200], 4, 1, 128, True, True),
+    ("bfloat16", [129, 64], 6, 1, 128, False, False),
+    ("bfloat16", [129, 64], 3, 1, 128, True, False),
+    ("bfloat16", [150, 77], 8, 2, 64, False, True),
+    ("bfloat16", [8, 3, 1, 7], 4, 2, 64, True, True),
+    ("bfloat16", [8, 3, 1, 7], 4, 2, 128, True, False),
     ("float32", [1, 0, 2, 5], 4, 2, 64, True, True),
+    ("float32", [20, 21, 3], 4, 2, 64, False, True),
     ("float32", [64, 129, 33], 4, 2, 64, True, True),
     ("float32", [200, 31], 3, 3, 80, False, False),
     ("float32", [140, 65], 2, 1, 128, True, True),
@@ -222,9 +229,11 @@ def test_rectangles_agree_with_attention(dtype, dim):
         within(name, got[name], download(x).reshape(value.shape), 2 * bound)
 
 
-def test_many_short_sequences():
-    lengths = [1, 2, 3, 5, 0, 8] * 100
-    case = ("bfloat16", lengths, 4, 2, 64, True, True)
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [
+    ([1, 2, 3, 5, 0, 8] * 100, 4, 2, 64), ([9, 2, 3, 5, 0, 8] * 100, 4, 1, 64), ([9, 40] * 150, 8, 4, 128),
+    ([65, 2] * 140, 4, 4, 64)])
+def test_many_short_sequences(lengths, heads, kv_heads, dim):
+    case = ("bfloat16", lengths, heads, kv_heads, dim, True, True)
     q, k, v, g = inputs(case, 23)
     got, rest = run(case, q, k, v, g)
     for name, (value, bound) in reference(q, k, v, g, lengths, True, "bfloat16", rest is not None).items():

@@ -124,3 +124,24 @@ def test_labels_of_packed_documents():
             total += n * model.loss([d], [l]).item()
             count += n
     assert abs(loss - total / count) <= 1e-5 * loss
+
+
+def test_checkpoints_keep_the_rotation(tmp_path):
+    """A model whose positions are not the reference's is saved and read back."""
+    from qutai_amd.lm import load_checkpoint, save_checkpoint
+
+    config = Config(**{**SMALL, **VARIANTS["part"]})
+    model = Decoder(config, seed=11)
+    model.loss_packed(DOCUMENTS).backward()
+    save_checkpoint(tmp_path, model)
+    other = Decoder(Config(**config.to_dict()), seed=12)
+    load_checkpoint(tmp_path, other)
+    assert model.loss_packed(DOCUMENTS).item() == other.loss_packed(DOCUMENTS).item()
+    with pytest.raises(ValueError):  # another rotation is another model
+        load_checkpoint(tmp_path, Decoder(Config(**SMALL, qk_norm=True), seed=12))
+
+
+def test_evaluation_records_nothing():
+    model = Decoder(Config(**SMALL), seed=13)
+    loss = model.loss_packed(DOCUMENTS, train=False)
+    assert not loss.requires_grad
