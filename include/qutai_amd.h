@@ -411,9 +411,10 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * to itself).  q, k and v rows start q_row, k_row and v_row elements after the
  * previous token's (columns of wider matrices), heads `dim` elements after each
  * other; out is contiguous [tokens][heads][dim], lse fp32 [tokens][heads].  `tiles`
- * (device, int64 triples) says which rows the workgroups take, `tile_rows` each
- * and in this order: the sequence's first token, its length, and the tile's first
- * row in it, a multiple of tile_rows; tiles cover every row once.  tile_rows is
+ * (device) says which rows the workgroups take, `tile_rows` each and in this order:
+ * tile_count int64 that hold the sequence's first token and, 32 bits up, the tile's
+ * first row in it, a multiple of tile_rows, then tile_count lengths of these
+ * sequences; tiles cover every row once.  tile_rows is
  * what qutai_amd_attention_packed_rows returns for the call's `tokens` (of all
  * `sequences`), `longest` sequence, sizes, scale and pass (0: forward, 1: the backward's query tiles, 2: its key
  * tiles); aligned: every pointer and pitch is a multiple of 16 bytes.  rest (NULL, or
@@ -453,6 +454,12 @@ int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, con
                      int64_t heads, int64_t kv_heads, int64_t dim, int64_t rotary, int64_t q_row, int64_t k_row,
                      int64_t q_out_row, int64_t k_out_row, int half, double magnitude, int inverse, int dtype,
                      void* stream);
+
+/* Places of the tokens of sequences that lie one behind the other: positions[t] = t
+ * less the start of its sequence for t < used (`starts`: rising, the first 0), 0 for
+ * used <= t < total. */
+int qutai_amd_positions(const int64_t* starts, int64_t sequences, int64_t used, int64_t total, int64_t* positions,
+                        void* stream);
 
 /* One AdamW step over `count` tensors.  `tensors` is HOST memory, eight int64 each:
  * addresses of the parameter, its gradient, its first and second moments and its

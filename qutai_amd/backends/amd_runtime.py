@@ -84,6 +84,7 @@ SIGNATURES = {
     "qutai_amd_qk_norm_rope_workspace": [_i64],
     "qutai_amd_rotary": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
                          _f64, _i32, _i32, _p],
+    "qutai_amd_positions": [_p, _i64, _i64, _i64, _p, _p],
     "qutai_amd_adamw": [_p, _i64, _i32, _f64, _f64, _f64, _f64, _f64, _i64, ctypes.c_uint64, _f64, _p, _i64, _p, _p],
     "qutai_amd_adamw_workspace": [_i64, _i64],
     "qutai_amd_adamw_moments": [_p, _p, _p, _p, _p, _i64, _p],

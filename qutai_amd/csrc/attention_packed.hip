@@ -135,6 +135,7 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, con
                   int64_t rows, hipStream_t stream) {
   if (!count) return hipSuccess;
   a.tiles = tiles;
+  a.lengths = tiles + count;
   a.pack = packed_heads(a.heads, a.kv_heads, WAVES);
   const unsigned n = (unsigned)(count * groups_of(pass, dtype, a.heads, a.kv_heads, a.dim, rows));
   if (rows == GEN_WAVES) {

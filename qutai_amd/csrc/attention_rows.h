@@ -39,10 +39,12 @@ struct AttnGenArgs {
 };
 
 // Sequences of different lengths, one behind the other in rows of tokens (b = 0):
-// a workgroup's tile is (start of its sequence, the sequence's length, first row
-// in it), and q, k, v and their gradients may be columns of wider matrices.
+// of a workgroup's tile the tables hold its sequence's start with the tile's first
+// row in it (32 bits up) and the sequence's length, and q, k, v and their gradients may
+// be columns of wider matrices.
 struct AttnPackedArgs : AttnGenArgs {
   const int64_t* tiles;
+  const int64_t* lengths;
   int64_t vt, ot, dqt, dkt, dvt;  // elements from row to row of v, of out and its gradient, and of dq, dk, dv
   void* rest;                     // what out's rounding left, or null
   int pack;                       // query heads of a kv head that share a workgroup
@@ -65,8 +67,8 @@ __device__ __forceinline__ int64_t part_pitch(const AttnPackedArgs& p) { return 
 // The arguments of tile `tile`'s sequence alone; returns the tile's first row in it.
 template <class T>
 __device__ __forceinline__ int enter_sequence(AttnPackedArgs& p, int64_t tile) {
-  const int64_t start = uniform64(p.tiles[3 * tile]);
-  p.time = uniform64(p.tiles[3 * tile + 1]);
+  const int64_t word = uniform64(p.tiles[tile]), start = word & 0xffffffff;
+  p.time = uniform64(p.lengths[tile]);
   const auto at = [&](const void* x, int64_t pitch) { return (const void*)((const T*)x + start * pitch); };
   p.q = at(p.q, p.qt);
   p.k = at(p.k, p.kt);
@@ -81,7 +83,7 @@ __device__ __forceinline__ int enter_sequence(AttnPackedArgs& p, int64_t tile) {
   p.delta += start * p.lt;
   p.part_k += start * part_pitch(p);
   p.part_v += start * part_pitch(p);
-  return uniform32((int)p.tiles[3 * tile + 2]);
+  return (int)(word >> 32);
 }
 
 template <class T> __device__ __forceinline__ float ld(const void* p, int64_t i);

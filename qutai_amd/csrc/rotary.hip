@@ -1,4 +1,5 @@
-// Rotary positions of query and key heads: C ABI `qutai_amd_rotary`.
+// Rotary positions of query and key heads: C ABI `qutai_amd_rotary`, and the places of
+// packed sequences' tokens: `qutai_amd_positions`.
 //
 // Pair i of a head's first R channels is turned by its token's position p times
 // turns[i] whole turns and scaled by `magnitude`:
@@ -154,9 +155,37 @@ hipError_t launch(RotaryArgs& a, bool half, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// A token's place in its sequence, found among the sequences' starts by halving; 0
+// behind the last one.
+__global__ void __launch_bounds__(THREADS) positions_kernel(const int64_t* starts, int64_t sequences, int64_t used,
+                                                            int64_t total, int64_t* positions) {
+  const int64_t t = (int64_t)blockIdx.x * THREADS + threadIdx.x;
+  if (t >= total) return;
+  int64_t lo = 0, hi = sequences;
+  while (hi - lo > 1) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (starts[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  positions[t] = t < used ? t - starts[lo] : 0;
+}
+
 }  // namespace
 
-extern "C" int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, const double* turns,
+extern "C" {
+
+int qutai_amd_positions(const int64_t* starts, int64_t sequences, int64_t used, int64_t total, int64_t* positions,
+                        void* stream) {
+  if (sequences < 0 || used < 0 || used > total || total >= 1ll << 31 || (used && !sequences)) return QA_EINVAL;
+  if (!total) return QA_OK;
+  if (!positions || (used && !starts)) return QA_EINVAL;
+  const unsigned grid = (unsigned)((total + THREADS - 1) / THREADS);
+  hipLaunchKernelGGL(positions_kernel, dim3(grid), dim3(THREADS), 0, (hipStream_t)stream, starts, used ? sequences : 0, used,
+                     total, positions);
+  return (int)hipGetLastError();
+}
+
+int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, const double* turns,
                                 const int64_t* positions, const int64_t* starts, int64_t offset, int64_t batch,
                                 int64_t time, int64_t heads, int64_t kv_heads, int64_t dim, int64_t rotary,
                                 int64_t q_row, int64_t k_row, int64_t q_out_row, int64_t k_out_row, int half,
@@ -211,3 +240,5 @@ extern "C" int qutai_amd_rotary(const void* q, const void* k, void* q_out, void*
   }
   return e == hipErrorInvalidValue ? QA_EINVAL : (int)e;
 }
+
+}  // extern "C"

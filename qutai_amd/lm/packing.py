@@ -3,7 +3,8 @@ tokens: what attention and positions need to keep them apart."""
 from __future__ import annotations
 
 from array import array
-from itertools import accumulate, chain
+from bisect import bisect_right
+from itertools import accumulate
 
 from ..backends import amd
 from ..backends.amd_runtime import get_runtime
@@ -33,9 +34,11 @@ class Packing:
     @property
     def positions(self):
         if self._positions is None:
-            places = array("q", chain.from_iterable(map(range, self.lengths)))
-            places.extend([0] * (self.total - self.used))
-            self._positions = amd.storage(places, dtype="int64")
+            self._positions = positions = amd.AMDStorage(self.total, "int64")
+            if self.total:
+                starts = amd.storage(array("q", self.starts), dtype="int64")
+                positions.runtime.call("qutai_amd_positions", starts.ptr, len(self.starts), self.used, self.total,
+                                       positions.ptr)
         return self._positions
 
     def plan(self, number, heads, kv_heads, dim, dtype, whole, scale, causal):
@@ -50,17 +53,31 @@ class Packing:
         return found
 
     def tiles(self, rows, longest_first):
-        """(storage, count): for every tile of ``rows`` tokens of a sequence its
-        start, its length and the tile's first token in it, as int64 triples (a
-        tile per workgroup of attention).  Tiles that have most to do come first:
+        """(storage, count): the tiles of ``rows`` tokens of a sequence that the
+        workgroups of attention take: an int64 for each that holds the sequence's
+        start and, 32 bits up, the tile's first token in it, then as many of the
+        sequences' lengths.  Tiles that have most to do come first, by whole tiles:
         causal queries see what lies before them (``longest_first`` "end"), causal
         keys are seen by what lies behind ("start"), and without a mask the work
         goes by the length ("length")."""
         key = rows, longest_first
         if key not in self._tiles:
-            tiles = [(n, start, first) for start, n in zip(self.starts, self.lengths) for first in range(0, n, rows)]
-            work = {"end": lambda t: -min(t[2] + rows, t[0]), "start": lambda t: t[2] - t[0], "length": lambda t: -t[0]}
-            tiles.sort(key=work[longest_first])
-            table = array("q", chain.from_iterable((start, n, first) for n, start, first in tiles))
-            self._tiles[key] = amd.storage(table, dtype="int64"), len(tiles)
+            order = sorted((i for i, n in enumerate(self.lengths) if n), key=self.lengths.__getitem__, reverse=True)
+            lengths = array("q", map(self.lengths.__getitem__, order))
+            starts = [self.starts[i] for i in order]
+            words, sizes, shift = [], array("q"), rows << 32
+            if longest_first == "length":
+                for start, n in zip(starts, lengths):
+                    count = -(-n // rows)
+                    words += range(start, start + count * shift, shift)
+                    sizes.extend([n] * count)
+            else:  # the sequences of more than `level` tiles are the first ones
+                if longest_first == "start":  # their tiles counted from the last
+                    starts, shift = [s + (n - 1) // rows * shift for s, n in zip(starts, lengths)], -shift
+                rising = lengths[::-1]
+                for level in range((self.longest - 1) // rows, -1, -1):
+                    many, first = len(lengths) - bisect_right(rising, level * rows), level * shift
+                    words += [s + first for s in starts[:many]]
+                    sizes += lengths[:many]
+            self._tiles[key] = amd.storage(array("q", words) + sizes, dtype="int64"), len(words)
         return self._tiles[key]

@@ -20,16 +20,28 @@ def test_packing_places(monkeypatch):
     monkeypatch.setattr(amd, "storage", lambda values, dtype: list(values))
     packing = Packing([3, 0, 300, 1], total=310)
     assert (packing.starts, packing.used, packing.total, packing.longest) == ((0, 3, 3, 303), 304, 310, 300)
-    assert packing.positions == [0, 1, 2, *range(300), 0] + [0] * 6
-    for rows in (4, 32, 128, 256):
+    lengths_at = {0: 3, 3: 300, 303: 1}
+
+    def tiles(rows, order):
+        table, count = packing.tiles(rows, order)
+        found = [(word & 0xFFFFFFFF, word >> 32, n) for word, n in zip(table[:count], table[count:])]
+        assert len(table) == 2 * count and all(lengths_at[start] == n for start, _, n in found)
+        return found
+
+    for rows in (4, 32, 64, 128, 256):
         for order in ("end", "start", "length"):
-            table, count = packing.tiles(rows, order)
-            triples = [tuple(table[3 * i:3 * i + 3]) for i in range(count)]
-            covered = [start + t for start, n, first in triples for t in range(first, min(first + rows, n))]
-            assert sorted(covered) == list(range(304)) and all(first % rows == 0 for _, _, first in triples)
-    order = [first for _, n, first in [packing.tiles(128, "end")[0][3 * i:3 * i + 3] for i in range(3)]]
-    assert order == [256, 128, 0]
-    assert [packing.tiles(128, "start")[0][3 * i + 2] for i in range(3)] == [0, 128, 256]
+            found = tiles(rows, order)
+            covered = [start + t for start, first, n in found for t in range(first, min(first + rows, n))]
+            assert sorted(covered) == list(range(304)) and all(first % rows == 0 for _, first, _ in found)
+    assert [first for _, first, _ in tiles(128, "end")] == [256, 128, 0, 0, 0]
+    assert [(start, first) for start, first, _ in tiles(128, "start")] == [(3, 0), (3, 128), (3, 256), (0, 0), (303, 0)]
+    assert [start for start, _, _ in tiles(128, "length")] == [3, 3, 3, 0, 303]
+
+
+def test_packing_of_large_starts(monkeypatch):
+    monkeypatch.setattr(amd, "storage", lambda values, dtype: list(values))
+    table, count = Packing([1 << 30, 5]).tiles(1 << 29, "end")
+    assert [(w & 0xFFFFFFFF, w >> 32) for w in table[:count]] == [(0, 1 << 29), (0, 0), (1 << 30, 0)]
 
 
 @pytest.mark.parametrize("lengths,total", [([-1], None), ([1.0], None), ([True], None), ([4], 3), ([1 << 31], None),
@@ -201,6 +213,10 @@ def test_c_entry_points_refuse():
                    dict(kor=15), dict(q=None), dict(ko=None), dict(batch=1 << 30, time=4)):
         assert turn(**change) == EINVAL, change
     assert turn(batch=0) == 0
+
+    for wrong in ((None, 1, 5, 5, p), (p, 0, 5, 5, p), (p, 1, 6, 5, p), (p, 1, -1, 5, p), (p, 1, 5, 1 << 31, p), (p, 1, 5, 5, None)):
+        assert library.qutai_amd_positions(*wrong, None) == EINVAL, wrong
+    assert library.qutai_amd_positions(None, 0, 0, 0, None, None) == 0
 
     def forward(**change):
         a = dict(q=p, k=p, v=p, out=p, lse=p, rest=None, tiles=p, count=2, rows=64, tokens=200, sequences=3, heads=4, kv=2, dim=64, qr=256, kr=128,

@@ -173,3 +173,11 @@ def test_no_tokens():
     turns = Rotary(64)
     empty = amd.AMDStorage(0, "float32")
     assert [x.size for x in amd_lm.rotary(empty, empty, turns, 0, 5, 2, 1, 64)] == [0, 0]
+
+
+@pytest.mark.parametrize("lengths,total", [([1], 1), ([0, 3, 0, 0, 2, 0], 9), ([], 4), ([0, 0], 0), (list(range(130)), None),
+                                           ([70000, 1, 5], 70100)])
+def test_places_of_packed_tokens(lengths, total):
+    packing = Packing(lengths, total)
+    places = [t for n in lengths for t in range(n)]
+    assert packing.positions.tolist() == places + [0] * (packing.total - len(places))
