@@ -34,11 +34,12 @@ class Packing:
     @property
     def positions(self):
         if self._positions is None:
-            self._positions = positions = amd.AMDStorage(self.total, "int64")
+            positions = amd.AMDStorage(self.total, "int64")
             if self.total:
                 starts = amd.storage(array("q", self.starts), dtype="int64")
                 positions.runtime.call("qutai_amd_positions", starts.ptr, len(self.starts), self.used, self.total,
                                        positions.ptr)
+            self._positions = positions
         return self._positions
 
     def plan(self, number, heads, kv_heads, dim, dtype, whole, scale, causal):

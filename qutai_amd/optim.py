@@ -19,7 +19,8 @@ class AdamW:
     for every 256 values, rounded up or down by chance (``seed``: the same run
     gives the same bits).  With ``max_norm`` gradients whose norm over all tensors
     exceeds it are scaled down to it, and a step whose norm is not finite changes
-    nothing; ``norm()`` is the last step's.  ``lr`` may be changed between steps."""
+    nothing (t counts it all the same: nothing is read from the device); ``norm()``
+    is the last step's.  ``lr`` may be changed between steps."""
 
     def __init__(self, parameters, lr=1e-3, *, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, max_norm=None,
                  seed=0):
@@ -27,6 +28,9 @@ class AdamW:
         if not parameters or any(not isinstance(p, Tensor) or p.device != "amd" or p.dtype not in ("float32", "bfloat16")
                                  for p in parameters):
             raise ValueError("AdamW takes float32 or bfloat16 Tensors of the amd device")
+        spans = sorted((p.storage.ptr, p.storage.ptr + p.storage.nbytes) for p in parameters if p.size)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("parameters must not share memory: every value is stepped once")
         if bits not in (8, 32) or type(seed) is not int or not 0 <= seed < 1 << 32:
             raise ValueError("moments have 8 or 32 bits, the seed is an integer below 2^32")
         if len(betas) != 2 or any(not 0 <= b < 1 for b in betas) or not 0 < eps < float("inf"):
@@ -91,4 +95,4 @@ class AdamW:
             for x, values in zip(own.storages(), given):
                 if len(x):
                     x.runtime.upload(x.ptr, array(values.typecode, values))
-        self.steps, self.seed = state["steps"], state["seed"]
+        self.steps, self.seed, self._norm = state["steps"], state["seed"], None

@@ -44,6 +44,25 @@ def test_packing_of_large_starts(monkeypatch):
     assert [(w & 0xFFFFFFFF, w >> 32) for w in table[:count]] == [(0, 1 << 29), (0, 0), (1 << 30, 0)]
 
 
+def test_positions_that_failed_are_made_again(monkeypatch):
+    """Positions whose kernel could not be sent (an upload inside a capture) are not
+    kept as if they were there."""
+    packing, sent = Packing([2, 3]), []
+    block, starts = fake(5, "int64"), fake(2, "int64")
+    block.runtime.call = lambda name, *arguments: sent.append(name)
+    monkeypatch.setattr(amd, "AMDStorage", lambda size, dtype: block)
+
+    def failing(values, dtype):
+        raise RuntimeError("no upload here")
+
+    monkeypatch.setattr(amd, "storage", failing)
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            packing.positions
+    monkeypatch.setattr(amd, "storage", lambda values, dtype: starts)
+    assert packing.positions is block and packing.positions is block and sent == ["qutai_amd_positions"]
+
+
 @pytest.mark.parametrize("lengths,total", [([-1], None), ([1.0], None), ([True], None), ([4], 3), ([1 << 31], None),
                                            ([2], 2.0)])
 def test_packing_refusals(lengths, total):
@@ -173,6 +192,17 @@ def parameter(size=8, dtype="float32"):
 def test_adamw_refusals(change):
     with pytest.raises(ValueError):
         AdamW(**{"parameters": [parameter()], **change})
+
+
+def test_adamw_refuses_parameters_that_share_memory(monkeypatch):
+    monkeypatch.setattr(amd_lm, "AdamWMoments", lambda size, bits: SimpleNamespace(size=size, bits=bits))
+    p, inside, behind = parameter(64), fake(8, "float32"), fake(8, "float32")
+    inside.ptr, behind.ptr = p.storage.ptr + 4 * 60, p.storage.ptr + 4 * 64
+    with pytest.raises(ValueError):
+        AdamW([p, Tensor(p.storage, shape=(64,), requires_grad=True)])
+    with pytest.raises(ValueError):
+        AdamW([Tensor(inside, shape=(8,), requires_grad=True), p])
+    assert len(AdamW([p, Tensor(behind, shape=(8,), requires_grad=True), p]).parameters) == 2  # the same one once
 
 
 def test_adamw_step_refusals(monkeypatch):
