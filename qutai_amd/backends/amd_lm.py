@@ -667,27 +667,29 @@ def attention_backward(gradient, q, k, v, out, lse, batch, time, heads, kv_heads
     return dq, dk, dv
 
 
-def _packed_places(q, k, v, packing, heads, kv_heads, dim, places):
-    """Pointers and pitches of the q, k and v rows of a packed call, which it
-    checks, and whether all of them are whole 16-byte chunks."""
-    if len({q.dtype, k.dtype, v.dtype}) != 1 or q.dtype not in ("bfloat16", "float32"):
+def _packed_places(q, k, v, packing, heads, kv_heads, dim, q_column, q_row, k_column, k_row, v_column, v_row):
+    """Addresses of the first q, k and v rows of a packed call, which it checks, the
+    elements from row to row, and all of them or'd in bytes: whole 16-byte chunks if
+    that is."""
+    dtype = q.dtype
+    if dtype not in ("bfloat16", "float32") or k.dtype != dtype or v.dtype != dtype:
         raise ValueError("attention takes q, k, v of one dtype, bfloat16 or float32")
     if not 0 < dim <= 256 or kv_heads <= 0 or heads <= 0 or heads % kv_heads:
         raise ValueError("attention needs 0 < head dimension <= 256 and heads divisible by kv_heads")
-    sides = ((q, heads, *places[0]), (k, kv_heads, *places[1]), (v, kv_heads, *places[2]))
-    found = [_qk_rows(x, packing.total, n, dim, column, row, q.dtype) for x, n, column, row in sides]
-    item = _TYPES[q.dtype][1]
-    return found, all(at % 16 == 0 and row * item % 16 == 0 for at, row in found) and dim * item % 16 == 0
+    total = packing.total
+    q_at, q_row = _qk_rows(q, total, heads, dim, q_column, q_row, dtype)
+    k_at, k_row = _qk_rows(k, total, kv_heads, dim, k_column, k_row, dtype)
+    v_at, v_row = _qk_rows(v, total, kv_heads, dim, v_column, v_row, dtype)
+    return q_at, k_at, v_at, q_row, k_row, v_row, q_at | k_at | v_at | (q_row | k_row | v_row | dim) * _TYPES[dtype][1]
 
 
 def _packed_tail(packing, *blocks):
     """Zeros in the rows behind the last sequence of contiguous results."""
-    if packing.used < packing.total:
-        for x in blocks:
-            if x is not None:
-                width = x.size // packing.total
-                start = packing.used * width
-                x.runtime.call("qutai_amd_fill", x.ptr + start * _TYPES[x.dtype][1], x.size - start, 0.0, code(x.dtype))
+    for x in blocks:
+        if x is not None:
+            width = x.size // packing.total
+            start = packing.used * width
+            x.runtime.call("qutai_amd_fill", x.ptr + start * _TYPES[x.dtype][1], x.size - start, 0.0, code(x.dtype))
 
 
 def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, scale=None, q_column=0, q_row=None,
@@ -699,20 +701,21 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
     [total][heads][dim], lse [total][heads]; rows behind the last sequence are
     zero.  With ``rest`` also what out's rounding left, for the backward (None
     where there is none)."""
-    ((q_at, q_row), (k_at, k_row), (v_at, v_row)), whole = _packed_places(
-        q, k, v, packing, heads, kv_heads, dim, ((q_column, q_row), (k_column, k_row), (v_column, v_row)))
-    runtime, dtype = get_runtime(), code(q.dtype)
-    out, lse = AMDStorage(packing.total * heads * dim, q.dtype), AMDStorage(packing.total * heads, "float32")
+    q_at, k_at, v_at, q_row, k_row, v_row, odd = _packed_places(q, k, v, packing, heads, kv_heads, dim, q_column, q_row,
+                                                                k_column, k_row, v_column, v_row)
+    name, total = q.dtype, packing.total
+    out, lse, left, dtype = AMDStorage(total * heads * dim, name), AMDStorage(total * heads, "float32"), None, code(name)
     scale = dim ** -0.5 if scale is None else float(scale)
-    left = None
     if packing.used:
-        tiles, count, rows = packing.plan(0, heads, kv_heads, dim, dtype, whole, scale, causal)
-        if rest and rows > 4 and q.dtype == "bfloat16" and dim <= 128:
-            left = AMDStorage(out.size, q.dtype)
-        runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count, rows,
-                     *packing.extent[:2], heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
-                     mfma=_on_matrix_cores(q.dtype, dim))
-    _packed_tail(packing, out, lse, left)
+        tiles, count, rows = packing.plan(0, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal)
+        if rest and rows > 4 and name == "bfloat16" and dim <= 128:
+            left = AMDStorage(out.size, name)
+        tokens, sequences, _ = packing.extent
+        out.runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count,
+                         rows, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
+                         mfma=_on_matrix_cores(name, dim))
+    if packing.used < total:
+        _packed_tail(packing, out, lse, left)
     return (out, lse, left) if rest else (out, lse)
 
 
@@ -724,9 +727,10 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
     with ``into`` (a storage laid out as the one matrix that q, k and v are columns
     of) its columns q_column .., k_column .., v_column ...; every one is summed in
     a fixed order.  Rows behind the last sequence are zero."""
-    places = ((q_column, q_row), (k_column, k_row), (v_column, v_row))
-    ((q_at, q_row), (k_at, k_row), (v_at, v_row)), whole = _packed_places(q, k, v, packing, heads, kv_heads, dim, places)
-    total = packing.total
+    columns = q_column, k_column, v_column
+    q_at, k_at, v_at, q_row, k_row, v_row, odd = _packed_places(q, k, v, packing, heads, kv_heads, dim, q_column, q_row,
+                                                                k_column, k_row, v_column, v_row)
+    total, widths = packing.total, (heads * dim, kv_heads * dim, kv_heads * dim)
     if gradient.dtype != q.dtype or out.dtype != q.dtype or lse.dtype != "float32":
         raise ValueError("attention backward needs gradient/out of the activations' dtype and a float32 lse")
     if gradient.size != total * heads * dim or out.size != gradient.size or lse.size != total * heads:
@@ -734,36 +738,36 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
     if rest is not None and (rest.dtype != q.dtype or rest.size != out.size):
         raise ValueError("rest is what attention_packed returned beside out")
     if into is None:
-        results = tuple(AMDStorage(total * n * dim, q.dtype) for n in (heads, kv_heads, kv_heads))
-        targets = [(x.ptr, n * dim) for x, n in zip(results, (heads, kv_heads, kv_heads))]
+        results = tuple(AMDStorage(total * width, q.dtype) for width in widths)
+        targets, steps = tuple(x.ptr for x in results), widths
     else:
-        row, spans = q_row, sorted((column, column + n * dim) for (column, _), n in zip(places, (heads, kv_heads, kv_heads)))
+        spans = sorted((column, column + width) for column, width in zip(columns, widths))
         if not q_row == k_row == v_row or any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("into holds the gradients in separate columns of one row")
         for x in (gradient, q, k, v, out, *(() if rest is None else (rest,))):
             if into.ptr < x.ptr + x.nbytes and x.ptr < into.ptr + into.nbytes:
                 raise ValueError("into must not share memory with an input")
-        results = (into,) * 3
-        targets = [_qk_rows(into, total, n, dim, column, row, q.dtype)
-                   for (column, _), n in zip(places, (heads, kv_heads, kv_heads))]
-    whole = whole and all(at % 16 == 0 and row * _TYPES[q.dtype][1] % 16 == 0
-                          for at, row in (*targets, (gradient.ptr, 0), (out.ptr, 0)))
-    runtime, dtype = get_runtime(), code(q.dtype)
+        results, steps = (into,) * 3, (q_row,) * 3
+        targets = tuple(_qk_rows(into, total, n, dim, column, q_row, q.dtype)[0]
+                        for column, n in zip(columns, (heads, kv_heads, kv_heads)))
+    for at in (*targets, gradient.ptr, out.ptr):
+        odd |= at
+    dtype = code(q.dtype)
     scale = dim ** -0.5 if scale is None else float(scale)
     if packing.used:
         delta = AMDStorage(total * heads, "float32")
-        (q_tiles, q_count, q_rows), (k_tiles, k_count, k_rows) = (
-            packing.plan(n, heads, kv_heads, dim, dtype, whole, scale, causal) for n in (1, 2))
-        runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
-                     *(at for at, _ in targets), delta.ptr, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count, k_rows,
-                     *packing.extent[:2], heads, kv_heads, dim, q_row, k_row, v_row, *(row for _, row in targets), dtype, scale,
-                     int(bool(causal)), mfma=_on_matrix_cores(q.dtype, dim))
-    if into is None:
-        _packed_tail(packing, *results)
-    elif packing.used < total:
-        tail = total - packing.used
-        for (at, row), n in zip(targets, (heads, kv_heads, kv_heads)):
-            _zero_columns(into, at, tail, packing.used, row, n * dim)
+        query_tiles, key_tiles = (packing.plan(n, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal) for n in (1, 2))
+        tokens, sequences, _ = packing.extent
+        delta.runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
+                           *targets, delta.ptr, query_tiles[0].ptr, *query_tiles[1:], key_tiles[0].ptr, *key_tiles[1:], tokens,
+                           sequences, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),
+                           mfma=_on_matrix_cores(q.dtype, dim))
+    if packing.used < total:
+        if into is None:
+            _packed_tail(packing, *results)
+        else:
+            for at, width in zip(targets, widths):
+                _zero_columns(into, at, total - packing.used, packing.used, q_row, width)
     return results
 
 
@@ -1060,24 +1064,23 @@ def rotary(q, k, rotary, batch, time, heads, kv_heads, dim, *, positions=None, o
     dtype = (q if heads else k).dtype
     if dtype not in ("bfloat16", "float32"):
         raise ValueError("rotary takes bfloat16 or float32 rows")
-    sides = ((q, heads, q_column, q_row, out_q_column),
-             (k, kv_heads, k_column, k_row, heads * dim if out_k_column is None else out_k_column))
-    sources = [_qk_rows(x, tokens, n, dim, column, row, dtype) for x, n, column, row, _ in sides]
-    if out is not None:
-        targets = [_qk_rows(out, tokens, n, dim, column, out_row, dtype) for _, n, _, _, column in sides]
-        for (x, n, *_), source, target in zip(sides, sources, targets):
+    q_at, q_step = _qk_rows(q, tokens, heads, dim, q_column, q_row, dtype)
+    k_at, k_step = _qk_rows(k, tokens, kv_heads, dim, k_column, k_row, dtype)
+    if out is None:
+        q_out, k_out = heads * dim, kv_heads * dim
+        results = (AMDStorage(tokens * q_out, dtype) if heads else None, AMDStorage(tokens * k_out, dtype) if kv_heads else None)
+        q_to, k_to = amd._p(results[0]), amd._p(results[1])
+    else:
+        q_to, q_out = _qk_rows(out, tokens, heads, dim, out_q_column, out_row, dtype)
+        k_to, k_out = _qk_rows(out, tokens, kv_heads, dim, heads * dim if out_k_column is None else out_k_column, out_row, dtype)
+        for x, n, source, target in ((q, heads, (q_at, q_step), (q_to, q_out)), (k, kv_heads, (k_at, k_step), (k_to, k_out))):
             if n and source != target and out.ptr < x.ptr + x.nbytes and x.ptr < out.ptr + out.nbytes:
                 raise ValueError("out shares memory with an input that is not in its place")
-        (q_to, q_out), (k_to, k_out) = targets
         item = _TYPES[dtype][1]
         if heads and kv_heads and (q_out != k_out or not (q_to + heads * dim * item <= k_to
                                                           or k_to + kv_heads * dim * item <= q_to)):
             raise ValueError("out holds q's and k's results in separate columns of one row")
-        results = tuple(out if n else None for n in (heads, kv_heads))
-    else:
-        results = tuple(AMDStorage(tokens * n * dim, dtype) if n else None for n in (heads, kv_heads))
-        (q_to, q_out), (k_to, k_out) = ((amd._p(x), n * dim) for x, n in zip(results, (heads, kv_heads)))
-    (q_at, q_step), (k_at, k_step) = sources
+        results = out if heads else None, out if kv_heads else None
     if tokens:
         get_runtime().call("qutai_amd_rotary", q_at, k_at, q_to, k_to, rotary.turns, amd._p(positions), amd._p(starts),
                            offset, batch, time, heads, kv_heads, dim, rotary.rotary_dim, q_step, k_step, q_out, k_out,
