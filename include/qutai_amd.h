@@ -406,39 +406,45 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
                             double scale, int causal, void* stream);
 
 /* Attention among the tokens of each of several sequences of different lengths
- * that lie one behind the other in one matrix of tokens, as
+ * that lie one behind the other in one matrix of tokens, the first from row 0 on, as
  * qutai_amd_attention_fwd of each alone (causal != 0: a token sees its sequence up
  * to itself).  q, k and v rows start q_row, k_row and v_row elements after the
  * previous token's (columns of wider matrices), heads `dim` elements after each
  * other; out is contiguous [tokens][heads][dim], lse fp32 [tokens][heads].  `tiles`
- * (device) says which rows the workgroups take, `tile_rows` each and in this order:
+ * (device) says which rows the workgroups take, tile_rows each and in this order:
  * tile_count int64 that hold the sequence's first token and, 32 bits up, the tile's
  * first row in it, a multiple of tile_rows, then tile_count lengths of these
- * sequences; tiles cover every row once.  tile_rows is
- * what qutai_amd_attention_packed_rows returns for the call's `tokens` (of all
- * `sequences`), `longest` sequence, sizes, scale and pass (0: forward, 1: the backward's query tiles, 2: its key
- * tiles); aligned: every pointer and pitch is a multiple of 16 bytes.  rest (NULL, or
- * bf16 laid out as out; bf16 with dim up to 128 and tile_rows above 4) receives what
- * out's rounding left, for the backward.  Rows in no tile are left as they are.
- * dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up to 128 rounds probabilities and dS
- * to bf16 for their products, the others keep fp32's bits. */
-int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads,
-                                        int64_t dim, int dtype, int aligned, double scale, int pass);
+ * sequences; tiles cover every row once.  tile_rows is what
+ * qutai_amd_attention_packed_rows returns for the `tokens` of all `sequences`, the
+ * `longest` of them, the call's sizes and scale and its pass (0: forward, 1: the
+ * backward's query tiles, 2: its key tiles); aligned: every pointer and pitch is a
+ * multiple of 16 bytes.  rest (NULL, or bf16 laid out as out; bf16 with dim up to 128
+ * and tile_rows above 4) receives what out's rounding left, for the backward.  Rows
+ * in no tile are left as they are.  dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up
+ * to 128 rounds probabilities and dS to bf16 for their products, the others keep
+ * fp32's bits. */
+int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads,
+                                        int64_t kv_heads, int64_t dim, int dtype, int aligned, double scale, int pass);
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
-                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens, int64_t sequences,
-                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
-                                   double scale, int causal, void* stream);
+                                   const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens,
+                                   int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row,
+                                   int64_t k_row, int64_t v_row, int dtype, double scale, int causal, void* stream);
 /* Its gradients: grad is that of out (contiguous), out, lse and rest (or NULL) the
- * forward's; dq,
- * dk and dv rows start dq_row, dk_row and dv_row elements after each other; delta
- * is scratch, fp32 [tokens][heads].  Every gradient is summed in a fixed order. */
+ * forward's; dq, dk and dv rows start dq_row, dk_row and dv_row elements after each
+ * other; delta is scratch, fp32 [tokens][heads].  With a workspace (16-byte aligned)
+ * of at least qutai_amd_attention_packed_workspace bytes (0: none is used) the query
+ * heads of a kv head are worked on side by side where there are few key tiles.  Every
+ * gradient is summed in a fixed order. */
+size_t qutai_amd_attention_packed_workspace(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads,
+                                            int64_t dim, int dtype, int64_t key_rows);
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                    const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
-                                   const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
-                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
-                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
-                                   int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
-                                   void* stream);
+                                   void* workspace, size_t workspace_bytes, const int64_t* query_tiles,
+                                   int64_t query_count, int64_t query_rows, const int64_t* key_tiles,
+                                   int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
+                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
+                                   int64_t v_row, int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype,
+                                   double scale, int causal, void* stream);
 
 /* The first `rotary` channels (even) of every query and key head turned by their
  * token's position: pair i (channels 2i and 2i+1, or with half != 0 i and i +

@@ -707,7 +707,7 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
     out, lse, left, dtype = AMDStorage(total * heads * dim, name), AMDStorage(total * heads, "float32"), None, code(name)
     scale = dim ** -0.5 if scale is None else float(scale)
     if packing.used:
-        tiles, count, rows = packing.plan(0, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal)
+        tiles, count, rows, _ = packing.plan(0, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal)
         if rest and rows > 4 and name == "bfloat16" and dim <= 128:
             left = AMDStorage(out.size, name)
         tokens, sequences, _ = packing.extent
@@ -756,11 +756,13 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
     scale = dim ** -0.5 if scale is None else float(scale)
     if packing.used:
         delta = AMDStorage(total * heads, "float32")
-        query_tiles, key_tiles = (packing.plan(n, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal) for n in (1, 2))
+        (q_tiles, q_count, q_rows, _), (k_tiles, k_count, k_rows, need) = (
+            packing.plan(n, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal) for n in (1, 2))
+        workspace = AMDStorage(need // 4, "float32") if need else None
         tokens, sequences, _ = packing.extent
         delta.runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
-                           *targets, delta.ptr, query_tiles[0].ptr, *query_tiles[1:], key_tiles[0].ptr, *key_tiles[1:], tokens,
-                           sequences, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),
+                           *targets, delta.ptr, amd._p(workspace), need, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count,
+                           k_rows, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),
                            mfma=_on_matrix_cores(q.dtype, dim))
     if packing.used < total:
         if into is None:

@@ -95,8 +95,9 @@ SIGNATURES = {
     "qutai_amd_attention_packed_rows": [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _f64, _i32],
     "qutai_amd_attention_packed_fwd": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f64,
                                        _i32, _p],
-    "qutai_amd_attention_packed_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64,
-                                       _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f64, _i32, _p],
+    "qutai_amd_attention_packed_workspace": [_i64, _i64, _i64, _i64, _i64, _i32, _i64],
+    "qutai_amd_attention_packed_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _i64, _i64, _p, _i64, _i64, _i64,
+                                       _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f64, _i32, _p],
     "qutai_amd_attention_cached": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _f64, _p],
     "qutai_amd_sample": [_p, _p, _p, _p, _i64, _i64, _p, _f64, _p, _i64, _p, _f64, _p, _f64, _i32, _i32, _p],
     "qutai_amd_cache_quantize": [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32,
@@ -124,6 +125,7 @@ SIGNATURES = {
     "qutai_amd_gemm_static_capacity": [],
 }
 RESTYPES = {"qutai_amd_cache_pitch": _i64, "qutai_amd_adamw_workspace": _i64, "qutai_amd_attention_packed_rows": _i64,
+             "qutai_amd_attention_packed_workspace": _sz,
              "qutai_amd_attention_quantized_workspace_size": _sz,
             "qutai_amd_gemm_workspace_size": _sz, "qutai_amd_qk_norm_rope_workspace": _i64, "qutai_amd_rms_norm_workspace": _i64,
             "qutai_amd_attention_bwd_workspace_size": _sz, "qutai_amd_reduce_sum_workspace_size": _sz,

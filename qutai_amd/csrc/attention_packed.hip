@@ -1,6 +1,6 @@
 // Attention of sequences of different lengths that lie one behind the other in
 // one matrix of tokens: C ABI `qutai_amd_attention_packed_fwd`, `_bwd`, `_rows`,
-// `_bwd_workspace_size`.
+// `_workspace`.
 //
 //   forward:  S = scale Q K^T over a sequence's own (causal: no later) keys,
 //             O = softmax(S) V, lse = log sum exp S
@@ -124,6 +124,34 @@ int64_t groups_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t
   return rows != GEN_WAVES && packed_fits(dtype, dim) ? heads / packed_heads(heads, kv_heads, WAVES) : heads;
 }
 
+// Query heads of a group that take workgroups of their own in the key pass of
+// attention_mma.h's kernels, whose partial sums a kernel of its own adds up: all of
+// them with fewer workgroups than the GPU holds at once (two for a CU), else 1.  us,
+// side by side (with the sum) and one after the other: fp32, one sequence of 4000, 8
+// heads over 2 of 64, 412 and 1530; 4000 tokens of up to 1000, 16 over 4 of 64, 126 and
+// 400, 8000 with heads of 32, 96 and 238; bf16 of 256, 564 and 1134; with half as many
+// tiles again as the bound, 16384 of up to 1024, 16 over 4 of 64, 414 and 440, 8 over 4
+// of 96, 304 and 308, and with three times as many, 16 over 8 of 64, 424 and 375.
+int64_t heads_apart(int dtype, int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t rows) {
+  if (rows == GEN_WAVES || packed_fits(dtype, dim)) return 1;
+  return (tokens / MMA_ROWS + std::min(sequences, tokens)) * kv_heads < 2 * cu_count() ? heads / kv_heads : 1;
+}
+
+// dK = scale * sum_g part_k[g], dV = sum_g part_v[g] (g in order) of 4 channels a lane.
+template <class T>
+__global__ void __launch_bounds__(256) packed_dkv_sum(AttnPackedArgs p, int64_t tokens, int group) {
+  constexpr bool F32 = sizeof(T) == 4;
+  const int64_t chunks = p.kv_heads * p.dim / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x, t = i / chunks, at = i % chunks * 4;
+  if (t >= tokens) return;
+  f32x4 sk = global_load<f32x4>(p.part_k + 4 * i), sv = global_load<f32x4>(p.part_v + 4 * i);
+  for (int g = 1; g < group; g++) {
+    sk += global_load<f32x4>(p.part_k + g * p.part_stride + 4 * i);
+    sv += global_load<f32x4>(p.part_v + g * p.part_stride + 4 * i);
+  }
+  put4<F32>(p.dk, t * p.dkt + at, sk * p.scale);
+  put4<F32>(p.dv, t * p.dvt + at, sv);
+}
+
 // Rows of a tile of the matrix kernels.
 int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim, int64_t key_tiles) {
   if (!packed_fits(dtype, dim)) return MMA_ROWS;
@@ -137,7 +165,8 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, con
   a.tiles = tiles;
   a.lengths = tiles + count;
   a.pack = packed_heads(a.heads, a.kv_heads, WAVES);
-  const unsigned n = (unsigned)(count * groups_of(pass, dtype, a.heads, a.kv_heads, a.dim, rows));
+  const int64_t apart = pass == KEYS && a.split ? a.heads / a.kv_heads : 1;
+  const unsigned n = (unsigned)(count * groups_of(pass, dtype, a.heads, a.kv_heads, a.dim, rows) * apart);
   if (rows == GEN_WAVES) {
     if (dtype == BF16) launch_rows<bf16_t>(pass, a, n, stream);
     else launch_rows<float>(pass, a, n, stream);
@@ -215,6 +244,15 @@ int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64
   return rows_of((Pass)pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences));
 }
 
+size_t qutai_amd_attention_packed_workspace(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
+                                            int dtype, int64_t key_rows) {
+  if ((dtype != BF16 && dtype != F32) || dim <= 0 || dim > 256 || heads <= 0 || kv_heads <= 0 || heads % kv_heads ||
+      heads > 1 << 16 || tokens < 0 || tokens >= 1ll << 31 || sequences < 0)
+    return 0;
+  const int64_t apart = heads_apart(dtype, tokens, sequences, heads, kv_heads, dim, key_rows);
+  return apart == 1 ? 0 : (size_t)(2 * apart * tokens * kv_heads * dim) * sizeof(float);
+}
+
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
                                    const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens, int64_t sequences,
                                    int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
@@ -239,7 +277,7 @@ int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, 
 
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                    const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
-                                   const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
+                                   void* workspace, size_t workspace_bytes, const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
                                    const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
                                    int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
                                    int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
@@ -250,7 +288,7 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
   if (status != QA_OK) return status;
   if (dq_row < heads * dim || dk_row < kv_heads * dim || dv_row < kv_heads * dim) return QA_EINVAL;
   if (std::max({dq_row, dk_row, dv_row}) > 1 << 22) return QA_EINVAL;
-  if (!grid_fits(query_count, heads) || !grid_fits(key_count, kv_heads)) return QA_EINVAL;
+  if (!grid_fits(query_count, heads) || !grid_fits(key_count, heads)) return QA_EINVAL;
   if (!query_count && !key_count) return QA_OK;
   if (!grad || !q || !k || !v || !out || !dq || !dk || !dv || !lse || !delta || !query_tiles || !key_tiles)
     return QA_EINVAL;
@@ -271,10 +309,23 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
   a.dqt = dq_row;
   a.dkt = dk_row;
   a.dvt = dv_row;
+  const int64_t group = heads / kv_heads;
+  const size_t need = qutai_amd_attention_packed_workspace(tokens, sequences, heads, kv_heads, dim, dtype, key_rows);
+  if (need && workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0) {
+    a.split = 1;
+    a.part_stride = tokens * kv_heads * dim;
+    a.part_k = (float*)workspace;
+    a.part_v = a.part_k + group * a.part_stride;
+  }
   // the query pass writes delta, which the key pass reads
-  const hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), query_tiles, query_count, query_rows, (hipStream_t)stream);
+  hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), query_tiles, query_count, query_rows, (hipStream_t)stream);
   if (e != hipSuccess) return (int)e;
-  return (int)launch(KEYS, dtype, a, key_tiles_of(tokens, sequences), key_tiles, key_count, key_rows, (hipStream_t)stream);
+  e = launch(KEYS, dtype, a, key_tiles_of(tokens, sequences), key_tiles, key_count, key_rows, (hipStream_t)stream);
+  if (e != hipSuccess || !a.split || !key_count) return (int)e;
+  const dim3 grid((unsigned)((a.part_stride / 4 + 255) / 256));
+  if (dtype == BF16) hipLaunchKernelGGL(packed_dkv_sum<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, a, tokens, (int)group);
+  else hipLaunchKernelGGL(packed_dkv_sum<float>, grid, dim3(256), 0, (hipStream_t)stream, a, tokens, (int)group);
+  return (int)hipGetLastError();
 }
 
 }  // extern "C"

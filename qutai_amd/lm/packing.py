@@ -43,14 +43,17 @@ class Packing:
         return self._positions
 
     def plan(self, number, heads, kv_heads, dim, dtype, whole, scale, causal):
-        """(tiles, count, rows of a tile) of pass ``number`` of attention (forward,
-        queries of the backward, its keys) of these sizes; asked of the library once."""
+        """(tiles, count, rows of a tile, bytes of workspace) of pass ``number`` of
+        attention (forward, queries of the backward, its keys) of these sizes; asked of
+        the library once."""
         key = number, heads, kv_heads, dim, dtype, whole, scale, bool(causal)
         found = self._plans.get(key)
         if found is None:
-            rows = get_runtime().lib.qutai_amd_attention_packed_rows(*self.extent, heads, kv_heads, dim, dtype, int(whole),
-                                                                     scale, number)
-            found = self._plans[key] = (*self.tiles(rows, "length" if not causal else "start" if number == 2 else "end"), rows)
+            lib, sizes = get_runtime().lib, (heads, kv_heads, dim, dtype)
+            rows = lib.qutai_amd_attention_packed_rows(*self.extent, *sizes, int(whole), scale, number)
+            need = lib.qutai_amd_attention_packed_workspace(*self.extent[:2], *sizes, rows) if number == 2 else 0
+            found = (*self.tiles(rows, "length" if not causal else "start" if number == 2 else "end"), rows, need)
+            self._plans[key] = found
         return found
 
     def tiles(self, rows, longest_first):

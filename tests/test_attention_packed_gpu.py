@@ -277,3 +277,29 @@ def test_gradients_against_differences():
         slope = (value(ahead) - value(behind)) / 2
         # third derivatives of a softmax of scores of order 1 times 1e-6 a step, and fp32's sums of 18 * 32 values
         assert abs(slope - grads[which] @ step.reshape(-1)) <= 2e-4 * (np.abs(grads[which]) @ np.abs(step).reshape(-1)) + 1e-5
+
+
+@pytest.mark.parametrize("apart,dtype,lengths,heads,kv_heads,dim", [
+    (True, "float32", [330, 0, 41], 8, 1, 64), (True, "float32", [130, 129], 6, 2, 128), (True, "bfloat16", [200, 30], 4, 1, 136),
+    (False, "float32", [330, 41], 2, 2, 64), (False, "float32", [21 + i % 9 for i in range(70)], 16, 8, 32),
+    (False, "bfloat16", [21 + i % 9 for i in range(70)], 16, 8, 136)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_heads_of_a_group_side_by_side(apart, dtype, lengths, heads, kv_heads, dim, causal):
+    """The key pass of few tiles, whose heads' sums are added up by a kernel of their own,
+    and of many; the rows behind the sequences stay zero, the same sums come every time."""
+    runtime = amd.get_runtime()
+    packing = Packing(lengths)
+    need = packing.plan(2, heads, kv_heads, dim, amd.code(dtype), True, dim ** -0.5, causal)[3]
+    assert bool(need) == apart and need % (8 * packing.total * dim) == 0
+    case = dtype, lengths, heads, kv_heads, dim, causal, True
+    q, k, v, g = inputs(case, 31)
+    behind = [np.concatenate([x, np.full((3, *x.shape[1:]), 5.0)]) for x in (q, k, v, g)]
+    result, rest = run(case, *behind)
+    expected = reference(q, k, v, g, lengths, causal, dtype, rest is not None)
+    for name, (value, bound) in expected.items():
+        got = result[name].reshape(len(behind[0]), *value.shape[1:])
+        within(name, got[:-3], value, bound)
+        assert not got[-3:].any()
+    again, _ = run(case, *behind)
+    assert all(np.array_equal(result[name], again[name]) for name in result)
+    assert runtime.lib.qutai_amd_attention_packed_workspace(*packing.extent[:2], heads, kv_heads, dim, amd.code(dtype), 4) == 0

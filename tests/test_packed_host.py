@@ -11,7 +11,7 @@ from qutai_amd.backends import amd, amd_lm, amd_runtime
 from qutai_amd.lm import Config, Packing, Rotary
 from qutai_amd.lm.layers import attention, rotary
 from qutai_amd.optim import AdamW
-from tests.test_operators_host import built, fake
+from tests.test_operators_host import LIBRARY, built, fake
 
 EINVAL, EWORKSPACE = amd_runtime.QA_EINVAL, amd_runtime.QA_EWORKSPACE
 
@@ -287,3 +287,20 @@ def test_c_entry_points_refuse():
     assert library.qutai_amd_adamw_workspace(-1, 8) == 0 and library.qutai_amd_adamw_workspace(49, 8) == 2048
     assert library.qutai_amd_adamw_moments(p, p, None, p, p, 8, None) == EINVAL
     assert library.qutai_amd_adamw_moments(p, p, p, p, p, -1, None) == EINVAL
+
+
+@built
+def test_workspace_of_the_key_pass():
+    """Asked for where a group's heads work side by side: fp32 or wide bf16 heads that
+    share keys, few key tiles; nothing for sizes that are none."""
+    import ctypes
+
+    library = ctypes.CDLL(str(LIBRARY))
+    ask = library.qutai_amd_attention_packed_workspace
+    ask.restype, ask.argtypes = ctypes.c_size_t, amd_runtime.SIGNATURES["qutai_amd_attention_packed_workspace"]
+    assert ask(1000, 3, 8, 2, 64, 0, 128) == 2 * 4 * 1000 * 2 * 64 * 4 and ask(1000, 3, 4, 1, 136, 5, 128) == 2 * 4 * 1000 * 136 * 4
+    for sizes in ((1000, 3, 8, 8, 64, 0, 128), (1000, 3, 8, 2, 64, 5, 64), (1000, 3, 8, 2, 64, 0, 4), (1 << 20, 3, 8, 2, 64, 0, 128),
+                  (100000, 90000, 8, 2, 64, 0, 128), (0, 0, 8, 2, 64, 0, 128), (-1, 3, 8, 2, 64, 0, 128), (1000, -3, 8, 2, 64, 0, 128),
+                  (1000, 3, 8, 3, 64, 0, 128), (1000, 3, 0, 2, 64, 0, 128), (1000, 3, 8, 0, 64, 0, 128), (1000, 3, 8, 2, 0, 0, 128),
+                  (1000, 3, 8, 2, 264, 0, 128), (1000, 3, 8, 2, 64, 4, 128)):
+        assert ask(*sizes) == 0, sizes
