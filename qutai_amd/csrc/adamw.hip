@@ -1,4 +1,4 @@
-// One AdamW step over many tensors: C ABI `qutai_amd_adamw`, `_norm`, `_moments`.
+// One AdamW step over many tensors: C ABI `qutai_amd_adamw`, `_workspace`, `_moments`.
 //
 //   g' = g min(1, max_norm / norm)
 //   m' = b1 m + (1 - b1) g',  v' = b2 v + (1 - b2) g'^2
@@ -17,10 +17,18 @@
 // change in one step is far below a code's follows them: rounded to nearest, b2 =
 // 0.999 would never let a second moment fall.  A positive second moment keeps the
 // least code, so a step is never divided by a root that rounding made 0.  Moments
-// of 8 bits are computed in 64 (memory bounds the step all the same), so that the
-// codes are those of the definition whatever the order of operations.
+// are computed in 64 bits, so that codes are those of the definition whatever the order
+// of operations, and fp32's are rounded once.
 //
-// A block with an infinity or NaN has the exponent 127 and reads as NaN.
+// A block with an infinity, a NaN or a moment of 2^127 or more has the exponent 127 and
+// reads as NaN.
+//
+// One launch steps 48 tensors, whose records are its arguments: a workgroup takes 1024 or
+// 4096 values of one of them at a time, with 8 bits a wave a block.  Memory bounds it
+// where parameters are fp32 (61 million values in 20 tensors: 32-bit moments 290 us for 1.7
+// GB, 5.9 TB/s; 8 bits 205 for 973 MB, 4.7 TB/s, and 36 for the norm of 243 MB); 5 million
+// bf16 values in 17 tensors with moments of 8 bits take 17.5 us for 50 MB, bound by about
+// 90 vector instructions a value, an eighth of them in 64 bits.
 #include "common.h"
 #include "qutai_amd.h"
 
@@ -31,12 +39,21 @@ using namespace qa;
 namespace {
 
 constexpr int THREADS = 256, BLOCK = 256;     // BLOCK: values that share an exponent
-constexpr int CHUNK = 4096;                   // values of a workgroup's turn
-constexpr int TURNS = CHUNK / (4 * THREADS);  // a thread takes 4 values, and 4 more a thousand on
-constexpr int TENSORS = 48;                   // of a launch: their records fit the kernel's arguments
-constexpr int GROUPS = 2048;                  // workgroups of a launch at most: eight for a CU
+constexpr int NORM_CHUNK = 4096;              // values of a workgroup's turn of the norm
 constexpr int NORM_GROUPS = 1024;             // partial sums of a launch
+constexpr int TENSORS = 48;                   // of a launch: their records fit the kernel's arguments
 constexpr int NOT_FINITE = 127;
+
+// Values of a workgroup's turn of the step, and workgroups of a launch at most.  Moments
+// of 8 bits: a block for each wave.  fp32 moments: four loads of every array in flight
+// where there are turns enough for the GPU, shorter turns of more workgroups else.  us with
+// turns of 1024, 2048 and 4096: 61 million values, 8 bits 203, 205 and 225, fp32 351, 323
+// and 310; 15 million, fp32, 78 and 75 (1024, 4096), 4 million 17.9 and 18.9, 1 million 5.3
+// and 8.8; 5 million bf16 values, 8 bits, 17.6, 18.0 and 20.6.  With 16384 workgroups
+// instead of 2048 the 61 million take 290 instead of 309 (fp32) and 217 instead of 207.
+// (The norm: 53, 38 and 36.)
+constexpr int SHORT_CHUNK = 1024, LONG_CHUNK = 4096, SHORT_GROUPS = 2048, LONG_GROUPS = 16384;
+constexpr int64_t LONG_FROM = 1ll << 23;  // values of all tensors
 
 struct Tensor {
   void* p;
@@ -54,7 +71,7 @@ struct StepArgs {
   int n;
   uint32_t chunks;
   double b1, b1_rest, b2, b2_rest;
-  float keep, rate, root, eps;  // 1 - lr decay, lr / c1, 1 / sqrt(c2)
+  float decay, rate, root, eps;  // lr times the decay, lr / c1, 1 / sqrt(c2)
   const double* partial;        // sums of squares, or null
   int partials;
   double max_norm;
@@ -151,6 +168,7 @@ __device__ __forceinline__ double group_sum(double x, double* shared) {
 
 template <class T>
 __device__ __forceinline__ void square_sum(const Tensor& t, int64_t start, int64_t end, double& sum) {
+  constexpr int TURNS = NORM_CHUNK / (4 * THREADS);  // a thread takes 4 values, and 4 more a thousand on
   f32x4 g[TURNS];
   const int64_t i = start + 4 * threadIdx.x;
 #pragma unroll
@@ -170,7 +188,7 @@ __global__ void __launch_bounds__(THREADS) adamw_norm(NormArgs a) {
   const uint32_t starts = starts_of(a);
   for (uint32_t c = blockIdx.x; c < a.chunks; c += gridDim.x) {
     const Tensor& t = a.t[tensor_of(starts, c)];
-    const int64_t start = (int64_t)(c - t.chunks) * CHUNK, end = min(t.count, start + CHUNK);
+    const int64_t start = (int64_t)(c - t.chunks) * NORM_CHUNK, end = min(t.count, start + NORM_CHUNK);
     if (t.bf16) square_sum<bf16_t>(t, start, end, sum);
     else square_sum<float>(t, start, end, sum);
   }
@@ -279,7 +297,7 @@ struct Block8 {
       codes2 |= max(coded(v1[j], E2 - 30, bits >> 16), v1[j] > 0.0 ? 1u : 0u) << 8 * j;
       // the hardware's fp64 root holds fp32's bits for every value that fp64 holds
       const float root = (float)__builtin_amdgcn_sqrt(v1[j]);
-      p1[j] = fmaf(p[j], a.keep, -a.rate * (float)m1[j] * __builtin_amdgcn_rcpf(fmaf(root, a.root, a.eps)));
+      p1[j] = p[j] + fmaf(-a.decay, p[j], -a.rate * (float)m1[j] * __builtin_amdgcn_rcpf(fmaf(root, a.root, a.eps)));
     }
     if (E1 == NOT_FINITE) codes1 = 0;
     if (E2 == NOT_FINITE) codes2 = 0;
@@ -293,7 +311,7 @@ struct Block8 {
   }
 };
 
-template <class T>
+template <class T, int CHUNK>
 __device__ __forceinline__ void step8(const StepArgs& a, const Tensor& t, int64_t start, int64_t end, double factor) {
   const int lane = threadIdx.x & 63, wave = uniform32(threadIdx.x >> 6);
   constexpr int N = CHUNK / BLOCK / (THREADS / 64);  // blocks of a wave, whose loads go out together
@@ -304,10 +322,10 @@ __device__ __forceinline__ void step8(const StepArgs& a, const Tensor& t, int64_
   for (int u = 0; u < N; u++) b[u].step(a, t, start + (u * (THREADS / 64) + wave) * BLOCK, end, lane, factor);
 }
 
-template <class T>
+template <class T, int CHUNK>
 __device__ __forceinline__ void step32(const StepArgs& a, const Tensor& t, int64_t start, int64_t end, double factor) {
 #pragma clang fp contract(off)
-  const float f = (float)factor, b1 = (float)a.b1, r1 = (float)a.b1_rest, b2 = (float)a.b2, r2 = (float)a.b2_rest;
+  constexpr int TURNS = CHUNK / (4 * THREADS);
   f32x4 g[TURNS], p[TURNS], m[TURNS], v[TURNS];
 #pragma unroll
   for (int u = 0; u < TURNS; u++) {
@@ -324,10 +342,11 @@ __device__ __forceinline__ void step32(const StepArgs& a, const Tensor& t, int64
     const bool whole = t.whole && i + 4 <= end;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float gj = g[u][j] * f;
-      m[u][j] = b1 * m[u][j] + r1 * gj;
-      v[u][j] = b2 * v[u][j] + r2 * (gj * gj);
-      p[u][j] = p[u][j] * a.keep - a.rate * (m[u][j] / (sqrtf(v[u][j]) * a.root + a.eps));
+      // memory bounds the step: moments in 64 bits, rounded once
+      const double gj = (double)g[u][j] * factor;
+      m[u][j] = (float)fma(a.b1, (double)m[u][j], a.b1_rest * gj);
+      v[u][j] = (float)fma(a.b2, (double)v[u][j], a.b2_rest * (gj * gj));
+      p[u][j] += fmaf(-a.decay, p[u][j], -a.rate * (m[u][j] / fmaf(sqrtf(v[u][j]), a.root, a.eps)));
     }
     put4<float>(t.m, i, end, whole, m[u]);
     put4<float>(t.v, i, end, whole, v[u]);
@@ -335,7 +354,7 @@ __device__ __forceinline__ void step32(const StepArgs& a, const Tensor& t, int64
   }
 }
 
-template <bool EIGHT>
+template <bool EIGHT, int CHUNK>
 __global__ void __launch_bounds__(THREADS) adamw_step(StepArgs a) {
   __shared__ double shared[4];
   const uint32_t starts = starts_of(a);
@@ -352,11 +371,11 @@ __global__ void __launch_bounds__(THREADS) adamw_step(StepArgs a) {
     const Tensor& t = a.t[tensor_of(starts, c)];
     const int64_t start = (int64_t)(c - t.chunks) * CHUNK, end = min(t.count, start + CHUNK);
     if constexpr (EIGHT) {
-      if (t.bf16) step8<bf16_t>(a, t, start, end, factor);
-      else step8<float>(a, t, start, end, factor);
+      if (t.bf16) step8<bf16_t, CHUNK>(a, t, start, end, factor);
+      else step8<float, CHUNK>(a, t, start, end, factor);
     } else {
-      if (t.bf16) step32<bf16_t>(a, t, start, end, factor);
-      else step32<float>(a, t, start, end, factor);
+      if (t.bf16) step32<bf16_t, CHUNK>(a, t, start, end, factor);
+      else step32<float, CHUNK>(a, t, start, end, factor);
     }
   }
 }
@@ -371,17 +390,17 @@ __global__ void __launch_bounds__(THREADS) adamw_moments(const uint8_t* m, const
   }
 }
 
-// Records of up to TENSORS tensors from `first` on; returns how many tensors they
-// took (those without values among them).
+// Records of up to TENSORS tensors from `first` on, in turns of `chunk` values; returns
+// how many tensors they took (those without values among them).
 template <class Args>
-int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, uint32_t key) {
+int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, uint32_t key, int64_t chunk) {
   a.n = 0;
   a.chunks = 0;
   int64_t i = first;
   for (; i < count && a.n < TENSORS; i++) {
     const int64_t* r = tensors + 8 * i;
     if (r[5] == 0) continue;
-    const int64_t chunks = (r[5] + CHUNK - 1) / CHUNK;
+    const int64_t chunks = (r[5] + chunk - 1) / chunk;  // below 2^31: valid()
     if (a.chunks + chunks > 0x7fffffff) break;
     Tensor& t = a.t[a.n++];
     t.p = (void*)r[0];
@@ -402,7 +421,7 @@ int64_t take(Args& a, const int64_t* tensors, int64_t first, int64_t count, uint
 // Launches that any `tensors` tensors of `values` values need at most: one ends with
 // TENSORS of them, or with 2^30 chunks at least.
 int64_t launches(int64_t tensors, int64_t values) {
-  return (tensors + TENSORS - 1) / TENSORS + (values / CHUNK + tensors >> 30);
+  return (tensors + TENSORS - 1) / TENSORS + ((values / NORM_CHUNK + tensors) >> 30);
 }
 
 bool valid(const int64_t* tensors, int64_t count, int bits, int64_t& values) {
@@ -410,7 +429,7 @@ bool valid(const int64_t* tensors, int64_t count, int bits, int64_t& values) {
   if (count < 0 || count > 1 << 24 || (count && !tensors)) return false;
   for (int64_t i = 0; i < count; i++) {
     const int64_t* r = tensors + 8 * i;
-    if (r[5] < 0 || r[5] > (1ll << 42) || (r[6] != F32 && r[6] != BF16)) return false;
+    if (r[5] < 0 || r[5] > (1ll << 40) || (r[6] != F32 && r[6] != BF16)) return false;
     if (r[5] == 0) continue;
     values += r[5];
     if (values > 1ll << 48) return false;
@@ -442,7 +461,7 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
     if (!workspace || (uintptr_t)workspace % 8 || workspace_values < launches(count, values) * NORM_GROUPS) return QA_EWORKSPACE;
     NormArgs a = {};
     for (int64_t first = 0; first < count;) {
-      first += take(a, tensors, first, count, 0);
+      first += take(a, tensors, first, count, 0, NORM_CHUNK);
       if (!a.n) continue;
       a.partial = workspace + parts;
       const unsigned groups = std::min<uint32_t>(a.chunks, NORM_GROUPS);
@@ -458,7 +477,7 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
   a.b1_rest = 1.0 - beta1;
   a.b2 = beta2;
   a.b2_rest = 1.0 - beta2;
-  a.keep = (float)(1.0 - rate * weight_decay);
+  a.decay = (float)(rate * weight_decay);
   a.rate = (float)(rate / c1);
   a.root = (float)(1.0 / __builtin_sqrt(c2));
   a.eps = (float)eps;
@@ -469,12 +488,14 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
     a.norm = norm;
   }
   const uint32_t key = mixed(mixed((uint32_t)seed) + (uint32_t)step);
+  const bool longer = bits == 32 && values >= LONG_FROM;
   for (int64_t first = 0; first < count;) {
-    first += take(a, tensors, first, count, key);
+    first += take(a, tensors, first, count, key, longer ? LONG_CHUNK : SHORT_CHUNK);
     if (!a.n) continue;
-    const dim3 grid(std::min<uint32_t>(a.chunks, GROUPS));
-    if (bits == 8) hipLaunchKernelGGL(adamw_step<true>, grid, dim3(THREADS), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(adamw_step<false>, grid, dim3(THREADS), 0, (hipStream_t)stream, a);
+    const dim3 grid(std::min<uint32_t>(a.chunks, longer ? LONG_GROUPS : SHORT_GROUPS));
+    if (bits == 8) hipLaunchKernelGGL((adamw_step<true, SHORT_CHUNK>), grid, dim3(THREADS), 0, (hipStream_t)stream, a);
+    else if (longer) hipLaunchKernelGGL((adamw_step<false, LONG_CHUNK>), grid, dim3(THREADS), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((adamw_step<false, SHORT_CHUNK>), grid, dim3(THREADS), 0, (hipStream_t)stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
   }
