@@ -11,10 +11,18 @@
 //
 // The waves of a workgroup share the stream.  They take the query heads of one kv
 // head first and consecutive blocks of 32 queries after that: with four heads to a
-// kv head a tile is 64 queries of four heads instead of 256 of one.  Short documents
-// then fill tiles (70 documents of 10 to 1024 tokens: 291 tiles of 64 instead of 110
-// of 256, of which a third is padding), and causal waves of a tile end their work
-// within two blocks of each other.
+// kv head a query tile is 32 rows of four heads instead of 128 of one.  Short
+// documents then fill tiles (70 documents of 10 to 1024 tokens: 547 tiles of 32 hold
+// 17504 rows for 16384 tokens, 168 of 128 21504), and all waves of a causal tile end
+// their work together.
+//
+// What bounds them, 16384 tokens of those documents, 16 heads over 4 of 64, causal:
+// forward 49 us (350 TFLOP/s, 2.4 TB/s), dQ 60 (430, 3.1), dK and dV 75 (450): the
+// softmax's vector instructions (three and an exponential for each score) beside the
+// matrix ones, and each wave's own beginning and end, 40% of the forward's vector
+// instructions at 160 visible keys to a query.  16000 tokens of three documents, 32
+// heads over 8 of 128: 712 us (990 TFLOP/s), 960 (1100) and 1580 (890; V of the
+// wave's keys read from LDS): the matrix cores, where a product of 8192^3 reaches 1160.
 //
 // Roundings to fewer bits: the probabilities and dS go into the second products as
 // bf16 (2^-8 of each, of random sign, as their other operand has; the normaliser
@@ -436,7 +444,7 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnP
   }
 }
 
-// A key tile: 4 waves of 32 keys; QB: rows of a streamed block.  Two sums of 128
+// A key tile: waves of 32 keys; QB: rows of a streamed block.  Two sums of 128
 // channels and K and V of the wave's keys do not fit 256 registers beside the scores
 // (97 of them spilled): there V stays in LDS, for 8 reads more beside 32 products,
 // and blocks of 32 rows leave room for two workgroups on a CU.
@@ -455,8 +463,8 @@ template <int DP, bool MASK>
 __device__ __forceinline__ void packed_dkv_step(lds_bytes sq, lds_bytes sg, const typename PackedTile<DP>::Lane& at,
                                                 const float* slse, const float* sdl, const bf16x8 (&kf)[DP / 16],
                                                 const bf16x8 (&vf)[PackedKeys<DP>::VF], lds_bytes sv,
-                                                const typename PackedTile<DP>::Lane& own, f32x16 (&dkt)[DP / 32], f32x16 (&dvt)[DP / 32], int end, int before,
-                                                float c, int half, int mb) {
+                                                const typename PackedTile<DP>::Lane& own, f32x16 (&dkt)[DP / 32],
+                                                f32x16 (&dvt)[DP / 32], int end, int before, float c, int half, int mb) {
   typedef PackedTile<DP> Tile;
   f32x16 sc = {};
 #pragma unroll

