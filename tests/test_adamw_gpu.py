@@ -257,3 +257,28 @@ def test_saved_states_go_on_with_the_same_bits(bits):
     assert all(np.array_equal(download(p.storage), download(o.storage)) for p, o in zip(parameters, others))
     assert all(a.to_array() == b.to_array() for s, t in zip(optimizer._state, second._state)
                for a, b in zip(s.storages(), t.storages()))
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_tensor_beyond_32_bits(bits):
+    """Equal values behind element 2^32 are stepped as those at the beginning (the rounding's
+    hash takes an element's low 32 bits); the norm counts all of them."""
+    size, steps = (1 << 32) + 4096, 2
+    p = Tensor(amd.full(size, 0.5, dtype="float32"), shape=(size,), requires_grad=True)
+    p.grad = Tensor(amd.full(size, 2.0 ** -10, dtype="float32"), shape=(size,))
+    optimizer = AdamW([p], **OPTIONS, bits=bits, max_norm=1.0, seed=5)
+    for _ in range(steps):
+        optimizer.step()
+    assert abs(optimizer.norm() - 2.0 ** -10 * size ** 0.5) <= 1e-9 * optimizer.norm()
+    state = optimizer._of(p)
+    if bits == 8:  # bytes, seen as words of eight
+        ends = [(x, size // 8 - 512, 512) for x in (state.first, state.second)] + [(state.exponents, size // 128 // 8 - 4, 4)]
+    else:
+        ends = [(x, size - 4096, 4096) for x in (state.first, state.second)]
+    for x, start, count in [(p.storage, size - 4096, 4096), *ends]:
+        first, last = (amd.view(x, at, count).to_array() for at in (0, start))
+        assert first == last and any(first)
+    model = Model([np.full(4096, 0.5, np.float32)], bits, **OPTIONS, seed=5)
+    for _ in range(steps):
+        model.step([np.full(4096, 2.0 ** -10 / (2.0 ** -10 * size ** 0.5))])
+    assert np.abs(download(amd.view(p.storage, 0, 4096)) - model.p[0]).max() <= 40 * UNIT * (0.5 + 10 * OPTIONS["lr"])

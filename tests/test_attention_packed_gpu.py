@@ -303,3 +303,52 @@ def test_heads_of_a_group_side_by_side(apart, dtype, lengths, heads, kv_heads, d
     again, _ = run(case, *behind)
     assert all(np.array_equal(result[name], again[name]) for name in result)
     assert runtime.lib.qutai_amd_attention_packed_workspace(*packing.extent[:2], heads, kv_heads, dim, amd.code(dtype), 4) == 0
+
+
+@pytest.mark.parametrize("dtype,dim", [("bfloat16", 64), ("bfloat16", 128), ("float32", 64), ("bfloat16", 136)])
+def test_rows_beyond_32_bits(dtype, dim):
+    """Columns of matrices of more than 2^32 values: what the same rows give side by side."""
+    lengths, heads, kv_heads, row = [700] * 24 + [1, 80], 4, 2, 1 << 18
+    rows, wide, narrow = sum(lengths), heads * dim, kv_heads * dim
+    assert rows * row > 1 << 32
+    packing = Packing(lengths)
+    q, k, v, g = (upload(normal(41 + i, rows * n * dim), dtype) for i, n in enumerate((heads, kv_heads, kv_heads, heads)))
+    columns = (row - wide, 64, 4096)
+    block = amd.AMDStorage(rows * row, dtype)
+    for x, width, column in zip((q, k, v), (wide, narrow, narrow), columns):
+        amd_lm.copy_rows(x, rows, width, out=block, out_column=column, out_row=row)
+    place = dict(zip(("q_column", "k_column", "v_column"), columns), q_row=row, k_row=row, v_row=row)
+    dims = (packing, heads, kv_heads, dim)
+    near = amd_lm.attention_packed(q, k, v, *dims, rest=True)
+    far = amd_lm.attention_packed(block, block, block, *dims, **place, rest=True)
+    into = amd.AMDStorage(rows * row, dtype)
+    expected = amd_lm.attention_packed_backward(g, q, k, v, *near[:2], *dims, rest=near[2])
+    amd_lm.attention_packed_backward(g, block, block, block, *far[:2], *dims, rest=far[2], **place, into=into)
+    found = [amd_lm.copy_rows(into, rows, width, column=column, row=row) for width, column in zip((wide, narrow, narrow), columns)]
+    for x, y in zip((*near[:2], *expected), (*far[:2], *found)):
+        x, y = download(x), download(y)
+        assert np.isfinite(x).all() and x.any() and np.array_equal(x, y)
+
+
+@pytest.mark.parametrize("dtype,dim", [("bfloat16", 64), ("bfloat16", 128), ("float32", 64), ("bfloat16", 20)])
+def test_scales_and_a_packing_used_for_all(dtype, dim):
+    """Twice the queries at half the scale are the same scores: the same results, and half of
+    dQ's.  One packing serves every type, width, mask and scale."""
+    packing, heads, kv_heads = Packing([90, 3, 200]), 4, 2
+    for other in (32, 64, 80):  # tables and plans of other calls
+        x, y = (upload(normal(3, 293 * n * other), "float32") for n in (1, 1))
+        amd_lm.attention_packed_backward(x, x, y, y, *amd_lm.attention_packed(x, y, y, packing, 1, 1, other, causal=False),
+                                         packing, 1, 1, other, causal=False)
+    q, k, v, g = (stored(normal(51 + i, (293, n, dim)), dtype) for i, n in enumerate((heads, kv_heads, kv_heads, heads)))
+    for scale in (0.7, 2.0 ** -20, 8.0):
+        results = []
+        for factor, rows in ((1.0, packing), (2.0, packing), (2.0, Packing([90, 3, 200]))):
+            stores, dims = [upload(x, dtype) for x in (q * factor, k, v)], (rows, heads, kv_heads, dim)
+            out, lse, rest = amd_lm.attention_packed(*stores, *dims, scale=scale / factor, rest=True)
+            grads = amd_lm.attention_packed_backward(upload(g, dtype), *stores, out, lse, *dims, scale=scale / factor, rest=rest)
+            dq, dk, dv = map(download, grads)
+            results.append([download(out), download(lse), dq * factor, dk, dv])
+        # a factor of two changes no rounding but of what lies below fp32's least normal number, 2^-126: each of the at
+        # most 6 x 2 x 293 products in a sum moves by that at most, times the scale (8: less than 2^15 in all)
+        for x in results[1:]:
+            assert all(np.isfinite(a).all() and np.abs(a - b).max() <= 2.0 ** -111 for a, b in zip(results[0], x))

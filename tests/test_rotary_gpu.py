@@ -181,3 +181,19 @@ def test_places_of_packed_tokens(lengths, total):
     packing = Packing(lengths, total)
     places = [t for n in lengths for t in range(n)]
     assert packing.positions.tolist() == places + [0] * (packing.total - len(places))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_beyond_32_bits(dtype):
+    """In place in a matrix of more than 2^32 values: what the same rows give side by side."""
+    rows, row, heads, dim = 17000, 1 << 18, 3, 64
+    x, turns, columns = upload(normal(5, rows * heads * dim), dtype), Rotary(dim, layout="half", scaling=PARTS), (128, row - 192)
+    block = amd.AMDStorage(rows * row, dtype)
+    for column in columns:
+        amd_lm.copy_rows(x, rows, heads * dim, out=block, out_column=column, out_row=row)
+    dims = (turns, 1, rows, heads, heads, dim)
+    near = amd_lm.rotary(x, x, *dims)
+    amd_lm.rotary(block, block, *dims, q_column=columns[0], q_row=row, k_column=columns[1], k_row=row, out=block, out_row=row,
+                  out_q_column=columns[0], out_k_column=columns[1])
+    for y, column in zip(near, columns):
+        assert np.array_equal(download(y), download(amd_lm.copy_rows(block, rows, heads * dim, column=column, row=row)))
