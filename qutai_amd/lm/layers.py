@@ -22,7 +22,7 @@ from ..core.context import is_recording, set_recording
 from ..core.grad import DeferredGradient, owned, record
 from ..core.tensor import Tensor
 from ..nn.cache import unchanged_on_failure
-from .rotary import Rotary
+from .rotary import default_rotary
 
 
 def backend(value):
@@ -492,7 +492,7 @@ class GQA:
         elif turns is None and packing is None:
             q, k = rope(q, self.heads, self.theta), rope(k, self.kv_heads, self.theta)
         elif turns is None:
-            turns = Rotary(q.shape[2] // self.heads, self.theta)
+            turns = default_rotary(q.shape[2] // self.heads, self.theta)
         if turns is not None:
             q, k = rotary(q, k, *sizes, turns, positions=positions)
         return self.out(attention(q, k, self.v(x), *sizes, packing))
@@ -873,7 +873,7 @@ def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turn
     columns = dict(q_row=total, k_column=dq, k_row=total)
     into = dict(out_row=total, out_k_column=dq)
     if turns is None and q_norm is None:
-        turns = Rotary(head, theta)
+        turns = default_rotary(head, theta)
     turned = (turns, batch, time, heads, kv_heads, head)
     if q_norm is None:
         q, k = b.rotary(qkv, qkv, *turned, positions=positions, **columns, out=qkv, **into)

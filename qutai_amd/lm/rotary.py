@@ -4,6 +4,7 @@ contexts longer than those a model was trained on."""
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from math import isfinite, log, pi
 
 LAYOUTS = ("interleaved", "half")
@@ -85,3 +86,10 @@ class Rotary:
     def turns(self):
         """Address of the whole turns a position of every pair (fp64, host)."""
         return ctypes.addressof(self._turns)
+
+
+@lru_cache(maxsize=16)
+def default_rotary(dim, theta):
+    """The Decoder's own rotation as a Rotary, made once for a width and theta: a block
+    asks for it every time it runs over packed sequences."""
+    return Rotary(dim, theta)
