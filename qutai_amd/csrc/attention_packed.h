@@ -52,11 +52,14 @@ __device__ __forceinline__ lds_bytes lds_at(const void* x) {
   return (lds_bytes)(lds_ptr_t)const_cast<void*>(x);
 }
 
+// DP: channels in steps of 32 that hold a head's.  Heads of 65 to 96 have kernels of their
+// own rather than those of 128: dK and dV of 8000 tokens, 16 heads over 4 of 96, 132 us
+// (178), dQ 68 (75), forward 61 (65).
 template <int DP>
 struct PackedTile {
   static constexpr int S = DP / 16, DB = DP / 32;  // MFMA k-steps over d, 32-wide d blocks
-  static constexpr int PC = DP / 8;                // 16-byte chunks of a row
-  static constexpr int ROW = DP * 2;               // bytes
+  static constexpr int PC = DP > 64 ? 16 : 8;      // 16-byte chunks of a row in LDS, a power of two
+  static constexpr int LP = PC * 8, ROW = LP * 2;  // a row in LDS: elements, bytes
 
   // Chunk c of row r lies at c ^ swz(r).  16 rows' same chunk (a read of 16 lanes) and 4
   // rows' 64 bytes (a transposed read of 32) fall into different banks, and rows 16
@@ -235,7 +238,7 @@ __device__ __forceinline__ void put_rest(void* base, int64_t at, const f32x4& v,
 template <int DP, int NW, int KB>
 __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : KB == 32 ? 3 : 2) packed_fwd(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
-  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * DP];  // [stage][K, V]
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * Tile::LP];  // [stage][K, V]
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
   const PackedPlace at = enter_queries<NW>(p, wave);
   const int T = (int)p.time, D = (int)p.dim, q0 = at.q0, t = q0 + col, tile_rows = NW / p.pack * 32;
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : KB == 32 ? 3 : 2) pack
     if (kbk + 1 < nkb) issue(kbk + 1);
   };
   if (nkb > 0) issue(0);
-  constexpr int STAGE = 2 * KB * DP * 2;
+  constexpr int STAGE = 2 * KB * Tile::ROW;
   typename Tile::Lane in;  // in the stage of block kbk
   in.plan(lane);
   const lds_bytes sk = lds_at(&lds[0][0][0]), sv = lds_at(&lds[0][1][0]);
@@ -353,7 +356,7 @@ template <int DP, int NW>
 __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
   constexpr int KB = 64;
-  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * DP];
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * Tile::LP];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
   const PackedPlace at = enter_queries<NW>(p, wave);
   const int T = (int)p.time, D = (int)p.dim, q0 = at.q0, t = q0 + col, tile_rows = NW / p.pack * 32;
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnP
     if (kbk + 1 < nkb) issue(kbk + 1);
   };
   if (nkb > 0) issue(0);
-  constexpr int STAGE = 2 * KB * DP * 2;
+  constexpr int STAGE = 2 * KB * Tile::ROW;
   typename Tile::Lane in;  // in the stage of block kbk
   in.plan(lane);
   const lds_bytes sk = lds_at(&lds[0][0][0]), sv = lds_at(&lds[0][1][0]);
@@ -446,12 +449,12 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnP
 
 // A key tile: waves of 32 keys; QB: rows of a streamed block.  Two sums of 128
 // channels and K and V of the wave's keys do not fit 256 registers beside the scores
-// (97 of them spilled): there V stays in LDS, for 8 reads more beside 32 products,
-// and blocks of 32 rows leave room for two workgroups on a CU.
+// (97 of them spilled): there V stays in LDS, for 8 reads more beside 32 products.
+// Blocks of 32 rows leave room for two workgroups on a CU.
 template <int DP>
 struct PackedKeys {
   static constexpr int QB = DP > 64 ? 32 : 64;
-  static constexpr bool V_IN_LDS = DP > 64;
+  static constexpr bool V_IN_LDS = DP > 96;
   static constexpr int VF = V_IN_LDS ? 1 : DP / 16;
 };
 
@@ -522,9 +525,9 @@ __global__ void __launch_bounds__(KW * SPLIT * 64, 2) packed_bwd_dkv(AttnPackedA
   typedef PackedTile<DP> Tile;
   constexpr int QB = PackedKeys<DP>::QB;
   constexpr bool V_IN_LDS = PackedKeys<DP>::V_IN_LDS;
-  __shared__ __attribute__((aligned(16))) bf16_t lds[2][SPLIT][2][QB * DP];  // [stage][set][Q, dO]
+  __shared__ __attribute__((aligned(16))) bf16_t lds[2][SPLIT][2][QB * Tile::LP];  // [stage][set][Q, dO]
   __shared__ __attribute__((aligned(16))) float stats[2][SPLIT][2][QB];      // [stage][set][-lse log2(e), delta]
-  __shared__ __attribute__((aligned(16))) bf16_t own_v[V_IN_LDS ? KW * 32 * DP : 8];
+  __shared__ __attribute__((aligned(16))) bf16_t own_v[V_IN_LDS ? KW * 32 * Tile::LP : 8];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int set = uniform32(tid >> 6) / KW, wave = uniform32(tid >> 6) % KW;
   const int group = (int)(p.heads / p.kv_heads);
@@ -557,7 +560,7 @@ __global__ void __launch_bounds__(KW * SPLIT * 64, 2) packed_bwd_dkv(AttnPackedA
   auto issue = [&](int it, int h, int qs) {
     bf16_t* to = &lds[it & 1][set][0][0];
     cq.issue(to, uniform_ptr((const bf16_t*)p.q + h * p.qh + (int64_t)qs * p.qt), p.qt, T - qs, wave);
-    cg.issue(to + QB * DP, uniform_ptr((const bf16_t*)p.g + h * p.qh + (int64_t)qs * p.ot), p.ot, T - qs, wave);
+    cg.issue(to + QB * Tile::LP, uniform_ptr((const bf16_t*)p.g + h * p.qh + (int64_t)qs * p.ot), p.ot, T - qs, wave);
     if (wave < 2 && lane < QB) {
       const float* from = wave ? p.delta : p.lse;
       next = qs + lane < T ? from[h + (int64_t)(qs + lane) * p.lt] : 0.f;
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(KW * SPLIT * 64, 2) packed_bwd_dkv(AttnPackedA
   const int tail = none ? steps : clamped(rows / 32, diagonal);
   const int end = none ? steps : clamped((rows + 31) / 32, tail);
   if (iterations > 0) issue(0, kvh * group + set, qs0);
-  constexpr int STAGE = SPLIT * 2 * QB * DP * 2;
+  constexpr int STAGE = SPLIT * 2 * QB * Tile::ROW;
   typename Tile::Lane in, own;  // in the stage of block `it`, in the wave's rows of V
   in.plan(lane);
   own = in;

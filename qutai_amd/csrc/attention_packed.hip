@@ -65,13 +65,15 @@ struct KeyShape {
 // tile ends in a quarter of the time.  Measured, us: 16384 tokens of up to 1024, 16
 // heads over 4 of 64, {2, 2} 76, {4, 2} 92-99, {2, 4} 114, {4, 1} 155; one of 2000, 8
 // over 2 of 64, {2, 2} 103, {2, 4} 76; 16000 of up to 6000, 32 over 8 of 128, {4, 1}
-// 1866, {4, 2} 1993 (an older form of both); 8000 of up to 2000, 16 over 4 of 96,
-// {4, 1} 398, {2, 4} 177; 8000 of up to 8, 16 over 4 of 64, {2, 2} 157, {2, 4} 335.
+// 1580, {2, 2} 2146 (its sums spill to the accumulation registers); 500 at most, 193 and
+// 247; 16384 of up to 1024, 16 over 4 of 80, {4, 1} 165, {2, 2} 116, 12 over 12 of 96, {4, 1}
+// 102, {2, 1} 99; 8000 of up to 2000, 16 over 4 of 96, {2, 2} 172, {2, 4} 136; 8000 of up
+// to 8, 16 over 4 of 64, {2, 2} 157, {2, 4} 335.
 KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles) {
   const int64_t group = heads / kv_heads;
   const bool few = tiles * kv_heads < 2 * cu_count() * (dim > 64 ? 2 : 1);
   if (few && group % 4 == 0) return {2, 4};
-  if (dim <= 64) return group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
+  if (dim <= 96) return group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
   return few && group % 2 == 0 ? KeyShape{4, 2} : KeyShape{4, 1};
 }
 
@@ -84,7 +86,7 @@ void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape
   else {
     const auto [waves, sets] = shape;
     const dim3 block(waves * sets * 64);
-    if constexpr (DP == 64) {
+    if constexpr (DP <= 96) {
       if (sets == 4) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 4>), dim3(blocks), block, 0, stream, a);
       else if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 2>), dim3(blocks), block, 0, stream, a);
       else hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 1>), dim3(blocks), block, 0, stream, a);
@@ -178,6 +180,7 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, con
   } else if (dtype == BF16) {
     const KeyShape shape = key_shape(a.heads, a.kv_heads, a.dim, key_tiles);
     if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, stream);
+    else if (a.dim <= 96) launch_packed<96>(pass, a, n, shape, stream);
     else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, stream);
     else launch_mma<false, 256>(pass, a, n, stream);
   } else {
