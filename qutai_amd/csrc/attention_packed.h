@@ -54,18 +54,20 @@ __device__ __forceinline__ lds_bytes lds_at(const void* x) {
 
 // DP: channels in steps of 32 that hold a head's.  Heads of 65 to 96 have kernels of their
 // own rather than those of 128: dK and dV of 8000 tokens, 16 heads over 4 of 96, 132 us
-// (178), dQ 68 (75), forward 61 (65).
+// (178), dQ 68 (75), forward 61 (65); heads of up to 32 rather than those of 64: 16384
+// tokens, 16 over 4 of 32, 53 (72), 36 (48), 30 (39).
 template <int DP>
 struct PackedTile {
   static constexpr int S = DP / 16, DB = DP / 32;  // MFMA k-steps over d, 32-wide d blocks
-  static constexpr int PC = DP > 64 ? 16 : 8;      // 16-byte chunks of a row in LDS, a power of two
+  static constexpr int PC = DP > 64 ? 16 : DP / 8;  // 16-byte chunks of a row in LDS, a power of two
   static constexpr int LP = PC * 8, ROW = LP * 2;  // a row in LDS: elements, bytes
 
   // Chunk c of row r lies at c ^ swz(r).  16 rows' same chunk (a read of 16 lanes) and 4
   // rows' 64 bytes (a transposed read of 32) fall into different banks, and rows 16
   // apart are swizzled alike, so that a lane's addresses in a tile differ by constants.
   __device__ static __forceinline__ int swz(int r) {
-    if constexpr (PC == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
+    if constexpr (PC == 4) return r >> 2 & 3;
+    else if constexpr (PC == 8) return (r >> 1 & 1) << 2 | (r >> 2 & 1) << 1 | (r >> 3 & 1);
     else return (r & 3) << 2 | (r >> 2 & 3);
   }
 
@@ -236,7 +238,7 @@ __device__ __forceinline__ void put_rest(void* base, int64_t at, const f32x4& v,
 }
 
 template <int DP, int NW, int KB>
-__global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : KB == 32 ? 3 : 2) packed_fwd(AttnPackedArgs p) {
+__global__ void __launch_bounds__(NW * 64, DP <= 64 ? 4 : KB == 32 ? 3 : 2) packed_fwd(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
   __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * Tile::LP];  // [stage][K, V]
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform32(tid >> 6), half = lane >> 5, col = lane & 31;
@@ -353,7 +355,7 @@ __device__ __forceinline__ void packed_dq_step(lds_bytes sk, lds_bytes sv, const
 }
 
 template <int DP, int NW>
-__global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnPackedArgs p) {
+__global__ void __launch_bounds__(NW * 64, DP <= 64 ? 4 : 2) packed_bwd_dq(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
   constexpr int KB = 64;
   __shared__ __attribute__((aligned(16))) bf16_t lds[2][2][KB * Tile::LP];
@@ -451,6 +453,8 @@ __global__ void __launch_bounds__(NW * 64, DP == 64 ? 4 : 2) packed_bwd_dq(AttnP
 // channels and K and V of the wave's keys do not fit 256 registers beside the scores
 // (97 of them spilled): there V stays in LDS, for 8 reads more beside 32 products.
 // Blocks of 32 rows leave room for two workgroups on a CU.
+// Heads of up to 32 leave registers for three waves of a SIMD (16384 tokens, 53 us; for
+// four, with 20 spilled, 62).
 template <int DP>
 struct PackedKeys {
   static constexpr int QB = DP > 64 ? 32 : 64;
@@ -521,7 +525,7 @@ __device__ __forceinline__ void packed_dkv_step(lds_bytes sq, lds_bytes sg, cons
 // SPLIT sets of KW waves take the query heads of a group in turns, each with a stream
 // of its own, and add up their sums at the end in the order of the sets.
 template <int DP, int KW, int SPLIT>
-__global__ void __launch_bounds__(KW * SPLIT * 64, 2) packed_bwd_dkv(AttnPackedArgs p) {
+__global__ void __launch_bounds__(KW * SPLIT * 64, DP == 32 ? 3 : 2) packed_bwd_dkv(AttnPackedArgs p) {
   typedef PackedTile<DP> Tile;
   constexpr int QB = PackedKeys<DP>::QB;
   constexpr bool V_IN_LDS = PackedKeys<DP>::V_IN_LDS;

@@ -81,7 +81,7 @@ int64_t key_tiles_of(int64_t tokens, int64_t sequences) { return tokens / 64 + s
 
 template <int DP>
 void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape shape, hipStream_t stream) {
-  if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP == 64 ? 64 : 32>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
+  if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP <= 64 ? 64 : 32>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
   else if (pass == QUERIES) hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
   else {
     const auto [waves, sets] = shape;
@@ -179,7 +179,8 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, con
     else launch_rows<float>(pass, a, n, stream);
   } else if (dtype == BF16) {
     const KeyShape shape = key_shape(a.heads, a.kv_heads, a.dim, key_tiles);
-    if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, stream);
+    if (a.dim <= 32) launch_packed<32>(pass, a, n, shape, stream);
+    else if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, stream);
     else if (a.dim <= 96) launch_packed<96>(pass, a, n, shape, stream);
     else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, stream);
     else launch_mma<false, 256>(pass, a, n, stream);

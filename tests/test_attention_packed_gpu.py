@@ -56,6 +56,9 @@ CASES = [
     ("bfloat16", [150, 77, 1], 8, 2, 96, True, True),
     ("bfloat16", [150, 64], 6, 1, 72, False, False),
     ("bfloat16", [33, 64, 130], 4, 4, 88, True, False),
+    ("bfloat16", [150, 77, 1], 8, 2, 32, True, True),
+    ("bfloat16", [150, 64], 6, 1, 24, False, True),
+    ("bfloat16", [33, 64, 130], 3, 3, 16, False, False),
 ]
 
 
@@ -234,7 +237,8 @@ def test_rectangles_agree_with_attention(dtype, dim):
 
 @pytest.mark.parametrize("lengths,heads,kv_heads,dim", [
     ([1, 2, 3, 5, 0, 8] * 100, 4, 2, 64), ([9, 2, 3, 5, 0, 8] * 100, 4, 1, 64), ([9, 40] * 150, 8, 4, 128),
-    ([65, 2] * 140, 4, 4, 64), ([65, 2] * 140, 8, 4, 96), ([65, 2] * 140, 4, 4, 80)])
+    ([65, 2] * 140, 4, 4, 64), ([65, 2] * 140, 8, 4, 96), ([65, 2] * 140, 4, 4, 80),
+    ([65, 2] * 140, 8, 4, 32), ([65, 2] * 140, 4, 4, 24)])
 def test_many_short_sequences(lengths, heads, kv_heads, dim):
     case = ("bfloat16", lengths, heads, kv_heads, dim, True, True)
     q, k, v, g = inputs(case, 23)
