@@ -421,14 +421,15 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * multiple of 16 bytes.  rest (NULL, or bf16 laid out as out; bf16 with dim up to 128
  * and tile_rows above 4) receives what out's rounding left, for the backward.  Rows
  * in no tile are left as they are.  dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up
- * to 128 rounds probabilities and dS to bf16 for their products, the others keep
- * fp32's bits. */
+ * to 128 rounds probabilities and dS to bf16 for their products (in two parts where no
+ * sequence has more than 64 tokens), the others keep fp32's bits. */
 int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads,
                                         int64_t kv_heads, int64_t dim, int dtype, int aligned, double scale, int pass);
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
                                    const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens,
-                                   int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row,
-                                   int64_t k_row, int64_t v_row, int dtype, double scale, int causal, void* stream);
+                                   int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim,
+                                   int64_t q_row, int64_t k_row, int64_t v_row, int dtype, double scale, int causal,
+                                   void* stream);
 /* Its gradients: grad is that of out (contiguous), out, lse and rest (or NULL) the
  * forward's; dq, dk and dv rows start dq_row, dk_row and dv_row elements after each
  * other; delta is scratch, fp32 [tokens][heads].  With a workspace (16-byte aligned)
@@ -442,7 +443,7 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
                                    void* workspace, size_t workspace_bytes, const int64_t* query_tiles,
                                    int64_t query_count, int64_t query_rows, const int64_t* key_tiles,
                                    int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
-                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
+                                   int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
                                    int64_t v_row, int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype,
                                    double scale, int causal, void* stream);
 

@@ -710,9 +710,8 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
         tiles, count, rows, _ = packing.plan(0, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal)
         if rest and rows > 4 and name == "bfloat16" and dim <= 128:
             left = AMDStorage(out.size, name)
-        tokens, sequences, _ = packing.extent
         out.runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count,
-                         rows, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
+                         rows, *packing.extent, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
                          mfma=_on_matrix_cores(name, dim))
     if packing.used < total:
         _packed_tail(packing, out, lse, left)
@@ -759,10 +758,9 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
         (q_tiles, q_count, q_rows, _), (k_tiles, k_count, k_rows, need) = (
             packing.plan(n, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal) for n in (1, 2))
         workspace = AMDStorage(need // 4, "float32") if need else None
-        tokens, sequences, _ = packing.extent
         delta.runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
                            *targets, delta.ptr, amd._p(workspace), need, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count,
-                           k_rows, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),
+                           k_rows, *packing.extent, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),
                            mfma=_on_matrix_cores(q.dtype, dim))
     if packing.used < total:
         if into is None:

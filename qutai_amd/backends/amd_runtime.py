@@ -93,10 +93,10 @@ SIGNATURES = {
     "qutai_amd_head_gradient": [_p, _p, _p, _i64, _i64, _f64, _i32, _p],
     "qutai_amd_attention_fwd": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _f64, _i32, _p],
     "qutai_amd_attention_packed_rows": [_i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _f64, _i32],
-    "qutai_amd_attention_packed_fwd": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f64,
+    "qutai_amd_attention_packed_fwd": [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f64,
                                        _i32, _p],
     "qutai_amd_attention_packed_workspace": [_i64, _i64, _i64, _i64, _i64, _i32, _i64],
-    "qutai_amd_attention_packed_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _i64, _i64, _p, _i64, _i64, _i64,
+    "qutai_amd_attention_packed_bwd": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _sz, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64,
                                        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _f64, _i32, _p],
     "qutai_amd_attention_cached": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i32, _f64, _p],
     "qutai_amd_sample": [_p, _p, _p, _p, _i64, _i64, _p, _f64, _p, _i64, _p, _f64, _p, _f64, _i32, _i32, _p],

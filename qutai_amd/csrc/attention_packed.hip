@@ -69,8 +69,11 @@ struct KeyShape {
 // 247; 16384 of up to 1024, 16 over 4 of 80, {4, 1} 165, {2, 2} 116, 12 over 12 of 96, {4, 1}
 // 102, {2, 1} 99; 8000 of up to 2000, 16 over 4 of 96, {2, 2} 172, {2, 4} 136; 8000 of up
 // to 8, 16 over 4 of 64, {2, 2} 157, {2, 4} 335.
-KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles) {
+// Short sequences (PARTS kernels): tiles of 64 rows, which hold one; 16000 of up to 64, 32
+// heads over 8 of 128, {2, 1} 253, {2, 2} 280, {4, 1} 291.
+KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles, int64_t longest) {
   const int64_t group = heads / kv_heads;
+  if (longest <= FINE) return dim <= 96 && group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
   const bool few = tiles * kv_heads < 2 * cu_count() * (dim > 64 ? 2 : 1);
   if (few && group % 4 == 0) return {2, 4};
   if (dim <= 96) return group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
@@ -79,22 +82,35 @@ KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles) 
 
 int64_t key_tiles_of(int64_t tokens, int64_t sequences) { return tokens / 64 + std::min(sequences, tokens); }
 
+template <int DP, bool PARTS>
+void launch_queries(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
+  const dim3 block(WAVES * 64);
+  if (pass == FORWARD)
+    hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP <= 64 ? 64 : 32, PARTS>), dim3(blocks), block, 0, stream, a);
+  else hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES, PARTS>), dim3(blocks), block, 0, stream, a);
+}
+
 template <int DP>
-void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape shape, hipStream_t stream) {
-  if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP <= 64 ? 64 : 32>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
-  else if (pass == QUERIES) hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), dim3(WAVES * 64), 0, stream, a);
-  else {
-    const auto [waves, sets] = shape;
-    const dim3 block(waves * sets * 64);
-    if constexpr (DP <= 96) {
-      if (sets == 4) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 4>), dim3(blocks), block, 0, stream, a);
-      else if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 2>), dim3(blocks), block, 0, stream, a);
-      else hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 1>), dim3(blocks), block, 0, stream, a);
-    } else {
-      if (sets == 4) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 4>), dim3(blocks), block, 0, stream, a);
-      else if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 2>), dim3(blocks), block, 0, stream, a);
-      else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), block, 0, stream, a);
-    }
+void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape shape, bool parts, hipStream_t stream) {
+  if (pass != KEYS) {
+    if (parts) launch_queries<DP, true>(pass, a, blocks, stream);
+    else launch_queries<DP, false>(pass, a, blocks, stream);
+    return;
+  }
+  const auto [waves, sets] = shape;
+  const dim3 block(waves * sets * 64);
+  if (parts) {
+    constexpr int MOST = DP <= 96 ? 2 : 1;
+    if (sets == MOST) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, MOST, true>), dim3(blocks), block, 0, stream, a);
+    else hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 1, true>), dim3(blocks), block, 0, stream, a);
+  } else if (sets == 4) {
+    hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 4>), dim3(blocks), block, 0, stream, a);
+  } else if constexpr (DP <= 96) {
+    if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 2>), dim3(blocks), block, 0, stream, a);
+    else hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 1>), dim3(blocks), block, 0, stream, a);
+  } else {
+    if (sets == 2) hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 2>), dim3(blocks), block, 0, stream, a);
+    else hipLaunchKernelGGL((packed_bwd_dkv<DP, 4, 1>), dim3(blocks), block, 0, stream, a);
   }
 }
 
@@ -160,14 +176,15 @@ __global__ void __launch_bounds__(256) packed_dkv_sum(AttnPackedArgs p, int64_t 
 }
 
 // Rows of a tile of the matrix kernels.
-int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim, int64_t key_tiles) {
+int64_t rows_of(Pass pass, int dtype, int64_t heads, int64_t kv_heads, int64_t dim, int64_t key_tiles, int64_t longest) {
   if (!packed_fits(dtype, dim)) return MMA_ROWS;
-  return pass == KEYS ? 32 * key_shape(heads, kv_heads, dim, key_tiles).waves : WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
+  if (pass == KEYS) return 32 * key_shape(heads, kv_heads, dim, key_tiles, longest).waves;
+  return WAVES * 32 / packed_heads(heads, kv_heads, WAVES);
 }
 
 // One pass over the tiles of `rows` rows each.
-hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, const int64_t* tiles, int64_t count,
-                  int64_t rows, hipStream_t stream) {
+hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, int64_t longest, const int64_t* tiles,
+                  int64_t count, int64_t rows, hipStream_t stream) {
   if (!count) return hipSuccess;
   a.tiles = tiles;
   a.lengths = tiles + count;
@@ -178,11 +195,12 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, con
     if (dtype == BF16) launch_rows<bf16_t>(pass, a, n, stream);
     else launch_rows<float>(pass, a, n, stream);
   } else if (dtype == BF16) {
-    const KeyShape shape = key_shape(a.heads, a.kv_heads, a.dim, key_tiles);
-    if (a.dim <= 32) launch_packed<32>(pass, a, n, shape, stream);
-    else if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, stream);
-    else if (a.dim <= 96) launch_packed<96>(pass, a, n, shape, stream);
-    else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, stream);
+    const KeyShape shape = key_shape(a.heads, a.kv_heads, a.dim, key_tiles, longest);
+    const bool parts = longest <= FINE;
+    if (a.dim <= 32) launch_packed<32>(pass, a, n, shape, parts, stream);
+    else if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, parts, stream);
+    else if (a.dim <= 96) launch_packed<96>(pass, a, n, shape, parts, stream);
+    else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, parts, stream);
     else launch_mma<false, 256>(pass, a, n, stream);
   } else {
     if (a.dim <= 32) launch_mma<true, 32>(pass, a, n, stream);
@@ -194,17 +212,17 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, con
 }
 
 // What forward and backward share: sizes, scale, pitches.  rows: of a tile.
-int set_packed(AttnPackedArgs& a, int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
+int set_packed(AttnPackedArgs& a, int64_t tokens, int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim,
                int64_t q_row, int64_t k_row, int64_t v_row, int dtype, double scale, int causal,
                std::initializer_list<std::pair<Pass, int64_t>> tiles) {
   if ((dtype != BF16 && dtype != F32) || heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1 << 16) return QA_EINVAL;
-  if (tokens < 0 || tokens >= 1ll << 31 || sequences < 0) return QA_EINVAL;
+  if (tokens < 0 || tokens >= 1ll << 31 || sequences < 0 || longest < 0) return QA_EINVAL;
   if (dim <= 0 || dim > 256 || !(scale > 0.0) || scale > 1e30) return QA_EINVAL;
   if (q_row < heads * dim || k_row < kv_heads * dim || v_row < kv_heads * dim) return QA_EINVAL;
   if (std::max({q_row, k_row, v_row, heads * dim}) > 1 << 22) return QA_EINVAL;  // 64 rows within a buffer descriptor
   for (const auto& [pass, rows] : tiles) {
     if (rows == GEN_WAVES) continue;
-    if (rows != rows_of(pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences)) || !mma_fits(dtype, dim) ||
+    if (rows != rows_of(pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences), longest) || !mma_fits(dtype, dim) ||
         scale < 0x1p-50)
       return QA_EINVAL;
   }
@@ -243,7 +261,7 @@ extern "C" {
 int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads,
                                         int64_t dim, int dtype, int aligned, double scale, int pass) {
   if ((dtype != BF16 && dtype != F32) || dim <= 0 || dim > 256 || pass < 0 || pass > 2 || heads <= 0 || kv_heads <= 0 ||
-      heads % kv_heads || tokens < 0 || tokens >= 1ll << 31 || sequences < 0)
+      heads % kv_heads || tokens < 0 || tokens >= 1ll << 31 || sequences < 0 || longest < 0)
     return 0;
   if (!aligned || !mma_fits(dtype, dim) || scale < 0x1p-50) return GEN_WAVES;
   // Tiles of sequences of a few tokens are mostly empty.  8000 tokens, us, tiles and one
@@ -253,7 +271,7 @@ int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64
   // 32 82 and 202, 132 and 217, 144 and 197.
   const int64_t few = packed_fits(dtype, dim) ? (pass == KEYS ? 8 : 0) : 20;
   if (longest <= few) return GEN_WAVES;
-  return rows_of((Pass)pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences));
+  return rows_of((Pass)pass, dtype, heads, kv_heads, dim, key_tiles_of(tokens, sequences), longest);
 }
 
 size_t qutai_amd_attention_packed_workspace(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t dim,
@@ -267,10 +285,10 @@ size_t qutai_amd_attention_packed_workspace(int64_t tokens, int64_t sequences, i
 
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
                                    const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens, int64_t sequences,
-                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
+                                   int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
                                    double scale, int causal, void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
+  const int status = set_packed(a, tokens, sequences, longest, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
   if (status != QA_OK) return status;
   if (!grid_fits(tile_count, heads)) return QA_EINVAL;
   if (rest && (tile_rows == GEN_WAVES || !packed_fits(dtype, dim))) return QA_EINVAL;
@@ -284,18 +302,18 @@ int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, 
   a.dqt = a.ot;
   a.lse = lse;
   a.rest = rest;
-  return (int)launch(FORWARD, dtype, a, key_tiles_of(tokens, sequences), tiles, tile_count, tile_rows, (hipStream_t)stream);
+  return (int)launch(FORWARD, dtype, a, key_tiles_of(tokens, sequences), longest, tiles, tile_count, tile_rows, (hipStream_t)stream);
 }
 
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                    const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
                                    void* workspace, size_t workspace_bytes, const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
                                    const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
-                                   int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
+                                   int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
                                    int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
                                    void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, tokens, sequences, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
+  const int status = set_packed(a, tokens, sequences, longest, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
                                 {{QUERIES, query_rows}, {KEYS, key_rows}});
   if (status != QA_OK) return status;
   if (dq_row < heads * dim || dk_row < kv_heads * dim || dv_row < kv_heads * dim) return QA_EINVAL;
@@ -330,9 +348,9 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
     a.part_v = a.part_k + group * a.part_stride;
   }
   // the query pass writes delta, which the key pass reads
-  hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), query_tiles, query_count, query_rows, (hipStream_t)stream);
+  hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), longest, query_tiles, query_count, query_rows, (hipStream_t)stream);
   if (e != hipSuccess) return (int)e;
-  e = launch(KEYS, dtype, a, key_tiles_of(tokens, sequences), key_tiles, key_count, key_rows, (hipStream_t)stream);
+  e = launch(KEYS, dtype, a, key_tiles_of(tokens, sequences), longest, key_tiles, key_count, key_rows, (hipStream_t)stream);
   if (e != hipSuccess || !a.split || !key_count) return (int)e;
   const dim3 grid((unsigned)((a.part_stride / 4 + 255) / 256));
   if (dtype == BF16) hipLaunchKernelGGL(packed_dkv_sum<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, a, tokens, (int)group);

@@ -70,14 +70,15 @@ def inputs(case, seed):
     return q, k, v, g
 
 
-def reference(q, k, v, g, lengths, causal, dtype, exact_rest):
+def reference(q, k, v, g, lengths, causal, dtype, exact_rest, weight=None):
     """{name: (value, bound)}: the formulas in float64, and how far roundings may
     take a kernel that holds scores, statistics and sums in fp32 and rounds bf16's
     probabilities and dS to bf16 (fp32's keep 2^-24 of theirs)."""
     total, heads, dim = q.shape
     kv_heads, scale = k.shape[1], q.shape[2] ** -0.5
     group, step = heads // k.shape[1], STEP[dtype]
-    weight = 2.0 ** -8 if dtype == "bfloat16" else 8 * UNIT  # a probability's or dS's rounding
+    if weight is None:  # a probability's or dS's rounding
+        weight = 2.0 ** -8 if dtype == "bfloat16" else 8 * UNIT
     out = {n: (np.zeros(s), np.zeros(s)) for n, s in (("out", q.shape), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape))}
     lse = np.zeros((total, heads)), np.zeros((total, heads))
     start = 0
@@ -359,3 +360,18 @@ def test_scales_and_a_packing_used_for_all(dtype, dim):
         # most 6 x 2 x 293 products in a sum moves by that at most, times the scale (8: less than 2^15 in all)
         for x in results[1:]:
             assert all(np.isfinite(a).all() and np.abs(a - b).max() <= 2.0 ** -111 for a, b in zip(results[0], x))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,causal", [
+    (4, 2, 64, True), (3, 1, 64, False), (8, 2, 128, True), (2, 2, 128, False), (6, 3, 96, True), (4, 4, 80, False), (8, 2, 32, True),
+    (3, 3, 24, False)])
+def test_short_sequences_keep_more_of_probabilities(heads, kv_heads, dim, causal):
+    """No sequence of more than 64 tokens: probabilities and dS in two bf16 parts, the second
+    of what the first left, so 2^-8 of 2^-8 is lost."""
+    lengths = [64, 1, 0, 33, 2, 9, 64, 31, 32, 47]
+    case = ("bfloat16", lengths, heads, kv_heads, dim, causal, True)
+    q, k, v, g = inputs(case, 61)
+    got, rest = run(case, q, k, v, g)
+    assert rest is not None
+    for name, (value, bound) in reference(q, k, v, g, lengths, causal, "bfloat16", True, 2.0 ** -16).items():
+        within(name, got[name], value, bound)

@@ -249,14 +249,14 @@ def test_c_entry_points_refuse():
     assert library.qutai_amd_positions(None, 0, 0, 0, None, None) == 0
 
     def forward(**change):
-        a = dict(q=p, k=p, v=p, out=p, lse=p, rest=None, tiles=p, count=2, rows=64, tokens=200, sequences=3, heads=4, kv=2, dim=64, qr=256, kr=128,
+        a = dict(q=p, k=p, v=p, out=p, lse=p, rest=None, tiles=p, count=2, rows=64, tokens=200, sequences=3, longest=1000, heads=4, kv=2, dim=64, qr=256, kr=128,
                  vr=128, dtype=5, scale=0.125, causal=1, stream=None)
         a.update(change)
         return library.qutai_amd_attention_packed_fwd(*a.values())
 
     wrong = (dict(heads=3), dict(kv=0), dict(dim=0), dict(dim=264), dict(qr=255), dict(kr=127), dict(vr=64), dict(dtype=4),
              dict(scale=0.0), dict(scale=float("nan")), dict(rows=100), dict(rows=0), dict(q=None), dict(lse=None),
-             dict(tiles=None), dict(count=-1), dict(count=1 << 40), dict(tokens=-1), dict(sequences=-1), dict(tokens=1 << 31), dict(q=p + 2), dict(qr=1 << 30), dict(dim=20))
+             dict(tiles=None), dict(count=-1), dict(count=1 << 40), dict(tokens=-1), dict(sequences=-1), dict(longest=-1), dict(tokens=1 << 31), dict(q=p + 2), dict(qr=1 << 30), dict(dim=20))
     for change in wrong:
         assert forward(**change) == EINVAL, change
     assert forward(count=0) == 0
