@@ -8,6 +8,11 @@ from .backends import amd, amd_lm
 from .core.tensor import Tensor
 
 
+def _check_seed(seed):
+    if type(seed) is not int or not 0 <= seed < 1 << 32:
+        raise ValueError("the seed is an integer of 0 or more, below 2^32")
+
+
 class AdamW:
     """``step()`` applies the gradients of ``parameters`` (float32 or bfloat16
     Tensors; those without a ``grad`` are left as they are):
@@ -31,8 +36,9 @@ class AdamW:
         spans = sorted((p.storage.ptr, p.storage.ptr + p.storage.nbytes) for p in parameters if p.size)
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters must not share memory: every value is stepped once")
-        if bits not in (8, 32) or type(seed) is not int or not 0 <= seed < 1 << 32:
-            raise ValueError("moments have 8 or 32 bits, the seed is an integer below 2^32")
+        if bits not in (8, 32):
+            raise ValueError("moments have 8 or 32 bits")
+        _check_seed(seed)
         if len(betas) != 2 or any(not 0 <= b < 1 for b in betas) or not 0 < eps < float("inf"):
             raise ValueError("betas lie in [0, 1), eps is positive")
         if max_norm is not None and not 0 < max_norm < float("inf"):
@@ -84,15 +90,26 @@ class AdamW:
                 "moments": [[x.to_array() for x in state.storages()] for state in self._state]}
 
     def load_state_dict(self, state):
-        moments = state["moments"]
-        if state["bits"] != self.bits or len(moments) != len(self._state) or type(state["steps"]) is not int \
-                or state["steps"] < 0:
+        """Goes on from a ``state_dict`` of an optimizer of the same tensors and bits;
+        ValueError, and nothing changed, where it is not one."""
+        try:
+            steps, bits, seed, moments = (state[name] for name in ("steps", "bits", "seed", "moments"))
+        except (KeyError, TypeError):
+            raise ValueError("a state holds steps, bits, seed and moments") from None
+        if bits != self.bits or not isinstance(moments, (list, tuple)) or len(moments) != len(self._state) \
+                or type(steps) is not int or not 0 <= steps < (1 << 63) - 1:
             raise ValueError("the state is of another optimizer")
-        for own, given in zip(self._state, moments):
-            if len(given) != len(own.storages()) or any(len(x) != len(g) for x, g in zip(own.storages(), given)):
-                raise ValueError("the state's moments have other sizes")
-        for own, given in zip(self._state, moments):
-            for x, values in zip(own.storages(), given):
+        _check_seed(seed)
+        own = [state.storages() for state in self._state]
+        for kept, given in zip(own, moments):
+            if not isinstance(given, (list, tuple)) or len(given) != len(kept):
+                raise ValueError("the state's moments are of another optimizer")
+            # the items' type too: what is uploaded is as many bytes as the array has
+            if any(not isinstance(values, array) or values.typecode != amd._TYPES[x.dtype][0] or len(values) != len(x)
+                   for x, values in zip(kept, given)):
+                raise ValueError("the state's moments are arrays of the sizes and item types of state_dict")
+        for kept, given in zip(own, moments):
+            for x, values in zip(kept, given):
                 if len(x):
-                    x.runtime.upload(x.ptr, array(values.typecode, values))
-        self.steps, self.seed, self._norm = state["steps"], state["seed"], None
+                    x.runtime.upload(x.ptr, values)
+        self.steps, self.seed, self._norm = steps, seed, None
