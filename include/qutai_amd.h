@@ -477,6 +477,8 @@ int qutai_amd_positions(const int64_t* starts, int64_t sequences, int64_t used, 
  * every 256 values; zeros stand for zeros.
  *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *   p' = p (1 - rate weight_decay) - rate m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
+ * eps, rate / (1 - beta1^step) and rate weight_decay are fp32 in the kernels: QA_EINVAL
+ * where eps is no normal number of fp32 (2^-126 or more) or the others exceed it.
  * With max_norm > 0 gradients are scaled to that norm over all tensors where they
  * exceed it, the norm goes to `norm` (fp64, device, may be NULL), a norm that is not
  * finite leaves everything as it is, and `workspace` holds at least

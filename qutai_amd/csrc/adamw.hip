@@ -33,6 +33,7 @@
 #include "qutai_amd.h"
 
 #include <algorithm>
+#include <cfloat>
 
 using namespace qa;
 
@@ -453,9 +454,13 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
                     int64_t workspace_values, double* norm, void* stream) {
   int64_t values;
   if ((bits != 8 && bits != 32) || !valid(tensors, count, bits, values)) return QA_EINVAL;
-  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) || !(eps > 0.0) || step < 1) return QA_EINVAL;
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0) || step < 1) return QA_EINVAL;
   if (!(rate >= 0.0) || !(rate < 1e30) || !(weight_decay >= 0.0) || !(weight_decay < 1e30) || !(max_norm >= 0.0))
     return QA_EINVAL;
+  // The kernels take these in fp32: an eps that is 0 there, or whose reciprocal is infinite,
+  // makes 0 / 0 of a value without a gradient, an infinite rate or decay inf * 0.
+  const double c1 = 1.0 - __builtin_pow(beta1, (double)step), c2 = 1.0 - __builtin_pow(beta2, (double)step);
+  if (!(eps >= FLT_MIN) || !(eps <= FLT_MAX) || !(rate / c1 <= FLT_MAX) || !(rate * weight_decay <= FLT_MAX)) return QA_EINVAL;
   int64_t parts = 0;
   if (max_norm > 0.0 && values) {
     if (!workspace || (uintptr_t)workspace % 8 || workspace_values < launches(count, values) * NORM_GROUPS) return QA_EWORKSPACE;
@@ -472,7 +477,6 @@ int qutai_amd_adamw(const int64_t* tensors, int64_t count, int bits, double rate
     }
   }
   StepArgs a = {};
-  const double c1 = 1.0 - __builtin_pow(beta1, (double)step), c2 = 1.0 - __builtin_pow(beta2, (double)step);
   a.b1 = beta1;
   a.b1_rest = 1.0 - beta1;
   a.b2 = beta2;

@@ -8,6 +8,9 @@ from .backends import amd, amd_lm
 from .core.tensor import Tensor
 
 
+FP32_NORMAL = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127  # fp32's least and largest normal numbers
+
+
 def _check_seed(seed):
     if type(seed) is not int or not 0 <= seed < 1 << 32:
         raise ValueError("the seed is an integer of 0 or more, below 2^32")
@@ -25,7 +28,8 @@ class AdamW:
     gives the same bits).  With ``max_norm`` gradients whose norm over all tensors
     exceeds it are scaled down to it, and a step whose norm is not finite changes
     nothing (t counts it all the same: nothing is read from the device); ``norm()``
-    is the last step's.  ``lr`` may be changed between steps."""
+    is the last step's.  ``lr`` may be changed between steps.  ``eps`` and each
+    step's rate are fp32 in the kernels: eps is 2^-126 or more."""
 
     def __init__(self, parameters, lr=1e-3, *, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, max_norm=None,
                  seed=0):
@@ -39,8 +43,10 @@ class AdamW:
         if bits not in (8, 32):
             raise ValueError("moments have 8 or 32 bits")
         _check_seed(seed)
-        if len(betas) != 2 or any(not 0 <= b < 1 for b in betas) or not 0 < eps < float("inf"):
-            raise ValueError("betas lie in [0, 1), eps is positive")
+        if len(betas) != 2 or any(not 0 <= b < 1 for b in betas):
+            raise ValueError("betas lie in [0, 1)")
+        if not FP32_NORMAL[0] <= eps <= FP32_NORMAL[1]:  # else 0 in the kernels, and a value without a gradient 0 / 0
+            raise ValueError("eps is a normal number of fp32: 2^-126 (1.2e-38) or more")
         if max_norm is not None and not 0 < max_norm < float("inf"):
             raise ValueError("max_norm is a positive number")
         self.parameters, self.lr, self.betas, self.eps = parameters, lr, tuple(map(float, betas)), eps

@@ -6,9 +6,11 @@ from types import SimpleNamespace
 import pytest
 
 from qutai_amd import Tensor
-from qutai_amd.backends import amd_lm
+from qutai_amd.backends import amd_lm, amd_runtime
 from qutai_amd.optim import AdamW
-from tests.test_operators_host import fake
+from tests.test_operators_host import built, fake
+
+EINVAL = amd_runtime.QA_EINVAL
 
 SIZES = (8, 300)
 
@@ -95,3 +97,36 @@ def test_moments_of_other_sizes_write_nothing(optimizer):
         with pytest.raises(ValueError):
             optimizer.load_state_dict(state)
     assert not optimizer.uploads.written and (optimizer.steps, optimizer.seed) == (0, 3)
+
+
+LEAST, MOST = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127  # fp32's normal numbers
+
+
+@pytest.mark.parametrize("eps", [5e-324, 7e-46, 1e-39, LEAST * (1 - 2.0 ** -52), 2.0 ** 128, 1e300, float("nan"), float("inf"), -1e-8])
+def test_eps_that_fp32_does_not_hold_as_a_normal_number_is_refused(eps):
+    """It would be 0 in the kernels (or its reciprocal infinite), and a value without a
+    gradient 0 / 0."""
+    parameter = Tensor(fake(8, "float32"), shape=(8,), requires_grad=True)
+    with pytest.raises(ValueError):
+        AdamW([parameter], eps=eps)
+
+
+@built
+def test_c_refuses_numbers_that_fp32_does_not_hold():
+    """eps, the rate over 1 - beta1^step and the rate's decay are fp32 in the kernels."""
+    import ctypes
+
+    library, p = amd_runtime.load_library(), 4096
+    row = (ctypes.c_int64 * 8)(p, p, p, p, p, 0, 0, 0)  # no values: nothing is launched
+
+    def step(**change):
+        a = dict(tensors=ctypes.addressof(row), count=1, bits=32, rate=1e-3, b1=0.9, b2=0.99, eps=1e-8, decay=0.0, step=1, seed=0,
+                 max_norm=0.0, workspace=None, values=0, norm=None, stream=None)
+        a.update(change)
+        return library.qutai_amd_adamw(*a.values())
+
+    for change in (dict(), dict(eps=LEAST), dict(eps=MOST), dict(rate=1e25), dict(rate=1e18, decay=1e20), dict(b1=1 - 2.0 ** -53, rate=1e20)):
+        assert step(**change) == 0, change
+    for change in (dict(eps=LEAST / 2), dict(eps=1e-46), dict(eps=2.0 ** 128), dict(eps=float("nan")),
+                   dict(b1=1 - 2.0 ** -53, rate=1e25), dict(rate=1e19, decay=1e20)):
+        assert step(**change) == EINVAL, change
