@@ -246,6 +246,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, heads, kv_heads, theta, eps, offset=0
         raise ValueError("qk_norm_rope takes q (batch, time, heads*dim) and k (batch, time, kv_heads*dim)")
     batch, time, features = q.shape
     if positions is not None:  # every token a sequence of its own
+        if offset:
+            raise ValueError("positions hold one int64 for every token, without offset")
         batch, time = batch * time, 1
     dims = (batch, time, heads, kv_heads, features // heads, theta, eps)
     where = dict(offset=offset, starts=positions)
