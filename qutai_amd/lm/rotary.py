@@ -13,7 +13,13 @@ SCALINGS = {"linear": {"factor"}, "base": {"factor"},
 
 
 def _number(value, low):
-    return isinstance(value, (int, float)) and not isinstance(value, bool) and isfinite(value) and value > low
+    """Whether this is a finite number above ``low`` that a float holds."""
+    if not isinstance(value, (int, float)) or isinstance(value, bool):
+        return False
+    try:
+        return isfinite(value) and value > low
+    except OverflowError:  # an integer beyond every float
+        return False
 
 
 def checked_scaling(scaling, rotary_dim):
@@ -21,7 +27,7 @@ def checked_scaling(scaling, rotary_dim):
     ValueError where it is not one."""
     if scaling is None:
         return None
-    if not isinstance(scaling, dict) or scaling.get("kind") not in SCALINGS:
+    if not isinstance(scaling, dict) or scaling.get("kind") not in tuple(SCALINGS):
         raise ValueError(f"a rotary scaling is a dict whose kind is one of {', '.join(SCALINGS)}")
     kind = scaling["kind"]
     if set(scaling) - {"kind"} - SCALINGS[kind] or not _number(scaling.get("factor"), 0):
@@ -32,9 +38,11 @@ def checked_scaling(scaling, rotary_dim):
     if kind == "parts":
         result = {"low": 1.0, "high": 32.0, **result}
         result.setdefault("magnitude", 0.1 * log(result["factor"]) + 1.0 if result["factor"] > 1 else 1.0)
-        if not _number(result.get("original_length"), 0) or not _number(result["magnitude"], 0):
-            raise ValueError("parts scaling needs the original_length, above 0, and a magnitude above 0")
-        if not _number(result["low"], -1) or not _number(result["high"], result["low"]):
+        if not _number(result.get("original_length"), 0):
+            raise ValueError("parts scaling needs the original_length, above 0")
+        if not _number(result["magnitude"], 0) or not 2.0 ** -126 <= result["magnitude"] < 1e30:
+            raise ValueError("parts scaling needs a magnitude that fp32 holds, from 2^-126 to 1e30")
+        if not _number(result["low"], -1) or result["low"] < 0 or not _number(result["high"], result["low"]):
             raise ValueError("parts scaling needs 0 <= low < high turns")
     return result
 
@@ -66,9 +74,12 @@ class Rotary:
         self.dim, self.theta, self.rotary_dim, self.layout = dim, float(theta), rotary_dim, layout
         self.magnitude, base = 1.0, self.theta
         kind = None if scaling is None else scaling["kind"]
-        if kind == "base":
-            base *= scaling["factor"] ** (rotary_dim / (rotary_dim - 2))
-        frequencies = [base ** (-2 * i / rotary_dim) for i in range(rotary_dim // 2)]
+        try:
+            if kind == "base":
+                base *= scaling["factor"] ** (rotary_dim / (rotary_dim - 2))
+            frequencies = [base ** (-2 * i / rotary_dim) for i in range(rotary_dim // 2)]
+        except OverflowError:
+            raise ValueError("theta and the scaling's factor give frequencies beyond every float") from None
         if kind == "linear":
             frequencies = [f / scaling["factor"] for f in frequencies]
         elif kind == "parts":
@@ -78,7 +89,7 @@ class Rotary:
                 kept = min(1.0, max(0.0, (scaling["original_length"] * f / (2 * pi) - low) / (high - low)))
                 frequencies[i] = f * (kept + (1 - kept) / scaling["factor"])
         self.frequencies = tuple(frequencies)  # radians a position
-        if not all(isfinite(f) for f in frequencies):
+        if not isfinite(base) or not all(isfinite(f) for f in frequencies):
             raise ValueError("the scaled frequencies are not finite")
         self._turns = (ctypes.c_double * len(frequencies))(*(f / (2 * pi) for f in frequencies))
 
