@@ -421,8 +421,8 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * multiple of 16 bytes.  rest (NULL, or bf16 laid out as out; bf16 with dim up to 128
  * and tile_rows above 4) receives what out's rounding left, for the backward.  Rows
  * in no tile are left as they are.  dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up
- * to 128 rounds probabilities and dS to bf16 for their products (in two parts where no
- * sequence has more than 64 tokens), the others keep fp32's bits. */
+ * to 128 rounds probabilities and dS to bf16 for their products, in two parts where their
+ * sequence has no more than 64 tokens; the others keep fp32's bits. */
 int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads,
                                         int64_t kv_heads, int64_t dim, int dtype, int aligned, double scale, int pass);
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,

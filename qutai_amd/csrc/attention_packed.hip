@@ -69,11 +69,12 @@ struct KeyShape {
 // 247; 16384 of up to 1024, 16 over 4 of 80, {4, 1} 165, {2, 2} 116, 12 over 12 of 96, {4, 1}
 // 102, {2, 1} 99; 8000 of up to 2000, 16 over 4 of 96, {2, 2} 172, {2, 4} 136; 8000 of up
 // to 8, 16 over 4 of 64, {2, 2} 157, {2, 4} 335.
-// Short sequences (PARTS kernels): tiles of 64 rows, which hold one; 16000 of up to 64, 32
-// heads over 8 of 128, {2, 1} 253, {2, 2} 280, {4, 1} 291.
+// Short sequences (ONLY kernels): tiles of 64 rows, which hold one; 16000 of up to 64, 32
+// heads over 8 of 128, {2, 1} 173; 8000, 16 over 4 of 96, {2, 1} 29, {2, 2} 40 to 77 (it
+// spills); 16384, 16 over 4 of 64, {2, 2} 60.
 KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles, int64_t longest) {
   const int64_t group = heads / kv_heads;
-  if (longest <= FINE) return dim <= 96 && group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
+  if (longest <= FINE) return dim <= 64 && group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
   const bool few = tiles * kv_heads < 2 * cu_count() * (dim > 64 ? 2 : 1);
   if (few && group % 4 == 0) return {2, 4};
   if (dim <= 96) return group % 2 == 0 ? KeyShape{2, 2} : KeyShape{2, 1};
@@ -82,25 +83,18 @@ KeyShape key_shape(int64_t heads, int64_t kv_heads, int64_t dim, int64_t tiles, 
 
 int64_t key_tiles_of(int64_t tokens, int64_t sequences) { return tokens / 64 + std::min(sequences, tokens); }
 
-template <int DP, bool PARTS>
-void launch_queries(Pass pass, const AttnPackedArgs& a, unsigned blocks, hipStream_t stream) {
-  const dim3 block(WAVES * 64);
-  if (pass == FORWARD)
-    hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP <= 64 ? 64 : 32, PARTS>), dim3(blocks), block, 0, stream, a);
-  else hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES, PARTS>), dim3(blocks), block, 0, stream, a);
-}
-
 template <int DP>
-void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape shape, bool parts, hipStream_t stream) {
+void launch_packed(Pass pass, const AttnPackedArgs& a, unsigned blocks, KeyShape shape, bool only, hipStream_t stream) {
   if (pass != KEYS) {
-    if (parts) launch_queries<DP, true>(pass, a, blocks, stream);
-    else launch_queries<DP, false>(pass, a, blocks, stream);
+    const dim3 block(WAVES * 64);
+    if (pass == FORWARD) hipLaunchKernelGGL((packed_fwd<DP, WAVES, DP <= 64 ? 64 : 32>), dim3(blocks), block, 0, stream, a);
+    else hipLaunchKernelGGL((packed_bwd_dq<DP, WAVES>), dim3(blocks), block, 0, stream, a);
     return;
   }
   const auto [waves, sets] = shape;
   const dim3 block(waves * sets * 64);
-  if (parts) {
-    constexpr int MOST = DP <= 96 ? 2 : 1;
+  if (only) {
+    constexpr int MOST = DP <= 64 ? 2 : 1;
     if (sets == MOST) hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, MOST, true>), dim3(blocks), block, 0, stream, a);
     else hipLaunchKernelGGL((packed_bwd_dkv<DP, 2, 1, true>), dim3(blocks), block, 0, stream, a);
   } else if (sets == 4) {
@@ -196,11 +190,10 @@ hipError_t launch(Pass pass, int dtype, AttnPackedArgs a, int64_t key_tiles, int
     else launch_rows<float>(pass, a, n, stream);
   } else if (dtype == BF16) {
     const KeyShape shape = key_shape(a.heads, a.kv_heads, a.dim, key_tiles, longest);
-    const bool parts = longest <= FINE;
-    if (a.dim <= 32) launch_packed<32>(pass, a, n, shape, parts, stream);
-    else if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, parts, stream);
-    else if (a.dim <= 96) launch_packed<96>(pass, a, n, shape, parts, stream);
-    else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, parts, stream);
+    if (a.dim <= 32) launch_packed<32>(pass, a, n, shape, longest <= FINE, stream);
+    else if (a.dim <= 64) launch_packed<64>(pass, a, n, shape, longest <= FINE, stream);
+    else if (a.dim <= 96) launch_packed<96>(pass, a, n, shape, longest <= FINE, stream);
+    else if (a.dim <= 128) launch_packed<128>(pass, a, n, shape, longest <= FINE, stream);
     else launch_mma<false, 256>(pass, a, n, stream);
   } else {
     if (a.dim <= 32) launch_mma<true, 32>(pass, a, n, stream);
