@@ -758,6 +758,8 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
         (q_tiles, q_count, q_rows, _), (k_tiles, k_count, k_rows, need) = (
             packing.plan(n, heads, kv_heads, dim, dtype, odd % 16 == 0, scale, causal) for n in (1, 2))
         workspace = AMDStorage(need // 4, "float32") if need else None
+        if rest is not None and rest.ptr % 16 and odd % 16 == 0:  # read with the others' whole chunks
+            rest = copy_rows(rest, 1, rest.size)
         delta.runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
                            *targets, delta.ptr, amd._p(workspace), need, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count,
                            k_rows, *packing.extent, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),

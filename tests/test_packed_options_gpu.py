@@ -1,0 +1,41 @@
+"""Packed attention with operands at addresses of their own, many tiles, and what it counts
+as a launch on the matrix cores."""
+import numpy as np
+import pytest
+
+from qutai_amd.backends import amd, amd_lm
+from qutai_amd.lm import Packing
+from tests.helpers import download, normal, stored, upload
+
+pytestmark = pytest.mark.gpu
+
+
+def shifted(values, dtype, shift=1):
+    """A storage of these values whose address is no multiple of 16 bytes."""
+    flat = np.concatenate([np.zeros(shift), np.asarray(values).reshape(-1)])
+    return amd.view(upload(flat, dtype), shift, flat.size - shift)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", ["rest", "out", "gradient", "k"])
+def test_operands_at_any_address(which, dim):
+    """An operand that is not 16-byte aligned: the same bits for the rest of out, which is
+    copied; gradients within the roundings of two kernels for the others, whose rows are
+    then worked on one at a time without the rest."""
+    packing, heads, kv_heads, dtype = Packing([70, 3, 31]), 4, 2, "bfloat16"
+    q, k, v, g = (stored(normal(81 + i, (104, n, dim)), dtype) for i, n in enumerate((heads, kv_heads, kv_heads, heads)))
+    stores, dims = [upload(x, dtype) for x in (q, k, v)], (packing, heads, kv_heads, dim)
+    out, lse, rest = amd_lm.attention_packed(*stores, *dims, rest=True)
+    operands = dict(gradient=upload(g, dtype), q=stores[0], k=stores[1], v=stores[2], out=out, lse=lse)
+    expected = [download(x) for x in amd_lm.attention_packed_backward(**operands, packing=packing, heads=heads, kv_heads=kv_heads,
+                                                                      dim=dim, rest=rest)]
+    if which == "rest":
+        rest = shifted(download(rest), dtype)
+        assert rest.ptr % 16
+    else:
+        operands[which] = shifted(download(operands[which]), dtype)
+    got = [download(x) for x in amd_lm.attention_packed_backward(**operands, packing=packing, heads=heads, kv_heads=kv_heads, dim=dim,
+                                                                 rest=rest)]
+    for a, b in zip(got, expected):
+        # one wave per row knows out as bf16 alone, whose half step of 2^-8 is an error of delta and so of every dS
+        assert np.array_equal(a, b) if which == "rest" else np.abs(a - b).max() <= 2.0 ** -5 * np.abs(b).max()
