@@ -420,7 +420,9 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * backward's query tiles, 2: its key tiles); aligned: every pointer and pitch is a
  * multiple of 16 bytes.  rest (NULL, or bf16 laid out as out; bf16 with dim up to 128
  * and tile_rows above 4) receives what out's rounding left, for the backward.  Rows
- * in no tile are left as they are.  dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up
+ * in no tile are left as they are.  A launch holds less than 2^23 workgroups, a tile's
+ * being the heads of its side (QA_EINVAL beyond; up to four query heads of a kv head share
+ * one in bf16 up to 128).  dtype QA_F32 or QA_BF16, dim up to 256.  bf16 up
  * to 128 rounds probabilities and dS to bf16 for their products, in two parts where their
  * sequence has no more than 64 tokens; the others keep fp32's bits. */
 int64_t qutai_amd_attention_packed_rows(int64_t tokens, int64_t sequences, int64_t longest, int64_t heads,

@@ -244,8 +244,11 @@ bool whole(std::initializer_list<const void*> pointers, std::initializer_list<in
   return aligned16(pointers);
 }
 
-// Workgroups of 512 threads that a launch can hold.
-bool grid_fits(int64_t tiles, int64_t blocks) { return tiles >= 0 && tiles <= ((1ll << 23) - 1) / blocks; }
+// Whether a launch can hold a pass's workgroups, of 512 threads at most (`apart`: heads of a
+// group that take workgroups of their own).
+bool grid_fits(int64_t tiles, int64_t groups, int64_t apart = 1) {
+  return tiles >= 0 && tiles <= ((1ll << 23) - 1) / (groups * apart);
+}
 
 }  // namespace
 
@@ -283,7 +286,7 @@ int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, 
   AttnPackedArgs a = {};
   const int status = set_packed(a, tokens, sequences, longest, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
   if (status != QA_OK) return status;
-  if (!grid_fits(tile_count, heads)) return QA_EINVAL;
+  if (!grid_fits(tile_count, groups_of(FORWARD, dtype, heads, kv_heads, dim, tile_rows))) return QA_EINVAL;
   if (rest && (tile_rows == GEN_WAVES || !packed_fits(dtype, dim))) return QA_EINVAL;
   if (!tile_count) return QA_OK;
   if (!q || !k || !v || !out || !lse || !tiles) return QA_EINVAL;
@@ -311,7 +314,9 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
   if (status != QA_OK) return status;
   if (dq_row < heads * dim || dk_row < kv_heads * dim || dv_row < kv_heads * dim) return QA_EINVAL;
   if (std::max({dq_row, dk_row, dv_row}) > 1 << 22) return QA_EINVAL;
-  if (!grid_fits(query_count, heads) || !grid_fits(key_count, heads)) return QA_EINVAL;
+  if (!grid_fits(query_count, groups_of(QUERIES, dtype, heads, kv_heads, dim, query_rows)) ||
+      !grid_fits(key_count, kv_heads, heads_apart(dtype, tokens, sequences, heads, kv_heads, dim, key_rows)))
+    return QA_EINVAL;
   if (!query_count && !key_count) return QA_OK;
   if (!grad || !q || !k || !v || !out || !dq || !dk || !dv || !lse || !delta || !query_tiles || !key_tiles)
     return QA_EINVAL;

@@ -39,3 +39,25 @@ def test_operands_at_any_address(which, dim):
     for a, b in zip(got, expected):
         # one wave per row knows out as bf16 alone, whose half step of 2^-8 is an error of delta and so of every dS
         assert np.array_equal(a, b) if which == "rest" else np.abs(a - b).max() <= 2.0 ** -5 * np.abs(b).max()
+
+
+def test_many_sequences_of_many_heads():
+    """More tiles times heads than workgroups fit a launch, of heads that share workgroups:
+    sequences of one token, whose out is their value, and whose dV is their heads' gradient
+    summed (four bf16 terms in fp32, rounded to bf16)."""
+    count, heads, kv_heads, dim = 140000, 64, 16, 8
+    assert count * heads >= 1 << 23
+    packing = Packing([1] * count)
+    q, k, v, g = (stored(np.tile(normal(91 + i, 1000 * n * dim), count // 1000), "bfloat16")
+                  for i, n in enumerate((heads, kv_heads, kv_heads, heads)))
+    stores, dims = [upload(x, "bfloat16") for x in (q, k, v)], (packing, heads, kv_heads, dim)
+    out, lse, rest = amd_lm.attention_packed(*stores, *dims, rest=True)
+    expected = np.repeat(v.reshape(count, kv_heads, 1, dim), heads // kv_heads, 2)
+    assert np.array_equal(download(out), expected.reshape(-1))
+    dq, dk, dv = amd_lm.attention_packed_backward(upload(g, "bfloat16"), *stores, out, lse, *dims, rest=rest)
+    terms = g.astype(np.float64).reshape(count, kv_heads, heads // kv_heads, dim)
+    total = terms.sum(2).reshape(-1)
+    assert (np.abs(download(dv) - total) <= 2.0 ** -8 * np.abs(total) + 2.0 ** -22 * np.abs(terms).sum(2).reshape(-1)).all()
+    # dS is what two fp32 sums of the same 8 products, of up to 60 in all, leave: 8 x 2^-24 x 60 each; times |q| or |k| of up
+    # to 5, the scale of 0.36 and the four heads of dK: 4e-4 at most
+    assert np.abs(download(dq)).max() <= 4e-4 and np.abs(download(dk)).max() <= 4e-4
