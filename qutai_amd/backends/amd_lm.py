@@ -712,7 +712,7 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
             left = AMDStorage(out.size, name)
         out.runtime.call("qutai_amd_attention_packed_fwd", q_at, k_at, v_at, out.ptr, lse.ptr, amd._p(left), tiles.ptr, count,
                          rows, *packing.extent, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, int(bool(causal)),
-                         mfma=_on_matrix_cores(name, dim))
+                         mfma=rows > 4)
     if packing.used < total:
         _packed_tail(packing, out, lse, left)
     return (out, lse, left) if rest else (out, lse)
@@ -763,7 +763,7 @@ def attention_packed_backward(gradient, q, k, v, out, lse, packing, heads, kv_he
         delta.runtime.call("qutai_amd_attention_packed_bwd", gradient.ptr, q_at, k_at, v_at, out.ptr, amd._p(rest), lse.ptr,
                            *targets, delta.ptr, amd._p(workspace), need, q_tiles.ptr, q_count, q_rows, k_tiles.ptr, k_count,
                            k_rows, *packing.extent, heads, kv_heads, dim, q_row, k_row, v_row, *steps, dtype, scale, int(bool(causal)),
-                           mfma=_on_matrix_cores(q.dtype, dim))
+                           mfma=max(q_rows, k_rows) > 4)
     if packing.used < total:
         if into is None:
             _packed_tail(packing, *results)

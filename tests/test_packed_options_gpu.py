@@ -61,3 +61,22 @@ def test_many_sequences_of_many_heads():
     # dS is what two fp32 sums of the same 8 products, of up to 60 in all, leave: 8 x 2^-24 x 60 each; times |q| or |k| of up
     # to 5, the scale of 0.36 and the four heads of dK: 4e-4 at most
     assert np.abs(download(dq)).max() <= 4e-4 and np.abs(download(dk)).max() <= 4e-4
+
+
+@pytest.mark.parametrize("dtype,dim,lengths,shift,forward,backward", [
+    ("bfloat16", 64, [70, 3], 0, True, True), ("bfloat16", 64, [70, 3], 1, False, False), ("bfloat16", 20, [70, 3], 0, False, False),
+    ("bfloat16", 64, [2, 3], 0, True, True),  # queries in tiles, keys one at a time
+    ("bfloat16", 136, [70, 3], 0, True, True), ("bfloat16", 136, [20, 3], 0, False, False),
+    ("float32", 64, [70, 3], 0, True, True), ("float32", 64, [20, 3], 0, False, False), ("float32", 160, [70, 3], 0, False, False)])
+def test_what_counts_as_a_launch_on_the_matrix_cores(dtype, dim, lengths, shift, forward, backward):
+    """The calls whose rows are worked on in tiles, in one of the passes at least."""
+    runtime, packing, heads, kv_heads = amd.get_runtime(), Packing(lengths), 4, 2
+    q, k, v, g = (shifted(normal(95 + i, packing.total * n * dim), dtype, shift)
+                  for i, n in enumerate((heads, kv_heads, kv_heads, heads)))
+    dims = (packing, heads, kv_heads, dim)
+    before = runtime.mfma_launches
+    out, lse = amd_lm.attention_packed(q, k, v, *dims)
+    assert runtime.mfma_launches - before == forward
+    before = runtime.mfma_launches
+    amd_lm.attention_packed_backward(g, q, k, v, out, lse, *dims)
+    assert runtime.mfma_launches - before == backward
