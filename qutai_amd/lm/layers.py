@@ -857,10 +857,11 @@ def gqa_attention(x, wq, wk, wv, heads, kv_heads, theta, q_norm=None, k_norm=Non
 
 
 def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turns, packing):
-    """gqa_attention with a Rotary or over packed sequences.  The heads are turned
-    in the product's own columns; normed heads, whose product the backward needs,
-    go to new rows (the norm's launch turns them too, but by a Rotary's turns, which
-    take a launch of their own)."""
+    """gqa_attention with a Rotary or over packed sequences, whose heads are turned in
+    the product's own columns, which attention reads.  Without a packing the turned heads
+    go to rows of their own, as do normed ones, whose product the backward needs (the
+    norm's launch turns them too, but by a Rotary's turns, which take a launch of their
+    own)."""
     b = backend(x)
     batch, time, width = x.shape
     if packing is not None and (batch, time) != (1, packing.total):
@@ -878,17 +879,15 @@ def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turn
         turns = default_rotary(head, theta)
     turned = (turns, batch, time, heads, kv_heads, head)
     if q_norm is None:
-        q, k = b.rotary(qkv, qkv, *turned, positions=positions, **columns, out=qkv, **into)
+        q, k = b.rotary(qkv, qkv, *turned, positions=positions, **columns,
+                        **({} if packing is None else dict(out=qkv, **into)))
         parents = (x, wq, wk, wv)
     else:  # a position for each token: 0 turns nothing
         starts = positions if turns is None else None
-        norm_dims = (q_norm.storage, k_norm.storage, *((batch, time) if turns is None and packing is None else (rows, 1)),
-                     heads, kv_heads, head, theta, eps)
+        norm_dims = q_norm.storage, k_norm.storage, rows, 1, heads, kv_heads, head, theta, eps
         q, k = b.qk_norm_rope(qkv, qkv, *norm_dims, **columns, starts=starts)
         if turns is not None:
-            for side, block in ((0, q), (1, k)):
-                n = (0, kv_heads) if side else (heads, 0)
-                b.rotary(q, k, turns, batch, time, *n, head, positions=positions, out=block, out_k_column=0)
+            q, k = b.rotary(q, k, *turned, positions=positions)
         parents = (x, wq, wk, wv, q_norm, k_norm)
     if packing is not None:
         place = dict(v_column=dq + dkv, v_row=total, **(columns if q_norm is None else {}))
@@ -896,8 +895,6 @@ def _gqa_turned(x, wq, wk, wv, heads, kv_heads, theta, q_norm, k_norm, eps, turn
         keep = is_recording() and any(t.requires_grad for t in parents)
         out, lse, *rest = b.attention_packed(q, k, qkv, *dims, **place, rest=keep)
     else:
-        if q_norm is None:
-            q, k = (b.copy_rows(qkv, rows, n, column=c, row=total) for n, c in ((dq, 0), (dkv, dq)))
         v = b.copy_rows(qkv, rows, dkv, column=dq + dkv, row=total)
         dims = (batch, time, heads, kv_heads, head)
         out, lse = b.attention(q, k, v, *dims)
