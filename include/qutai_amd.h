@@ -476,7 +476,8 @@ int qutai_amd_positions(const int64_t* starts, int64_t sequences, int64_t used, 
  * gradient's too) and a number that tells it from the others (8 bits: part of what
  * decides how its codes are rounded, with `seed` and `step`).  bits 32: moments are
  * fp32.  bits 8: one byte a value, and two exponents (int8, first and second) for
- * every 256 values; zeros stand for zeros.
+ * every 256 values; zeros stand for zeros; where one moment is not finite or 2^127 or more
+ * all 256 read as NaN in the next step.
  *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *   p' = p (1 - rate weight_decay) - rate m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
  * eps, rate / (1 - beta1^step) and rate weight_decay are fp32 in the kernels: QA_EINVAL

@@ -21,7 +21,8 @@
 // of operations, and fp32's are rounded once.
 //
 // A block with an infinity, a NaN or a moment of 2^127 or more has the exponent 127 and
-// reads as NaN.
+// reads as NaN, so the next step makes NaN of all 256 parameters (the codes have none for a
+// single value; without a norm to find it by, a gradient that is not finite is the caller's).
 //
 // One launch steps 48 tensors, whose records are its arguments: a workgroup takes 1024 or
 // 4096 values of one of them at a time, with 8 bits a wave a block.  Memory bounds it

@@ -28,7 +28,9 @@ class AdamW:
     gives the same bits).  With ``max_norm`` gradients whose norm over all tensors
     exceeds it are scaled down to it, and a step whose norm is not finite changes
     nothing (t counts it all the same: nothing is read from the device); ``norm()``
-    is the last step's.  ``lr`` may be changed between steps.  ``eps`` and each
+    is the last step's.  Without it a gradient that is not finite makes its value NaN
+    for good, and with 8 bits, from the next step on, all 256 values that share its
+    moments' exponent.  ``lr`` may be changed between steps.  ``eps`` and each
     step's rate are fp32 in the kernels: eps is 2^-126 or more."""
 
     def __init__(self, parameters, lr=1e-3, *, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, bits=32, max_norm=None,

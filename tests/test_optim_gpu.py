@@ -27,3 +27,28 @@ def test_the_least_eps_leaves_values_without_a_gradient(bits):
     assert np.array_equal(after[::3], start[::3])
     expected = start.astype(np.float64) - 1e-2 * np.sign(g)
     assert (np.abs(after - expected) <= UNIT * (np.abs(expected) + 8 * 1e-2)).all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+@pytest.mark.parametrize("bits,lost", [(32, slice(600, 601)), (8, slice(512, 768))])
+def test_what_a_bad_gradient_costs_for_good(bits, lost, bad):
+    """Without max_norm an infinity or NaN among the gradients takes its own value with
+    moments of 32 bits, with 8 bits from the next step on all 256 that share its moments'
+    exponent; every other value goes on to the bit as if that gradient had been 0."""
+    runs = []
+    for value in (bad, 0.0):
+        p = Tensor(upload(normal(3, 1024), "float32"), shape=(1024,), requires_grad=True)
+        optimizer = AdamW([p], bits=bits, seed=2)
+        for step in range(3):
+            g = normal(10 + step, 1024)
+            if step == 0:
+                g[600] = value
+            p.grad = Tensor(upload(g, "float32"), shape=(1024,))
+            optimizer.step()
+        runs.append([download(p.storage), *(download(x.storage) for x in optimizer.moments(p))])
+    expected = np.zeros(1024, bool)
+    expected[lost] = True
+    for i, (got, clean) in enumerate(zip(*runs)):
+        if i == 0 or bits == 8 or np.isnan(bad):  # fp32's moments of an infinity are infinite: 0.9 inf and more
+            assert np.array_equal(np.isnan(got), expected), i
+        assert np.array_equal(got[~expected], clean[~expected]) and not np.isfinite(got[expected]).any()
