@@ -7,6 +7,7 @@ from qutai_amd import Tensor
 from qutai_amd.backends import amd
 from qutai_amd.optim import AdamW
 from tests.helpers import download, normal, stored, upload
+from tests.test_adamw_gpu import Model
 
 pytestmark = pytest.mark.gpu
 
@@ -52,3 +53,29 @@ def test_what_a_bad_gradient_costs_for_good(bits, lost, bad):
         if i == 0 or bits == 8 or np.isnan(bad):  # fp32's moments of an infinity are infinite: 0.9 inf and more
             assert np.array_equal(np.isnan(got), expected), i
         assert np.array_equal(got[~expected], clean[~expected]) and not np.isfinite(got[expected]).any()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_parameters_of_both_types(bits):
+    """float32 and bfloat16 tensors in one optimizer, whose norm is that of all gradients."""
+    sizes, types = [700, 513, 3, 4096], ["float32", "bfloat16", "bfloat16", "float32"]
+    values = [stored(normal(20 + i, n), t) for i, (n, t) in enumerate(zip(sizes, types))]
+    parameters = [Tensor(upload(x, t), shape=x.shape, requires_grad=True) for x, t in zip(values, types)]
+    options = dict(lr=1e-2, betas=(0.9, 0.99), weight_decay=0.1, max_norm=0.5, seed=6)
+    optimizer, model = AdamW(parameters, **options, bits=bits), Model(values, bits, **options)
+    for step in range(2):
+        given = [stored(normal(40 + 10 * step + i, n), t) for i, (n, t) in enumerate(zip(sizes, types))]
+        for p, g, t in zip(parameters, given, types):
+            p.grad = Tensor(upload(g, t), shape=p.shape)
+        optimizer.step()
+        norm = model.step(given)
+        assert abs(optimizer.norm() - norm) <= 1e-12 * norm
+        for i, (p, t) in enumerate(zip(parameters, types)):
+            got, value = download(p.storage), model.p[i]
+            # a dozen fp32 roundings of a quotient of some ten times lr at most, and the parameter's own
+            bound = 40 * UNIT * (np.abs(value) + 10 * options["lr"]) + (2.0 ** -8 * np.abs(value) if t == "bfloat16" else 0)
+            assert (np.abs(got - value) <= bound).all(), (step, i)
+            model.p[i] = got.astype(np.float64)  # each step on its own
+            first, second = (download(x.storage) for x in optimizer.moments(p))
+            if bits == 8:
+                assert np.array_equal(first, model.m[i]) and np.array_equal(second, model.v[i]), (step, i)
