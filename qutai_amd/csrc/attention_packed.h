@@ -200,6 +200,11 @@ __device__ __forceinline__ void add_columns(lds_bytes tile, const typename Packe
   }
 }
 
+// All waves have a block in LDS and are done with the one before, whose stage is copied into
+// next: a wave's reads of it, and what it wrote, are waited for here, wherever the compiler
+// puts their uses.
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 // The tile, heads and rows of a wave of a query tile.
 struct PackedPlace {
   int h, kvh, first, q0;  // first row of the tile, of the wave
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(NW * 64, DP <= 64 ? 4 : 3) packed_fwd(AttnPack
   const int n_full = T <= FINE ? 0 : min(seen, p.causal ? q0 + 1 : T) / KB;
   auto advance = [&](int kbk) {  // wait for a block, start the next one's copies
     wait_vmcnt<0>();
-    asm volatile("s_barrier" ::: "memory");
+    stage_barrier();
     if (kbk + 1 < nkb) issue(kbk + 1);
   };
   if (nkb > 0) issue(0);
@@ -442,7 +447,7 @@ __global__ void __launch_bounds__(NW * 64, DP <= 64 ? 4 : 2) packed_bwd_dq(AttnP
   const int n_full = T <= FINE ? 0 : min(seen, p.causal ? q0 + 1 : T) / KB;
   auto advance = [&](int kbk) {
     wait_vmcnt<0>();
-    asm volatile("s_barrier" ::: "memory");
+    stage_barrier();
     if (kbk + 1 < nkb) issue(kbk + 1);
   };
   if (nkb > 0) issue(0);
@@ -600,11 +605,8 @@ __global__ void __launch_bounds__(KW * SPLIT * 64, DP == 32 ? 3 : 2) packed_bwd_
   // first of the set's next
   auto advance = [&](int it, int h, int qi) {
     wait_vmcnt<0>();
-    if (wave < 2 && lane < QB) {
-      stats[it & 1][set][wave][lane] = wave ? next : -next * LOG2E;
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): in LDS before the barrier
-    }
-    asm volatile("s_barrier" ::: "memory");
+    if (wave < 2 && lane < QB) stats[it & 1][set][wave][lane] = wave ? next : -next * LOG2E;
+    stage_barrier();
     if (it + 1 < iterations) {
       const bool wrap = qi + 1 == nq;
       issue(it + 1, wrap ? h + SPLIT : h, qs0 + (wrap ? 0 : qi + 1) * QB);
