@@ -1042,6 +1042,17 @@ def qk_norm_rope_backward(gq, gk, q, k, q_weight, k_weight, batch, time, heads, 
     return dq, dk, dwq, dwk
 
 
+def _int64(value):
+    """A whole number as the int that an int64 argument holds."""
+    try:
+        whole = int(value)
+    except (TypeError, ValueError, OverflowError):
+        whole = None
+    if whole is None or whole != value or not -(1 << 63) <= whole < 1 << 63:
+        raise ValueError("the offset is an integer of 64 bits")
+    return whole
+
+
 def rotary(q, k, rotary, batch, time, heads, kv_heads, dim, *, positions=None, offset=0, starts=None, inverse=False,
            q_column=0, q_row=None, k_column=0, k_row=None, out=None, out_row=None, out_q_column=0, out_k_column=None):
     """(q, k) with the first channels of every head turned by their tokens'
@@ -1056,8 +1067,9 @@ def rotary(q, k, rotary, batch, time, heads, kv_heads, dim, *, positions=None, o
     side out (its result is None)."""
     if rotary.dim != dim or min(batch, time, heads, kv_heads) < 0 or heads + kv_heads == 0:
         raise ValueError("rotary turns query or key heads of its own width")
-    if inverse not in (False, True) or offset != int(offset):
-        raise ValueError("inverse is True or False, the offset an integer")
+    if inverse not in (False, True):
+        raise ValueError("inverse is True or False")
+    offset = _int64(offset)
     tokens = batch * time
     if positions is not None and (starts is not None or offset or positions.dtype != "int64" or positions.size != tokens):
         raise ValueError("positions hold one int64 for every token, without offset and starts")
