@@ -27,7 +27,6 @@ using namespace qa;
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int64_t CACHED = 128 << 20;  // bytes of results that stay in the memory-side cache (256 MB)
 
 struct RotaryArgs {
   const void* x[2];  // queries, keys
@@ -39,13 +38,12 @@ struct RotaryArgs {
   int heads[2], dim, rotary;
   int pair_lanes, lanes, slots;  // lanes of a token that turn pairs, all of its lanes, lanes that share its heads
   float magnitude, sign;
-  bool past;  // results are stored past the caches
   double turns[128];
 };
 
 // N elements at once: 16 or 8 bytes, or one.  Inputs are read once, past the caches;
-// results stay there for the attention that reads them next, unless (`past`) they do
-// not fit: 336 MB of them take 123 us past the caches and 133 through them.
+// results stay there for the attention that reads them next (336 MB of them, more than the
+// caches hold, take 133 us either way).
 template <class T, int N>
 __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
   if constexpr (N == 1) {
@@ -62,7 +60,7 @@ __device__ __forceinline__ void load(const T* p, float (&v)[N]) {
   }
 }
 template <class T, int N>
-__device__ __forceinline__ void store(T* p, const float (&v)[N], bool past) {
+__device__ __forceinline__ void store(T* p, const float (&v)[N]) {
   if constexpr (N == 1) {
     if constexpr (sizeof(T) == 4) p[0] = v[0];
     else p[0] = f32_to_bf16(v[0]);
@@ -74,13 +72,13 @@ __device__ __forceinline__ void store(T* p, const float (&v)[N], bool past) {
       if constexpr (sizeof(T) == 4) w[e] = __float_as_uint(v[e]);
       else w[e] = pack_bf16x2(v[2 * e], v[2 * e + 1]);
     }
-    if (past) global_store_nt(p, w);
-    else global_store(p, w);
+    global_store(p, w);
   }
 }
 
 // V elements of T at a time: 16 or 8 bytes, or one where widths, pitches or addresses
-// are no whole chunks of that.
+// are no whole chunks of that (32768 tokens, 16 and 4 bf16 heads of 80: 54 us with 32
+// channels turned, 124 with 20, whose halves of 10 are 20 bytes).
 template <class T, int V, bool HALF>
 __global__ void __launch_bounds__(THREADS) rotary_kernel(RotaryArgs a) {
   const int64_t id = (int64_t)blockIdx.x * THREADS + threadIdx.x;
@@ -140,8 +138,8 @@ __global__ void __launch_bounds__(THREADS) rotary_kernel(RotaryArgs a) {
         for (int e = 0; e < V; e++) u[e] = y[e], w[e] = y[V + e];
       }
     }
-    store<T, V>(out + first, u, a.past);
-    if (both) store<T, V>(out + second, w, a.past);
+    store<T, V>(out + first, u);
+    if (both) store<T, V>(out + second, w);
   }
 }
 
@@ -226,7 +224,6 @@ int qutai_amd_rotary(const void* q, const void* k, void* q_out, void* k_out, con
   a.rotary = (int)rotary;
   a.magnitude = (float)magnitude;
   a.sign = inverse ? -1.f : 1.f;
-  a.past = a.tokens * (heads + kv_heads) * dim * item > CACHED;
   for (int64_t i = 0; i < rotary / 2; i++) a.turns[i] = turns[i];
   const hipStream_t s = (hipStream_t)stream;
   hipError_t e;
