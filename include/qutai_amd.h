@@ -409,7 +409,7 @@ int qutai_amd_attention_fwd(const void* q, const void* k, const void* v, void* o
  * that lie one behind the other in one matrix of tokens, the first from row 0 on, as
  * qutai_amd_attention_fwd of each alone (causal != 0: a token sees its sequence up
  * to itself).  q, k and v rows start q_row, k_row and v_row elements after the
- * previous token's (columns of wider matrices), heads `dim` elements after each
+ * previous token's (columns of wider matrices; up to 2^22 each), heads `dim` elements after each
  * other; out is contiguous [tokens][heads][dim], lse fp32 [tokens][heads].  `tiles`
  * (device) says which rows the workgroups take, tile_rows each and in this order:
  * tile_count int64 that hold the sequence's first token and, 32 bits up, the tile's
@@ -480,6 +480,7 @@ int qutai_amd_positions(const int64_t* starts, int64_t sequences, int64_t used, 
  * all 256 read as NaN in the next step.
  *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2,
  *   p' = p (1 - rate weight_decay) - rate m' / (1 - beta1^step) / (sqrt(v' / (1 - beta2^step)) + eps)
+ * Parameters and moments share no memory with each other or with the gradients.
  * eps, rate / (1 - beta1^step) and rate weight_decay are fp32 in the kernels: QA_EINVAL
  * where eps is no normal number of fp32 (2^-126 or more) or the others exceed it.
  * With max_norm > 0 gradients are scaled to that norm over all tensors where they

@@ -700,7 +700,8 @@ def attention_packed(q, k, v, packing, heads, kv_heads, dim, *, causal=True, sca
     of matrices of q_row elements per token (and so on).  out is contiguous
     [total][heads][dim], lse [total][heads]; rows behind the last sequence are
     zero.  With ``rest`` also what out's rounding left, for the backward (None
-    where there is none)."""
+    where there is none).  bf16 heads of up to 128 channels round probabilities (and
+    dS) to bf16 for their products, in two parts in sequences of up to 64 tokens."""
     q_at, k_at, v_at, q_row, k_row, v_row, odd = _packed_places(q, k, v, packing, heads, kv_heads, dim, q_column, q_row,
                                                                 k_column, k_row, v_column, v_row)
     name, total = q.dtype, packing.total

@@ -166,7 +166,8 @@ __device__ __forceinline__ bf16x8 left_of(const float* v, const bf16x8& kept) {
 // tokens of sequences of up to 6: dQ 1.5 times as far off as in fp32), and the products are
 // not what bounds them.  In the query passes every masked block carries two parts (all blocks
 // of such sequences take the masked form; those on the diagonal or at the end of longer ones
-// gain by it at no measured cost), in the key pass a loop of its own, which is all that a
+// gain by it for 0 to 4% of the time, most for the forward of one document of 2000 tokens, 16
+// heads over 4 of 128, 57 us and 55), in the key pass a loop of its own, which is all that a
 // batch of only such sequences needs (ONLY).  Forward, dQ, dK and dV in two parts and in one,
 // us: 16384 tokens of up to 64, 16 heads over 4 of 64, 40 and 38, 44 and 42, 60 and 60; 16000,
 // 32 over 8 of 128, 143 and 141, 220 and 215, 173 and 203.

@@ -216,7 +216,9 @@ class Decoder:
         than max_seq_len), which lie one behind the other in one row of tokens: no
         padding, no token sees another sequence, and positions start at 0 in each.
         The mean runs over the predictions of all sequences (a sequence's last token
-        predicts nothing); labels have the sequences' shape, -100 is ignored."""
+        predicts nothing); labels have the sequences' shape, -100 is ignored.  Under
+        autocast attention rounds probabilities to bf16 (amd_lm.attention_packed), where
+        that of ``loss`` does so for heads of 64 channels only."""
         if chunk_size <= 0:
             raise ValueError("chunk_size must be positive")
         rows = [row if isinstance(row, (list, tuple)) else list(row) for row in sequences]
