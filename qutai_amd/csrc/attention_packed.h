@@ -643,9 +643,9 @@ __global__ void __launch_bounds__(KW * SPLIT * 64, DP == 32 ? 3 : 2) packed_bwd_
     };
     auto step = [&](int st, auto mask, auto parts) {
       const int qi = st / HB, qs = qs0 + qi * QB;
-      packed_dkv_step<DP, decltype(mask)::value, decltype(parts)::value>(sq, sg, in, &stats[it & 1][set][0][0], &stats[it & 1][set][1][0], kf, vf,
-                                                 sv, own, dkt, dvt, T - qs, p.causal ? key - qs : -1, p.scale_log2,
-                                                 half, st % HB);
+      packed_dkv_step<DP, decltype(mask)::value, decltype(parts)::value>(
+          sq, sg, in, &stats[it & 1][set][0][0], &stats[it & 1][set][1][0], kf, vf, sv, own, dkt, dvt, T - qs,
+          p.causal ? key - qs : -1, p.scale_log2, half, st % HB);
     };
     int st = 0;
     for (; st < skipped; st++) enter(st);

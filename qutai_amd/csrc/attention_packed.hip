@@ -283,10 +283,11 @@ size_t qutai_amd_attention_packed_workspace(int64_t tokens, int64_t sequences, i
 
 int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, void* out, float* lse, void* rest,
                                    const int64_t* tiles, int64_t tile_count, int64_t tile_rows, int64_t tokens, int64_t sequences,
-                                   int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int dtype,
-                                   double scale, int causal, void* stream) {
+                                   int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row,
+                                   int64_t v_row, int dtype, double scale, int causal, void* stream) {
   AttnPackedArgs a = {};
-  const int status = set_packed(a, tokens, sequences, longest, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal, {{FORWARD, tile_rows}});
+  const int status = set_packed(a, tokens, sequences, longest, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
+                                {{FORWARD, tile_rows}});
   if (status != QA_OK) return status;
   if (!grid_fits(tile_count, groups_of(FORWARD, dtype, heads, kv_heads, dim, tile_rows))) return QA_EINVAL;
   if (rest && (tile_rows == GEN_WAVES || !packed_fits(dtype, dim))) return QA_EINVAL;
@@ -305,11 +306,11 @@ int qutai_amd_attention_packed_fwd(const void* q, const void* k, const void* v, 
 
 int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* k, const void* v, const void* out,
                                    const void* rest, const float* lse, void* dq, void* dk, void* dv, float* delta,
-                                   void* workspace, size_t workspace_bytes, const int64_t* query_tiles, int64_t query_count, int64_t query_rows,
-                                   const int64_t* key_tiles, int64_t key_count, int64_t key_rows, int64_t tokens, int64_t sequences,
-                                   int64_t longest, int64_t heads, int64_t kv_heads, int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row,
-                                   int64_t dq_row, int64_t dk_row, int64_t dv_row, int dtype, double scale, int causal,
-                                   void* stream) {
+                                   void* workspace, size_t workspace_bytes, const int64_t* query_tiles, int64_t query_count,
+                                   int64_t query_rows, const int64_t* key_tiles, int64_t key_count, int64_t key_rows,
+                                   int64_t tokens, int64_t sequences, int64_t longest, int64_t heads, int64_t kv_heads,
+                                   int64_t dim, int64_t q_row, int64_t k_row, int64_t v_row, int64_t dq_row, int64_t dk_row,
+                                   int64_t dv_row, int dtype, double scale, int causal, void* stream) {
   AttnPackedArgs a = {};
   const int status = set_packed(a, tokens, sequences, longest, heads, kv_heads, dim, q_row, k_row, v_row, dtype, scale, causal,
                                 {{QUERIES, query_rows}, {KEYS, key_rows}});
@@ -348,7 +349,8 @@ int qutai_amd_attention_packed_bwd(const void* grad, const void* q, const void* 
     a.part_v = a.part_k + group * a.part_stride;
   }
   // the query pass writes delta, which the key pass reads
-  hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), longest, query_tiles, query_count, query_rows, (hipStream_t)stream);
+  hipError_t e = launch(QUERIES, dtype, a, key_tiles_of(tokens, sequences), longest, query_tiles, query_count, query_rows,
+                        (hipStream_t)stream);
   if (e != hipSuccess) return (int)e;
   e = launch(KEYS, dtype, a, key_tiles_of(tokens, sequences), longest, key_tiles, key_count, key_rows, (hipStream_t)stream);
   if (e != hipSuccess || !a.split || !key_count) return (int)e;
